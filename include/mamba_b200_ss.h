@@ -58,6 +58,10 @@ extern "C" {
 /* the reference's kernels dispatch dstate up to 256 (csrc/selective_scan/static_switch.h:15-35) */
 #define SS_MAX_DSTATE 256
 #define SS_MAX_CONV_WIDTH 4
+/* largest key_dim and value_dim of the linear-attention calls */
+#define SS_MAX_LINEAR_DIM 128
+/* longest row of the block-norm calls */
+#define SS_MAX_BLOCK_NORM_DIM 8192
 /* capacity (floats) of the library-held state array used by ss_bwd_noalloc: 16 MiB */
 #define SS_NOALLOC_MAX_CKPT_ELEMS 4194304
 
@@ -255,6 +259,127 @@ typedef struct ss_mamba_step_args {
   void* y;               int64_t y_batch_stride;    /* (batch, dim): the gated output         */
 } ss_mamba_step_args;
 
+/* Linear attention with a decay per head (no counterpart in the reference; the selective scan's
+ * sibling with a matrix state).  Per batch row and head, in fp32:
+ *   S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T       (key_dim x value_dim)
+ *   o_t = scale * q_t S_t
+ * heads is a multiple of key_heads; head j uses q and k of key head j / (heads / key_heads).
+ * key_dim and value_dim are at most SS_MAX_LINEAR_DIM.  The innermost axis of q, k, v, o has stride 1.
+ * A log decay of -infinity resets the state.  With seq_lens, tokens t >= seq_lens[b] (clamped to
+ * [0, seqlen]) are not read into anything and their o is zero. */
+typedef struct ss_linear_args {
+  int batch, seqlen, heads, key_heads, key_dim, value_dim;
+  int io_dtype;             /* dtype of q, k, v, o                                        */
+  int decay_dtype;          /* SS_F32 or io_dtype                                         */
+  float scale;
+  const void* q;     int64_t q_batch_stride, q_seq_stride, q_head_stride;
+  const void* k;     int64_t k_batch_stride, k_seq_stride, k_head_stride;
+  const void* v;     int64_t v_batch_stride, v_seq_stride, v_head_stride;
+  const void* log_decay; int64_t decay_batch_stride, decay_seq_stride, decay_head_stride;
+                            /* batch and seq strides 0: one decay per head                */
+  const int32_t* seq_lens;  /* (batch) nullable                                           */
+  const float* state_in;    /* (batch, heads, key_dim, value_dim) packed; nullable: zeros  */
+  float* state_out;         /* same shape; nullable                                       */
+  void* o;           int64_t o_batch_stride, o_seq_stride, o_head_stride;
+  void* work;               /* 16-byte aligned scratch of ss_linear_work_bytes(args, 0) bytes (not
+                               needed between calls); nullable when that is 0              */
+} ss_linear_args;
+
+/* Gradients of ss_linear_fwd.  f holds the forward's inputs (f.o and f.work are ignored; f.state_out
+ * is the final state that the forward wrote, read when dstate_out is given). */
+typedef struct ss_linear_bwd_args {
+  ss_linear_args f;
+  const void* dout;  int64_t do_batch_stride, do_seq_stride, do_head_stride;
+  const float* dstate_out;  /* gradient of state_out, packed; nullable: zeros              */
+  void* dq;          int64_t dq_batch_stride, dq_seq_stride, dq_head_stride;
+  void* dk;          int64_t dk_batch_stride, dk_seq_stride, dk_head_stride;
+  void* dv;          int64_t dv_batch_stride, dv_seq_stride, dv_head_stride;
+  void* dlog_decay;         /* nullable; decay_dtype, packed: (batch, seqlen, heads), or (heads) when
+                               f's batch and seq decay strides are 0                       */
+  float* dstate_in;         /* nullable; packed                                            */
+  void* work;               /* ss_linear_work_bytes(&f, 1) bytes                           */
+} ss_linear_bwd_args;
+
+/* One token: state <- exp(log_decay) state + k v^T; o = scale * q state. */
+typedef struct ss_linear_step_args {
+  int batch, heads, key_heads, key_dim, value_dim, io_dtype, decay_dtype;
+  float scale;
+  float* state;      int64_t state_batch_stride;  /* (batch, heads, key_dim, value_dim) fp32, heads packed */
+  const void* q;     int64_t q_batch_stride, q_head_stride;
+  const void* k;     int64_t k_batch_stride, k_head_stride;
+  const void* v;     int64_t v_batch_stride, v_head_stride;
+  const void* log_decay; int64_t decay_batch_stride, decay_head_stride;
+  void* o;           int64_t o_batch_stride, o_head_stride;
+} ss_linear_step_args;
+
+/* The norms before and after a block with its gate and the residual scale, over rows of length dim
+ * (dim <= SS_MAX_BLOCK_NORM_DIM; no counterpart in the reference).  In fp32, rounded once:
+ *   n = post_weight ? y * rsqrt(mean(y^2) + eps) * w(post_weight) : y       w(p) = unit_offset ? 1 + p : p
+ *   h = residual + scale * act(gate) * n          (the next residual stream)
+ *   x = h * rsqrt(mean(h^2) + pre_eps) * w(pre_weight)   from the unrounded h; only with pre_weight
+ * activation: 0 none, 1 SiLU, 2 sigmoid.  A gate row stride of 0 uses one gate row for all rows. */
+typedef struct ss_block_norm_args {
+  int rows, dim, io_dtype, unit_offset, activation;
+  float eps, pre_eps;                                        /* of the norm of y, and of h    */
+  float scale_const;                                         /* used when scale is NULL       */
+  const void* y;         int64_t y_row_stride;
+  const void* residual;  int64_t residual_row_stride;
+  const void* gate;      int64_t gate_row_stride;            /* nullable                      */
+  const float* post_weight;                                  /* (dim) fp32, nullable          */
+  const float* pre_weight;                                   /* (dim) fp32, nullable          */
+  const float* scale;                                        /* (dim) fp32, nullable          */
+  void* h;               int64_t h_row_stride;
+  void* x;               int64_t x_row_stride;               /* iff pre_weight                */
+  float* rstd;                                               /* (rows, 2) fp32 for the backward, nullable */
+} ss_block_norm_args;
+
+/* Its backward from dx (iff pre_weight) and dh (nullable).  f holds the forward's inputs and rstd
+ * (f.h and f.x are ignored: h is recomputed unrounded).  The column gradients are summed in a
+ * fixed order. */
+typedef struct ss_block_norm_bwd_args {
+  ss_block_norm_args f;
+  const void* dx;        int64_t dx_row_stride;
+  const void* dh;        int64_t dh_row_stride;              /* nullable                      */
+  void* dy;              int64_t dy_row_stride;
+  void* dresidual;       int64_t dresidual_row_stride;
+  void* dgate;           int64_t dgate_row_stride;           /* iff gate                      */
+  float* dpost_weight;                                       /* (dim) nullable, overwritten   */
+  float* dpre_weight;                                        /* (dim) nullable, overwritten   */
+  float* dscale;                                             /* (dim) nullable, overwritten   */
+  float* work;                                               /* ss_block_norm_work_elems floats */
+} ss_block_norm_bwd_args;
+
+/* One step of beam search over the beams of each batch row:
+ *   cand[w, v] = scores[w] + logits[w, v] - logsumexp(logits[w])
+ *   finished beam: its score at eos_token, -infinity elsewhere
+ * and the num_select largest of (beams x vocab), the lowest index first among equals.  A candidate
+ * that is not a number, and every candidate of a beam whose score is NaN or +infinity, counts as
+ * -infinity.  Candidates are compared in fp64. */
+typedef struct ss_beam_args {
+  int batch, beams, vocab, num_select, io_dtype;
+  int eos_token;                                             /* used with finished            */
+  const void* logits;    int64_t logits_batch_stride, logits_beam_stride;  /* vocab stride 1  */
+  const float* scores;                                       /* (batch, beams) packed         */
+  const uint8_t* finished;                                   /* (batch, beams) packed, nullable */
+  float* out_scores;                                         /* (batch, num_select) packed    */
+  int64_t* parents;                                          /* (batch, num_select) packed    */
+  int64_t* tokens;                                           /* (batch, num_select) packed    */
+  void* work;                                                /* ss_beam_work_bytes bytes, 16-byte aligned */
+} ss_beam_args;
+
+#define SS_MAX_BEAMS 32
+#define SS_MAX_REORDER 64
+
+/* Rows of per-beam state gathered in place: for every tensor and batch row, row w <- row parents[w]
+ * of the rows before the call.  Tensor i is (batch * beams) packed rows of row_bytes[i] bytes, a multiple of 4.
+ * A parent outside [0, beams) leaves its row as it was and raises bit 2 of the device status. */
+typedef struct ss_reorder_args {
+  int batch, beams, count;                                   /* count <= SS_MAX_REORDER       */
+  const int64_t* parents; int64_t parents_batch_stride;      /* beam stride 1                 */
+  void* data[SS_MAX_REORDER];
+  int64_t row_bytes[SS_MAX_REORDER];
+} ss_reorder_args;
+
 /* Number of fp32 elements of the forward-to-backward state buffer. */
 SS_API size_t ss_ckpt_elems(int batch, int dim, int seqlen, int dstate);
 
@@ -315,6 +440,37 @@ SS_API int ss_rmsnorm_fwd(const ss_rmsnorm_args* args, void* stream);
 /* Its backward (see ss_rmsnorm_bwd_args). */
 SS_API int ss_rmsnorm_bwd(const ss_rmsnorm_bwd_args* args, void* stream);
 
+/* Linear attention over a sequence (see ss_linear_args). */
+SS_API int ss_linear_fwd(const ss_linear_args* args, void* stream);
+
+/* Its backward (see ss_linear_bwd_args). */
+SS_API int ss_linear_bwd(const ss_linear_bwd_args* args, void* stream);
+
+/* One token of linear attention (see ss_linear_step_args). */
+SS_API int ss_linear_step(const ss_linear_step_args* args, void* stream);
+
+/* Scratch bytes of ss_linear_fwd (backward = 0) or ss_linear_bwd (1) for these sizes, types and
+ * strides (data pointers and seq_lens' values are not looked at); 0 for invalid sizes. */
+SS_API size_t ss_linear_work_bytes(const ss_linear_args* args, int backward);
+
+/* Norms before and after a block with gate and residual scale (see ss_block_norm_args). */
+SS_API int ss_block_norm_fwd(const ss_block_norm_args* args, void* stream);
+
+/* Its backward (see ss_block_norm_bwd_args). */
+SS_API int ss_block_norm_bwd(const ss_block_norm_bwd_args* args, void* stream);
+
+/* Floats of ss_block_norm_bwd_args.work. */
+SS_API size_t ss_block_norm_work_elems(int64_t rows, int dim, int io_dtype);
+
+/* One step of beam search (see ss_beam_args). */
+SS_API int ss_beam_select(const ss_beam_args* args, void* stream);
+
+/* Bytes of ss_beam_args.work. */
+SS_API size_t ss_beam_work_bytes(int batch, int beams, int vocab, int num_select);
+
+/* Reorders per-beam states in place (see ss_reorder_args). */
+SS_API int ss_reorder(const ss_reorder_args* args, void* stream);
+
 /* Static description of a status code. */
 SS_API const char* ss_status_string(int status);
 
@@ -322,7 +478,7 @@ SS_API const char* ss_status_string(int status);
 SS_API int ss_last_cuda_error(void);
 
 /* Error bits that kernels raised on the current device since the last reset (1: a bounded
- * wait for a TMA tile gave up), or -1 if the status cannot be read.  Synchronizes `stream`;
+ * wait for a TMA tile or a matrix instruction gave up; 2: ss_reorder met a parent out of range), or -1 if the status cannot be read.  Synchronizes `stream`;
  * reset != 0 clears the bits. */
 SS_API int ss_device_status(int reset, void* stream);
 
@@ -345,8 +501,9 @@ SS_API int ss_abi_version(void);
 
 /* sizeof the argument structs as compiled into the library (0: ss_fwd_args,
  * 1: ss_bwd_args, 2: ss_step_args, 3: ss_conv_args, 4: ss_conv_bwd_args,
- * 5: ss_conv_step_args, 6: ss_rmsnorm_args, 7: ss_rmsnorm_bwd_args, 8: ss_mamba_step_args;
- * 0 for other values) — lets an FFI binding check its own struct
+ * 5: ss_conv_step_args, 6: ss_rmsnorm_args, 7: ss_rmsnorm_bwd_args, 8: ss_mamba_step_args,
+ * 9: ss_linear_args, 10: ss_linear_bwd_args, 11: ss_linear_step_args, 12: ss_block_norm_args,
+ * 13: ss_block_norm_bwd_args, 14: ss_beam_args, 15: ss_reorder_args; 0 for other values) — lets an FFI binding check its own struct
  * layout against the library's. */
 SS_API size_t ss_struct_size(int which);
 

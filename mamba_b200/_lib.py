@@ -141,16 +141,108 @@ class MambaStepArgs(ctypes.Structure):
     ]
 
 
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int), ("seqlen", c_int), ("heads", c_int), ("key_heads", c_int), ("key_dim", c_int),
+        ("value_dim", c_int), ("io_dtype", c_int), ("decay_dtype", c_int), ("scale", ctypes.c_float),
+        ("q", c_vp), ("q_batch_stride", c_i64), ("q_seq_stride", c_i64), ("q_head_stride", c_i64),
+        ("k", c_vp), ("k_batch_stride", c_i64), ("k_seq_stride", c_i64), ("k_head_stride", c_i64),
+        ("v", c_vp), ("v_batch_stride", c_i64), ("v_seq_stride", c_i64), ("v_head_stride", c_i64),
+        ("log_decay", c_vp), ("decay_batch_stride", c_i64), ("decay_seq_stride", c_i64), ("decay_head_stride", c_i64),
+        ("seq_lens", c_vp), ("state_in", c_vp), ("state_out", c_vp),
+        ("o", c_vp), ("o_batch_stride", c_i64), ("o_seq_stride", c_i64), ("o_head_stride", c_i64),
+        ("work", c_vp),
+    ]
+
+
+class LinearBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("f", LinearArgs),
+        ("dout", c_vp), ("do_batch_stride", c_i64), ("do_seq_stride", c_i64), ("do_head_stride", c_i64),
+        ("dstate_out", c_vp),
+        ("dq", c_vp), ("dq_batch_stride", c_i64), ("dq_seq_stride", c_i64), ("dq_head_stride", c_i64),
+        ("dk", c_vp), ("dk_batch_stride", c_i64), ("dk_seq_stride", c_i64), ("dk_head_stride", c_i64),
+        ("dv", c_vp), ("dv_batch_stride", c_i64), ("dv_seq_stride", c_i64), ("dv_head_stride", c_i64),
+        ("dlog_decay", c_vp), ("dstate_in", c_vp), ("work", c_vp),
+    ]
+
+
+class LinearStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int), ("heads", c_int), ("key_heads", c_int), ("key_dim", c_int), ("value_dim", c_int),
+        ("io_dtype", c_int), ("decay_dtype", c_int), ("scale", ctypes.c_float),
+        ("state", c_vp), ("state_batch_stride", c_i64),
+        ("q", c_vp), ("q_batch_stride", c_i64), ("q_head_stride", c_i64),
+        ("k", c_vp), ("k_batch_stride", c_i64), ("k_head_stride", c_i64),
+        ("v", c_vp), ("v_batch_stride", c_i64), ("v_head_stride", c_i64),
+        ("log_decay", c_vp), ("decay_batch_stride", c_i64), ("decay_head_stride", c_i64),
+        ("o", c_vp), ("o_batch_stride", c_i64), ("o_head_stride", c_i64),
+    ]
+
+
+class BlockNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", c_int), ("dim", c_int), ("io_dtype", c_int), ("unit_offset", c_int), ("activation", c_int),
+        ("eps", ctypes.c_float), ("pre_eps", ctypes.c_float), ("scale_const", ctypes.c_float),
+        ("y", c_vp), ("y_row_stride", c_i64),
+        ("residual", c_vp), ("residual_row_stride", c_i64),
+        ("gate", c_vp), ("gate_row_stride", c_i64),
+        ("post_weight", c_vp), ("pre_weight", c_vp), ("scale", c_vp),
+        ("h", c_vp), ("h_row_stride", c_i64),
+        ("x", c_vp), ("x_row_stride", c_i64),
+        ("rstd", c_vp),
+    ]
+
+
+class BlockNormBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("f", BlockNormArgs),
+        ("dx", c_vp), ("dx_row_stride", c_i64),
+        ("dh", c_vp), ("dh_row_stride", c_i64),
+        ("dy", c_vp), ("dy_row_stride", c_i64),
+        ("dresidual", c_vp), ("dresidual_row_stride", c_i64),
+        ("dgate", c_vp), ("dgate_row_stride", c_i64),
+        ("dpost_weight", c_vp), ("dpre_weight", c_vp), ("dscale", c_vp), ("work", c_vp),
+    ]
+
+
+class BeamArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int), ("beams", c_int), ("vocab", c_int), ("num_select", c_int), ("io_dtype", c_int),
+        ("eos_token", c_int),
+        ("logits", c_vp), ("logits_batch_stride", c_i64), ("logits_beam_stride", c_i64),
+        ("scores", c_vp), ("finished", c_vp),
+        ("out_scores", c_vp), ("parents", c_vp), ("tokens", c_vp), ("work", c_vp),
+    ]
+
+
+MAX_REORDER = 64  # SS_MAX_REORDER
+
+
+class ReorderArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", c_int), ("beams", c_int), ("count", c_int),
+        ("parents", c_vp), ("parents_batch_stride", c_i64),
+        ("data", c_vp * MAX_REORDER), ("row_bytes", c_i64 * MAX_REORDER),
+    ]
+
+
 # ss_struct_size index order
 STRUCTS = (FwdArgs, BwdArgs, StepArgs, ConvArgs, ConvBwdArgs, ConvStepArgs, RmsNormArgs, RmsNormBwdArgs,
-           MambaStepArgs)
+           MambaStepArgs, LinearArgs, LinearBwdArgs, LinearStepArgs, BlockNormArgs, BlockNormBwdArgs, BeamArgs,
+           ReorderArgs)
 ABI_VERSION = 8
 MAX_CONV_WIDTH = 4
+MAX_LINEAR_DIM = 128        # SS_MAX_LINEAR_DIM
+MAX_BLOCK_NORM_DIM = 8192   # SS_MAX_BLOCK_NORM_DIM
+MAX_BEAMS = 32              # SS_MAX_BEAMS, and the largest num_select
 
 EXPORTS = ("ss_fwd", "ss_bwd", "ss_step", "ss_ckpt_elems", "ss_work_elems", "ss_status_string",
            "ss_last_cuda_error", "ss_abi_version", "ss_struct_size", "ss_device_status",
            "ss_bwd_noalloc", "ss_conv_fwd", "ss_conv_bwd", "ss_conv_step", "ss_rmsnorm_fwd", "ss_rmsnorm_bwd",
-           "ss_mamba_step", "ss_set_wait_limit", "ss_set_time_chunks")
+           "ss_mamba_step", "ss_set_wait_limit", "ss_set_time_chunks", "ss_linear_fwd", "ss_linear_bwd",
+           "ss_linear_step", "ss_linear_work_bytes", "ss_block_norm_fwd", "ss_block_norm_bwd",
+           "ss_block_norm_work_elems", "ss_beam_select", "ss_beam_work_bytes", "ss_reorder")
 NOALLOC_MAX_CKPT_ELEMS = 4194304  # SS_NOALLOC_MAX_CKPT_ELEMS
 
 _lib = None
@@ -179,6 +271,17 @@ def lib():
                 L.ss_rmsnorm_fwd.argtypes = [ctypes.POINTER(RmsNormArgs), c_vp]
                 L.ss_rmsnorm_bwd.argtypes = [ctypes.POINTER(RmsNormBwdArgs), c_vp]
                 L.ss_mamba_step.argtypes = [ctypes.POINTER(MambaStepArgs), c_vp]
+                for f, st in (("ss_linear_fwd", LinearArgs), ("ss_linear_bwd", LinearBwdArgs),
+                              ("ss_linear_step", LinearStepArgs), ("ss_block_norm_fwd", BlockNormArgs),
+                              ("ss_block_norm_bwd", BlockNormBwdArgs), ("ss_beam_select", BeamArgs),
+                              ("ss_reorder", ReorderArgs)):
+                    getattr(L, f).argtypes = [ctypes.POINTER(st), c_vp]
+                    getattr(L, f).restype = c_int
+                L.ss_linear_work_bytes.argtypes = [ctypes.POINTER(LinearArgs), c_int]
+                L.ss_block_norm_work_elems.argtypes = [c_i64, c_int, c_int]
+                L.ss_beam_work_bytes.argtypes = [c_int, c_int, c_int, c_int]
+                for f in ("ss_linear_work_bytes", "ss_block_norm_work_elems", "ss_beam_work_bytes"):
+                    getattr(L, f).restype = ctypes.c_size_t
                 for f in ("ss_fwd", "ss_bwd", "ss_step", "ss_last_cuda_error", "ss_abi_version",
                           "ss_conv_fwd", "ss_conv_bwd", "ss_conv_step", "ss_rmsnorm_fwd", "ss_rmsnorm_bwd",
                           "ss_mamba_step", "ss_set_wait_limit", "ss_set_time_chunks"):
@@ -242,14 +345,15 @@ def stream_of(device: torch.device) -> int:
 
 
 def device_status(device, reset: bool = True) -> int:
-    """Error bits raised by kernels on `device` (1 = a bounded TMA wait timed out)."""
+    """Error bits raised by kernels on `device` (STATUS_BITS)."""
     import torch
 
     with torch.cuda.device(device):
         return int(lib().ss_device_status(int(reset), stream_of(torch.device(device))))
 
 
-STATUS_BITS = {1: "a bounded wait for a TMA tile gave up (the CTA ended early; its outputs are incomplete)"}
+STATUS_BITS = {1: "a bounded wait for a TMA tile gave up (the CTA ended early; its outputs are incomplete)",
+               2: "reorder_states met a parent outside its beams (its row was left as it was)"}
 
 
 def check_device_status(device=None, what: str = "mamba_b200") -> None:

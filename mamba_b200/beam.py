@@ -1,0 +1,95 @@
+"""Beam search's step over the sm_100a kernels ``ss_beam_select`` and ``ss_reorder``: the best
+continuations over the beams and the vocabulary, and the beams' states put in their new order in
+place.  ``mamba_b200.beam_search`` runs a model with them; the reference has no counterpart (its
+``generate`` is a stub, models/causal_lm.py:61-62)."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib as L
+from .selective_scan_interface import _cuda_device
+
+
+@torch.no_grad()
+def beam_select(logits, scores, num_select=None, finished=None, eos_token_id=None):
+    """The num_select best continuations of every batch row.
+
+    logits: (batch, beams, vocab) in float32, bfloat16 or float16; scores: (batch, beams) fp32 sums of
+    log probabilities.  A candidate's score is scores + log_softmax(logits).  finished (batch, beams)
+    bool: such a beam offers itself alone, at eos_token_id with its score unchanged, and its logits
+    are not read.  Candidates that are not a number count as -inf, as does every candidate of a beam
+    whose score is NaN or +inf.  Returns (scores, parents, tokens), each (batch, num_select), in falling
+    order of score, equal candidates in order of (beam, token); scores fp32, indices int64.
+    num_select (beams when None) and beams are at most 32."""
+    dev = _cuda_device(logits, scores, finished)
+    if logits.dim() != 3:
+        raise ValueError(f"logits must be (batch, beams, vocab), got {tuple(logits.shape)}")
+    b, w, vocab = logits.shape
+    k = w if num_select is None else int(num_select)
+    if w < 1 or vocab < 1 or not 1 <= k <= w * vocab:
+        raise ValueError(f"num_select {k} of {w} beams x {vocab} tokens")
+    if w > L.MAX_BEAMS or k > L.MAX_BEAMS:
+        raise NotImplementedError(f"beams {w} and num_select {k} are at most {L.MAX_BEAMS}")
+    if tuple(scores.shape) != (b, w):
+        raise ValueError(f"scores must be {(b, w)}, got {tuple(scores.shape)}")
+    if (finished is not None) != (eos_token_id is not None):
+        raise ValueError("finished and eos_token_id go together")
+    eos = 0
+    if finished is not None:
+        if tuple(finished.shape) != (b, w) or finished.dtype != torch.bool:
+            raise ValueError(f"finished must be {(b, w)} bool, got {finished.dtype} {tuple(finished.shape)}")
+        eos = int(eos_token_id)
+        if not 0 <= eos < vocab:
+            raise ValueError(f"eos_token_id {eos} of {vocab} tokens")
+        finished = finished.contiguous()
+    io = L.dtype_code(logits.dtype)
+    x = logits if (logits.stride(-1) == 1 or vocab == 1) and min(logits.stride()) >= 0 else logits.contiguous()
+    s = scores.to(torch.float32).contiguous()
+    out = torch.empty((b, k), dtype=torch.float32, device=dev)
+    parents, tokens = (torch.empty((b, k), dtype=torch.int64, device=dev) for _ in range(2))
+    n = int(L.lib().ss_beam_work_bytes(b, w, vocab, k))
+    work = torch.empty(n, dtype=torch.uint8, device=dev)
+    args = L.BeamArgs(b, w, vocab, k, io, eos, x.data_ptr(), x.stride(0), x.stride(1), s.data_ptr(), L.ptr(finished),
+                      out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), work.data_ptr())
+    with torch.cuda.device(dev):
+        L.check(L.lib().ss_beam_select(args, L.stream_of(dev)), "ss_beam_select")
+    return out, parents, tokens
+
+
+@torch.no_grad()
+def reorder_states(states, parents):
+    """Put per-beam rows in their new order, in place: for every tensor of ``states`` ((batch * beams, ...)
+    contiguous, rows of a multiple of 4 bytes) and every batch row, row w becomes what row
+    parents[:, w] was.  parents: (batch, beams) int64 (its beams may be a slice of a wider result of
+    ``beam_select``).  A parent outside the beams leaves its row as it was, and the next
+    ``check_device_status`` raises.  Tensors that share memory are refused."""
+    states = list(states)
+    dev = _cuda_device(parents, *states)
+    if parents.dim() != 2 or parents.dtype != torch.int64:
+        raise ValueError(f"parents must be (batch, beams) int64, got {parents.dtype} {tuple(parents.shape)}")
+    b, w = parents.shape
+    if w < 1:
+        raise ValueError("parents must name at least one beam")
+    if w > L.MAX_BEAMS:
+        raise NotImplementedError(f"{w} beams are more than {L.MAX_BEAMS}")
+    rows = []
+    for t in states:
+        if t.dim() < 1 or t.shape[0] != b * w or not t.is_contiguous():
+            raise ValueError(f"a state must have {b * w} contiguous rows, got {tuple(t.shape)}")
+        n = t.numel() // max(t.shape[0], 1) * t.element_size()
+        if n % 4:
+            raise NotImplementedError(f"rows of {n} bytes (a multiple of 4 is supported)")
+        if n and b:
+            rows.append((t.data_ptr(), n))
+    rows.sort()
+    for (p, n), (q, _) in zip(rows, rows[1:]):
+        if p + n * b * w > q:
+            raise ValueError("states must not share memory")
+    p = parents if parents.stride(1) == 1 or w == 1 else parents.contiguous()
+    with torch.cuda.device(dev):
+        for i in range(0, len(rows), L.MAX_REORDER):
+            part = rows[i:i + L.MAX_REORDER]
+            args = L.ReorderArgs(b, w, len(part), p.data_ptr(), p.stride(0) if b > 1 else w)
+            args.data[:len(part)] = [q for q, _ in part]
+            args.row_bytes[:len(part)] = [n for _, n in part]
+            L.check(L.lib().ss_reorder(args, L.stream_of(dev)), "ss_reorder")

@@ -1,0 +1,290 @@
+// One step of beam search: the num_select best continuations over the beams and the vocabulary of
+// each batch row, and the reordering of the beams' states.
+//
+//   cand[w, v] = score[w] + logit[w, v] - log sum_v' e^{logit[w, v']}
+//
+// Selection, pass 1: CTAs own slices of one beam's vocabulary, read once.  Inside a beam the order
+// of the candidates is the order of the logits, so a slice needs only its largest num_select logits
+// (the first among equals), beside its running maximum and sum of exponentials.  A warp keeps the
+// best so far sorted over its lanes, as 64-bit keys (the logit's bits mapped to ascending integers,
+// then the complement of the index, so one comparison orders both); an element enters only above
+// the current last, which for n elements in no particular order happens about k ln(n / k) times.
+// Pass 2, one CTA per batch row and one warp per beam: slices' sums (in fp64) and keys merged, then
+// the beams' lists, compared as fp64 values.  The sums of exponentials are fp32 inside a lane (tens
+// of terms) and fp64 across lanes, which leaves the logarithm good to about 1e-8, so that two
+// candidates of different beams change places against exact arithmetic only when they are that near.
+// Pass 1 is bound by its latency up to a few million logits, and by the read of the logits above.
+#pragma once
+#include "ss_common.cuh"
+
+namespace ssb {
+
+constexpr int kBsThreads = 256;
+constexpr int kBsWarps = kBsThreads / 32;
+constexpr unsigned kFull = 0xffffffffu;
+
+typedef unsigned long long u64;
+
+// float order as ascending unsigned integers; NaN sorts as -infinity (a beam with one has no valid
+// candidate, which the merge sees from its sum)
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) x = -INFINITY;
+  const uint32_t b = __float_as_uint(x + 0.f);  // -0 as +0
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// the best 32 of a warp, lane i the i-th best (0: none)
+struct WarpBest {
+  u64 mine = 0;
+  // offer one key a lane (0: none); every lane takes part
+  __device__ __forceinline__ void offer(u64 key, int k) {
+    const int lane = threadIdx.x & 31;
+    u64 last = __shfl_sync(kFull, mine, k - 1);
+    unsigned want = __ballot_sync(kFull, key > last);
+    while (want) {
+      const int src = __ffs(want) - 1;
+      want &= want - 1;
+      const u64 x = __shfl_sync(kFull, key, src);
+      if (x <= last) continue;  // the last rose since the ballot
+      const u64 up = __shfl_up_sync(kFull, mine, 1);
+      const bool here = mine < x;                       // x goes at the first lane that holds less
+      const bool before = lane > 0 && up < x;
+      if (here) mine = before ? up : x;
+      last = __shfl_sync(kFull, mine, k - 1);
+    }
+  }
+};
+
+struct BeamSlice {
+  double sum;  // of e^{logit - max}
+  float max;
+  float pad;
+};
+
+struct BeamK {
+  ss_beam_args a;
+  int slices, slice_len;  // slice_len: a multiple of the vector width
+  int vec;
+  BeamSlice* part;        // [batch * beams][slices]
+  u64* keys;              // [batch * beams][slices][num_select]
+};
+
+template <typename IT>
+__global__ void __launch_bounds__(kBsThreads) beam_slice_kernel(const __grid_constant__ BeamK P) {
+  constexpr int VW = 16 / sizeof(IT);
+  __shared__ float s_max[kBsWarps];
+  __shared__ double s_sum[kBsWarps];
+  __shared__ u64 s_keys[kBsWarps][32];
+  griddep_launch_dependents();
+  const ss_beam_args& a = P.a;
+  const int row = blockIdx.x / P.slices, slice = blockIdx.x % P.slices;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, k = a.num_select;
+  if (a.finished && a.finished[row]) return;  // the merge does not look at its slices
+  const IT* x = static_cast<const IT*>(a.logits) + (int64_t)(row / a.beams) * a.logits_batch_stride +
+                (int64_t)(row % a.beams) * a.logits_beam_stride;
+  const int v0 = slice * P.slice_len, v1 = min(v0 + P.slice_len, a.vocab);
+  WarpBest best;
+  float m = -INFINITY, sum = 0.f;
+  for (int base = v0; base < v1; base += kBsThreads * VW) {
+    const int e0 = base + threadIdx.x * VW;
+    float v[VW];
+    if (P.vec && e0 + VW <= v1) {
+      const uint4 q = ld_stream16(x + e0);
+#pragma unroll
+      for (int i = 0; i < VW; ++i) v[i] = to_f<IT>(reinterpret_cast<const IT*>(&q)[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VW; ++i) v[i] = e0 + i < v1 ? to_f<IT>(x[e0 + i]) : -INFINITY;
+    }
+    float vm = v[0];
+#pragma unroll
+    for (int i = 1; i < VW; ++i) vm = fmaxf(vm, v[i]);
+    if (vm > m) {
+      sum *= expf(m - vm);  // 0 at the first finite value
+      m = vm;
+    }
+#pragma unroll
+    for (int i = 0; i < VW; ++i)  // an infinite maximum, or NaN, makes the sum NaN
+      if (e0 + i < v1 && v[i] != -INFINITY) sum += expf(v[i] - m);
+    // the warp's elements, one of each lane at a time
+    const u64 last = __shfl_sync(kFull, best.mine, k - 1);
+    const float floor_v = last ? key_value((uint32_t)(last >> 32)) : -INFINITY;
+    bool any = last == 0;
+#pragma unroll
+    for (int i = 0; i < VW; ++i) any |= !(v[i] < floor_v);
+    if (__any_sync(kFull, any)) {
+#pragma unroll
+      for (int i = 0; i < VW; ++i)
+        best.offer(e0 + i < v1 ? ((u64)order_key(v[i]) << 32) | (uint32_t)~(uint32_t)(e0 + i) : 0, k);
+    }
+  }
+  // the CTA's maximum and sum
+  float wm = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(kFull, wm, o));
+  double ws = (m == -INFINITY && sum == 0.f) ? 0.0 : (double)sum * (double)expf(m - wm);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(kFull, ws, o);
+  if (lane == 0) s_max[wid] = wm, s_sum[wid] = ws;
+  s_keys[wid][lane] = lane < k ? best.mine : 0;
+  __syncthreads();
+  if (wid == 0) {
+    float cm = -INFINITY;
+    for (int i = 0; i < kBsWarps; ++i) cm = fmaxf(cm, s_max[i]);
+    double cs = 0.0;
+    for (int i = 0; i < kBsWarps; ++i)
+      if (!(s_sum[i] == 0.0)) cs += s_sum[i] * (double)expf(s_max[i] - cm);
+    for (int i = 1; i < kBsWarps; ++i) best.offer(s_keys[i][lane], k);
+    const int64_t at = (int64_t)row * P.slices + slice;
+    if (lane == 0) P.part[at] = BeamSlice{cs, cm, 0.f};
+    if (lane < k) P.keys[at * k + lane] = best.mine;
+  }
+}
+
+// order of the merge: larger value first, then the smaller flat index
+__device__ __forceinline__ bool beats(double v, int i, double w, int j) { return v > w || (v == w && i < j); }
+
+// One CTA per batch row, a warp per beam.
+__global__ void __launch_bounds__(32 * SS_MAX_BEAMS) beam_merge_kernel(const __grid_constant__ BeamK P) {
+  __shared__ double s_val[SS_MAX_BEAMS][32];
+  __shared__ int s_tok[SS_MAX_BEAMS][32];
+  const ss_beam_args& a = P.a;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, k = a.num_select;
+  const int64_t row = (int64_t)blockIdx.x * a.beams + wid;
+  const bool done = a.finished && a.finished[row];
+  double score = a.scores[row];
+  const bool dead = !(score < INFINITY);  // NaN or +infinity
+  griddep_wait();
+  double val = -INFINITY;
+  int tok = -1;
+  if (done) {
+    // its score at the end token, then -infinity in the order of the tokens
+    if (dead || score == -INFINITY) {
+      tok = lane;
+    } else if (lane == 0) {
+      tok = a.eos_token;
+      val = score;
+    } else {
+      tok = lane - 1 + (lane - 1 >= a.eos_token);
+    }
+  } else {
+    float m = -INFINITY;
+    const BeamSlice* part = P.part + row * P.slices;
+    for (int s = lane; s < P.slices; s += 32) m = fmaxf(m, part[s].max);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+    double sum = 0.0;
+    for (int s = lane; s < P.slices; s += 32)
+      if (!(part[s].sum == 0.0)) sum += part[s].sum * exp((double)part[s].max - (double)m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    const double lse = (double)m + log(sum);
+    WarpBest best;
+    const u64* keys = P.keys + row * P.slices * k;
+    const int n = P.slices * k;
+    for (int i = 0; i < n; i += 32) best.offer(i + lane < n ? keys[i + lane] : 0, k);
+    const float logit = key_value((uint32_t)(best.mine >> 32));
+    const bool valid = lse > -INFINITY && lse < INFINITY && !dead && score > -INFINITY;  // false for NaN
+    if (valid) {
+      val = score + ((double)logit - lse);
+      tok = best.mine ? (int)~(uint32_t)best.mine : -1;
+      // candidates of -infinity follow in the order of the tokens, as the keys have them
+    } else {
+      tok = lane;
+    }
+  }
+  // a beam offers as many candidates as it has tokens
+  if (lane >= k || lane >= a.vocab) tok = -1;
+  s_val[wid][lane] = val;
+  s_tok[wid][lane] = tok;
+  __syncthreads();
+  if (wid != 0) return;
+  double bv = -INFINITY;  // lane i: the i-th best of the row
+  int bi = INT32_MAX;
+  for (int w = 0; w < a.beams; ++w) {
+    const double v = s_val[w][lane];
+    const int t = s_tok[w][lane];
+    const int idx = t < 0 ? INT32_MAX : w * a.vocab + t;
+    double lv = __shfl_sync(kFull, bv, k - 1);
+    int li = __shfl_sync(kFull, bi, k - 1);
+    unsigned want = __ballot_sync(kFull, t >= 0 && beats(v, idx, lv, li));
+    while (want) {
+      const int src = __ffs(want) - 1;
+      want &= want - 1;
+      const double x = __shfl_sync(kFull, v, src);
+      const int xi = __shfl_sync(kFull, idx, src);
+      if (!beats(x, xi, lv, li)) continue;
+      const double uv = __shfl_up_sync(kFull, bv, 1);
+      const int ui = __shfl_up_sync(kFull, bi, 1);
+      const bool here = beats(x, xi, bv, bi);
+      const bool before = lane > 0 && beats(x, xi, uv, ui);
+      if (here) bv = before ? uv : x, bi = before ? ui : xi;
+      lv = __shfl_sync(kFull, bv, k - 1);
+      li = __shfl_sync(kFull, bi, k - 1);
+    }
+  }
+  if (lane < k) {
+    const int64_t at = (int64_t)blockIdx.x * k + lane;
+    a.out_scores[at] = (float)bv;
+    a.parents[at] = bi / a.vocab;
+    a.tokens[at] = bi % a.vocab;
+  }
+}
+
+// ------------------------------------------------------------------------------------ reordering
+// Each thread owns one 16-byte (or 4-byte) column of a batch row's beams: it loads what its rows
+// take from other beams, then stores, so the gather needs no second buffer.  Rows that keep their
+// place are neither read nor written.  Bound by the memory traffic of the rows that move.
+struct ReorderK {
+  ss_reorder_args a;
+  int* status;
+  int64_t first[SS_MAX_REORDER + 1];  // tensor i's first block of 256 columns
+};
+
+template <int W, typename V>
+__device__ __forceinline__ void reorder_columns(char* rows, int64_t row_bytes, const int* from, int beams, int64_t col) {
+  V v[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+    if (w < beams && from[w] != w) v[w] = *reinterpret_cast<const V*>(rows + from[w] * row_bytes + col);
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+    if (w < beams && from[w] != w) *reinterpret_cast<V*>(rows + w * row_bytes + col) = v[w];
+}
+
+template <int W>
+__global__ void __launch_bounds__(256) reorder_kernel(const __grid_constant__ ReorderK P) {
+  __shared__ int from[SS_MAX_BEAMS];
+  const ss_reorder_args& a = P.a;
+  griddep_wait();
+  const int b = blockIdx.y;
+  if (threadIdx.x < a.beams) {
+    const int64_t p = a.parents[(int64_t)b * a.parents_batch_stride + threadIdx.x];
+    const bool ok = p >= 0 && p < a.beams;
+    from[threadIdx.x] = ok ? (int)p : threadIdx.x;
+    if (!ok && blockIdx.x == 0 && P.status) atomicOr(P.status, kStatusParent);
+  }
+  __syncthreads();
+  for (int64_t blk = blockIdx.x; blk < P.first[a.count]; blk += gridDim.x) {
+    int i = 0;  // the block's tensor
+    for (int hi = a.count; hi - i > 1;) {
+      const int mid = (i + hi) / 2;
+      if (P.first[mid] <= blk) i = mid;
+      else hi = mid;
+    }
+    const int64_t bytes = a.row_bytes[i];
+    char* rows = static_cast<char*>(a.data[i]) + (int64_t)b * a.beams * bytes;
+    const bool wide = bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(a.data[i]) & 15) == 0;
+    const int64_t at = (blk - P.first[i]) * 256 + threadIdx.x;
+    if (wide) {
+      if (at * 16 < bytes) reorder_columns<W, uint4>(rows, bytes, from, a.beams, at * 16);
+    } else {
+      if (at * 4 < bytes) reorder_columns<W, uint32_t>(rows, bytes, from, a.beams, at * 4);
+    }
+  }
+}
+
+}  // namespace ssb

@@ -1,0 +1,179 @@
+// C ABI of the norms around a block (ss_block_norm_fwd / ss_block_norm_bwd): validation and dispatch
+// over dtype, vectors a lane and warps a row.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/mamba_b200_ss.h"
+#include "ss_block_norm.cuh"
+
+namespace {
+
+using namespace ssb;
+
+bool rows16(const void* p, int64_t stride, size_t es) {
+  return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((stride * (int64_t)es) & 15) == 0);
+}
+
+struct Shape {
+  int nv, wpr;  // 16-byte vectors a lane, warps a row; nv 0: the row is too long
+};
+
+// A row in as few warps as its vectors allow: up to 4 a lane in the forward, 3 in the backward
+// (whose column sums take two more registers a value)
+Shape shape_of(int dim, size_t es, int most) {
+  const int vw = (int)(16 / es);
+  for (int wpr : {1, 2, 4, 8}) {
+    const int need = (dim + 32 * wpr * vw - 1) / (32 * wpr * vw);
+    if (need <= most) return {need, wpr};
+  }
+  const int need = (dim + 32 * 8 * vw - 1) / (32 * 8 * vw);
+  return need <= 8 ? Shape{need <= 4 ? 4 : need <= 6 ? 6 : 8, 8} : Shape{0, 8};
+}
+
+int sm_count() {
+  int sms = 148, dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaGetLastError();
+  return sms;
+}
+
+// CTAs of the backward (the workspace holds two sums per column of each); the same rule wherever
+// the library runs, so that ss_block_norm_work_elems needs no device
+int bwd_ctas(int64_t rows, int wpr) {
+  const int rpc = kBnWarps / wpr;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rpc - 1) / rpc, 2 * 148));
+}
+
+int check(const ss_block_norm_args& a) {
+  if (a.rows < 0 || a.dim < 1 || !(a.eps >= 0.f) || !(a.pre_eps >= 0.f) || !std::isfinite(a.scale_const)) return SS_ERR_INVALID;
+  if (a.io_dtype != SS_F32 && a.io_dtype != SS_BF16 && a.io_dtype != SS_F16) return SS_ERR_UNSUPPORTED;
+  if (a.activation < kActNone || a.activation > kActSigmoid) return SS_ERR_INVALID;
+  if (a.dim > SS_MAX_BLOCK_NORM_DIM) return SS_ERR_UNSUPPORTED;
+  if (a.rows == 0) return SS_OK;
+  if (!a.y || !a.residual) return SS_ERR_INVALID;
+  if (a.y_row_stride < a.dim || a.residual_row_stride < a.dim) return SS_ERR_INVALID;
+  if (a.gate && a.gate_row_stride != 0 && a.gate_row_stride < a.dim) return SS_ERR_INVALID;
+  return SS_OK;
+}
+
+template <typename F>
+int by_dtype(int io, F&& f) {
+  switch (io) {
+    case SS_F32: return record_cuda_status(f(float{}));
+    case SS_BF16: return record_cuda_status(f(__nv_bfloat16{}));
+    default: return record_cuda_status(f(__half{}));
+  }
+}
+
+template <typename IT, int NV, int WPR>
+cudaError_t fwd(const BlockNormK& P, cudaStream_t st) {
+  constexpr size_t smem = sizeof(float) * 2 * NV * WPR * 32 * (16 / sizeof(IT));
+  auto kern = block_norm_fwd_kernel<IT, NV, WPR>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), smem + 256);  // and the static part
+  if (e != cudaSuccess) return e;
+  const int rpc = kBnWarps / WPR;
+  const int64_t ctas = ((int64_t)P.a.rows + rpc - 1) / rpc;
+  kern<<<(unsigned)std::min<int64_t>(ctas, 4 * sm_count()), 32 * kBnWarps, smem, st>>>(P);
+  return cudaGetLastError();
+}
+
+template <typename IT, int NV, int WPR>
+cudaError_t bwd(const BlockNormBwdK& P, cudaStream_t st) {
+  constexpr size_t smem = sizeof(float) * 2 * NV * WPR * 32 * (16 / sizeof(IT));
+  auto kern = block_norm_bwd_kernel<IT, NV, WPR>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), smem + 256);  // and the static part
+  if (e != cudaSuccess) return e;
+  kern<<<(unsigned)bwd_ctas(P.a.f.rows, WPR), 32 * kBnWarps, smem, st>>>(P);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+#define SSB_BN_SHAPES(F, MOST)                                    \
+  if (s.wpr == 1) {                                               \
+    if (s.nv == 1) return F<IT, 1, 1>(P, st);                     \
+    if (s.nv == 2) return F<IT, 2, 1>(P, st);                     \
+    if (s.nv == 3) return F<IT, 3, 1>(P, st);                     \
+    return F<IT, MOST, 1>(P, st);                                 \
+  }                                                               \
+  if (s.wpr == 2) { SSB_BN_WIDE(F, MOST, 2) }                     \
+  if (s.wpr == 4) { SSB_BN_WIDE(F, MOST, 4) }                     \
+  if (s.nv <= 2) return F<IT, 2, 8>(P, st);                       \
+  if (s.nv <= 3) return F<IT, 3, 8>(P, st);                       \
+  if (s.nv <= 4) return F<IT, 4, 8>(P, st);                       \
+  if (s.nv <= 6) return F<IT, 6, 8>(P, st);                       \
+  return F<IT, 8, 8>(P, st);
+
+// a row that did not fit half as many warps has at least 2 vectors a lane here
+#define SSB_BN_WIDE(F, MOST, WPR)                                 \
+  if (s.nv <= 2) return F<IT, 2, WPR>(P, st);                     \
+  if (s.nv == 3) return F<IT, 3, WPR>(P, st);                     \
+  return F<IT, MOST, WPR>(P, st);
+
+extern "C" {
+
+size_t ss_block_norm_work_elems(int64_t rows, int dim, int io_dtype) {
+  if (rows < 1 || dim < 1 || dim > SS_MAX_BLOCK_NORM_DIM) return 0;
+  return (size_t)bwd_ctas(rows, shape_of(dim, io_dtype == SS_F32 ? 4 : 2, 3).wpr) * 2 * dim;
+}
+
+int ss_block_norm_fwd(const ss_block_norm_args* a, void* stream) {
+  if (a == nullptr) return SS_ERR_INVALID;
+  const int rc = check(*a);
+  if (rc != SS_OK) return rc;
+  if (a->rows == 0) return SS_OK;
+  if (!a->h || a->h_row_stride < a->dim) return SS_ERR_INVALID;
+  if (a->pre_weight && (!a->x || a->x_row_stride < a->dim)) return SS_ERR_INVALID;
+  const size_t es = a->io_dtype == SS_F32 ? 4 : 2;
+  BlockNormK P;
+  P.a = *a;
+  P.vec = a->dim % (int)(16 / es) == 0 && rows16(a->y, a->y_row_stride, es) &&
+          rows16(a->residual, a->residual_row_stride, es) && rows16(a->gate, a->gate_row_stride, es) &&
+          rows16(a->h, a->h_row_stride, es) && (!a->pre_weight || rows16(a->x, a->x_row_stride, es));
+  cudaStream_t st = (cudaStream_t)stream;
+  return by_dtype(a->io_dtype, [&](auto tag) -> cudaError_t {
+    using IT = decltype(tag);
+    const Shape s = shape_of(a->dim, sizeof(IT), 4);
+    SSB_BN_SHAPES(fwd, 4)
+  });
+}
+
+int ss_block_norm_bwd(const ss_block_norm_bwd_args* g, void* stream) {
+  if (g == nullptr) return SS_ERR_INVALID;
+  const ss_block_norm_args& a = g->f;
+  const int rc = check(a);
+  if (rc != SS_OK) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  const float ofs = a.unit_offset ? 1.f : 0.f;
+  const size_t es = a.io_dtype == SS_F32 ? 4 : 2;
+  const Shape s = shape_of(a.dim, es, 3);
+  if (a.rows > 0) {
+    if (!a.rstd || !g->dresidual || !g->dy || !g->work || (a.gate && !g->dgate) || (a.pre_weight && !g->dx))
+      return SS_ERR_INVALID;
+    if (g->dy_row_stride < a.dim || g->dresidual_row_stride < a.dim || (a.gate && g->dgate_row_stride < a.dim) ||
+        (a.pre_weight && g->dx_row_stride < a.dim) || (g->dh && g->dh_row_stride < a.dim))
+      return SS_ERR_INVALID;
+    BlockNormBwdK P;
+    P.a = *g;
+    P.vec = a.dim % (int)(16 / es) == 0 && rows16(a.y, a.y_row_stride, es) &&
+            rows16(a.residual, a.residual_row_stride, es) && rows16(a.gate, a.gate_row_stride, es) &&
+            (!a.pre_weight || rows16(g->dx, g->dx_row_stride, es)) && rows16(g->dh, g->dh_row_stride, es) &&
+            rows16(g->dy, g->dy_row_stride, es) && rows16(g->dresidual, g->dresidual_row_stride, es) &&
+            (!a.gate || rows16(g->dgate, g->dgate_row_stride, es));
+    const int r = by_dtype(a.io_dtype, [&](auto tag) -> cudaError_t {
+      using IT = decltype(tag);
+      SSB_BN_SHAPES(bwd, 3)
+    });
+    if (r != SS_OK) return r;
+  }
+  if (!g->dpost_weight && !g->dpre_weight && !g->dscale) return SS_OK;
+  const dim3 grid((unsigned)((a.dim + 31) / 32), 2);
+  block_norm_cols_kernel<<<grid, 256, 0, st>>>(g->work, a.rows > 0 ? bwd_ctas(a.rows, s.wpr) : 0, a.dim, a.post_weight,
+                                               a.scale, a.scale_const, ofs, g->dpost_weight, g->dpre_weight, g->dscale);
+  return record_cuda_status(cudaGetLastError());
+}
+
+}  // extern "C"

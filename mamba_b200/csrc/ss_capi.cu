@@ -73,9 +73,7 @@ int ssb::record_cuda_status(cudaError_t e) {
   return SS_ERR_CUDA;
 }
 
-namespace {
-
-int* status_ptr() {
+int* ssb::device_status_word() {
   void* p = nullptr;
   if (cudaGetSymbolAddress(&p, g_ss_status) != cudaSuccess) {
     cudaGetLastError();
@@ -83,6 +81,10 @@ int* status_ptr() {
   }
   return static_cast<int*>(p);
 }
+
+namespace {
+
+int* status_ptr() { return ssb::device_status_word(); }
 
 // cuTensorMapEncodeTiled from the driver, fetched through the runtime (no -lcuda link)
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -527,6 +529,13 @@ size_t ss_struct_size(int which) {
     case 6: return sizeof(ss_rmsnorm_args);
     case 7: return sizeof(ss_rmsnorm_bwd_args);
     case 8: return sizeof(ss_mamba_step_args);
+    case 9: return sizeof(ss_linear_args);
+    case 10: return sizeof(ss_linear_bwd_args);
+    case 11: return sizeof(ss_linear_step_args);
+    case 12: return sizeof(ss_block_norm_args);
+    case 13: return sizeof(ss_block_norm_bwd_args);
+    case 14: return sizeof(ss_beam_args);
+    case 15: return sizeof(ss_reorder_args);
     default: return 0;
   }
 }

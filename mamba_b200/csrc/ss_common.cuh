@@ -26,6 +26,8 @@ namespace ssb {
 
 // Records e as the thread's last CUDA error (ss_last_cuda_error) and maps it to a status.
 int record_cuda_status(cudaError_t e);
+// The current device's status word (ss_device_status), or null if it cannot be found.
+int* device_status_word();
 // Argument checks of a backward call (ss_capi.cu); own_states: f.ckpt and y not required.
 int check_bwd(const ss_bwd_args* args, bool own_states);
 // Raises the dynamic shared-memory limit of kernel `fn` to `smem` bytes (when above the 48 KB
@@ -42,6 +44,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // device status word codes (OR-ed into the caller-visible status buffer)
 constexpr int kStatusTimeout = 1;   // a bounded wait on a TMA barrier gave up
+constexpr int kStatusParent = 2;    // a beam's parent was out of range
 // default limit of a bounded wait for a TMA tile (SM clock cycles, ~2 s at 1.9 GHz); a launch
 // takes its limit from ss_set_wait_limit.  The drain after a timeout (waiting for the CTA's
 // own copies still in flight before it exits) always uses the default.

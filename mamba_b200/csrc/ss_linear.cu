@@ -1,0 +1,288 @@
+// C ABI of linear attention: validation, the runs of the recurrence that make up a call, the
+// segments that a long sequence is cut into, and dispatch.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "../../include/mamba_b200_ss.h"
+#include "ss_linear.cuh"
+
+namespace {
+
+using namespace ssb;
+
+int sm_count() {
+  int sms = 148, dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaGetLastError();
+  return sms;
+}
+
+size_t align16(size_t n) { return (n + 15) & ~size_t(15); }
+
+int tiles_of(int dim) { return (dim + kLsN - 1) / kLsN; }
+
+bool sizes_ok(const ss_linear_args& a) {
+  return a.batch >= 0 && a.seqlen >= 0 && a.heads >= 1 && a.key_heads >= 1 && a.heads % a.key_heads == 0 &&
+         a.key_dim >= 1 && a.value_dim >= 1;
+}
+
+bool dtypes_ok(int io, int decay) {
+  return (io == SS_F32 || io == SS_BF16 || io == SS_F16) && (decay == SS_F32 || decay == io);
+}
+
+// Segments that run side by side: enough CTAs for the GPU when batch x heads are few, at least two
+// chunks each (a segment's own state costs a pass over its keys and values), at most 32 (every
+// segment folds the states of those before it).
+struct Split {
+  int segs, chunks;
+};
+
+Split split_of(const ss_linear_args& a, int chunk, int passes, int tiles) {
+  const int64_t n = (a.seqlen + chunk - 1) / chunk;
+  const int64_t ctas = (int64_t)a.batch * a.heads * passes * tiles;
+  int64_t segs = 1;
+  if (ctas > 0 && ctas < 148) segs = std::max<int64_t>(1, std::min<int64_t>({148 / ctas, n / 2, 32}));
+  Split s;
+  s.chunks = (int)std::max<int64_t>(1, (n + segs - 1) / segs);
+  s.segs = (int)std::max<int64_t>(1, (n + s.chunks - 1) / s.chunks);
+  return s;
+}
+
+// The scratch of a call, cut into its parts (offsets in bytes; absent parts are -1)
+struct Work {
+  size_t bytes = 0;
+  int64_t sums = -1, seg_decay = -1, dots = -1, parts = -1;
+  Split split;
+};
+
+Work work_of(const ss_linear_args& a, int backward) {
+  Work w;
+  const int passes = backward ? 3 : 1;
+  const int tiles = backward ? std::max(tiles_of(a.key_dim), tiles_of(a.value_dim)) : tiles_of(a.value_dim);
+  w.split = split_of(a, kLsC, passes, tiles);
+  const size_t bh = (size_t)a.batch * a.heads;
+  auto take = [&](size_t n) {
+    const int64_t at = (int64_t)w.bytes;
+    w.bytes += align16(n);
+    return at;
+  };
+  if (w.split.segs > 1) {
+    w.sums = take(sizeof(float) * passes * bh * w.split.segs * a.key_dim * a.value_dim);
+    w.seg_decay = take(sizeof(float) * 2 * bh * w.split.segs);
+  }
+  if (backward) {
+    w.dots = take(sizeof(float) * 2 * tiles_of(a.key_dim) * bh * a.seqlen);
+    if (a.heads != a.key_heads) w.parts = take(sizeof(float) * 2 * bh * a.seqlen * a.key_dim);
+  }
+  return w;
+}
+
+template <typename IT>
+cudaError_t run_passes(const LinK& P, int passes, int tiles, cudaStream_t st) {
+  constexpr size_t smem = sizeof(LsSmem);
+  auto main_k = linear_simt_kernel<IT, false>;
+  auto sum_k = linear_simt_kernel<IT, true>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(main_k), smem);
+  if (e == cudaSuccess) e = ensure_smem_limit(reinterpret_cast<const void*>(sum_k), smem);
+  if (e != cudaSuccess) return e;
+  (void)tiles;
+  const int kt = (kLinMaxDim + kLsN - 1) / kLsN;
+  const dim3 grid((unsigned)((int64_t)P.batch * P.heads * P.segs), (unsigned)(passes * kt));
+  if (P.segs > 1) {
+    sum_k<<<grid, kLsThreads, smem, st>>>(P);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  main_k<<<grid, kLsThreads, smem, st>>>(P);
+  return cudaGetLastError();
+}
+
+cudaError_t run_by_type(int io, const LinK& P, int passes, int tiles, cudaStream_t st) {
+  switch (io) {
+    case SS_F32: return run_passes<float>(P, passes, tiles, st);
+    case SS_BF16: return run_passes<__nv_bfloat16>(P, passes, tiles, st);
+    default: return run_passes<__half>(P, passes, tiles, st);
+  }
+}
+
+LinK problem(const ss_linear_args& a, const Work& w, void* work) {
+  LinK P{};
+  P.g = a.log_decay;
+  P.g_f32 = a.decay_dtype == SS_F32;
+  P.gb = a.decay_batch_stride, P.gl = a.decay_seq_stride, P.gh = a.decay_head_stride;
+  P.lens = a.seq_lens;
+  P.batch = a.batch, P.seqlen = a.seqlen, P.heads = a.heads;
+  P.segs = w.split.segs, P.seg_chunks = w.split.chunks;
+  if (w.seg_decay >= 0) P.seg_decay = reinterpret_cast<float*>(static_cast<char*>(work) + w.seg_decay);
+  return P;
+}
+
+// status of the arguments that both directions share (a zero batch may carry null pointers)
+int check_fwd(const ss_linear_args& a) {
+  if (!sizes_ok(a)) return SS_ERR_INVALID;
+  if (!dtypes_ok(a.io_dtype, a.decay_dtype)) return SS_ERR_UNSUPPORTED;
+  if (a.key_dim > SS_MAX_LINEAR_DIM || a.value_dim > SS_MAX_LINEAR_DIM) return SS_ERR_UNSUPPORTED;
+  if ((int64_t)a.batch * a.heads > (1 << 24)) return SS_ERR_UNSUPPORTED;
+  if (!std::isfinite(a.scale) || a.scale == 0.f) return SS_ERR_INVALID;
+  const bool empty = a.batch == 0 || a.seqlen == 0;
+  if (!empty && (!a.q || !a.k || !a.v || !a.log_decay)) return SS_ERR_INVALID;
+  return SS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ss_linear_work_bytes(const ss_linear_args* a, int backward) {
+  if (a == nullptr || !sizes_ok(*a) || a->key_dim > SS_MAX_LINEAR_DIM || a->value_dim > SS_MAX_LINEAR_DIM) return 0;
+  return work_of(*a, backward != 0).bytes;
+}
+
+int ss_linear_fwd(const ss_linear_args* a, void* stream) {
+  if (a == nullptr) return SS_ERR_INVALID;
+  const int rc = check_fwd(*a);
+  if (rc != SS_OK) return rc;
+  if (a->batch == 0) return SS_OK;
+  if (a->seqlen > 0 && !a->o) return SS_ERR_INVALID;
+  if (a->seqlen == 0 && !a->state_out) return SS_OK;
+  const Work w = work_of(*a, 0);
+  if (w.bytes && !a->work) return SS_ERR_INVALID;
+  LinK P = problem(*a, w, a->work);
+  LinPass& A = P.pass[0];
+  const int rep = a->heads / a->key_heads;
+  A.q = a->q, A.qb = a->q_batch_stride, A.ql = a->q_seq_stride, A.qh = a->q_head_stride, A.rq = rep;
+  A.k = a->k, A.kb = a->k_batch_stride, A.kl = a->k_seq_stride, A.kh = a->k_head_stride, A.rk = rep;
+  A.v = a->v, A.vb = a->v_batch_stride, A.vl = a->v_seq_stride, A.vh = a->v_head_stride, A.rv = 1;
+  A.o = a->o, A.ob = a->o_batch_stride, A.ol = a->o_seq_stride, A.oh = a->o_head_stride;
+  A.dk = a->key_dim, A.dv = a->value_dim;
+  A.scale = a->scale;
+  A.s_in = a->state_in, A.s_in_scale = 1.f;
+  A.s_out = a->state_out, A.s_out_scale = 1.f;
+  A.s_row = a->value_dim, A.s_col = 1;
+  if (w.sums >= 0) A.sum = reinterpret_cast<float*>(static_cast<char*>(a->work) + w.sums);
+  return record_cuda_status(run_by_type(a->io_dtype, P, 1, tiles_of(a->value_dim), (cudaStream_t)stream));
+}
+
+int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
+  if (g == nullptr) return SS_ERR_INVALID;
+  const ss_linear_args& a = g->f;
+  const int rc = check_fwd(a);
+  if (rc != SS_OK) return rc;
+  if (a.batch == 0) return SS_OK;
+  if (a.seqlen > 0 && (!g->dout || !g->dq || !g->dk || !g->dv)) return SS_ERR_INVALID;
+  if (g->dstate_out && g->dlog_decay && !a.state_out) return SS_ERR_INVALID;
+  const Work w = work_of(a, 1);
+  if (w.bytes && !g->work) return SS_ERR_INVALID;
+  char* base = static_cast<char*>(g->work);
+  LinK P = problem(a, w, base);
+  const int rep = a.heads / a.key_heads;
+  const int64_t bh = (int64_t)a.batch * a.heads, block = (int64_t)a.key_dim * a.value_dim;
+  const int tq = tiles_of(a.key_dim);
+  float* dots = g->dlog_decay ? reinterpret_cast<float*>(base + w.dots) : nullptr;
+  float* parts = w.parts >= 0 ? reinterpret_cast<float*>(base + w.parts) : nullptr;
+  float* sums = w.sums >= 0 ? reinterpret_cast<float*>(base + w.sums) : nullptr;
+  struct T {
+    const void* p;
+    int64_t b, l, h;
+    int rep;
+  };
+  const T q{a.q, a.q_batch_stride, a.q_seq_stride, a.q_head_stride, rep};
+  const T k{a.k, a.k_batch_stride, a.k_seq_stride, a.k_head_stride, rep};
+  const T v{a.v, a.v_batch_stride, a.v_seq_stride, a.v_head_stride, 1};
+  const T dout{g->dout, g->do_batch_stride, g->do_seq_stride, g->do_head_stride, 1};
+  auto set = [&](int i, const T& x, const T& y, const T& z, int dk, int dv, bool reverse) -> LinPass& {
+    LinPass& A = P.pass[i];
+    A.q = x.p, A.qb = x.b, A.ql = x.l, A.qh = x.h, A.rq = x.rep;
+    A.k = y.p, A.kb = y.b, A.kl = y.l, A.kh = y.h, A.rk = y.rep;
+    A.v = z.p, A.vb = z.b, A.vl = z.l, A.vh = z.h, A.rv = z.rep;
+    A.dk = dk, A.dv = dv, A.reverse = reverse, A.scale = a.scale;
+    A.s_in_scale = reverse ? 1.f / a.scale : 1.f;  // a reverse run's state times scale is the state's gradient
+    if (sums) A.sum = sums + (int64_t)i * bh * w.split.segs * block;
+    return A;
+  };
+  auto grad = [&](LinPass& A, int i, void* out, int64_t b, int64_t l, int64_t h, const T& p) {
+    if (parts) {  // fp32 parts per head, summed below
+      A.o = parts + (int64_t)i * bh * a.seqlen * a.key_dim;
+      A.o_f32 = 1;
+      A.oh = a.key_dim, A.ol = (int64_t)a.heads * a.key_dim, A.ob = (int64_t)a.seqlen * A.ol;
+    } else {
+      A.o = out, A.ob = b, A.ol = l, A.oh = h;
+    }
+    if (dots) {
+      A.dot = dots + (int64_t)i * tq * bh * a.seqlen;
+      A.p = p.p, A.pb = p.b, A.pl = p.l, A.ph = p.h, A.rp = p.rep;
+    }
+  };
+  LinPass& Q = set(0, dout, v, k, a.value_dim, a.key_dim, false);
+  grad(Q, 0, g->dq, g->dq_batch_stride, g->dq_seq_stride, g->dq_head_stride, q);
+  Q.s_in = a.state_in, Q.s_row = 1, Q.s_col = a.value_dim;
+  LinPass& K = set(1, v, dout, q, a.value_dim, a.key_dim, true);
+  grad(K, 1, g->dk, g->dk_batch_stride, g->dk_seq_stride, g->dk_head_stride, k);
+  K.s_in = g->dstate_out, K.s_row = 1, K.s_col = a.value_dim;
+  LinPass& V = set(2, k, q, dout, a.key_dim, a.value_dim, true);
+  V.o = g->dv, V.ob = g->dv_batch_stride, V.ol = g->dv_seq_stride, V.oh = g->dv_head_stride;
+  V.s_in = g->dstate_out, V.s_row = a.value_dim, V.s_col = 1;
+  V.s_out = g->dstate_in, V.s_out_scale = a.scale;
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e = run_by_type(a.io_dtype, P, 3, std::max(tq, tiles_of(a.value_dim)), st);
+  if (e != cudaSuccess) return record_cuda_status(e);
+  if (parts && a.seqlen > 0) {
+    LinGroupK G{};
+    G.batch = a.batch, G.seqlen = a.seqlen, G.key_heads = a.key_heads, G.rep = rep, G.dim = a.key_dim;
+    G.parts[0] = parts, G.out[0] = g->dq, G.ob[0] = g->dq_batch_stride, G.ol[0] = g->dq_seq_stride, G.oh[0] = g->dq_head_stride;
+    G.parts[1] = parts + bh * a.seqlen * a.key_dim;
+    G.out[1] = g->dk, G.ob[1] = g->dk_batch_stride, G.ol[1] = g->dk_seq_stride, G.oh[1] = g->dk_head_stride;
+    const int64_t n = (int64_t)a.batch * a.seqlen * a.key_heads * a.key_dim;
+    const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 8 * sm_count()), 2);
+    if (a.io_dtype == SS_F32) linear_group_sum_kernel<float><<<grid, 256, 0, st>>>(G);
+    else if (a.io_dtype == SS_BF16) linear_group_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(G);
+    else linear_group_sum_kernel<__half><<<grid, 256, 0, st>>>(G);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return record_cuda_status(e);
+  }
+  if (g->dlog_decay) {
+    LinDecayK D{};
+    D.xq = dots, D.yk = dots + (int64_t)tq * bh * a.seqlen, D.tq = D.tk = tq;
+    if (g->dstate_out) D.d_last = g->dstate_out, D.last = a.state_out;
+    D.block = block;
+    D.g = a.log_decay, D.dg = g->dlog_decay;
+    D.g_f32 = a.decay_dtype == SS_F32, D.g_bf16 = a.io_dtype == SS_BF16;
+    D.per_head = a.decay_batch_stride == 0 && a.decay_seq_stride == 0;
+    D.gb = a.decay_batch_stride, D.gl = a.decay_seq_stride, D.gh = a.decay_head_stride;
+    D.lens = a.seq_lens;
+    D.batch = a.batch, D.seqlen = a.seqlen, D.heads = a.heads;
+    linear_decay_grad_kernel<<<(unsigned)(D.per_head ? a.heads : bh), kLdThreads, 0, st>>>(D);
+    e = cudaGetLastError();
+  }
+  return record_cuda_status(e);
+}
+
+int ss_linear_step(const ss_linear_step_args* a, void* stream) {
+  if (a == nullptr) return SS_ERR_INVALID;
+  if (a->batch < 0 || a->heads < 1 || a->key_heads < 1 || a->heads % a->key_heads != 0 || a->key_dim < 1 ||
+      a->value_dim < 1 || !std::isfinite(a->scale))
+    return SS_ERR_INVALID;
+  if (!dtypes_ok(a->io_dtype, a->decay_dtype)) return SS_ERR_UNSUPPORTED;
+  if (a->key_dim > SS_MAX_LINEAR_DIM || a->value_dim > SS_MAX_LINEAR_DIM) return SS_ERR_UNSUPPORTED;
+  if ((int64_t)a->batch * a->heads > 2147483647LL) return SS_ERR_UNSUPPORTED;
+  if (a->batch == 0) return SS_OK;
+  if (!a->state || !a->q || !a->k || !a->v || !a->log_decay || !a->o) return SS_ERR_INVALID;
+  if (a->state_batch_stride < (int64_t)a->heads * a->key_dim * a->value_dim) return SS_ERR_INVALID;
+  LinStepK P;
+  P.a = *a;
+  P.vec = a->value_dim % 4 == 0 && a->state_batch_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a->state) & 15) == 0;
+  const unsigned grid = (unsigned)((int64_t)a->batch * a->heads);
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (a->io_dtype) {
+    case SS_F32: linear_step_kernel<float><<<grid, 32 * kLstWarps, 0, st>>>(P); break;
+    case SS_BF16: linear_step_kernel<__nv_bfloat16><<<grid, 32 * kLstWarps, 0, st>>>(P); break;
+    default: linear_step_kernel<__half><<<grid, 32 * kLstWarps, 0, st>>>(P); break;
+  }
+  return record_cuda_status(cudaGetLastError());
+}
+
+}  // extern "C"

@@ -1,0 +1,518 @@
+// Linear attention with a decay per head.  Per batch row and head, over tokens t:
+//
+//   S_t = e^{g_t} S_{t-1} + k_t v_t^T        (state dk x dv, fp32)
+//   o_t = scale * q_t S_t
+//
+// in chunks of C tokens.  With G the inclusive sum of g inside the chunk, T its last value and H
+// the state before the chunk,
+//
+//   o_i = scale * ( e^{G_i} q_i H + sum_{j <= i} e^{G_i - G_j} (q_i . k_j) v_j )
+//   H  <- e^T H + sum_j e^{T - G_j} k_j v_j^T
+//
+// Every exponent is <= 0 for g <= 0.  The gradients are three more runs of the same recurrence, two
+// of them from the last token to the first ("reverse": pairs j >= i, output weight e^{T - G_i},
+// update weight e^{G_j}):
+//
+//   dq = run(q: do, k: v, v: k)   dv = reverse run(q: k, k: q, v: do)   dk = reverse run(q: v, k: do, v: q)
+//
+// The state of the dv run, times scale, is the gradient of the state (dS_0 at its end); and with
+// D_i = q_i . dq_i - k_i . dk_i, dg_t = sum_{i >= t} D_i + <dS_last, S_last>: each weight e^{G_i - G_j}
+// holds g_t once for every pair j < t <= i, and the sums telescope to the pairs that span t.
+#pragma once
+#include <type_traits>
+
+#include "ss_common.cuh"
+
+namespace ssb {
+
+// one run of the recurrence over a (batch, seqlen, heads) problem
+struct LinPass {
+  const void *q, *k, *v;
+  void* o;
+  int64_t qb, ql, qh, kb, kl, kh, vb, vl, vh, ob, ol, oh;  // element strides of batch, token, head
+  int rq, rk, rv;      // heads that share one head of q, k, v
+  int dk, dv;
+  int reverse;
+  int o_f32;           // o is fp32 (per-head parts of a gradient that a later kernel sums), else the I/O dtype
+  float scale;
+  const float* s_in;   // initial state, nullable: element (i, j) at i * s_row + j * s_col of a (dk * dv) block per (b, h)
+  float s_in_scale;
+  float* s_out;        // final state, nullable
+  float s_out_scale;
+  int s_row, s_col;
+  // dot[tile][b][h][t] = sum over the tile's output columns of p[.., t, ..] * o (before rounding)
+  const void* p;
+  int64_t pb, pl, ph;
+  int rp;
+  float* dot;
+  float* sum;          // segment states: [b * h][segment][dk * dv], nullable when there is one segment
+};
+
+constexpr int kLinMaxPasses = 3;
+
+struct LinK {
+  LinPass pass[kLinMaxPasses];
+  const void* g;       // log decay: I/O dtype or fp32
+  int g_f32;
+  int64_t gb, gl, gh;
+  const int* lens;     // nullable
+  float* seg_decay;    // [direction][b * h][segment]: the segment's total log decay
+  int batch, seqlen, heads;
+  int segs, seg_chunks;  // segments of the sequence, chunks of each
+};
+
+// log decays below this act as a reset: e^x is 0 in fp32 already, and sums of -1e4 stay exact
+constexpr float kLinReset = -1.0e4f;
+constexpr float kLinZeroBelow = -104.f;  // e^x rounds to zero in fp32
+
+__device__ __forceinline__ float lin_decay(const LinK& P, int b, int t, int h, bool bf16) {
+  const int64_t at = (int64_t)b * P.gb + (int64_t)t * P.gl + (int64_t)h * P.gh;
+  float g;
+  if (P.g_f32) g = static_cast<const float*>(P.g)[at];
+  else if (bf16) g = to_f<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(P.g)[at]);
+  else g = to_f<__half>(static_cast<const __half*>(P.g)[at]);
+  return g < kLinReset ? kLinReset : g;  // keeps NaN
+}
+
+// ------------------------------------------------------------------ fp32 units, any size and stride
+// One CTA per (segment, batch row and head, 64 value columns, pass); chunks of 64 tokens in shared
+// memory as fp32, each thread a 4 x 4 tile of every product.  This path serves fp32 I/O, where
+// 16-bit tensor-core operands would lose half the mantissa.
+constexpr int kLsC = 64;          // tokens of a chunk
+constexpr int kLsN = 64;          // value columns of a CTA
+constexpr int kLsThreads = 256;
+constexpr int kLsLd = 68;         // row stride (floats): 16-byte aligned, rows 4 banks apart
+constexpr int kLinMaxDim = 128;
+
+struct LsSmem {
+  float qt[kLinMaxDim][kLsLd];  // [d][token]
+  float kt[kLinMaxDim][kLsLd];
+  float v[kLsC][kLsLd];         // [token][column]
+  float h[kLinMaxDim][kLsLd];   // [d][column]
+  float at[kLsC][kLsLd];        // weighted scores, [j][i]
+  double G[kLsC];
+  float w_out[kLsC], w_upd[kLsC];
+  double total;
+};
+
+template <typename IT, bool STATE_ONLY>
+__global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_constant__ LinK P) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  LsSmem& S = *reinterpret_cast<LsSmem*>(smem_raw);
+  const int tiles = (kLinMaxDim + kLsN - 1) / kLsN;
+  const LinPass& A = P.pass[blockIdx.y / tiles];
+  const int tile = blockIdx.y % tiles;
+  const int n0 = tile * kLsN;
+  const int dk = A.dk, dv = A.dv;
+  if (n0 >= dv) return;
+  const int nv = min(kLsN, dv - n0);
+  const int bh = blockIdx.x / P.segs, seg = blockIdx.x % P.segs;
+  if (STATE_ONLY && seg == P.segs - 1) return;  // nothing follows the last segment
+  const int b = bh / P.heads, head = bh % P.heads;
+  const int len = P.lens ? max(0, min(P.lens[b], P.seqlen)) : P.seqlen;
+  const int n_chunks = (P.seqlen + kLsC - 1) / kLsC, n_live = (len + kLsC - 1) / kLsC;
+  const int c0 = seg * P.seg_chunks, c1 = min(c0 + P.seg_chunks, n_chunks);
+  const IT* q = static_cast<const IT*>(A.q) + (int64_t)b * A.qb + (int64_t)(head / A.rq) * A.qh;
+  const IT* k = static_cast<const IT*>(A.k) + (int64_t)b * A.kb + (int64_t)(head / A.rk) * A.kh;
+  const IT* v = static_cast<const IT*>(A.v) + (int64_t)b * A.vb + (int64_t)(head / A.rv) * A.vh + n0;
+  const int tid = threadIdx.x;
+  const int ti = tid / 16 * 4, tj = tid % 16 * 4;  // 4 x 4 tile of a 64 x 64 product
+  const int hi = tid / 16 * 8;                     // 8 x 4 tile of the state
+  const int64_t block = (int64_t)dk * dv;
+
+  // the state before this segment: the initial state folded with the earlier segments' own states
+  for (int e = tid; e < kLinMaxDim * kLsN; e += kLsThreads) {
+    const int i = e / kLsN, j = e % kLsN;
+    float s = 0.f;
+    if (!STATE_ONLY && i < dk && j < nv) {
+      if (A.s_in) s = A.s_in_scale * A.s_in[bh * block + (int64_t)i * A.s_row + (int64_t)(n0 + j) * A.s_col];
+      for (int r = 0; r < seg; ++r) {
+        const float d = expf(P.seg_decay[((int64_t)A.reverse * P.batch * P.heads + bh) * P.segs + r]);
+        s = fmaf(d, s, A.sum[((int64_t)bh * P.segs + r) * block + (int64_t)i * dv + n0 + j]);
+      }
+    }
+    S.h[i][j] = s;
+  }
+  double seg_total = 0.0;
+
+  for (int c = c0; c < (STATE_ONLY ? min(c1, n_live) : c1); ++c) {
+    if (!STATE_ONLY && c >= n_live) {  // behind the row's end: zero outputs
+      for (int e = tid; e < kLsC * kLsN; e += kLsThreads) {
+        const int t = c * kLsC + e / kLsN, j = e % kLsN;
+        if (t < P.seqlen && j < nv) {
+          const int64_t at = (int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0 + j;
+          if (A.o_f32) static_cast<float*>(A.o)[at] = 0.f;
+          else static_cast<IT*>(A.o)[at] = zero_v<IT>();
+        }
+      }
+      if (A.dot && tid < kLsC && c * kLsC + tid < P.seqlen)
+        A.dot[(((int64_t)tile * P.batch + b) * P.heads + head) * P.seqlen + c * kLsC + tid] = 0.f;
+      continue;
+    }
+    const int t0 = (A.reverse ? n_live - 1 - c : c) * kLsC;
+    const int m = min(kLsC, len - t0);  // valid tokens
+    __syncthreads();                    // the chunk before is done with shared memory
+    for (int e = tid; e < kLsC * dk; e += kLsThreads) {
+      const int t = e / dk, d = e % dk;
+      const bool on = t < m;
+      if (!STATE_ONLY) S.qt[d][t] = on ? to_f<IT>(q[(int64_t)(t0 + t) * A.ql + d]) : 0.f;
+      S.kt[d][t] = on ? to_f<IT>(k[(int64_t)(t0 + t) * A.kl + d]) : 0.f;
+    }
+    for (int e = tid; e < kLsC * kLsN; e += kLsThreads) {
+      const int t = e / kLsN, j = e % kLsN;
+      S.v[t][j] = (t < m && j < nv) ? to_f<IT>(v[(int64_t)(t0 + t) * A.vl + j]) : 0.f;
+    }
+    if (tid < 32) {  // inclusive sums of two tokens a lane, in 64 bits: differences stay exact behind a reset
+      constexpr bool bf = sizeof(IT) == 2 && std::is_same<IT, __nv_bfloat16>::value;
+      const double g0 = 2 * tid < m ? (double)lin_decay(P, b, t0 + 2 * tid, head, bf) : 0.0;
+      const double g1 = 2 * tid + 1 < m ? (double)lin_decay(P, b, t0 + 2 * tid + 1, head, bf) : 0.0;
+      double s = g0 + g1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double x = __shfl_up_sync(0xffffffffu, s, o);
+        if (tid >= o) s += x;
+      }
+      const double T = __shfl_sync(0xffffffffu, s, 31);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const double G = r ? s : s - g1;
+        const int t = 2 * tid + r;
+        S.G[t] = G;
+        const float a = expf((float)G), z = expf((float)(T - G));
+        S.w_out[t] = A.reverse ? z : a;
+        S.w_upd[t] = t < m ? (A.reverse ? a : z) : 0.f;
+      }
+      if (tid == 0) S.total = T;
+    }
+    __syncthreads();
+    seg_total += S.total;
+    if constexpr (!STATE_ONLY) {
+      // scores, weighted by the decay between the two tokens
+      float acc[4][4] = {};
+      for (int d = 0; d < dk; ++d) {
+        const float4 x = *reinterpret_cast<const float4*>(&S.qt[d][ti]);
+        const float4 y = *reinterpret_cast<const float4*>(&S.kt[d][tj]);
+        const float xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xa[i], ya[j], acc[i][j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = ti + i, s = tj + j;
+          const bool on = A.reverse ? s >= r : s <= r;
+          const double d = A.reverse ? S.G[s] - S.G[r] : S.G[r] - S.G[s];
+          S.at[s][r] = on && s < m ? acc[i][j] * expf((float)d) : 0.f;
+        }
+      // e^{G_i} q_i H
+      float o[4][4] = {};
+      for (int d = 0; d < dk; ++d) {
+        const float4 x = *reinterpret_cast<const float4*>(&S.qt[d][ti]);
+        const float4 y = *reinterpret_cast<const float4*>(&S.h[d][tj]);
+        const float xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][j] = fmaf(xa[i], ya[j], o[i][j]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] *= S.w_out[ti + i];
+      __syncthreads();  // scores written, H read
+      for (int s = 0; s < kLsC; ++s) {
+        const float4 x = *reinterpret_cast<const float4*>(&S.at[s][ti]);
+        const float4 y = *reinterpret_cast<const float4*>(&S.v[s][tj]);
+        const float xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][j] = fmaf(xa[i], ya[j], o[i][j]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + ti + i;
+        const bool on = ti + i < m;
+        float dot = 0.f;
+        if (t < P.seqlen) {
+          const int64_t at = (int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0 + tj;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (tj + j < nv) {
+              const float r = on ? A.scale * o[i][j] : 0.f;
+              if (A.o_f32) static_cast<float*>(A.o)[at + j] = r;
+              else static_cast<IT*>(A.o)[at + j] = from_f<IT>(r);
+              if (A.dot && on)
+                dot = fmaf(r, to_f<IT>(static_cast<const IT*>(A.p)[(int64_t)b * A.pb + (int64_t)t * A.pl +
+                                                                   (int64_t)(head / A.rp) * A.ph + n0 + tj + j]), dot);
+            }
+        }
+        if (A.dot) {
+#pragma unroll
+          for (int s = 8; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
+          if (tid % 16 == 0 && t < P.seqlen)
+            A.dot[(((int64_t)tile * P.batch + b) * P.heads + head) * P.seqlen + t] = dot;
+        }
+      }
+    }
+    // H <- e^T H + sum_j w_j k_j v_j^T: each thread updates its own 8 x 4 entries
+    if (hi < dk) {
+      const float d = expf((float)S.total);
+      float h[8][4];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(&S.h[hi + i][tj]);
+        h[i][0] = d * x.x, h[i][1] = d * x.y, h[i][2] = d * x.z, h[i][3] = d * x.w;
+      }
+      for (int s = 0; s < m; s += 4) {
+        float4 y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          y[r] = *reinterpret_cast<const float4*>(&S.v[s + r][tj]);
+          const float w = S.w_upd[s + r];
+          y[r].x *= w, y[r].y *= w, y[r].z *= w, y[r].w *= w;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (hi + i >= dk) break;
+          const float4 x = *reinterpret_cast<const float4*>(&S.kt[hi + i][s]);
+          const float xa[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            h[i][0] = fmaf(xa[r], y[r].x, h[i][0]);
+            h[i][1] = fmaf(xa[r], y[r].y, h[i][1]);
+            h[i][2] = fmaf(xa[r], y[r].z, h[i][2]);
+            h[i][3] = fmaf(xa[r], y[r].w, h[i][3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<float4*>(&S.h[hi + i][tj]) = make_float4(h[i][0], h[i][1], h[i][2], h[i][3]);
+    }
+  }
+  __syncthreads();
+  if (STATE_ONLY) {
+    for (int e = tid; e < dk * nv; e += kLsThreads) {
+      const int i = e / nv, j = e % nv;
+      A.sum[((int64_t)bh * P.segs + seg) * block + (int64_t)i * dv + n0 + j] = S.h[i][j];
+    }
+    if (tid == 0 && tile == 0)  // the same value from every pass of a direction
+      P.seg_decay[((int64_t)A.reverse * P.batch * P.heads + bh) * P.segs + seg] = (float)seg_total;
+  } else if (A.s_out && seg == P.segs - 1) {
+    for (int e = tid; e < dk * nv; e += kLsThreads) {
+      const int i = e / nv, j = e % nv;
+      A.s_out[bh * block + (int64_t)i * A.s_row + (int64_t)(n0 + j) * A.s_col] = A.s_out_scale * S.h[i][j];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------- gradient tails
+// Gradients of shared heads: out[b, t, kh, d] = sum over the group's heads of parts[b, t, h, d]
+// (fp32, contiguous), in a fixed order, rounded once.
+struct LinGroupK {
+  const float* parts[2];
+  void* out[2];
+  int64_t ob[2], ol[2], oh[2];
+  int batch, seqlen, key_heads, rep, dim;
+};
+
+template <typename IT>
+__global__ void __launch_bounds__(256) linear_group_sum_kernel(const __grid_constant__ LinGroupK P) {
+  const int which = blockIdx.y;
+  const int64_t n = (int64_t)P.batch * P.seqlen * P.key_heads * P.dim;
+  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (int64_t)gridDim.x * blockDim.x) {
+    const int d = (int)(e % P.dim);
+    const int64_t r = e / P.dim;  // (b, t, kh)
+    const float* src = P.parts[which] + (r * P.rep) * P.dim + d;
+    float s = 0.f;
+    for (int i = 0; i < P.rep; ++i) s += src[(int64_t)i * P.dim];
+    const int kh = (int)(r % P.key_heads);
+    const int64_t bt = r / P.key_heads;
+    static_cast<IT*>(P.out[which])[(bt / P.seqlen) * P.ob[which] + (bt % P.seqlen) * P.ol[which] + kh * P.oh[which] + d] =
+        from_f<IT>(s);
+  }
+}
+
+// dg_t = sum_{i >= t} (q_i . dq_i - k_i . dk_i) + <dS_last, S_last>, summed in 64 bits from the last
+// token.  One CTA per (b, h), 512 tokens a step; for a decay per head one CTA per head, which sums
+// over its rows and tokens in a fixed order.
+struct LinDecayK {
+  const float *xq, *yk;  // [tile][b][h][t]
+  int tq, tk;            // tiles of each
+  const float *d_last, *last;  // nullable (b, h, dk * dv)
+  int64_t block;
+  const void* g;
+  void* dg;
+  int g_f32, per_head, g_bf16;
+  int64_t gb, gl, gh;
+  const int* lens;
+  int batch, seqlen, heads;
+};
+
+constexpr int kLdThreads = 512;
+
+__global__ void __launch_bounds__(kLdThreads) linear_decay_grad_kernel(const __grid_constant__ LinDecayK P) {
+  __shared__ double part[kLdThreads / 32];
+  __shared__ double carry_s;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const int head = P.per_head ? blockIdx.x : blockIdx.x % P.heads;
+  const int b0 = P.per_head ? 0 : blockIdx.x / P.heads, b1 = P.per_head ? P.batch : b0 + 1;
+  const int64_t bhl = (int64_t)P.batch * P.heads * P.seqlen;
+  double sum = 0.0;  // per head: this thread's part of the total
+  auto store = [&](int64_t at, float x) {
+    if (P.g_f32) static_cast<float*>(P.dg)[at] = x;
+    else if (P.g_bf16) static_cast<__nv_bfloat16*>(P.dg)[at] = from_f<__nv_bfloat16>(x);
+    else static_cast<__half*>(P.dg)[at] = from_f<__half>(x);
+  };
+  for (int b = b0; b < b1; ++b) {
+    const int64_t bh = (int64_t)b * P.heads + head;
+    const int len = P.lens ? max(0, min(P.lens[b], P.seqlen)) : P.seqlen;
+    double x = 0.0;
+    if (P.d_last)
+      for (int64_t e = tid; e < P.block; e += kLdThreads)
+        x += (double)P.d_last[bh * P.block + e] * (double)P.last[bh * P.block + e];
+    __syncthreads();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (lane == 0) part[wid] = x;
+    __syncthreads();
+    if (tid == 0) {
+      double s = 0.0;
+      for (int i = 0; i < kLdThreads / 32; ++i) s += part[i];
+      carry_s = s;
+    }
+    __syncthreads();
+    double carry = carry_s;
+    // thread i holds token end - 1 - i, so a prefix over threads is a suffix over tokens
+    for (int end = P.seqlen; end > 0; end -= kLdThreads) {
+      const int t = end - 1 - tid;
+      double d = 0.0;
+      if (t >= 0 && t < len) {
+        for (int i = 0; i < P.tq; ++i) d += (double)P.xq[i * bhl + bh * P.seqlen + t];
+        for (int i = 0; i < P.tk; ++i) d -= (double)P.yk[i * bhl + bh * P.seqlen + t];
+      }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double u = __shfl_up_sync(0xffffffffu, d, o);
+        if (lane >= o) d += u;
+      }
+      __syncthreads();
+      if (lane == 31) part[wid] = d;
+      __syncthreads();
+      double before = 0.0, all = 0.0;
+      for (int i = 0; i < kLdThreads / 32; ++i) {
+        if (i < wid) before += part[i];
+        all += part[i];
+      }
+      if (t >= 0) {
+        const int64_t at = (int64_t)b * P.gb + (int64_t)t * P.gl + (int64_t)head * P.gh;
+        float g;
+        if (P.g_f32) g = static_cast<const float*>(P.g)[at];
+        else if (P.g_bf16) g = to_f<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(P.g)[at]);
+        else g = to_f<__half>(static_cast<const __half*>(P.g)[at]);
+        // a reset passes nothing from before the token, and behind the row's end there is nothing
+        const double r = t >= len || g < kLinZeroBelow ? 0.0 : carry + before + d;
+        if (P.per_head) sum += r;
+        else store(((int64_t)b * P.seqlen + t) * P.heads + head, (float)r);
+      }
+      carry += all;
+    }
+  }
+  if (P.per_head) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
+    if (lane == 0) part[wid] = sum;
+    __syncthreads();
+    if (tid == 0) {
+      double s = 0.0;
+      for (int i = 0; i < kLdThreads / 32; ++i) s += part[i];
+      store(head, (float)s);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------ single token
+// S <- e^g S + k v^T, o = scale q S.  The state is read and written once: a warp owns 4 x 32
+// consecutive columns (a float4 a lane; narrower values leave lanes idle) and a slice of the rows.
+struct LinStepK {
+  ss_linear_step_args a;
+  int vec;
+};
+
+constexpr int kLstWarps = 8;
+
+template <typename IT>
+__global__ void __launch_bounds__(32 * kLstWarps) linear_step_kernel(const __grid_constant__ LinStepK P) {
+  const ss_linear_step_args& a = P.a;
+  __shared__ float4 red[kLstWarps][32];
+  __shared__ float qs[kLinMaxDim], ks[kLinMaxDim];
+  const int bh = blockIdx.x, b = bh / a.heads, head = bh % a.heads;
+  const int dk = a.key_dim, dv = a.value_dim;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int kh = head / (a.heads / a.key_heads);
+  for (int d = threadIdx.x; d < dk; d += blockDim.x) {
+    qs[d] = to_f<IT>(static_cast<const IT*>(a.q)[(int64_t)b * a.q_batch_stride + (int64_t)kh * a.q_head_stride + d]);
+    ks[d] = to_f<IT>(static_cast<const IT*>(a.k)[(int64_t)b * a.k_batch_stride + (int64_t)kh * a.k_head_stride + d]);
+  }
+  const int64_t gat = (int64_t)b * a.decay_batch_stride + (int64_t)head * a.decay_head_stride;
+  const float g = a.decay_dtype == SS_F32 ? static_cast<const float*>(a.log_decay)[gat]
+                                          : to_f<IT>(static_cast<const IT*>(a.log_decay)[gat]);
+  const float decay = expf(g);
+  const int n0 = lane * 4;
+  float v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    v[j] = n0 + j < dv ? to_f<IT>(static_cast<const IT*>(a.v)[(int64_t)b * a.v_batch_stride +
+                                                             (int64_t)head * a.v_head_stride + n0 + j]) : 0.f;
+  __syncthreads();
+  float* st = a.state + (int64_t)b * a.state_batch_stride + (int64_t)head * dk * dv;
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+  if (n0 < dv) {
+#pragma unroll 8
+    for (int d = wid; d < dk; d += kLstWarps) {
+      float* row = st + (int64_t)d * dv + n0;
+      float s[4];
+      if (P.vec) {
+        const float4 x = *reinterpret_cast<const float4*>(row);
+        s[0] = x.x, s[1] = x.y, s[2] = x.z, s[3] = x.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = n0 + j < dv ? row[j] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[j] = fmaf(decay, s[j], ks[d] * v[j]);
+        o[j] = fmaf(qs[d], s[j], o[j]);
+      }
+      if (P.vec) {
+        *reinterpret_cast<float4*>(row) = make_float4(s[0], s[1], s[2], s[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n0 + j < dv) row[j] = s[j];
+      }
+    }
+  }
+  red[wid][lane] = make_float4(o[0], o[1], o[2], o[3]);
+  __syncthreads();
+  if (wid == 0) {
+    float4 s = red[0][lane];
+#pragma unroll
+    for (int w = 1; w < kLstWarps; ++w) {
+      const float4 x = red[w][lane];
+      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+    }
+    const float r[4] = {s.x, s.y, s.z, s.w};
+    IT* out = static_cast<IT*>(a.o) + (int64_t)b * a.o_batch_stride + (int64_t)head * a.o_head_stride;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n0 + j < dv) out[n0 + j] = from_f<IT>(a.scale * r[j]);
+  }
+}
+
+}  // namespace ssb

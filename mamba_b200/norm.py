@@ -7,10 +7,16 @@ prenorm=True)`` does both in one pass — the sum (the next residual stream, rou
 I/O dtype as the reference's in-place add) and its normalisation — and is differentiable in
 x, residual and weight.  ``rms_norm(module, x, ...)`` takes a reference ``RMSNorm`` module
 (its ``weight`` and ``eps``).
+
+``block_norm_fn`` (``ss_block_norm_fwd`` / ``ss_block_norm_bwd``) is for models whose blocks have a
+norm behind them as well, a gate, or a scale on the residual branch (the reference's have none): the
+norm after the block, the gate, the scaled residual add and the norm before the next block in one
+pass each way.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .selective_scan_interface import _cuda_device
@@ -86,3 +92,99 @@ def rms_norm(norm, x, residual=None, prenorm=False):
     """A reference ``RMSNorm`` module's forward (modules/rms_norm.py:21-30) through the fused
     kernel, optionally adding ``residual`` first (see rms_norm_fn)."""
     return rms_norm_fn(x, norm.weight, residual, norm.eps, True, prenorm)
+
+
+_ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
+
+
+class BlockNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, residual, post_weight, pre_weight, gate, scale, scale_const, activation, eps, pre_eps,
+                unit_offset):
+        _cuda_device(y, residual, post_weight, pre_weight, gate, scale)
+        dim, io = y.shape[-1], y.dtype
+        L.dtype_code(io)
+        rows = [None if t is None else _rows(t if t.dtype == io else t.to(io), dim) for t in (y, residual, gate)]
+        cols = [None if t is None else t.to(torch.float32).contiguous() for t in (post_weight, pre_weight, scale)]
+        n = rows[0].shape[0]
+        ctx.set_materialize_grads(False)
+        ctx.meta = (y.shape, activation, float(eps), float(pre_eps), bool(unit_offset), float(scale_const))
+        ctx.dtypes = tuple(None if t is None else t.dtype
+                           for t in (y, residual, post_weight, pre_weight, gate, scale))
+        new = lambda *s, dtype=io: torch.empty(s, dtype=dtype, device=y.device)  # noqa: E731
+        h = new(n, dim)
+        x = new(n, dim) if pre_weight is not None else None
+        rstd = new(n, 2, dtype=torch.float32)
+        ctx.save_for_backward(*rows, *cols, rstd)
+        args = BlockNormFn._args(ctx, rows, cols, rstd, h, x)
+        with torch.cuda.device(y.device):
+            L.check(L.lib().ss_block_norm_fwd(args, L.stream_of(y.device)), "ss_block_norm_fwd")
+        h = h.reshape(y.shape)
+        return h if x is None else (x.reshape(y.shape), h)
+
+    @staticmethod
+    def _args(ctx, rows, cols, rstd, h=None, x=None):
+        (y, residual, gate), (post, pre, scale) = rows, cols
+        shape, activation, eps, pre_eps, unit, const = ctx.meta
+        at = lambda t: (None, 0) if t is None else (t.data_ptr(), t.stride(0))  # noqa: E731
+        return L.BlockNormArgs(y.shape[0], shape[-1], L.dtype_code(y.dtype), int(unit), activation, eps, pre_eps, const,
+                               *at(y), *at(residual), *at(gate), L.ptr(post), L.ptr(pre), L.ptr(scale), *at(h), *at(x),
+                               rstd.data_ptr())
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        *rows, post, pre, scale, rstd = ctx.saved_tensors
+        y, residual, gate = rows
+        n, dim, io = y.shape[0], ctx.meta[0][-1], y.dtype
+        dx, dh = grads if pre is not None else (None, grads[0])
+        if dx is None and dh is None:
+            return (None,) * 11
+        if pre is not None and dx is None:
+            dx = torch.zeros_like(y)
+        dx, dh = (None if t is None else _rows(t if t.dtype == io else t.to(io), dim) for t in (dx, dh))
+        new = lambda t: None if t is None else torch.empty((n, dim), dtype=io, device=y.device)  # noqa: E731
+        dy, dres, dgate = new(y), new(residual), new(gate)
+        col = lambda t: None if t is None else torch.empty(dim, dtype=torch.float32, device=y.device)  # noqa: E731
+        dpost, dpre, dscale = col(post), col(pre), col(scale)
+        work = torch.empty(int(L.lib().ss_block_norm_work_elems(n, dim, L.dtype_code(io))), dtype=torch.float32,
+                           device=y.device)
+        at = lambda t: (None, 0) if t is None else (t.data_ptr(), t.stride(0))  # noqa: E731
+        args = L.BlockNormBwdArgs(BlockNormFn._args(ctx, rows, (post, pre, scale), rstd), *at(dx), *at(dh), *at(dy), *at(dres),
+                                  *at(dgate), L.ptr(dpost), L.ptr(dpre), L.ptr(dscale), work.data_ptr())
+        with torch.cuda.device(y.device):
+            L.check(L.lib().ss_block_norm_bwd(args, L.stream_of(y.device)), "ss_block_norm_bwd")
+        shape = ctx.meta[0]
+        out = [None if t is None else t.reshape(shape) for t in (dy, dres)] + [dpost, dpre]
+        out += [None if dgate is None else dgate.reshape(shape), dscale]
+        return (*(t if t is None or t.dtype == d else t.to(d) for t, d in zip(out, ctx.dtypes)),) + (None,) * 5
+
+
+def block_norm_fn(y, residual, post_weight=None, pre_weight=None, gate=None, residual_scale=None, activation="silu",
+                  eps=1e-6, pre_eps=None, unit_offset=True):
+    """What stands between two blocks, in one pass over the block's output ``y`` (..., dim):
+
+        h = residual + residual_scale * act(gate) * RMSNorm(y; post_weight)
+        x = RMSNorm(h; pre_weight)
+
+    post_weight (dim,): the norm after the block (none when None); gate (y's shape), through
+    ``activation`` ("silu", "sigmoid" or None: as it is); residual_scale: a (dim,) tensor or a number;
+    pre_weight (dim,): the norm before the next block.  Norms scale by 1 + weight (unit_offset) or
+    weight.  Everything is computed in fp32 and rounded once, x from the unrounded h.  dim is at most
+    8192.  Returns (x, h), or h alone without pre_weight; differentiable in every tensor."""
+    if residual.shape != y.shape or (gate is not None and gate.shape != y.shape):
+        raise ValueError("residual and gate must have the shape of y")
+    dim = y.shape[-1] if y.dim() else 0
+    if dim < 1:
+        raise ValueError("y must have a last dimension of at least 1")
+    if dim > L.MAX_BLOCK_NORM_DIM:
+        raise NotImplementedError(f"rows of {dim} values (at most {L.MAX_BLOCK_NORM_DIM})")
+    scale, const = (residual_scale, 1.0) if isinstance(residual_scale, torch.Tensor) else (
+        None, 1.0 if residual_scale is None else float(residual_scale))
+    for t, name in ((post_weight, "post_weight"), (pre_weight, "pre_weight"), (scale, "residual_scale")):
+        if t is not None and tuple(t.shape) != (dim,):
+            raise ValueError(f"{name} must be ({dim},), got {tuple(t.shape)}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation {activation!r} (one of {list(_ACTIVATIONS)})")
+    return BlockNormFn.apply(y, residual, post_weight, pre_weight, gate, scale, const, _ACTIVATIONS[activation], eps,
+                             eps if pre_eps is None else pre_eps, unit_offset)

@@ -1,0 +1,360 @@
+"""Linear attention with a decay per head against the recurrence in float64, token by token.
+
+Tolerances.  Every result is a sum of products; ``magnitude`` is the same sum with every factor's
+absolute value, computed by running the reference on absolute values (its gradients are sums of
+positive products too).  With u the half step of the I/O dtype, the result is rounded once (u |want|),
+and of each product's factors at most the weighted score and the carried state, or one of them twice,
+are rounded to 16 bits on the way: 2 u magnitude, for gradients of grouped heads as well (they are
+summed in fp32).  fp32 sums of n terms add n 2^-24 magnitude at most; n here is below 1024 and an
+exponential adds 2^-22, so 1024 * 2^-24 = 2^-14 covers the fp32 path in the worst case; random signs
+leave about sqrt(n), and 2^-17 magnitude is asked for.  States are fp32 results: with 16-bit I/O one
+factor of each product is split into two 16-bit parts (u^2), so 2^-14 magnitude holds with bf16 (u^2 =
+2^-16) and is asked of all types there."""
+import pytest
+import torch
+
+from sequence_ref import linear_ref
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def make(b, l, h, hk, dk, dv, dtype, *, per_head=False, state=False, lens=None, seed=0, bias=2.0):
+    g = torch.Generator().manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    t = dict(q=rn(b, l, hk, dk).to(dtype), k=rn(b, l, hk, dk).to(dtype), v=rn(b, l, h, dv).to(dtype))
+    if per_head:
+        t["g"] = -torch.nn.functional.softplus(rn(h) - bias)
+    else:
+        t["g"] = (-torch.nn.functional.softplus(rn(b, l, h) - bias)).to(dtype)
+    t["s0"] = rn(b, h, dk, dv) if state else None
+    t["lens"] = None if lens is None else torch.tensor(lens, dtype=torch.int32)
+    t["do"], t["dF"] = rn(b, l, h, dv).to(dtype), rn(b, h, dk, dv)
+    return {k: None if v is None else v.cuda() for k, v in t.items()}
+
+
+def reference(t, scale, want_final, absolute=False):
+    """o, final and the gradients in float64 (of the inputs' absolute values: the magnitudes)."""
+    f = (lambda x: x.double().abs()) if absolute else (lambda x: x.double())
+    leaves = [f(t[n]).requires_grad_() for n in ("q", "k", "v")]
+    g = t["g"].double().requires_grad_()
+    s0 = None if t["s0"] is None else f(t["s0"]).requires_grad_()
+    if t["lens"] is not None:  # what stands behind a row's end is not part of the mathematics
+        live = torch.arange(t["v"].shape[1], device="cuda")[None] < t["lens"][:, None]
+        clean = [torch.where(live[..., None, None], x, 0.0) for x in leaves]
+        gg = torch.where(live[..., None], g, 0.0) if g.dim() == 3 else g
+    else:
+        clean, gg = leaves, g
+    o, final = linear_ref(*clean, gg, scale, s0, t["lens"])
+    loss = (torch.where(live[..., None, None], f(t["do"]), 0.0) * o).sum() if t["lens"] is not None else (f(t["do"]) * o).sum()
+    if want_final:
+        loss = loss + (f(t["dF"]) * final).sum()
+    every = leaves + [g] + ([s0] if s0 is not None else [])
+    grads = torch.autograd.grad(loss, every, allow_unused=True)
+    return o.detach(), final.detach(), [torch.zeros_like(x) if d is None else d for d, x in zip(grads, every)]
+
+
+def close(name, got, want, mag, dtype, factor):
+    """|got - want| <= (half a step of got's dtype) |want| + factor * magnitude, everywhere."""
+    err = (got.double() - want).abs()
+    tol = HALF[got.dtype] * want.abs() * 1.001 + factor * mag + 1e-30
+    bad = err / tol
+    bad = torch.where(err == 0, 0.0, bad)
+    assert bool(torch.isfinite(got.double()).all()), f"{name}: not finite"
+    worst = float(bad.max()) if bad.numel() else 0.0
+    assert worst <= 1.0, f"{name}: {worst:.3g} of the tolerance"
+
+
+def decay_magnitude(t, scale, mags, mag_final, want_final):
+    """Magnitude of the decays' gradient: the telescoped sum of |q| dq + |k| dk, and <dF, S>."""
+    q, k = t["q"].double().abs(), t["k"].double().abs()
+    h = t["v"].shape[2]
+    rep = h // q.shape[2]
+    # per key head the magnitudes of the group's parts are summed; each part is at most that
+    x = sum((torch.where(torch.isfinite(a), a, 0.0) * m).sum(-1) for a, m in ((q, mags[0]), (k, mags[1])))
+    x = x.repeat_interleave(rep, 2).flip(1).cumsum(1).flip(1)
+    if want_final:
+        x = x + (t["dF"].double().abs() * mag_final).sum((-1, -2))[:, None]
+    return x if t["g"].dim() == 3 else x.sum((0, 1))
+
+
+def check(t, scale=0.3, want_final=True, tensors=None):
+    from mamba_b200 import linear_attention_fn
+
+    dtype = t["v"].dtype
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g")]
+    s0 = None if t["s0"] is None else t["s0"].detach().requires_grad_()
+    out = linear_attention_fn(*(tensors(leaves) if tensors else leaves), scale=scale, initial_state=s0,
+                              seq_lens=t["lens"], return_final_state=want_final)
+    o, final = out if want_final else (out, None)
+    seeds = [t["do"]] + ([t["dF"]] if want_final else [])
+    every = leaves + ([s0] if s0 is not None else [])
+    grads = torch.autograd.grad([o] + ([final] if want_final else []), every, seeds, allow_unused=True)
+    want_o, want_f, want_g = reference(t, scale, want_final)
+    mag_o, mag_f, mag_g = reference(t, scale, want_final, absolute=True)
+    f32 = dtype == torch.float32
+    soft = 2.0 ** -17 if f32 else 2 * HALF[dtype] + 2.0 ** -17
+    hard = 2.0 ** -17 if f32 else 2.0 ** -14
+    close("o", o, want_o, mag_o, dtype, soft)
+    if want_final:
+        assert final.dtype == torch.float32
+        close("final", final, want_f, mag_f, dtype, hard)
+    for name, got, want, mag in zip(("dq", "dk", "dv"), grads, want_g, mag_g):
+        assert got.dtype == dtype
+        close(name, got, want, mag, dtype, soft)
+    close("dlog_decay", grads[3], want_g[3], decay_magnitude(t, scale, mag_g, mag_f, want_final), dtype, soft)
+    if s0 is not None:
+        close("dinitial_state", grads[4], want_g[4], mag_g[4], dtype, hard)
+
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,l,h,hk,dk,dv", [(2, 1, 2, 2, 64, 64), (1, 2, 3, 1, 8, 16), (2, 63, 2, 2, 64, 64),
+                                           (1, 64, 2, 1, 128, 128), (2, 65, 4, 2, 64, 128), (1, 129, 2, 2, 128, 64),
+                                           (2, 200, 2, 1, 40, 57), (1, 300, 1, 1, 33, 128), (1, 257, 2, 2, 1, 1),
+                                           (1, 130, 6, 2, 72, 24)])
+def test_sizes(dtype, b, l, h, hk, dk, dv):
+    check(make(b, l, h, hk, dk, dv, dtype, state=True, seed=l))
+    check(make(b, l, h, hk, dk, dv, dtype, seed=l + 1), want_final=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bias", [-3.0, 0.0, 7.0])
+def test_decays_from_forgetful_to_lasting(dtype, bias):
+    check(make(1, 200, 2, 2, 64, 64, dtype, state=True, bias=bias, seed=5))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_decay_per_head(dtype):
+    check(make(2, 150, 4, 2, 64, 64, dtype, per_head=True, state=True, seed=6))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens", [[100, 0, 1, 170], [64, 128, 129, 65]])
+def test_padded_rows(dtype, lens):
+    """Rows end anywhere, one of them before its first token; what stands behind is NaN or infinite."""
+    t = make(4, 170, 2, 1, 64, 64, dtype, state=True, lens=lens, seed=7)
+    for i, n in enumerate(lens):
+        for name in ("q", "k", "v", "g"):
+            t[name][i, n:] = float("nan") if i % 2 else float("inf")
+    check(t)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_resets(dtype):
+    """A log decay of -inf forgets what came before; its own gradient is zero."""
+    t = make(1, 190, 2, 2, 64, 64, dtype, state=True, seed=8)
+    t["g"][0, [0, 5, 6, 100, 128, 189]] = float("-inf")
+    from mamba_b200 import linear_attention_fn
+
+    g = t["g"].clone().requires_grad_()
+    o, final = linear_attention_fn(t["q"], t["k"], t["v"], g, 0.3, t["s0"], None, True)
+    want_o, want_f, _ = reference(t, 0.3, True)
+    mag_o, mag_f, _ = reference(t, 0.3, True, absolute=True)
+    soft = 2.0 ** -17 if dtype == torch.float32 else 2 * HALF[dtype] + 2.0 ** -17
+    close("o", o, want_o, mag_o, dtype, soft)
+    close("final", final, want_f, mag_f, dtype, 2.0 ** -17 if dtype == torch.float32 else 2.0 ** -14)
+    (dg,) = torch.autograd.grad([o, final], [g], [t["do"], t["dF"]])
+    assert bool(torch.isfinite(dg).all()) and float(dg[0, [0, 5, 6, 100, 128, 189]].abs().max()) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strided_inputs(dtype):
+    """(batch, heads, seqlen, dim) storage, a slice of a wider projection, an expanded decay."""
+    t = make(2, 140, 4, 4, 64, 64, dtype, state=True, seed=9)
+
+    def views(leaves):
+        q, k, v, g = leaves
+        q = q.transpose(1, 2).contiguous().transpose(1, 2)
+        wide = torch.cat([k, v], -1)
+        return q, wide[..., :64], wide[..., 64:], g.transpose(0, 2).contiguous().transpose(0, 2)
+
+    check(t, tensors=views)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_misaligned_inputs(dtype):
+    """Rows that start off the 16-byte boundary."""
+    t = make(1, 70, 2, 2, 64, 64, dtype, seed=10)
+
+    def views(leaves):
+        q, k, v, g = leaves
+        pad = lambda x: torch.cat([x.new_zeros(*x.shape[:-1], 1), x], -1)[..., 1:]  # noqa: E731
+        return pad(q), pad(k), pad(v), g
+
+    check(t, tensors=views)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_sequence_is_its_halves(dtype):
+    """A long row with few heads (cut into segments that run side by side) against the same row in two
+    calls with the state carried over: the same sums in another grouping, so 2 roundings apart."""
+    from mamba_b200 import linear_attention_fn
+
+    t = make(1, 5000, 2, 1, 64, 64, dtype, state=True, bias=5.0, seed=11)
+    o, f = linear_attention_fn(t["q"], t["k"], t["v"], t["g"], None, t["s0"], None, True)
+    cut = 2113
+    a, s = linear_attention_fn(t["q"][:, :cut], t["k"][:, :cut], t["v"][:, :cut], t["g"][:, :cut], None, t["s0"], None, True)
+    c, s = linear_attention_fn(t["q"][:, cut:], t["k"][:, cut:], t["v"][:, cut:], t["g"][:, cut:], None, s, None, True)
+    two = torch.cat([a, c], 1)
+    rel = lambda x, y: float((x.double() - y.double()).norm() / y.double().norm())  # noqa: E731
+    # relative 2-norms: independent roundings of u each (4 of them for 16 bits), fp32 sums below 1e-5
+    assert rel(o, two) <= (1e-5 if dtype == torch.float32 else 4 * HALF[dtype])
+    assert rel(f, s) <= 1e-4
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_results_do_not_vary(dtype):
+    from mamba_b200 import linear_attention_fn
+
+    t = make(1, 1500, 4, 2, 64, 64, dtype, state=True, seed=12)
+
+    def once():
+        leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g", "s0")]
+        o, f = linear_attention_fn(*leaves[:4], None, leaves[4], None, True)
+        return [o, f, *torch.autograd.grad([o, f], leaves, [t["do"], t["dF"]])]
+
+    for a, b in zip(once(), once()):
+        assert torch.equal(a, b)
+
+
+def test_gradient_against_differences():
+    """fp32 gradients against central differences of the operator itself along random directions."""
+    from mamba_b200 import linear_attention_fn
+
+    t = make(2, 90, 2, 1, 24, 20, torch.float32, state=True, lens=[90, 41], seed=13)
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g", "s0")]
+
+    def loss(ls):
+        o, f = linear_attention_fn(*ls[:4], 0.3, ls[4], t["lens"], True)
+        return (o.double() * t["do"].double()).sum() + (f.double() * t["dF"].double()).sum()
+
+    grads = torch.autograd.grad(loss(leaves), leaves)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for i in range(5):
+        d = torch.randn(leaves[i].shape, generator=gen, device="cuda")
+        d = d / d.norm()
+        with torch.no_grad():
+            hi, lo = ([x + s * d if j == i else x for j, x in enumerate(leaves)] for s in (1e-2, -1e-2))
+            num = float(loss(hi) - loss(lo)) / 2e-2
+        # third-order term of the difference (step^2 = 1e-4 of the gradient's scale) and fp32 noise / step
+        assert abs(num - float((grads[i] * d).sum())) <= 2e-3 * float(grads[i].norm()) + 2e-3
+
+
+def test_only_the_final_state_is_used():
+    from mamba_b200 import linear_attention_fn
+
+    t = make(2, 70, 2, 2, 16, 16, torch.float32, seed=14)
+    leaves = [t[n].detach().requires_grad_() for n in ("k", "v")]
+    _, f = linear_attention_fn(t["q"], *leaves, t["g"], return_final_state=True)
+    got = torch.autograd.grad(f, leaves, t["dF"])
+    ref = [x.detach().double().requires_grad_() for x in leaves]
+    _, rf = linear_ref(t["q"].double(), *ref, t["g"].double(), 1.0)
+    for a, b in zip(got, torch.autograd.grad(rf, ref, t["dF"].double())):
+        assert float((a.double() - b).abs().max()) <= 2.0 ** -17 * float(b.abs().max()) * 16
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_empty_calls(dtype):
+    from mamba_b200 import linear_attention_fn
+
+    t = make(2, 0, 2, 2, 16, 16, dtype, state=True)
+    o, f = linear_attention_fn(t["q"], t["k"], t["v"], t["g"], 0.5, t["s0"], None, True)
+    assert o.shape == (2, 0, 2, 16) and torch.equal(f, t["s0"])
+    t = make(0, 5, 2, 2, 16, 16, dtype)
+    o, f = linear_attention_fn(t["q"], t["k"], t["v"], t["g"], return_final_state=True)
+    assert o.shape == (0, 5, 2, 16) and f.shape == (0, 2, 16, 16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,h,hk,dk,dv,per_head", [(1, 2, 2, 64, 64, False), (3, 6, 2, 128, 128, True), (2, 3, 1, 33, 57, False),
+                                                  (5, 4, 4, 128, 64, True), (1, 1, 1, 1, 1, False), (70, 2, 1, 16, 100, False)])
+def test_step(dtype, b, h, hk, dk, dv, per_head):
+    """Tokens one by one against the float64 recurrence; the state is fp32 arithmetic throughout
+    (a step: three roundings of 2^-24 each), the output rounded once."""
+    from mamba_b200 import linear_attention_step
+
+    t = make(b, 5, h, hk, dk, dv, dtype, per_head=per_head, state=True, seed=b + dk)
+    s = t["s0"].clone()
+    at = lambda x, i: x[:, i] if x.dim() > 1 else x  # noqa: E731
+    outs = [linear_attention_step(s, t["q"][:, i], t["k"][:, i], t["v"][:, i], at(t["g"], i), 0.3) for i in range(5)]
+    want_o, want_f = linear_ref(*(t[n].double() for n in ("q", "k", "v", "g")), 0.3, t["s0"].double())
+    mag_o, mag_f = linear_ref(*(t[n].double().abs() for n in ("q", "k", "v")), t["g"].double(), 0.3, t["s0"].double().abs())
+    close("o", torch.stack(outs, 1), want_o, mag_o, dtype, 2.0 ** -18)
+    close("state", s, want_f, mag_f, dtype, 2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_steps_continue_a_prompt(dtype):
+    from mamba_b200 import linear_attention_fn, linear_attention_step
+
+    t = make(2, 90, 4, 2, 64, 64, dtype, seed=21)
+    whole, f = linear_attention_fn(t["q"], t["k"], t["v"], t["g"], return_final_state=True)
+    _, s = linear_attention_fn(*(t[n][:, :80] for n in ("q", "k", "v", "g")), return_final_state=True)
+    for i in range(80, 90):
+        o = linear_attention_step(s, t["q"][:, i], t["k"][:, i], t["v"][:, i], t["g"][:, i])
+        err = float((o.double() - whole[:, i].double()).norm() / whole[:, i].double().norm())
+        assert err <= (1e-5 if dtype == torch.float32 else 4 * HALF[dtype])
+    assert float((s - f).norm() / f.norm()) <= 1e-4
+
+
+def test_step_on_strided_state_rows():
+    """A slice of a larger cache (batch stride wider than the state); the rows between stay as they are."""
+    from mamba_b200 import linear_attention_step
+
+    t = make(3, 1, 2, 2, 16, 16, torch.float32, state=True, seed=22)
+    cache = torch.full((3, 5, 16, 16), 7.0, device="cuda")
+    cache[:, 1:3] = t["s0"]
+    packed = t["s0"].clone()
+    args = t["q"][:, 0], t["k"][:, 0], t["v"][:, 0], t["g"][:, 0]
+    o = linear_attention_step(cache[:, 1:3], *args)
+    assert torch.equal(o, linear_attention_step(packed, *args))
+    assert torch.equal(cache[:, 1:3], packed) and bool((cache[:, [0, 3, 4]] == 7).all())
+
+
+def test_runs_on_another_stream_and_in_a_graph():
+    from mamba_b200 import linear_attention_fn
+
+    t = make(2, 300, 2, 2, 64, 64, torch.bfloat16, state=True, seed=23)
+    call = lambda: linear_attention_fn(t["q"], t["k"], t["v"], t["g"], None, t["s0"], None, True)  # noqa: E731
+    o, f = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        o2, f2 = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(o, o2) and torch.equal(f, f2)
+    graphs = []
+    for _ in range(2):  # two graphs alive at once, replayed in turn
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out))
+    t["v"].mul_(0.5)
+    want = call()
+    for graph, out in graphs + graphs:
+        graph.replay()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_training_step_in_a_graph():
+    from mamba_b200 import linear_attention_fn
+
+    t = make(2, 200, 4, 2, 64, 64, torch.bfloat16, seed=24)
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g")]
+    step = lambda: torch.autograd.grad(linear_attention_fn(*leaves), leaves, t["do"])  # noqa: E731
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    graph.replay()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
