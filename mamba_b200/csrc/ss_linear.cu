@@ -9,6 +9,7 @@
 
 #include "../../include/mamba_b200_ss.h"
 #include "ss_linear.cuh"
+#include "ss_linear_tc.cuh"
 
 namespace {
 
@@ -52,27 +53,30 @@ Split split_of(const ss_linear_args& a, int chunk, int passes, int tiles) {
   return s;
 }
 
-// The scratch of a call, cut into its parts (offsets in bytes; absent parts are -1)
+// The scratch of a call, cut into its parts (offsets in bytes; absent parts are -1).  The segments of
+// both kernels fit.
 struct Work {
   size_t bytes = 0;
   int64_t sums = -1, seg_decay = -1, dots = -1, parts = -1;
-  Split split;
+  Split simt, tc;
 };
 
 Work work_of(const ss_linear_args& a, int backward) {
   Work w;
   const int passes = backward ? 3 : 1;
   const int tiles = backward ? std::max(tiles_of(a.key_dim), tiles_of(a.value_dim)) : tiles_of(a.value_dim);
-  w.split = split_of(a, kLsC, passes, tiles);
+  w.simt = split_of(a, kLsC, passes, tiles);
+  w.tc = a.io_dtype == SS_F32 ? Split{1, 1} : split_of(a, kTcC, passes, tiles);
+  const int segs = a.io_dtype == SS_F32 ? w.simt.segs : std::max(w.simt.segs, w.tc.segs);
   const size_t bh = (size_t)a.batch * a.heads;
   auto take = [&](size_t n) {
     const int64_t at = (int64_t)w.bytes;
     w.bytes += align16(n);
     return at;
   };
-  if (w.split.segs > 1) {
-    w.sums = take(sizeof(float) * passes * bh * w.split.segs * a.key_dim * a.value_dim);
-    w.seg_decay = take(sizeof(float) * 2 * bh * w.split.segs);
+  if (segs > 1) {
+    w.sums = take(sizeof(float) * passes * bh * segs * a.key_dim * a.value_dim);
+    w.seg_decay = take(sizeof(float) * 2 * bh * segs);
   }
   if (backward) {
     w.dots = take(sizeof(float) * 2 * tiles_of(a.key_dim) * bh * a.seqlen);
@@ -82,14 +86,13 @@ Work work_of(const ss_linear_args& a, int backward) {
 }
 
 template <typename IT>
-cudaError_t run_passes(const LinK& P, int passes, int tiles, cudaStream_t st) {
+cudaError_t run_simt(const LinK& P, int passes, cudaStream_t st) {
   constexpr size_t smem = sizeof(LsSmem);
   auto main_k = linear_simt_kernel<IT, false>;
   auto sum_k = linear_simt_kernel<IT, true>;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(main_k), smem);
   if (e == cudaSuccess) e = ensure_smem_limit(reinterpret_cast<const void*>(sum_k), smem);
   if (e != cudaSuccess) return e;
-  (void)tiles;
   const int kt = (kLinMaxDim + kLsN - 1) / kLsN;
   const dim3 grid((unsigned)((int64_t)P.batch * P.heads * P.segs), (unsigned)(passes * kt));
   if (P.segs > 1) {
@@ -101,11 +104,79 @@ cudaError_t run_passes(const LinK& P, int passes, int tiles, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-cudaError_t run_by_type(int io, const LinK& P, int passes, int tiles, cudaStream_t st) {
+template <typename IT, int DK>
+cudaError_t launch_tc(const LinTcK& P, cudaStream_t st) {
+  constexpr size_t smem = TcShape<DK>::kBytes;
+  static_assert(smem <= 232448, "shared memory of a CTA");
+  static_assert(sizeof(TcBars) <= 512, "barriers");
+  auto main_k = linear_tc_kernel<IT, DK, false>;
+  auto sum_k = linear_tc_kernel<IT, DK, true>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(main_k), smem);
+  if (e == cudaSuccess) e = ensure_smem_limit(reinterpret_cast<const void*>(sum_k), smem);
+  if (e != cudaSuccess) return e;
+  const unsigned grid = (unsigned)((int64_t)P.k.batch * P.k.heads * P.k.segs * P.parts);
+  if (P.k.segs > 1) {
+    sum_k<<<grid, kTcThreads, smem, st>>>(P);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  main_k<<<grid, kTcThreads, smem, st>>>(P);
+  return cudaGetLastError();
+}
+
+bool vec16(const void* p, int es, int64_t b, int64_t l, int64_t h) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((b * es) & 15) == 0 && ((l * es) & 15) == 0 && ((h * es) & 15) == 0;
+}
+
+// The tensor-core kernel takes every 16-bit call whose rows TMA can address; false: it cannot.
+// Runs are grouped by the width of their keys (up to 64, up to 128), each group one launch.
+bool run_tc(int io, const LinK& P, int passes, cudaStream_t st, cudaError_t* e) {
+  LinTcK T[2];
+  int n[2] = {0, 0};
+  for (int i = 0; i < passes; ++i) {
+    const LinPass& A = P.pass[i];
+    const int w = A.dk > 64;
+    LinTcK& t = T[w];
+    const struct {
+      const void* p;
+      int64_t d, b, l, h;
+      int r;
+    } x[3] = {{A.q, A.dk, A.qb, A.ql, A.qh, A.rq}, {A.k, A.dk, A.kb, A.kl, A.kh, A.rk}, {A.v, A.dv, A.vb, A.vl, A.vh, A.rv}};
+    for (int j = 0; j < 3; ++j)
+      if (!map_heads(&t.map[n[w]][j], x[j].p, io, x[j].d, P.heads / x[j].r, P.seqlen, P.batch, x[j].h, x[j].l, x[j].b, kTcC))
+        return false;
+    if (n[w] == 0) {
+      t.k = P;
+      t.tiles = 1;
+      t.status = device_status_word();
+      t.wait_limit = wait_limit();
+    }
+    t.k.pass[n[w]] = A;
+    t.k.pass[n[w]].o_vec = vec16(A.o, A.o_f32 ? 4 : 2, A.ob, A.ol, A.oh) && (!A.dot || vec16(A.p, 2, A.pb, A.pl, A.ph));
+    t.tiles = std::max(t.tiles, (A.dv + kTcN - 1) / kTcN);
+    ++n[w];
+  }
+  *e = cudaSuccess;
+  for (int w = 0; w < 2 && *e == cudaSuccess; ++w) {
+    if (n[w] == 0) continue;
+    T[w].parts = n[w] * T[w].tiles;
+    if (io == SS_BF16) *e = w ? launch_tc<__nv_bfloat16, 128>(T[w], st) : launch_tc<__nv_bfloat16, 64>(T[w], st);
+    else *e = w ? launch_tc<__half, 128>(T[w], st) : launch_tc<__half, 64>(T[w], st);
+  }
+  return true;
+}
+
+cudaError_t run_passes(int io, LinK& P, const Work& w, int passes, cudaStream_t st) {
+  if (io != SS_F32 && P.seqlen > 0) {
+    P.segs = w.tc.segs, P.seg_chunks = w.tc.chunks;
+    cudaError_t e;
+    if (run_tc(io, P, passes, st, &e)) return e;
+  }
+  P.segs = w.simt.segs, P.seg_chunks = w.simt.chunks;
   switch (io) {
-    case SS_F32: return run_passes<float>(P, passes, tiles, st);
-    case SS_BF16: return run_passes<__nv_bfloat16>(P, passes, tiles, st);
-    default: return run_passes<__half>(P, passes, tiles, st);
+    case SS_F32: return run_simt<float>(P, passes, st);
+    case SS_BF16: return run_simt<__nv_bfloat16>(P, passes, st);
+    default: return run_simt<__half>(P, passes, st);
   }
 }
 
@@ -116,7 +187,6 @@ LinK problem(const ss_linear_args& a, const Work& w, void* work) {
   P.gb = a.decay_batch_stride, P.gl = a.decay_seq_stride, P.gh = a.decay_head_stride;
   P.lens = a.seq_lens;
   P.batch = a.batch, P.seqlen = a.seqlen, P.heads = a.heads;
-  P.segs = w.split.segs, P.seg_chunks = w.split.chunks;
   if (w.seg_decay >= 0) P.seg_decay = reinterpret_cast<float*>(static_cast<char*>(work) + w.seg_decay);
   return P;
 }
@@ -164,7 +234,7 @@ int ss_linear_fwd(const ss_linear_args* a, void* stream) {
   A.s_out = a->state_out, A.s_out_scale = 1.f;
   A.s_row = a->value_dim, A.s_col = 1;
   if (w.sums >= 0) A.sum = reinterpret_cast<float*>(static_cast<char*>(a->work) + w.sums);
-  return record_cuda_status(run_by_type(a->io_dtype, P, 1, tiles_of(a->value_dim), (cudaStream_t)stream));
+  return record_cuda_status(run_passes(a->io_dtype, P, w, 1, (cudaStream_t)stream));
 }
 
 int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
@@ -201,7 +271,7 @@ int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
     A.v = z.p, A.vb = z.b, A.vl = z.l, A.vh = z.h, A.rv = z.rep;
     A.dk = dk, A.dv = dv, A.reverse = reverse, A.scale = a.scale;
     A.s_in_scale = reverse ? 1.f / a.scale : 1.f;  // a reverse run's state times scale is the state's gradient
-    if (sums) A.sum = sums + (int64_t)i * bh * w.split.segs * block;
+    if (sums) A.sum = sums + (int64_t)i * bh * std::max(w.simt.segs, w.tc.segs) * block;
     return A;
   };
   auto grad = [&](LinPass& A, int i, void* out, int64_t b, int64_t l, int64_t h, const T& p) {
@@ -228,7 +298,7 @@ int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
   V.s_in = g->dstate_out, V.s_row = a.value_dim, V.s_col = 1;
   V.s_out = g->dstate_in, V.s_out_scale = a.scale;
   cudaStream_t st = (cudaStream_t)stream;
-  cudaError_t e = run_by_type(a.io_dtype, P, 3, std::max(tq, tiles_of(a.value_dim)), st);
+  cudaError_t e = run_passes(a.io_dtype, P, w, 3, st);
   if (e != cudaSuccess) return record_cuda_status(e);
   if (parts && a.seqlen > 0) {
     LinGroupK G{};

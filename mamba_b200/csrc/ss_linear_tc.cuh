@@ -1,0 +1,636 @@
+// Linear attention on the 5th-generation tensor cores (tcgen05), for 16-bit I/O: one run of the
+// recurrence (ss_linear.cuh) with chunks of 128 tokens.
+//
+// One CTA walks the chunks of a segment of one (batch row, head) for 64 value columns.  Per chunk:
+//
+//   S   = Q K^T                 128 x 128 x dk    operands as TMA wrote them (K-major, 128-byte swizzle)
+//   P   = S * e^{G_i - G_j}     masked, rounded to 16 bits into TMEM, the A operand of the next product
+//   Oa  = P V                   128 x 64 x 128    V as the MN-major B operand
+//   Oi  = Q Hhi + Q Hlo         128 x 64 x dk     the state before the chunk, split into two 16-bit parts
+//   L   = K^T V'hi + K^T V'lo   dk x 64 x 128     V' = e^{T - G_j} v_j, split likewise; K as MN-major A
+//   o   = scale (e^{G_i} Oi + Oa),   H <- e^T H + L   (H in fp32 registers, one row a thread)
+//
+// Rounding: Q, K and V enter as they are.  The weighted scores P are the one place where 16 bits
+// (half a step) are accepted: an output is rounded to the same type anyway.  The state and the
+// weighted values would spread their rounding to every later token and to the fp32 final state, so
+// they are split: hi + lo keeps 16 (bf16) or 22 (fp16) bits, at two products of 64 columns each.
+// The dot products for the decays' gradient need it too: sums of q . dq - k . dk telescope only as far
+// as both runs round the same P alike and nothing else.
+//
+// What bounds it: a chunk moves 128 x (2 dk + 128) x 2 bytes through TMA; two value tiles of one head
+// run side by side, so keys and queries come from L2 the second time.
+// Roles (18 warps): 0-3 scores, 4-7 weighted values, 8-11 outputs, 12-15 state, 16 loads and decays,
+// 17 matrix instructions.  The only chain from chunk to chunk is H: L -> state warps -> Q H.
+#pragma once
+#include "ss_linear.cuh"
+
+namespace ssb {
+
+constexpr int kTcC = 128;   // tokens of a chunk
+constexpr int kTcN = 64;    // value columns of a CTA
+constexpr int kTcThreads = 18 * 32;
+constexpr uint32_t kBox = kTcC * 128;  // one TMA box: 128 rows of 128 bytes
+
+struct LinTcK {
+  LinK k;
+  int tiles, parts;      // value tiles of the widest pass; passes x tiles
+  int* status;
+  long long wait_limit;
+  alignas(64) CUtensorMap map[kLinMaxPasses][3];  // q, k, v of each pass
+};
+
+// ---------------------------------------------------------------------------------------- PTX
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar, bool lead) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+               " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+               "r"((uint32_t)lead)
+               : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Issued by one lane (`lead`) of a warp that runs the whole loop together: the descriptors then stay
+// in uniform registers.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, bool lead) {
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+               "r"((uint32_t)add), "r"((uint32_t)lead)
+               : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add, bool lead) {
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+               "r"((uint32_t)add), "r"((uint32_t)lead)
+               : "memory");
+}
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// shared-memory operand descriptors, 128-byte swizzle: K-major (rows of 64 elements along K, 8-row
+// groups 1024 bytes apart) and MN-major (rows of 64 elements along M or N, one K a row; `lead` bytes
+// between groups of 64)
+__device__ __forceinline__ uint64_t desc_of(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+template <typename IT>
+__device__ __forceinline__ constexpr uint32_t idesc_of(int m, int n, bool a_mn, bool b_mn) {
+  const uint32_t f = std::is_same<IT, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(m >> 4) << 24);
+}
+
+template <typename IT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<IT, __nv_bfloat16>::value) {
+    __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&p);
+  } else {
+    __half2 p = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&p);
+  }
+}
+template <typename IT>
+__device__ __forceinline__ float2 unpack2(uint32_t p) {
+  if constexpr (std::is_same<IT, __nv_bfloat16>::value)
+    return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+  else
+    return __half22float2(*reinterpret_cast<__half2*>(&p));
+}
+// 8 values of a row split into hi + lo and stored at 16-byte chunk j of row r of two swizzled tiles
+template <typename IT>
+__device__ __forceinline__ void store_split(unsigned char* hi, unsigned char* lo, int r, int j, const float (&v)[8]) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[i] = pack2<IT>(v[2 * i], v[2 * i + 1]);
+    const float2 b = unpack2<IT>(h[i]);
+    l[i] = pack2<IT>(v[2 * i] - b.x, v[2 * i + 1] - b.y);
+  }
+  const int at = r * 128 + ((j ^ (r & 7)) << 4);
+  *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+template <int DK>
+struct TcShape {
+  static constexpr int kBoxes = DK / 64;
+  static constexpr int kStages = DK == 128 ? 2 : 3;
+  static constexpr uint32_t kStageBytes = (2 * kBoxes + 1) * kBox;  // Q, K, V
+  static constexpr uint32_t kVp = kStages * kStageBytes;            // V' hi, lo
+  static constexpr uint32_t kH = kVp + 2 * kBox;                    // H hi, lo
+  static constexpr uint32_t kDec = kH + 2 * DK * 128;               // per stage: G and T - G, times log2 e
+  static constexpr uint32_t kBars = kDec + kStages * 2 * kTcC * 4;
+  static constexpr uint32_t kBytes = kBars + 512;
+};
+
+struct TcBars {
+  uint64_t full[3], empty[3];
+  uint64_t s_full[2], p_full[2];
+  uint64_t vp_full, l_full, l_empty, h_full, h_empty, o_full, o_empty, drain;
+  float total[3];  // e^T of the stage's chunk
+  uint32_t tmem;
+  int abort;
+};
+
+// TMEM columns: two score buffers (the weighted scores overwrite the first half of theirs), outputs, L
+constexpr uint32_t kTmS = 0, kTmOi = 256, kTmOa = 320, kTmL = 384, kTmCols = 512;
+
+// try_wait that may suspend the thread for up to ~1 ms instead of coming back at once: a waiting warp
+// that polls takes issue slots from the ones that work
+__device__ __forceinline__ bool mbar_try_wait_long(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+
+struct TcWait {
+  TcBars* s;
+  long long limit;
+  int* status;
+  // false: the wait gave up, here or in another role
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+    if (mbar_try_wait_long(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try_wait_long(bar, parity)) {
+      if (*reinterpret_cast<volatile int*>(&s->abort)) return false;
+      if (clock64() - t0 > limit) {
+        *reinterpret_cast<volatile int*>(&s->abort) = 1;
+        if (status) atomicOr(status, kStatusTimeout);
+        return false;
+      }
+    }
+    return true;
+  }
+};
+
+template <typename IT, int DK, bool STATE_ONLY>
+__global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_constant__ LinTcK P) {
+  using S = TcShape<DK>;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  TcBars& B = *reinterpret_cast<TcBars*>(smem + S::kBars);
+  const LinK& K = P.k;
+  // value tiles and runs of one head are neighbours in the grid, so that they share what they read in L2
+  const int part = blockIdx.x % P.parts, where = blockIdx.x / P.parts;
+  const int pass = part / P.tiles, tile = part % P.tiles;
+  const LinPass& A = K.pass[pass];
+  const int dk = A.dk, dv = A.dv, n0 = tile * kTcN;
+  const int bh = where / K.segs, seg = where % K.segs;
+  if (n0 >= dv || (STATE_ONLY && seg == K.segs - 1)) return;
+  const int nv = min(kTcN, dv - n0);
+  const int b = bh / K.heads, head = bh % K.heads;
+  const int len = K.lens ? max(0, min(K.lens[b], K.seqlen)) : K.seqlen;
+  const int n_chunks = (K.seqlen + kTcC - 1) / kTcC, n_live = (len + kTcC - 1) / kTcC;
+  const int c0 = seg * K.seg_chunks, c1 = min(c0 + K.seg_chunks, n_chunks), cn = min(c1, n_live);
+  const bool reverse = A.reverse != 0;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, wg = wid >> 2, row = tid & 127;
+  auto first_token = [&](int c) { return (reverse ? n_live - 1 - c : c) * kTcC; };
+  auto dec_G = [&](int st) { return reinterpret_cast<float*>(smem + S::kDec) + st * 2 * kTcC; };
+  const TcWait wait{&B, P.wait_limit, P.status};
+  const int64_t block = (int64_t)dk * dv;
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+
+  if (wid == 16 && lane == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&B.full[i], 2);                          // the copies, the decays
+      mbar_init(&B.empty[i], STATE_ONLY ? 1 + 4 : 1 + 8);  // the products, the warps that read the decays last
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&B.s_full[i], 1), mbar_init(&B.p_full[i], 4);
+    mbar_init(&B.vp_full, 4);
+    mbar_init(&B.l_full, 1), mbar_init(&B.l_empty, 4);
+    mbar_init(&B.h_full, 4), mbar_init(&B.h_empty, 1);
+    mbar_init(&B.o_full, 1), mbar_init(&B.o_empty, 4);
+    mbar_init(&B.drain, 1);
+    B.abort = 0;
+    mbar_fence_init();
+  }
+  if (wid == 17) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&B.tmem)), "r"(kTmCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tm = B.tmem;
+  const uint32_t lanes = tm + ((uint32_t)(wid & 3) << 21);  // this warp's 32 lanes
+
+  if (wid == 16) {
+    // ------------------------------------------------------------ loads, decays
+    double seg_total = 0.0;
+    const int hq = head / A.rq, hk = head / A.rk, hv = head / A.rv;
+    const uint32_t base = smem_u32(smem);
+    constexpr bool bf = std::is_same<IT, __nv_bfloat16>::value;
+    float gn[4];  // 4 tokens a lane of the chunk after the one at hand: its loads are under way
+    float4 to_here, to_end;
+    float total = 0.f;
+    auto load_decays = [&](int c) {
+      const int t = first_token(c) + 4 * lane;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) gn[r] = t + r < len ? lin_decay(K, b, t + r, head, bf) : 0.f;
+    };
+    auto sums = [&]() {  // inclusive, in 64 bits: a difference of two sums keeps its digits
+      const double s0 = (double)gn[0], s1 = s0 + (double)gn[1], s2 = s1 + (double)gn[2], s3 = s2 + (double)gn[3];
+      double x = s3;
+#pragma unroll 1
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const double T = __shfl_sync(0xffffffffu, x, 31);
+      const double before = x - s3, after = T - before;
+      constexpr double l2e = 1.4426950408889634;
+      to_here = make_float4((float)((before + s0) * l2e), (float)((before + s1) * l2e), (float)((before + s2) * l2e),
+                            (float)((before + s3) * l2e));
+      to_end = make_float4((float)((after - s0) * l2e), (float)((after - s1) * l2e), (float)((after - s2) * l2e),
+                           (float)((after - s3) * l2e));
+      total = expf((float)T);
+      seg_total += T;
+    };
+    if (c0 < cn) load_decays(c0);
+    for (int c = c0, i = 0, st = 0; c < cn; ++c, ++i, st = st + 1 == S::kStages ? 0 : st + 1) {
+      sums();
+      if (i >= S::kStages && !warp_wait(&B.empty[st], (uint32_t)(i / S::kStages - 1) & 1)) break;
+      const int t0 = first_token(c);
+      if (lane == 0) {
+        const uint32_t dst = base + st * S::kStageBytes;
+        mbar_expect_tx(&B.full[st], (STATE_ONLY ? S::kBoxes + 1 : 2 * S::kBoxes + 1) * kBox);
+#pragma unroll
+        for (int x = 0; x < S::kBoxes; ++x) {
+          if (!STATE_ONLY) tma_load_4d(dst + x * kBox, &P.map[pass][0], x * 64, hq, t0, b, &B.full[st]);
+          tma_load_4d(dst + (S::kBoxes + x) * kBox, &P.map[pass][1], x * 64, hk, t0, b, &B.full[st]);
+        }
+        tma_load_4d(dst + 2 * S::kBoxes * kBox, &P.map[pass][2], n0, hv, t0, b, &B.full[st]);
+      }
+      *reinterpret_cast<float4*>(dec_G(st) + 4 * lane) = to_here;
+      *reinterpret_cast<float4*>(dec_G(st) + kTcC + 4 * lane) = to_end;
+      if (lane == 0) B.total[st] = total;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B.full[st]);
+      if (c + 1 < cn) load_decays(c + 1);
+    }
+    if (STATE_ONLY && tile == 0 && lane == 0)
+      K.seg_decay[((int64_t)reverse * K.batch * K.heads + bh) * K.segs + seg] = (float)seg_total;
+  } else if (wid == 17) {
+    // ------------------------------------------------------------ matrix instructions
+    const uint32_t base = smem_u32(smem);
+    const bool lead = lane == 0;
+    constexpr uint32_t kIdQK = idesc_of<IT>(128, kTcC, false, false), kIdN = idesc_of<IT>(128, kTcN, false, true),
+                       kIdL = idesc_of<IT>(128, kTcN, true, true);
+    // descriptors of the first stage; a step of 16 along K is 32 bytes (K-major) or 2048 (MN-major)
+    const uint64_t q0 = desc_of(base, 16), kk0 = desc_of(base + S::kBoxes * kBox, 16),
+                   km0 = desc_of(base + S::kBoxes * kBox, kBox), v0 = desc_of(base + 2 * S::kBoxes * kBox, kBox),
+                   vp0 = desc_of(base + S::kVp, kBox), h0 = desc_of(base + S::kH, kBox);
+    auto scores = [&](int st, int buf) {
+      const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4));
+#pragma unroll
+      for (int x = 0; x < S::kBoxes * 4; ++x)
+        mma_ss(tm + kTmS + buf * 128, q0 + o + (x >> 2) * (kBox >> 4) + (x & 3) * 2,
+               kk0 + o + (x >> 2) * (kBox >> 4) + (x & 3) * 2, kIdQK, x > 0, lead);
+      tc_commit(&B.s_full[buf], lead);
+    };
+    const int n = cn - c0;
+    for (int i = 0, st = 0, ph = 0; i < n; ++i) {  // ph: the stages' phase
+      if (!warp_wait(&B.full[st], ph)) break;
+      tc_after();
+      if (!STATE_ONLY && i == 0) scores(0, 0);
+      // L = K^T V'
+      if (!warp_wait(&B.vp_full, i & 1) || (i > 0 && !warp_wait(&B.l_empty, (i - 1) & 1))) break;
+      tc_after();
+      const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4));
+#pragma unroll
+      for (int x = 0; x < 2 * kTcC / 16; ++x)
+        mma_ss(tm + kTmL, km0 + o + (x & 7) * 128, vp0 + (x >> 3) * (kBox >> 4) + (x & 7) * 128, kIdL, x > 0, lead);
+      tc_commit(&B.l_full, lead);
+      const int nst = st + 1 == S::kStages ? 0 : st + 1, nph = nst ? ph : ph ^ 1;
+      if constexpr (STATE_ONLY) {
+        tc_commit(&B.empty[st], lead);
+      } else {
+        // the next chunk's scores, into the buffer whose weighted scores were used a chunk ago
+        if (i + 1 < n) {
+          if (!warp_wait(&B.full[nst], nph) || (i > 0 && !warp_wait(&B.o_full, (i - 1) & 1))) break;
+          tc_after();
+          scores(nst, (i + 1) & 1);
+        }
+        // Oi = Q H
+        if (!warp_wait(&B.h_full, i & 1) || (i > 0 && !warp_wait(&B.o_empty, (i - 1) & 1))) break;
+        tc_after();
+#pragma unroll
+        for (int x = 0; x < 2 * DK / 16; ++x) {
+          const int k = x % (DK / 16);
+          mma_ss(tm + kTmOi, q0 + o + (k >> 2) * (kBox >> 4) + (k & 3) * 2, h0 + x * 128, kIdN, x > 0, lead);
+        }
+        tc_commit(&B.h_empty, lead);
+        // Oa = P V
+        if (!warp_wait(&B.p_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
+        tc_after();
+#pragma unroll
+        for (int x = 0; x < kTcC / 16; ++x)
+          mma_ts(tm + kTmOa, tm + kTmS + (i & 1) * 128 + x * 8, v0 + o + x * 128, kIdN, x > 0, lead);
+        tc_commit(&B.o_full, lead);
+        tc_commit(&B.empty[st], lead);
+      }
+      st = nst;
+      ph = nph;
+    }
+    // every product has ended before the CTA gives up its memory
+    tc_commit(&B.drain, lead);
+    const long long t0 = clock64();
+    while (!mbar_try_wait(&B.drain, 0) && clock64() - t0 < kWaitCycles) {
+    }
+    __syncwarp();
+  } else if (wg == 0) {
+    // ------------------------------------------------------------ weighted scores
+    if constexpr (!STATE_ONLY) {
+      const int w = wid & 3;
+      const float sign = reverse ? 1.f : -1.f;
+      for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
+        const int m = min(kTcC, len - first_token(c));
+        if (!warp_wait(&B.full[st], ph) || !warp_wait(&B.s_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
+        tc_after();
+        const float* G = dec_G(st);
+        const float2 gi = f2(-sign * G[row]), sg = f2(sign);  // exponent: sign * (G_j - G_i)
+        const uint32_t sp = lanes + kTmS + (i & 1) * 128;
+        // 32 columns at a time.  P's columns x .. x + 31 land on S's columns x / 2 .., always behind
+        // what is still to be read; blocks on the far side of the diagonal are zero
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          uint32_t p[16];
+          if (reverse ? x >= w : x <= w) {
+            float s[32];
+            tmem_ld32(sp + x * 32, s);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 gj = *reinterpret_cast<const float4*>(G + x * 32 + j);
+              const float2 d0 = fma2(sg, make_float2(gj.x, gj.y), gi), d1 = fma2(sg, make_float2(gj.z, gj.w), gi);
+              const float2 e0 = mul2(make_float2(s[j], s[j + 1]), make_float2(ex2_ordered(d0.x), ex2_ordered(d0.y)));
+              const float2 e1 = mul2(make_float2(s[j + 2], s[j + 3]), make_float2(ex2_ordered(d1.x), ex2_ordered(d1.y)));
+              s[j] = e0.x, s[j + 1] = e0.y, s[j + 2] = e1.x, s[j + 3] = e1.y;
+            }
+            if (x == w || m < kTcC) {  // the diagonal, or tokens behind the row's end
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const int col = x * 32 + j;
+                s[j] = (reverse ? col >= row && col < m : col <= row) ? s[j] : 0.f;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) p[j] = pack2<IT>(s[2 * j], s[2 * j + 1]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) p[j] = 0u;
+          }
+          tmem_st16(sp + x * 16, p);
+        }
+        tc_wait_st();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.p_full[i & 1]);
+        if (++st == S::kStages) st = 0, ph ^= 1;
+      }
+    }
+  } else if (wg == 1) {
+    // ------------------------------------------------------------ weighted values
+    for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
+      const int m = min(kTcC, len - first_token(c));
+      if (!warp_wait(&B.full[st], ph)) break;
+      unsigned char* k = smem + st * S::kStageBytes + S::kBoxes * kBox + row * 128;
+      unsigned char* v = smem + st * S::kStageBytes + 2 * S::kBoxes * kBox + row * 128;
+      if (row >= m) {  // behind the row's end: whatever was read there must not meet a product
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+          for (int x = 0; x < S::kBoxes; ++x) *reinterpret_cast<uint4*>(k + x * kBox + j * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(v + j * 16) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      __syncwarp();
+      const float2 w = f2(ex2(dec_G(st)[reverse ? row : kTcC + row]));
+      if (i > 0 && !warp_wait(&B.l_full, (i - 1) & 1)) break;  // the product over the buffer has ended
+#pragma unroll 2
+      for (int j = 0; j < 8; ++j) {
+        const uint4 q = *reinterpret_cast<const uint4*>(v + ((j ^ (row & 7)) << 4));
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+        float x[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float2 f = mul2(w, unpack2<IT>(u[r]));
+          x[2 * r] = f.x;
+          x[2 * r + 1] = f.y;
+        }
+        store_split<IT>(smem + S::kVp, smem + S::kVp + kBox, row, j, x);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B.vp_full);
+      if (++st == S::kStages) st = 0, ph ^= 1;
+    }
+  } else if (wg == 2) {
+    // ------------------------------------------------------------ outputs
+    if constexpr (!STATE_ONLY) {
+      auto zero_row = [&](int t) {
+        const int64_t at = (int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0;
+        for (int j = 0; j < nv; ++j) {
+          if (A.o_f32) static_cast<float*>(A.o)[at + j] = 0.f;
+          else static_cast<IT*>(A.o)[at + j] = zero_v<IT>();
+        }
+        if (A.dot) A.dot[(((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen + t] = 0.f;
+      };
+      const bool vec = A.o_vec && nv == kTcN;
+      const int64_t o_at = (int64_t)b * A.ob + (int64_t)head * A.oh + n0;
+      const IT* p_at = A.dot ? static_cast<const IT*>(A.p) + (int64_t)b * A.pb + (int64_t)(head / A.rp) * A.ph + n0 : nullptr;
+      float* dot_at = A.dot ? A.dot + (((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen : nullptr;
+      for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
+        const int t0 = first_token(c), m = min(kTcC, len - t0), t = t0 + row;
+        if (!warp_wait(&B.full[st], ph)) break;
+        const float2 w = f2(A.scale * ex2(dec_G(st)[reverse ? kTcC + row : row])), sc = f2(A.scale);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.empty[st]);
+        const bool on = row < m;
+        const int64_t at = o_at + (int64_t)t * A.ol;
+        const IT* p = p_at + (int64_t)t * A.pl;
+        if (!warp_wait(&B.o_full, i & 1)) break;
+        tc_after();
+        float2 dot = f2(0.f);
+#pragma unroll 1
+        for (int x = 0; x < 2; ++x) {
+          float o[32], oa[32];
+          tmem_ld32(lanes + kTmOi + x * 32, o);
+          tmem_ld32(lanes + kTmOa + x * 32, oa);
+          tc_wait_ld();
+          if (x == 1) {
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.o_empty);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float2 r = fma2(w, make_float2(o[j], o[j + 1]), mul2(sc, make_float2(oa[j], oa[j + 1])));
+            o[j] = r.x, o[j + 1] = r.y;
+          }
+          if (on && vec) {
+            if (A.o_f32) {
+              float4* dst = reinterpret_cast<float4*>(static_cast<float*>(A.o) + at + x * 32);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(static_cast<IT*>(A.o) + at + x * 32);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                dst[j] = make_uint4(pack2<IT>(o[8 * j], o[8 * j + 1]), pack2<IT>(o[8 * j + 2], o[8 * j + 3]),
+                                    pack2<IT>(o[8 * j + 4], o[8 * j + 5]), pack2<IT>(o[8 * j + 6], o[8 * j + 7]));
+            }
+            if (dot_at) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint4 q = *reinterpret_cast<const uint4*>(p + x * 32 + 8 * j);
+                const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  dot = fma2(make_float2(o[8 * j + 2 * r], o[8 * j + 2 * r + 1]), unpack2<IT>(u[r]), dot);
+              }
+            }
+          } else if (on) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (x * 32 + j < nv) {
+                if (A.o_f32) static_cast<float*>(A.o)[at + x * 32 + j] = o[j];
+                else static_cast<IT*>(A.o)[at + x * 32 + j] = from_f<IT>(o[j]);
+                if (dot_at) dot.x = fmaf(o[j], to_f<IT>(p[x * 32 + j]), dot.x);
+              }
+          }
+        }
+        if (on) {
+          if (dot_at) dot_at[t] = dot.x + dot.y;
+        } else if (t < K.seqlen) {
+          zero_row(t);
+        }
+        if (++st == S::kStages) st = 0, ph ^= 1;
+      }
+      for (int c = max(cn, c0); c < c1; ++c)  // chunks behind the row's end
+        if (c * kTcC + row < K.seqlen) zero_row(c * kTcC + row);
+    }
+  } else {
+    // ------------------------------------------------------------ state: row `row` of H
+    const bool on = row < dk;
+    float h[kTcN];
+#pragma unroll
+    for (int j = 0; j < kTcN; ++j) h[j] = 0.f;
+    if (!STATE_ONLY && on) {
+      if (A.s_in) {
+        const float* s = A.s_in + bh * block + (int64_t)row * A.s_row + (int64_t)n0 * A.s_col;
+#pragma unroll
+        for (int j = 0; j < kTcN; ++j)
+          if (j < nv) h[j] = A.s_in_scale * s[(int64_t)j * A.s_col];
+      }
+      for (int r = 0; r < seg; ++r) {
+        const float d = expf(K.seg_decay[((int64_t)reverse * K.batch * K.heads + bh) * K.segs + r]);
+        const float* s = A.sum + ((int64_t)bh * K.segs + r) * block + (int64_t)row * dv + n0;
+#pragma unroll
+        for (int j = 0; j < kTcN; ++j)
+          if (j < nv) h[j] = fmaf(d, h[j], s[j]);
+      }
+    }
+    unsigned char* hh = smem + S::kH;
+    auto publish = [&]() {
+      if (row < DK) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float x[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) x[r] = h[8 * j + r];
+          store_split<IT>(hh, hh + DK * 128, row, j, x);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B.h_full);
+    };
+    if (!STATE_ONLY && cn > c0) publish();
+    for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
+      if (!warp_wait(&B.full[st], ph)) break;
+      const float d = *reinterpret_cast<volatile float*>(&B.total[st]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B.empty[st]);
+      if (!warp_wait(&B.l_full, i & 1)) break;
+      tc_after();
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float l[32];
+        tmem_ld32(lanes + kTmL + x * 32, l);
+        tc_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 r = fma2(f2(d), make_float2(h[x * 32 + j], h[x * 32 + j + 1]), make_float2(l[j], l[j + 1]));
+          h[x * 32 + j] = r.x, h[x * 32 + j + 1] = r.y;
+        }
+      }
+      tc_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B.l_empty);
+      if (!STATE_ONLY && c + 1 < cn) {
+        if (!warp_wait(&B.h_empty, i & 1)) break;
+        publish();
+      }
+      if (++st == S::kStages) st = 0, ph ^= 1;
+    }
+    if (on && !*reinterpret_cast<volatile int*>(&B.abort)) {
+      if (STATE_ONLY) {
+        float* s = A.sum + ((int64_t)bh * K.segs + seg) * block + (int64_t)row * dv + n0;
+#pragma unroll
+        for (int j = 0; j < kTcN; ++j)
+          if (j < nv) s[j] = h[j];
+      } else if (A.s_out && seg == K.segs - 1) {
+        float* s = A.s_out + bh * block + (int64_t)row * A.s_row + (int64_t)n0 * A.s_col;
+#pragma unroll
+        for (int j = 0; j < kTcN; ++j)
+          if (j < nv) s[(int64_t)j * A.s_col] = A.s_out_scale * h[j];
+      }
+    }
+  }
+  tc_before();
+  __syncthreads();
+  if (B.abort && wid == 16 && lane == 0) {  // copies still in flight land before the memory is given up
+    const long long t0 = clock64();
+    for (int st = 0; st < S::kStages; ++st)
+      for (uint32_t par = 0; par < 2; ++par)
+        while (!mbar_try_wait(&B.full[st], par) && clock64() - t0 < kWaitCycles / 8) {
+        }
+  }
+  __syncthreads();
+  if (wid == 17) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(kTmCols) : "memory");
+  }
+}
+
+}  // namespace ssb
