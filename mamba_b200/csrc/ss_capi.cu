@@ -132,15 +132,16 @@ bool ssb::map_heads(CUtensorMap* m, const void* p, int dtype, int64_t dim, int64
                     int64_t head_stride, int64_t seq_stride, int64_t batch_stride, int rows) {
   auto fn = encode_fn();
   if (fn == nullptr || p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15)) return false;
+  const int64_t es = dtype == SS_F32 ? 4 : 2;
   const int64_t n[3] = {heads, seqlen, batch}, st[3] = {head_stride, seq_stride, batch_stride};
   cuuint64_t dims[4] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)seqlen, (cuuint64_t)batch};
   cuuint64_t strides[3];
   for (int i = 0; i < 3; ++i) {
-    const int64_t b = n[i] > 1 ? st[i] * 2 : 16;  // an axis of one element is never stepped along
+    const int64_t b = n[i] > 1 ? st[i] * es : 16;  // an axis of one element is never stepped along
     if (b <= 0 || (b & 15) || b >= (1ll << 40)) return false;
     strides[i] = (cuuint64_t)b;
   }
-  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
+  cuuint32_t box[4] = {(cuuint32_t)(128 / es), 1, (cuuint32_t)rows, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   return fn(m, tm_type(dtype), 4, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==

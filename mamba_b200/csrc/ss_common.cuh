@@ -26,8 +26,8 @@ namespace ssb {
 
 // Records e as the thread's last CUDA error (ss_last_cuda_error) and maps it to a status.
 int record_cuda_status(cudaError_t e);
-// Tensor map of a (batch, seqlen, heads, dim) tensor of 2-byte elements (strides in elements): boxes of
-// 64 elements x `rows` tokens of one head, 128-byte swizzle, zeros outside.  False when TMA cannot
+// Tensor map of a (batch, seqlen, heads, dim) tensor (strides in elements): boxes of 128 bytes x `rows`
+// tokens of one head, 128-byte swizzle, zeros outside.  False when TMA cannot
 // describe it (alignment, zero strides).
 bool map_heads(CUtensorMap* m, const void* p, int dtype, int64_t dim, int64_t heads, int64_t seqlen, int64_t batch,
                int64_t head_stride, int64_t seq_stride, int64_t batch_stride, int rows);

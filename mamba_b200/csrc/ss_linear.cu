@@ -108,7 +108,7 @@ template <typename IT, int DK>
 cudaError_t launch_tc(const LinTcK& P, cudaStream_t st) {
   constexpr size_t smem = TcShape<DK>::kBytes;
   static_assert(smem <= 232448, "shared memory of a CTA");
-  static_assert(sizeof(TcBars) <= 512, "barriers");
+  static_assert(sizeof(TcBars) <= 256, "barriers");
   auto main_k = linear_tc_kernel<IT, DK, false>;
   auto sum_k = linear_tc_kernel<IT, DK, true>;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(main_k), smem);
@@ -128,13 +128,17 @@ bool vec16(const void* p, int es, int64_t b, int64_t l, int64_t h) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((b * es) & 15) == 0 && ((l * es) & 15) == 0 && ((h * es) & 15) == 0;
 }
 
-// The tensor-core kernel takes every 16-bit call whose rows TMA can address; false: it cannot.
+// The tensor-core kernel takes every 16-bit call whose rows are whole 16-byte units (TMA loads, vector
+// stores); false: it cannot.
 // Runs are grouped by the width of their keys (up to 64, up to 128), each group one launch.
 bool run_tc(int io, const LinK& P, int passes, cudaStream_t st, cudaError_t* e) {
   LinTcK T[2];
   int n[2] = {0, 0};
   for (int i = 0; i < passes; ++i) {
     const LinPass& A = P.pass[i];
+    if (A.dk % 8 || A.dv % 8 || !vec16(A.o, A.o_f32 ? 4 : 2, A.ob, A.ol, A.oh) ||
+        (A.dot && !vec16(A.p, 2, A.pb, A.pl, A.ph)))
+      return false;
     const int w = A.dk > 64;
     LinTcK& t = T[w];
     const struct {
@@ -145,6 +149,8 @@ bool run_tc(int io, const LinK& P, int passes, cudaStream_t st, cudaError_t* e) 
     for (int j = 0; j < 3; ++j)
       if (!map_heads(&t.map[n[w]][j], x[j].p, io, x[j].d, P.heads / x[j].r, P.seqlen, P.batch, x[j].h, x[j].l, x[j].b, kTcC))
         return false;
+    if (!map_heads(&t.map[n[w]][3], A.o, A.o_f32 ? SS_F32 : io, A.dv, P.heads, P.seqlen, P.batch, A.oh, A.ol, A.ob, 32))
+      return false;
     if (n[w] == 0) {
       t.k = P;
       t.tiles = 1;
@@ -152,7 +158,6 @@ bool run_tc(int io, const LinK& P, int passes, cudaStream_t st, cudaError_t* e) 
       t.wait_limit = wait_limit();
     }
     t.k.pass[n[w]] = A;
-    t.k.pass[n[w]].o_vec = vec16(A.o, A.o_f32 ? 4 : 2, A.ob, A.ol, A.oh) && (!A.dot || vec16(A.p, 2, A.pb, A.pl, A.ph));
     t.tiles = std::max(t.tiles, (A.dv + kTcN - 1) / kTcN);
     ++n[w];
   }

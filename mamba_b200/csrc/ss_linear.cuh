@@ -34,7 +34,6 @@ struct LinPass {
   int dk, dv;
   int reverse;
   int o_f32;           // o is fp32 (per-head parts of a gradient that a later kernel sums), else the I/O dtype
-  int o_vec;           // rows of o (and of p) start on 16-byte boundaries
   float scale;
   const float* s_in;   // initial state, nullable: element (i, j) at i * s_row + j * s_col of a (dk * dv) block per (b, h)
   float s_in_scale;

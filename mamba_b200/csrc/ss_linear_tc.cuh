@@ -36,7 +36,7 @@ struct LinTcK {
   int tiles, parts;      // value tiles of the widest pass; passes x tiles
   int* status;
   long long wait_limit;
-  alignas(64) CUtensorMap map[kLinMaxPasses][3];  // q, k, v of each pass
+  alignas(64) CUtensorMap map[kLinMaxPasses][4];  // q, k, v, o of each pass
 };
 
 // ---------------------------------------------------------------------------------------- PTX
@@ -47,13 +47,28 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "[%6];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(z), "r"(w), "r"(src)
+               : "memory");
+}
+// every store of this thread has read its shared memory
+__device__ __forceinline__ void tma_store_read() {
+  asm volatile("cp.async.bulk.commit_group;\n cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void tc_commit(uint64_t* bar, bool lead) {
-  asm volatile("{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
-               " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
-               "r"((uint32_t)lead)
+// one lane of a converged warp, in the form the compiler knows to be one lane: operands of the
+// instructions under it go to uniform registers without a loop over lanes
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
+  return ok != 0;
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -62,24 +77,27 @@ __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sy
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Issued by one lane (`lead`) of a warp that runs the whole loop together: the descriptors then stay
-// in uniform registers.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, bool lead) {
-  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
-               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-               "r"((uint32_t)add), "r"((uint32_t)lead)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+               "r"((uint32_t)add)
                : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add, bool lead) {
-  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
-               " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-               "r"((uint32_t)add), "r"((uint32_t)lead)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+               "r"((uint32_t)add)
                : "memory");
 }
 // 32 columns of this warp's 32 lanes
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
                : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
@@ -143,9 +161,11 @@ struct TcShape {
   static constexpr uint32_t kStageBytes = (2 * kBoxes + 1) * kBox;  // Q, K, V
   static constexpr uint32_t kVp = kStages * kStageBytes;            // V' hi, lo
   static constexpr uint32_t kH = kVp + 2 * kBox;                    // H hi, lo
-  static constexpr uint32_t kDec = kH + 2 * DK * 128;               // per stage: G and T - G, times log2 e
-  static constexpr uint32_t kBars = kDec + kStages * 2 * kTcC * 4;
-  static constexpr uint32_t kBytes = kBars + 512;
+  // per stage: G and T - G (times log2 e) of every token, and the column factors of three blocks
+  static constexpr uint32_t kDecStage = (2 * kTcC + 96) * 4;
+  static constexpr uint32_t kDec = kH + 2 * DK * 128;
+  static constexpr uint32_t kBars = kDec + kStages * kDecStage;
+  static constexpr uint32_t kBytes = kBars + 256;
 };
 
 struct TcBars {
@@ -157,7 +177,8 @@ struct TcBars {
   int abort;
 };
 
-// TMEM columns: two score buffers (the weighted scores overwrite the first half of theirs), outputs, L
+// TMEM columns: two score buffers (the weighted scores overwrite the first half of theirs), outputs,
+// L of the high and of the low parts
 constexpr uint32_t kTmS = 0, kTmOi = 256, kTmOa = 320, kTmL = 384, kTmCols = 512;
 
 // try_wait that may suspend the thread for up to ~1 ms instead of coming back at once: a waiting warp
@@ -172,25 +193,19 @@ __device__ __forceinline__ bool mbar_try_wait_long(uint64_t* bar, uint32_t parit
   return ok != 0;
 }
 
-struct TcWait {
-  TcBars* s;
-  long long limit;
-  int* status;
-  // false: the wait gave up, here or in another role
-  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
-    if (mbar_try_wait_long(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!mbar_try_wait_long(bar, parity)) {
-      if (*reinterpret_cast<volatile int*>(&s->abort)) return false;
-      if (clock64() - t0 > limit) {
-        *reinterpret_cast<volatile int*>(&s->abort) = 1;
-        if (status) atomicOr(status, kStatusTimeout);
-        return false;
-      }
+// the part of a wait that is not over at once; false: it gave up, here or in another role
+__device__ __noinline__ bool tc_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, long long limit, int* status) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait_long(bar, parity)) {
+    if (*abort) return false;
+    if (clock64() - t0 > limit) {
+      *abort = 1;
+      if (status) atomicOr(status, kStatusTimeout);
+      return false;
     }
-    return true;
   }
-};
+  return true;
+}
 
 template <typename IT, int DK, bool STATE_ONLY>
 __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_constant__ LinTcK P) {
@@ -213,10 +228,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
   const bool reverse = A.reverse != 0;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, wg = wid >> 2, row = tid & 127;
   auto first_token = [&](int c) { return (reverse ? n_live - 1 - c : c) * kTcC; };
-  auto dec_G = [&](int st) { return reinterpret_cast<float*>(smem + S::kDec) + st * 2 * kTcC; };
-  const TcWait wait{&B, P.wait_limit, P.status};
+  auto dec_G = [&](int st) { return reinterpret_cast<float*>(smem + S::kDec + st * S::kDecStage); };
   const int64_t block = (int64_t)dk * dv;
-  auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+  // for whole warps: the lanes go on, or give up, together
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
+    const bool ok = mbar_try_wait_long(bar, parity) || tc_wait_slow(bar, parity, &B.abort, P.wait_limit, P.status);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
 
   if (wid == 16 && lane == 0) {
     for (int i = 0; i < S::kStages; ++i) {
@@ -250,7 +268,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     const uint32_t base = smem_u32(smem);
     constexpr bool bf = std::is_same<IT, __nv_bfloat16>::value;
     float gn[4];  // 4 tokens a lane of the chunk after the one at hand: its loads are under way
-    float4 to_here, to_end;
+    float4 to_here, to_end, factor;
     float total = 0.f;
     auto load_decays = [&](int c) {
       const int t = first_token(c) + 4 * lane;
@@ -274,13 +292,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
                            (float)((after - s3) * l2e));
       total = expf((float)T);
       seg_total += T;
+      if (!STATE_ONLY) {
+        // factors of a block's 32 columns towards the block's border on the side of the rows that use them
+        const float f = __shfl_sync(0xffffffffu, to_here.w, reverse ? (lane & 24) - 1 : lane | 7);
+        const float sg = reverse ? 1.f : -1.f;
+        factor = make_float4(ex2(sg * (to_here.x - f)), ex2(sg * (to_here.y - f)), ex2(sg * (to_here.z - f)),
+                             ex2(sg * (to_here.w - f)));
+      }
     };
     if (c0 < cn) load_decays(c0);
     for (int c = c0, i = 0, st = 0; c < cn; ++c, ++i, st = st + 1 == S::kStages ? 0 : st + 1) {
       sums();
       if (i >= S::kStages && !warp_wait(&B.empty[st], (uint32_t)(i / S::kStages - 1) & 1)) break;
       const int t0 = first_token(c);
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t dst = base + st * S::kStageBytes;
         mbar_expect_tx(&B.full[st], (STATE_ONLY ? S::kBoxes + 1 : 2 * S::kBoxes + 1) * kBox);
 #pragma unroll
@@ -292,6 +317,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       }
       *reinterpret_cast<float4*>(dec_G(st) + 4 * lane) = to_here;
       *reinterpret_cast<float4*>(dec_G(st) + kTcC + 4 * lane) = to_end;
+      if (!STATE_ONLY) {  // blocks 0 - 2, reverse 1 - 3: the far block has no rows beyond it
+        const int l = reverse ? lane - 8 : lane;
+        if (l >= 0 && l < 24) *reinterpret_cast<float4*>(dec_G(st) + 2 * kTcC + 4 * l) = factor;
+      }
       if (lane == 0) B.total[st] = total;
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.full[st]);
@@ -302,38 +331,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
   } else if (wid == 17) {
     // ------------------------------------------------------------ matrix instructions
     const uint32_t base = smem_u32(smem);
-    const bool lead = lane == 0;
     constexpr uint32_t kIdQK = idesc_of<IT>(128, kTcC, false, false), kIdN = idesc_of<IT>(128, kTcN, false, true),
-                       kIdL = idesc_of<IT>(128, kTcN, true, true);
+                       kIdL = idesc_of<IT>(128, 2 * kTcN, true, true);
     // descriptors of the first stage; a step of 16 along K is 32 bytes (K-major) or 2048 (MN-major)
     const uint64_t q0 = desc_of(base, 16), kk0 = desc_of(base + S::kBoxes * kBox, 16),
                    km0 = desc_of(base + S::kBoxes * kBox, kBox), v0 = desc_of(base + 2 * S::kBoxes * kBox, kBox),
                    vp0 = desc_of(base + S::kVp, kBox), h0 = desc_of(base + S::kH, kBox);
     auto scores = [&](int st, int buf) {
       const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4));
+      if (elect_one()) {
 #pragma unroll
-      for (int x = 0; x < S::kBoxes * 4; ++x)
-        mma_ss(tm + kTmS + buf * 128, q0 + o + (x >> 2) * (kBox >> 4) + (x & 3) * 2,
-               kk0 + o + (x >> 2) * (kBox >> 4) + (x & 3) * 2, kIdQK, x > 0, lead);
-      tc_commit(&B.s_full[buf], lead);
+        for (int x = 0; x < S::kBoxes * 4; ++x)
+          mma_ss(tm + kTmS + buf * 128, q0 + o + (x >> 2) * (kBox >> 4) + (x & 3) * 2,
+                 kk0 + o + (x >> 2) * (kBox >> 4) + (x & 3) * 2, kIdQK, x > 0);
+        tc_commit(&B.s_full[buf]);
+      }
+      __syncwarp();
     };
     const int n = cn - c0;
     for (int i = 0, st = 0, ph = 0; i < n; ++i) {  // ph: the stages' phase
       if (!warp_wait(&B.full[st], ph)) break;
       tc_after();
       if (!STATE_ONLY && i == 0) scores(0, 0);
-      // L = K^T V'
+      // L = K^T [V'hi, V'lo]: a product of 64 columns takes as long as one of 128
       if (!warp_wait(&B.vp_full, i & 1) || (i > 0 && !warp_wait(&B.l_empty, (i - 1) & 1))) break;
       tc_after();
       const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4));
+      if (elect_one()) {
 #pragma unroll
-      for (int x = 0; x < 2 * kTcC / 16; ++x)
-        mma_ss(tm + kTmL, km0 + o + (x & 7) * 128, vp0 + (x >> 3) * (kBox >> 4) + (x & 7) * 128, kIdL, x > 0, lead);
-      tc_commit(&B.l_full, lead);
+        for (int x = 0; x < kTcC / 16; ++x) mma_ss(tm + kTmL, km0 + o + x * 128, vp0 + x * 128, kIdL, x > 0);
+        tc_commit(&B.l_full);
+        if (STATE_ONLY) tc_commit(&B.empty[st]);
+      }
+      __syncwarp();
       const int nst = st + 1 == S::kStages ? 0 : st + 1, nph = nst ? ph : ph ^ 1;
-      if constexpr (STATE_ONLY) {
-        tc_commit(&B.empty[st], lead);
-      } else {
+      if constexpr (!STATE_ONLY) {
         // the next chunk's scores, into the buffer whose weighted scores were used a chunk ago
         if (i + 1 < n) {
           if (!warp_wait(&B.full[nst], nph) || (i > 0 && !warp_wait(&B.o_full, (i - 1) & 1))) break;
@@ -343,26 +375,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         // Oi = Q H
         if (!warp_wait(&B.h_full, i & 1) || (i > 0 && !warp_wait(&B.o_empty, (i - 1) & 1))) break;
         tc_after();
+        if (elect_one()) {
 #pragma unroll
-        for (int x = 0; x < 2 * DK / 16; ++x) {
-          const int k = x % (DK / 16);
-          mma_ss(tm + kTmOi, q0 + o + (k >> 2) * (kBox >> 4) + (k & 3) * 2, h0 + x * 128, kIdN, x > 0, lead);
+          for (int x = 0; x < 2 * DK / 16; ++x) {
+            const int k = x % (DK / 16);
+            mma_ss(tm + kTmOi, q0 + o + (k >> 2) * (kBox >> 4) + (k & 3) * 2, h0 + x * 128, kIdN, x > 0);
+          }
+          tc_commit(&B.h_empty);
         }
-        tc_commit(&B.h_empty, lead);
+        __syncwarp();
         // Oa = P V
         if (!warp_wait(&B.p_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
+        if (elect_one()) {
 #pragma unroll
-        for (int x = 0; x < kTcC / 16; ++x)
-          mma_ts(tm + kTmOa, tm + kTmS + (i & 1) * 128 + x * 8, v0 + o + x * 128, kIdN, x > 0, lead);
-        tc_commit(&B.o_full, lead);
-        tc_commit(&B.empty[st], lead);
+          for (int x = 0; x < kTcC / 16; ++x)
+            mma_ts(tm + kTmOa, tm + kTmS + (i & 1) * 128 + x * 8, v0 + o + x * 128, kIdN, x > 0);
+          tc_commit(&B.o_full);
+          tc_commit(&B.empty[st]);
+        }
+        __syncwarp();
       }
       st = nst;
       ph = nph;
     }
     // every product has ended before the CTA gives up its memory
-    tc_commit(&B.drain, lead);
+    if (elect_one()) tc_commit(&B.drain);
+    __syncwarp();
     const long long t0 = clock64();
     while (!mbar_try_wait(&B.drain, 0) && clock64() - t0 < kWaitCycles) {
     }
@@ -371,37 +410,52 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     // ------------------------------------------------------------ weighted scores
     if constexpr (!STATE_ONLY) {
       const int w = wid & 3;
-      const float sign = reverse ? 1.f : -1.f;
+      const float sign = reverse ? -1.f : 1.f;
+      const uint32_t diag = reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane);  // columns kept of the lane's row
       for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
         const int m = min(kTcC, len - first_token(c));
         if (!warp_wait(&B.full[st], ph) || !warp_wait(&B.s_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
         const float* G = dec_G(st);
-        const float2 gi = f2(-sign * G[row]), sg = f2(sign);  // exponent: sign * (G_j - G_i)
+        const float gi = G[row];
         const uint32_t sp = lanes + kTmS + (i & 1) * 128;
         // 32 columns at a time.  P's columns x .. x + 31 land on S's columns x / 2 .., always behind
-        // what is still to be read; blocks on the far side of the diagonal are zero
+        // what is still to be read; blocks on the far side of the diagonal are zero.  Off the diagonal
+        // e^{G_i - G_j} = e^{G_i - R} e^{R - G_j}, R the sum at the columns' border: one exponential a
+        // row, and the columns' factors from the loading warp
 #pragma unroll 1
         for (int x = 0; x < 4; ++x) {
           uint32_t p[16];
           if (reverse ? x >= w : x <= w) {
             float s[32];
             tmem_ld32(sp + x * 32, s);
-            tc_wait_ld();
+            if (x != w) {
+              const float2 rf = f2(ex2(sign * (gi - G[reverse ? x * 32 - 1 : x * 32 + 31])));
+              const float* cf = G + 2 * kTcC + (reverse ? x - 1 : x) * 32;
+              tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 gj = *reinterpret_cast<const float4*>(G + x * 32 + j);
-              const float2 d0 = fma2(sg, make_float2(gj.x, gj.y), gi), d1 = fma2(sg, make_float2(gj.z, gj.w), gi);
-              const float2 e0 = mul2(make_float2(s[j], s[j + 1]), make_float2(ex2_ordered(d0.x), ex2_ordered(d0.y)));
-              const float2 e1 = mul2(make_float2(s[j + 2], s[j + 3]), make_float2(ex2_ordered(d1.x), ex2_ordered(d1.y)));
-              s[j] = e0.x, s[j + 1] = e0.y, s[j + 2] = e1.x, s[j + 3] = e1.y;
-            }
-            if (x == w || m < kTcC) {  // the diagonal, or tokens behind the row's end
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int col = x * 32 + j;
-                s[j] = (reverse ? col >= row && col < m : col <= row) ? s[j] : 0.f;
+              for (int j = 0; j < 32; j += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(cf + j);
+                const float2 e0 = mul2(make_float2(s[j], s[j + 1]), mul2(rf, make_float2(f.x, f.y)));
+                const float2 e1 = mul2(make_float2(s[j + 2], s[j + 3]), mul2(rf, make_float2(f.z, f.w)));
+                s[j] = e0.x, s[j + 1] = e0.y, s[j + 2] = e1.x, s[j + 3] = e1.y;
               }
+            } else {
+              tc_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                const float4 gj = *reinterpret_cast<const float4*>(G + x * 32 + j);
+                const float g4[4] = {gj.x, gj.y, gj.z, gj.w};
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const float e = s[j + r] * ex2_ordered(sign * (gi - g4[r]));
+                  s[j + r] = diag & (1u << (j + r)) ? e : 0.f;
+                }
+              }
+            }
+            if (reverse && m < kTcC) {  // columns behind the row's end hold anything
+#pragma unroll
+              for (int j = 0; j < 32; ++j) s[j] = x * 32 + j < m ? s[j] : 0.f;
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j) p[j] = pack2<IT>(s[2 * j], s[2 * j + 1]);
@@ -457,85 +511,87 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
   } else if (wg == 2) {
     // ------------------------------------------------------------ outputs
     if constexpr (!STATE_ONLY) {
-      auto zero_row = [&](int t) {
-        const int64_t at = (int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0;
-        for (int j = 0; j < nv; ++j) {
-          if (A.o_f32) static_cast<float*>(A.o)[at + j] = 0.f;
-          else static_cast<IT*>(A.o)[at + j] = zero_v<IT>();
-        }
-        if (A.dot) A.dot[(((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen + t] = 0.f;
-      };
-      const bool vec = A.o_vec && nv == kTcN;
-      const int64_t o_at = (int64_t)b * A.ob + (int64_t)head * A.oh + n0;
+      const int w4 = wid & 3;
       const IT* p_at = A.dot ? static_cast<const IT*>(A.p) + (int64_t)b * A.pb + (int64_t)(head / A.rp) * A.ph + n0 : nullptr;
       float* dot_at = A.dot ? A.dot + (((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen : nullptr;
+      const float2 sc = f2(A.scale);
       for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
         const int t0 = first_token(c), m = min(kTcC, len - t0), t = t0 + row;
         if (!warp_wait(&B.full[st], ph)) break;
-        const float2 w = f2(A.scale * ex2(dec_G(st)[reverse ? kTcC + row : row])), sc = f2(A.scale);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B.empty[st]);
+        const float2 w = f2(A.scale * ex2(dec_G(st)[reverse ? kTcC + row : row]));
         const bool on = row < m;
-        const int64_t at = o_at + (int64_t)t * A.ol;
-        const IT* p = p_at + (int64_t)t * A.pl;
+        uint4 q[8];
+        if (dot_at) {
+          const IT* p = p_at + (int64_t)t * A.pl;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            q[j] = on && 8 * j < nv ? *reinterpret_cast<const uint4*>(p + 8 * j) : make_uint4(0, 0, 0, 0);
+        }
         if (!warp_wait(&B.o_full, i & 1)) break;
         tc_after();
+        // the chunk's Q (and K) have been used: their room takes the output tile, which TMA stores
+        unsigned char* out = smem + st * S::kStageBytes + row * 128;
         float2 dot = f2(0.f);
-#pragma unroll 1
-        for (int x = 0; x < 2; ++x) {
-          float o[32], oa[32];
-          tmem_ld32(lanes + kTmOi + x * 32, o);
-          tmem_ld32(lanes + kTmOa + x * 32, oa);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float o[16], oa[16];
+          tmem_ld16(lanes + kTmOi + x * 16, o);
+          tmem_ld16(lanes + kTmOa + x * 16, oa);
           tc_wait_ld();
-          if (x == 1) {
+          if (x == 3) {
             tc_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&B.o_empty);
           }
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
+          for (int j = 0; j < 16; j += 2) {
             const float2 r = fma2(w, make_float2(o[j], o[j + 1]), mul2(sc, make_float2(oa[j], oa[j + 1])));
-            o[j] = r.x, o[j + 1] = r.y;
+            o[j] = on ? r.x : 0.f, o[j + 1] = on ? r.y : 0.f;
           }
-          if (on && vec) {
-            if (A.o_f32) {
-              float4* dst = reinterpret_cast<float4*>(static_cast<float*>(A.o) + at + x * 32);
+          if (A.o_f32) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-            } else {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<IT*>(A.o) + at + x * 32);
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float4*>(out + (x >> 1) * kBox + ((((x & 1) * 4 + j) ^ (row & 7)) << 4)) =
+                  make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          } else {
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                dst[j] = make_uint4(pack2<IT>(o[8 * j], o[8 * j + 1]), pack2<IT>(o[8 * j + 2], o[8 * j + 3]),
-                                    pack2<IT>(o[8 * j + 4], o[8 * j + 5]), pack2<IT>(o[8 * j + 6], o[8 * j + 7]));
+            for (int j = 0; j < 2; ++j)
+              *reinterpret_cast<uint4*>(out + (((2 * x + j) ^ (row & 7)) << 4)) =
+                  make_uint4(pack2<IT>(o[8 * j], o[8 * j + 1]), pack2<IT>(o[8 * j + 2], o[8 * j + 3]),
+                             pack2<IT>(o[8 * j + 4], o[8 * j + 5]), pack2<IT>(o[8 * j + 6], o[8 * j + 7]));
+          }
+          if (dot_at) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t u[4] = {q[2 * x + j].x, q[2 * x + j].y, q[2 * x + j].z, q[2 * x + j].w};
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                dot = fma2(make_float2(o[8 * j + 2 * r], o[8 * j + 2 * r + 1]), unpack2<IT>(u[r]), dot);
             }
-            if (dot_at) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint4 q = *reinterpret_cast<const uint4*>(p + x * 32 + 8 * j);
-                const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  dot = fma2(make_float2(o[8 * j + 2 * r], o[8 * j + 2 * r + 1]), unpack2<IT>(u[r]), dot);
-              }
-            }
-          } else if (on) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (x * 32 + j < nv) {
-                if (A.o_f32) static_cast<float*>(A.o)[at + x * 32 + j] = o[j];
-                else static_cast<IT*>(A.o)[at + x * 32 + j] = from_f<IT>(o[j]);
-                if (dot_at) dot.x = fmaf(o[j], to_f<IT>(p[x * 32 + j]), dot.x);
-              }
           }
         }
-        if (on) {
-          if (dot_at) dot_at[t] = dot.x + dot.y;
-        } else if (t < K.seqlen) {
-          zero_row(t);
+        fence_async_smem();
+        __syncwarp();
+        if (elect_one()) {
+          if (t0 + w4 * 32 < K.seqlen) {
+            const uint32_t src = smem_u32(smem) + st * S::kStageBytes + w4 * 32 * 128;
+            tma_store_4d(&P.map[pass][3], src, n0, head, t0 + w4 * 32, b);
+            if (A.o_f32 && n0 + 32 < dv) tma_store_4d(&P.map[pass][3], src + kBox, n0 + 32, head, t0 + w4 * 32, b);
+            tma_store_read();
+          }
+          mbar_arrive(&B.empty[st]);
         }
+        __syncwarp();
+        if (dot_at && t < K.seqlen) dot_at[t] = on ? dot.x + dot.y : 0.f;
         if (++st == S::kStages) st = 0, ph ^= 1;
       }
+      auto zero_row = [&](int t) {
+        const int es = A.o_f32 ? 4 : 2;
+        char* o = static_cast<char*>(A.o) + ((int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0) * es;
+#pragma unroll 1
+        for (int j = 0; j < nv * es; j += 16) *reinterpret_cast<uint4*>(o + j) = make_uint4(0, 0, 0, 0);
+        if (dot_at) dot_at[t] = 0.f;
+      };
       for (int c = max(cn, c0); c < c1; ++c)  // chunks behind the row's end
         if (c * kTcC + row < K.seqlen) zero_row(c * kTcC + row);
     }
@@ -575,8 +631,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.h_full);
     };
-    if (!STATE_ONLY && cn > c0) publish();
     for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
+      if (!STATE_ONLY) {
+        if (i > 0 && !warp_wait(&B.h_empty, (i - 1) & 1)) break;
+        publish();
+      }
       if (!warp_wait(&B.full[st], ph)) break;
       const float d = *reinterpret_cast<volatile float*>(&B.total[st]);
       __syncwarp();
@@ -584,23 +643,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       if (!warp_wait(&B.l_full, i & 1)) break;
       tc_after();
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float l[32];
-        tmem_ld32(lanes + kTmL + x * 32, l);
+      for (int x = 0; x < 4; ++x) {
+        float l[16], lo[16];
+        tmem_ld16(lanes + kTmL + x * 16, l);
+        tmem_ld16(lanes + kTmL + kTcN + x * 16, lo);
         tc_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const float2 r = fma2(f2(d), make_float2(h[x * 32 + j], h[x * 32 + j + 1]), make_float2(l[j], l[j + 1]));
-          h[x * 32 + j] = r.x, h[x * 32 + j + 1] = r.y;
+        for (int j = 0; j < 16; j += 2) {
+          const float2 r = fma2(f2(d), make_float2(h[x * 16 + j], h[x * 16 + j + 1]),
+                                add2(make_float2(l[j], l[j + 1]), make_float2(lo[j], lo[j + 1])));
+          h[x * 16 + j] = r.x, h[x * 16 + j + 1] = r.y;
         }
       }
       tc_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.l_empty);
-      if (!STATE_ONLY && c + 1 < cn) {
-        if (!warp_wait(&B.h_empty, i & 1)) break;
-        publish();
-      }
       if (++st == S::kStages) st = 0, ph ^= 1;
     }
     if (on && !*reinterpret_cast<volatile int*>(&B.abort)) {
