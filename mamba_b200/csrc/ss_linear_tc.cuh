@@ -19,8 +19,8 @@
 //
 // What bounds it: a chunk moves 128 x (2 dk + 128) x 2 bytes through TMA; two value tiles of one head
 // run side by side, so keys and queries come from L2 the second time.
-// Roles (18 warps): 0-3 scores, 4-7 weighted values, 8-11 outputs, 12-15 state, 16 loads and decays,
-// 17 matrix instructions.  The only chain from chunk to chunk is H: L -> state warps -> Q H.
+// Roles (19 warps): 0-3 scores, 4-7 weighted values, 8-11 outputs, 12-15 state, 16 loads, 17 matrix
+// instructions, 18 decays.  The only chain from chunk to chunk is H: L -> state warps -> Q H.
 #pragma once
 #include "ss_linear.cuh"
 
@@ -28,7 +28,10 @@ namespace ssb {
 
 constexpr int kTcC = 128;   // tokens of a chunk
 constexpr int kTcN = 64;    // value columns of a CTA
-constexpr int kTcThreads = 18 * 32;
+// log decays below this are a reset: e^-128 times anything of 16 bits is zero in fp32, and sums that hold
+// it keep a score's digits (2^-16 of a step at the first reset, more only behind a dozen in one chunk)
+constexpr float kTcReset = -128.f;
+constexpr int kTcThreads = 19 * 32;
 constexpr uint32_t kBox = kTcC * 128;  // one TMA box: 128 rows of 128 bytes
 
 struct LinTcK {
@@ -262,48 +265,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
   const uint32_t lanes = tm + ((uint32_t)(wid & 3) << 21);  // this warp's 32 lanes
 
   if (wid == 16) {
-    // ------------------------------------------------------------ loads, decays
-    double seg_total = 0.0;
+    // ------------------------------------------------------------ loads
     const int hq = head / A.rq, hk = head / A.rk, hv = head / A.rv;
     const uint32_t base = smem_u32(smem);
-    constexpr bool bf = std::is_same<IT, __nv_bfloat16>::value;
-    float gn[4];  // 4 tokens a lane of the chunk after the one at hand: its loads are under way
-    float4 to_here, to_end, factor;
-    float total = 0.f;
-    auto load_decays = [&](int c) {
-      const int t = first_token(c) + 4 * lane;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) gn[r] = t + r < len ? lin_decay(K, b, t + r, head, bf) : 0.f;
-    };
-    auto sums = [&]() {  // inclusive, in 64 bits: a difference of two sums keeps its digits
-      const double s0 = (double)gn[0], s1 = s0 + (double)gn[1], s2 = s1 + (double)gn[2], s3 = s2 + (double)gn[3];
-      double x = s3;
-#pragma unroll 1
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      const double T = __shfl_sync(0xffffffffu, x, 31);
-      const double before = x - s3, after = T - before;
-      constexpr double l2e = 1.4426950408889634;
-      to_here = make_float4((float)((before + s0) * l2e), (float)((before + s1) * l2e), (float)((before + s2) * l2e),
-                            (float)((before + s3) * l2e));
-      to_end = make_float4((float)((after - s0) * l2e), (float)((after - s1) * l2e), (float)((after - s2) * l2e),
-                           (float)((after - s3) * l2e));
-      total = expf((float)T);
-      seg_total += T;
-      if (!STATE_ONLY) {
-        // factors of a block's 32 columns towards the block's border on the side of the rows that use them
-        const float f = __shfl_sync(0xffffffffu, to_here.w, reverse ? (lane & 24) - 1 : lane | 7);
-        const float sg = reverse ? 1.f : -1.f;
-        factor = make_float4(ex2(sg * (to_here.x - f)), ex2(sg * (to_here.y - f)), ex2(sg * (to_here.z - f)),
-                             ex2(sg * (to_here.w - f)));
-      }
-    };
-    if (c0 < cn) load_decays(c0);
-    for (int c = c0, i = 0, st = 0; c < cn; ++c, ++i, st = st + 1 == S::kStages ? 0 : st + 1) {
-      sums();
-      if (i >= S::kStages && !warp_wait(&B.empty[st], (uint32_t)(i / S::kStages - 1) & 1)) break;
+    for (int c = c0, i = 0, st = 0, ph = 1; c < cn; ++c, ++i) {
+      if (i >= S::kStages && !warp_wait(&B.empty[st], ph)) break;
       const int t0 = first_token(c);
       if (elect_one()) {
         const uint32_t dst = base + st * S::kStageBytes;
@@ -315,16 +281,68 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         }
         tma_load_4d(dst + 2 * S::kBoxes * kBox, &P.map[pass][2], n0, hv, t0, b, &B.full[st]);
       }
-      *reinterpret_cast<float4*>(dec_G(st) + 4 * lane) = to_here;
-      *reinterpret_cast<float4*>(dec_G(st) + kTcC + 4 * lane) = to_end;
-      if (!STATE_ONLY) {  // blocks 0 - 2, reverse 1 - 3: the far block has no rows beyond it
-        const int l = reverse ? lane - 8 : lane;
-        if (l >= 0 && l < 24) *reinterpret_cast<float4*>(dec_G(st) + 2 * kTcC + 4 * l) = factor;
+      __syncwarp();
+      if (++st == S::kStages) st = 0, ph ^= 1;
+    }
+  } else if (wid == 18) {
+    // ------------------------------------------------------------ decays
+    constexpr bool bf = std::is_same<IT, __nv_bfloat16>::value;
+    uint32_t raw[4];  // 4 tokens a lane of the next chunk, as they are in memory: the loads are under way
+    const int64_t g0 = (int64_t)b * K.gb + (int64_t)head * K.gh;
+    auto load = [&](int c) {
+      const int t = first_token(c) + 4 * lane;
+      const int64_t at = g0 + (int64_t)t * K.gl;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        raw[r] = 0u;
+        if (t + r < len)
+          raw[r] = K.g_f32 ? static_cast<const uint32_t*>(K.g)[at + r * K.gl]
+                           : (uint32_t)static_cast<const unsigned short*>(K.g)[at + r * K.gl];
       }
-      if (lane == 0) B.total[st] = total;
+    };
+    double seg_total = 0.0;
+    if (c0 < cn) load(c0);
+    for (int c = c0, i = 0, st = 0, ph = 1; c < cn; ++c, ++i) {
+      float g[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (K.g_f32) g[r] = __uint_as_float(raw[r]);
+        else if (bf) g[r] = __uint_as_float(raw[r] << 16);
+        else g[r] = __half2float(__ushort_as_half((unsigned short)raw[r]));
+        g[r] = g[r] < kTcReset ? kTcReset : g[r];  // keeps NaN
+      }
+      if (c + 1 < cn) load(c + 1);
+      // inclusive sums, in 64 bits: a difference of two sums keeps its digits
+      const double s0 = (double)g[0], s1 = s0 + (double)g[1], s2 = s1 + (double)g[2], s3 = s2 + (double)g[3];
+      double x = s3;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const double T = __shfl_sync(0xffffffffu, x, 31);
+      const double before = x - s3, after = T - before;
+      constexpr double l2e = 1.4426950408889634;
+      const float4 to_here = make_float4((float)((before + s0) * l2e), (float)((before + s1) * l2e),
+                                         (float)((before + s2) * l2e), (float)((before + s3) * l2e));
+      const float4 to_end = make_float4((float)((after - s0) * l2e), (float)((after - s1) * l2e),
+                                        (float)((after - s2) * l2e), (float)((after - s3) * l2e));
+      // factors of a block's 32 columns towards the block's border on the side of the rows that use them
+      const float f = __shfl_sync(0xffffffffu, to_here.w, reverse ? (lane & 24) - 1 : lane | 7);
+      const float sg = reverse ? 1.f : -1.f;
+      const float4 factor = make_float4(ex2(sg * (to_here.x - f)), ex2(sg * (to_here.y - f)),
+                                        ex2(sg * (to_here.z - f)), ex2(sg * (to_here.w - f)));
+      seg_total += T;
+      if (i >= S::kStages && !warp_wait(&B.empty[st], ph)) break;
+      float* G = dec_G(st);
+      *reinterpret_cast<float4*>(G + 4 * lane) = to_here;
+      *reinterpret_cast<float4*>(G + kTcC + 4 * lane) = to_end;
+      const int l = reverse ? lane - 8 : lane;  // blocks 0 - 2, reverse 1 - 3: the far block has no rows beyond it
+      if (!STATE_ONLY && l >= 0 && l < 24) *reinterpret_cast<float4*>(G + 2 * kTcC + 4 * l) = factor;
+      if (lane == 0) B.total[st] = ex2((float)(T * l2e));
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.full[st]);
-      if (c + 1 < cn) load_decays(c + 1);
+      if (++st == S::kStages) st = 0, ph ^= 1;
     }
     if (STATE_ONLY && tile == 0 && lane == 0)
       K.seg_decay[((int64_t)reverse * K.batch * K.heads + bh) * K.segs + seg] = (float)seg_total;
@@ -366,12 +384,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       __syncwarp();
       const int nst = st + 1 == S::kStages ? 0 : st + 1, nph = nst ? ph : ph ^ 1;
       if constexpr (!STATE_ONLY) {
-        // the next chunk's scores, into the buffer whose weighted scores were used a chunk ago
-        if (i + 1 < n) {
-          if (!warp_wait(&B.full[nst], nph) || (i > 0 && !warp_wait(&B.o_full, (i - 1) & 1))) break;
-          tc_after();
-          scores(nst, (i + 1) & 1);
-        }
         // Oi = Q H
         if (!warp_wait(&B.h_full, i & 1) || (i > 0 && !warp_wait(&B.o_empty, (i - 1) & 1))) break;
         tc_after();
@@ -384,6 +396,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
           tc_commit(&B.h_empty);
         }
         __syncwarp();
+        // the next chunk's scores, into the buffer whose weighted scores were used a chunk ago (o_empty says
+        // so): now if the chunk is here, else after this chunk's last product, which must not wait for it
+        bool ahead = i + 1 < n && __all_sync(0xffffffffu, mbar_test_wait(&B.full[nst], nph));
+        if (ahead) {
+          tc_after();
+          scores(nst, (i + 1) & 1);
+        }
         // Oa = P V
         if (!warp_wait(&B.p_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
@@ -395,6 +414,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
           tc_commit(&B.empty[st]);
         }
         __syncwarp();
+        if (!ahead && i + 1 < n) {
+          if (!warp_wait(&B.full[nst], nph)) break;
+          tc_after();
+          scores(nst, (i + 1) & 1);
+        }
       }
       st = nst;
       ph = nph;
