@@ -149,8 +149,8 @@ __device__ __forceinline__ void store_split(unsigned char* hi, unsigned char* lo
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     h[i] = pack2<IT>(v[2 * i], v[2 * i + 1]);
-    const float2 b = unpack2<IT>(h[i]);
-    l[i] = pack2<IT>(v[2 * i] - b.x, v[2 * i + 1] - b.y);
+    const float2 d = fma2(unpack2<IT>(h[i]), f2(-1.f), make_float2(v[2 * i], v[2 * i + 1]));
+    l[i] = pack2<IT>(d.x, d.y);
   }
   const int at = r * 128 + ((j ^ (r & 7)) << 4);
   *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
@@ -168,7 +168,11 @@ struct TcShape {
   static constexpr uint32_t kDecStage = (2 * kTcC + 96) * 4;
   static constexpr uint32_t kDec = kH + 2 * DK * 128;
   static constexpr uint32_t kBars = kDec + kStages * kDecStage;
-  static constexpr uint32_t kBytes = kBars + 256;
+  // the output tile on its way to the TMA store: room of its own where there is some, so that the
+  // stage is free for the next load as soon as its products have ended; else the chunk's Q
+  static constexpr bool kOwnOut = DK == 64;
+  static constexpr uint32_t kOut = (kBars + 256 + 1023) / 1024 * 1024;
+  static constexpr uint32_t kBytes = kOwnOut ? kOut + kBox : kBars + 256;
 };
 
 struct TcBars {
@@ -358,10 +362,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     auto scores = [&](int st, int buf) {
       const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4));
       if (elect_one()) {
-#pragma unroll
-        for (int x = 0; x < S::kBoxes * 4; ++x)
-          mma_ss(tm + kTmS + buf * 128, q0 + o + (x >> 2) * (kBox >> 4) + (x & 3) * 2,
-                 kk0 + o + (x >> 2) * (kBox >> 4) + (x & 3) * 2, kIdQK, x > 0);
+        for (int x = 0; x < S::kBoxes; ++x)
+#pragma unroll 1
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t at = o + x * (kBox >> 4) + k * 2;
+            mma_ss(tm + kTmS + buf * 128, q0 + at, kk0 + at, kIdQK, x + k > 0);
+          }
         tc_commit(&B.s_full[buf]);
       }
       __syncwarp();
@@ -376,7 +382,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       tc_after();
       const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4));
       if (elect_one()) {
-#pragma unroll
+#pragma unroll 1
         for (int x = 0; x < kTcC / 16; ++x) mma_ss(tm + kTmL, km0 + o + x * 128, vp0 + x * 128, kIdL, x > 0);
         tc_commit(&B.l_full);
         if (STATE_ONLY) tc_commit(&B.empty[st]);
@@ -388,7 +394,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         if (!warp_wait(&B.h_full, i & 1) || (i > 0 && !warp_wait(&B.o_empty, (i - 1) & 1))) break;
         tc_after();
         if (elect_one()) {
-#pragma unroll
+#pragma unroll 1
           for (int x = 0; x < 2 * DK / 16; ++x) {
             const int k = x % (DK / 16);
             mma_ss(tm + kTmOi, q0 + o + (k >> 2) * (kBox >> 4) + (k & 3) * 2, h0 + x * 128, kIdN, x > 0);
@@ -407,7 +413,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         if (!warp_wait(&B.p_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
         if (elect_one()) {
-#pragma unroll
+#pragma unroll 1
           for (int x = 0; x < kTcC / 16; ++x)
             mma_ts(tm + kTmOa, tm + kTmS + (i & 1) * 128 + x * 8, v0 + o + x * 128, kIdN, x > 0);
           tc_commit(&B.o_full);
@@ -514,7 +520,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       __syncwarp();
       const float2 w = f2(ex2(dec_G(st)[reverse ? row : kTcC + row]));
       if (i > 0 && !warp_wait(&B.l_full, (i - 1) & 1)) break;  // the product over the buffer has ended
-#pragma unroll 2
+#pragma unroll 1
       for (int j = 0; j < 8; ++j) {
         const uint4 q = *reinterpret_cast<const uint4*>(v + ((j ^ (row & 7)) << 4));
         const uint32_t u[4] = {q.x, q.y, q.z, q.w};
@@ -536,6 +542,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     // ------------------------------------------------------------ outputs
     if constexpr (!STATE_ONLY) {
       const int w4 = wid & 3;
+      const bool own_out = S::kOwnOut && !A.o_f32;  // fp32 tiles take Q's and K's room, 32 KB
       const IT* p_at = A.dot ? static_cast<const IT*>(A.p) + (int64_t)b * A.pb + (int64_t)(head / A.rp) * A.ph + n0 : nullptr;
       float* dot_at = A.dot ? A.dot + (((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen : nullptr;
       const float2 sc = f2(A.scale);
@@ -544,29 +551,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         if (!warp_wait(&B.full[st], ph)) break;
         const float2 w = f2(A.scale * ex2(dec_G(st)[reverse ? kTcC + row : row]));
         const bool on = row < m;
-        uint4 q[8];
-        if (dot_at) {
-          const IT* p = p_at + (int64_t)t * A.pl;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            q[j] = on && 8 * j < nv ? *reinterpret_cast<const uint4*>(p + 8 * j) : make_uint4(0, 0, 0, 0);
+        if (own_out) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B.empty[st]);
         }
+        // 16 columns at a time, the next ones of p under way
+        const IT* p = p_at + (int64_t)t * A.pl;
+        uint4 q0 = make_uint4(0, 0, 0, 0), q1 = q0;
+        auto load_p = [&](int x) {
+          q0 = on && 16 * x < nv ? *reinterpret_cast<const uint4*>(p + 16 * x) : make_uint4(0, 0, 0, 0);
+          q1 = on && 16 * x + 8 < nv ? *reinterpret_cast<const uint4*>(p + 16 * x + 8) : make_uint4(0, 0, 0, 0);
+        };
+        if (dot_at) load_p(0);
         if (!warp_wait(&B.o_full, i & 1)) break;
         tc_after();
-        // the chunk's Q (and K) have been used: their room takes the output tile, which TMA stores
-        unsigned char* out = smem + st * S::kStageBytes + row * 128;
+        if (elect_one()) tma_store_read();  // the tile before has left
+        __syncwarp();
+        const uint32_t tile_at = own_out ? S::kOut : st * S::kStageBytes;
+        unsigned char* out = smem + tile_at + row * 128;
         float2 dot = f2(0.f);
-#pragma unroll
+#pragma unroll 1
         for (int x = 0; x < 4; ++x) {
           float o[16], oa[16];
           tmem_ld16(lanes + kTmOi + x * 16, o);
           tmem_ld16(lanes + kTmOa + x * 16, oa);
+          const uint32_t u[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+          if (dot_at && x < 3) load_p(x + 1);
           tc_wait_ld();
-          if (x == 3) {
-            tc_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&B.o_empty);
-          }
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
             const float2 r = fma2(w, make_float2(o[j], o[j + 1]), mul2(sc, make_float2(oa[j], oa[j + 1])));
@@ -586,29 +597,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
           }
           if (dot_at) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t u[4] = {q[2 * x + j].x, q[2 * x + j].y, q[2 * x + j].z, q[2 * x + j].w};
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                dot = fma2(make_float2(o[8 * j + 2 * r], o[8 * j + 2 * r + 1]), unpack2<IT>(u[r]), dot);
-            }
+            for (int j = 0; j < 8; ++j) dot = fma2(make_float2(o[2 * j], o[2 * j + 1]), unpack2<IT>(u[j]), dot);
           }
         }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.o_empty);
         fence_async_smem();
         __syncwarp();
         if (elect_one()) {
           if (t0 + w4 * 32 < K.seqlen) {
-            const uint32_t src = smem_u32(smem) + st * S::kStageBytes + w4 * 32 * 128;
+            const uint32_t src = smem_u32(smem) + tile_at + w4 * 32 * 128;
             tma_store_4d(&P.map[pass][3], src, n0, head, t0 + w4 * 32, b);
             if (A.o_f32 && n0 + 32 < dv) tma_store_4d(&P.map[pass][3], src + kBox, n0 + 32, head, t0 + w4 * 32, b);
-            tma_store_read();
           }
-          mbar_arrive(&B.empty[st]);
+          if (!own_out) {
+            tma_store_read();
+            mbar_arrive(&B.empty[st]);
+          }
         }
         __syncwarp();
         if (dot_at && t < K.seqlen) dot_at[t] = on ? dot.x + dot.y : 0.f;
         if (++st == S::kStages) st = 0, ph ^= 1;
       }
+      if (elect_one()) tma_store_read();
+      __syncwarp();
       auto zero_row = [&](int t) {
         const int es = A.o_f32 ? 4 : 2;
         char* o = static_cast<char*>(A.o) + ((int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0) * es;
