@@ -157,29 +157,30 @@ __device__ __forceinline__ void store_split(unsigned char* hi, unsigned char* lo
   *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
+// Shared memory: stages of Q, K, V as TMA writes them; buffers of V' (hi, lo); H (hi, lo); per stage the
+// decays: X of every token and the column factors of three blocks; barriers.  Narrow heads have room for
+// three stages and for V' of the next chunk.  The output tile takes the room of its chunk's V on its
+// way to the TMA store (V is needed later in the stage's next chunk than Q and K are).
 template <int DK>
 struct TcShape {
   static constexpr int kBoxes = DK / 64;
   static constexpr int kStages = DK == 128 ? 2 : 3;
-  static constexpr uint32_t kStageBytes = (2 * kBoxes + 1) * kBox;  // Q, K, V
-  static constexpr uint32_t kVp = kStages * kStageBytes;            // V' hi, lo
-  static constexpr uint32_t kH = kVp + 2 * kBox;                    // H hi, lo
-  // per stage: G and T - G (times log2 e) of every token, and the column factors of three blocks
-  static constexpr uint32_t kDecStage = (2 * kTcC + 96) * 4;
+  static constexpr int kVps = DK == 128 ? 1 : 2;
+  static constexpr uint32_t kStageBytes = (2 * kBoxes + 1) * kBox;
+  static constexpr uint32_t kVAt = 2 * kBoxes * kBox;
+  static constexpr uint32_t kVp = kStages * kStageBytes;
+  static constexpr uint32_t kH = kVp + kVps * 2 * kBox;
+  static constexpr uint32_t kDecStage = (kTcC + 96) * 4;
   static constexpr uint32_t kDec = kH + 2 * DK * 128;
   static constexpr uint32_t kBars = kDec + kStages * kDecStage;
-  // the output tile on its way to the TMA store: room of its own where there is some, so that the
-  // stage is free for the next load as soon as its products have ended; else the chunk's Q
-  static constexpr bool kOwnOut = DK == 64;
-  static constexpr uint32_t kOut = (kBars + 256 + 1023) / 1024 * 1024;
-  static constexpr uint32_t kBytes = kOwnOut ? kOut + kBox : kBars + 256;
+  static constexpr uint32_t kBytes = kBars + 256;
 };
 
 struct TcBars {
-  uint64_t full[3], empty[3];
+  uint64_t full[3], empty[3], v_empty[3];
   uint64_t s_full[2], p_full[2];
-  uint64_t vp_full, l_full, l_empty, h_full, h_empty, o_full, o_empty, drain;
-  float total[3];  // e^T of the stage's chunk
+  uint64_t vp_full[2], vp_empty[2], l_full, l_empty, h_full, h_empty, o_full, o_empty, drain;
+  float total[3], total2[3];  // e^T of the stage's chunk, T log2 e
   uint32_t tmem;
   int abort;
 };
@@ -200,10 +201,24 @@ __device__ __forceinline__ bool mbar_try_wait_long(uint64_t* bar, uint32_t parit
   return ok != 0;
 }
 
+// a few tens of tries in a loop of four instructions: what a waiting warp issues, the others cannot
+__device__ __forceinline__ bool mbar_try_wait_often(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 0;\n"
+      "again:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n @p bra over;\n add.u32 n, n, 1;\n"
+      " setp.lt.u32 q, n, 64;\n @q bra again;\n"
+      "over:\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+
 // the part of a wait that is not over at once; false: it gave up, here or in another role
 __device__ __noinline__ bool tc_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, long long limit, int* status) {
   const long long t0 = clock64();
-  while (!mbar_try_wait_long(bar, parity)) {
+  while (!mbar_try_wait_often(bar, parity)) {
     if (*abort) return false;
     if (clock64() - t0 > limit) {
       *abort = 1;
@@ -235,7 +250,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
   const bool reverse = A.reverse != 0;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, wg = wid >> 2, row = tid & 127;
   auto first_token = [&](int c) { return (reverse ? n_live - 1 - c : c) * kTcC; };
-  auto dec_G = [&](int st) { return reinterpret_cast<float*>(smem + S::kDec + st * S::kDecStage); };
+  auto dec_X = [&](int st) { return reinterpret_cast<float*>(smem + S::kDec + st * S::kDecStage); };
   const int64_t block = (int64_t)dk * dv;
   // for whole warps: the lanes go on, or give up, together
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
@@ -247,9 +262,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&B.full[i], 2);                          // the copies, the decays
       mbar_init(&B.empty[i], STATE_ONLY ? 1 + 4 : 1 + 8);  // the products, the warps that read the decays last
+      mbar_init(&B.v_empty[i], STATE_ONLY ? 1 : 1 + 4);    // the products, the output tile that takes V's room
     }
     for (int i = 0; i < 2; ++i) mbar_init(&B.s_full[i], 1), mbar_init(&B.p_full[i], 4);
-    mbar_init(&B.vp_full, 4);
+    for (int i = 0; i < 2; ++i) mbar_init(&B.vp_full[i], 4), mbar_init(&B.vp_empty[i], 1);
     mbar_init(&B.l_full, 1), mbar_init(&B.l_empty, 4);
     mbar_init(&B.h_full, 4), mbar_init(&B.h_empty, 1);
     mbar_init(&B.o_full, 1), mbar_init(&B.o_empty, 4);
@@ -283,8 +299,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
           if (!STATE_ONLY) tma_load_4d(dst + x * kBox, &P.map[pass][0], x * 64, hq, t0, b, &B.full[st]);
           tma_load_4d(dst + (S::kBoxes + x) * kBox, &P.map[pass][1], x * 64, hk, t0, b, &B.full[st]);
         }
-        tma_load_4d(dst + 2 * S::kBoxes * kBox, &P.map[pass][2], n0, hv, t0, b, &B.full[st]);
       }
+      __syncwarp();
+      if (i >= S::kStages && !warp_wait(&B.v_empty[st], ph)) break;
+      if (elect_one())
+        tma_load_4d(base + st * S::kStageBytes + S::kVAt, &P.map[pass][2], n0, hv, t0, b, &B.full[st]);
       __syncwarp();
       if (++st == S::kStages) st = 0, ph ^= 1;
     }
@@ -327,23 +346,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       const double T = __shfl_sync(0xffffffffu, x, 31);
       const double before = x - s3, after = T - before;
       constexpr double l2e = 1.4426950408889634;
-      const float4 to_here = make_float4((float)((before + s0) * l2e), (float)((before + s1) * l2e),
-                                         (float)((before + s2) * l2e), (float)((before + s3) * l2e));
-      const float4 to_end = make_float4((float)((after - s0) * l2e), (float)((after - s1) * l2e),
-                                        (float)((after - s2) * l2e), (float)((after - s3) * l2e));
+      // X: what a token's update is weighted with (forward T - G, reverse G, times log2 e).  The decay
+      // between a row's and a column's token is e^{X_col - X_row} either way, the output's weight e^{T - X}
+      const double y0 = reverse ? before : after, ys = reverse ? l2e : -l2e, yb = y0 * l2e;
+      const float4 X = make_float4((float)fma(ys, s0, yb), (float)fma(ys, s1, yb), (float)fma(ys, s2, yb),
+                                   (float)fma(ys, s3, yb));
       // factors of a block's 32 columns towards the block's border on the side of the rows that use them
-      const float f = __shfl_sync(0xffffffffu, to_here.w, reverse ? (lane & 24) - 1 : lane | 7);
-      const float sg = reverse ? 1.f : -1.f;
-      const float4 factor = make_float4(ex2(sg * (to_here.x - f)), ex2(sg * (to_here.y - f)),
-                                        ex2(sg * (to_here.z - f)), ex2(sg * (to_here.w - f)));
+      const float f = __shfl_sync(0xffffffffu, X.w, reverse ? (lane & 24) - 1 : lane | 7);
+      const float4 factor = make_float4(ex2(X.x - f), ex2(X.y - f), ex2(X.z - f), ex2(X.w - f));
       seg_total += T;
       if (i >= S::kStages && !warp_wait(&B.empty[st], ph)) break;
-      float* G = dec_G(st);
-      *reinterpret_cast<float4*>(G + 4 * lane) = to_here;
-      *reinterpret_cast<float4*>(G + kTcC + 4 * lane) = to_end;
+      float* xs = dec_X(st);
+      *reinterpret_cast<float4*>(xs + 4 * lane) = X;
       const int l = reverse ? lane - 8 : lane;  // blocks 0 - 2, reverse 1 - 3: the far block has no rows beyond it
-      if (!STATE_ONLY && l >= 0 && l < 24) *reinterpret_cast<float4*>(G + 2 * kTcC + 4 * l) = factor;
-      if (lane == 0) B.total[st] = ex2((float)(T * l2e));
+      if (!STATE_ONLY && l >= 0 && l < 24) *reinterpret_cast<float4*>(xs + kTcC + 4 * l) = factor;
+      if (lane == 0) B.total2[st] = (float)(T * l2e), B.total[st] = ex2((float)(T * l2e));
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.full[st]);
       if (++st == S::kStages) st = 0, ph ^= 1;
@@ -357,7 +374,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
                        kIdL = idesc_of<IT>(128, 2 * kTcN, true, true);
     // descriptors of the first stage; a step of 16 along K is 32 bytes (K-major) or 2048 (MN-major)
     const uint64_t q0 = desc_of(base, 16), kk0 = desc_of(base + S::kBoxes * kBox, 16),
-                   km0 = desc_of(base + S::kBoxes * kBox, kBox), v0 = desc_of(base + 2 * S::kBoxes * kBox, kBox),
+                   km0 = desc_of(base + S::kBoxes * kBox, kBox), v0 = desc_of(base + S::kVAt, kBox),
                    vp0 = desc_of(base + S::kVp, kBox), h0 = desc_of(base + S::kH, kBox);
     auto scores = [&](int st, int buf) {
       const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4));
@@ -378,14 +395,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       tc_after();
       if (!STATE_ONLY && i == 0) scores(0, 0);
       // L = K^T [V'hi, V'lo]: a product of 64 columns takes as long as one of 128
-      if (!warp_wait(&B.vp_full, i & 1) || (i > 0 && !warp_wait(&B.l_empty, (i - 1) & 1))) break;
+      if (!warp_wait(&B.vp_full[S::kVps == 2 ? i & 1 : 0], (uint32_t)(i / S::kVps) & 1) || (i > 0 && !warp_wait(&B.l_empty, (i - 1) & 1))) break;
       tc_after();
-      const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4));
+      const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4)), vp = vp0 + (S::kVps == 2 ? (i & 1) * 2 * (kBox >> 4) : 0);
       if (elect_one()) {
 #pragma unroll 1
-        for (int x = 0; x < kTcC / 16; ++x) mma_ss(tm + kTmL, km0 + o + x * 128, vp0 + x * 128, kIdL, x > 0);
+        for (int x = 0; x < kTcC / 16; ++x) mma_ss(tm + kTmL, km0 + o + x * 128, vp + x * 128, kIdL, x > 0);
         tc_commit(&B.l_full);
-        if (STATE_ONLY) tc_commit(&B.empty[st]);
+        tc_commit(&B.vp_empty[S::kVps == 2 ? i & 1 : 0]);
+        if (STATE_ONLY) tc_commit(&B.empty[st]), tc_commit(&B.v_empty[st]);
       }
       __syncwarp();
       const int nst = st + 1 == S::kStages ? 0 : st + 1, nph = nst ? ph : ph ^ 1;
@@ -418,6 +436,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
             mma_ts(tm + kTmOa, tm + kTmS + (i & 1) * 128 + x * 8, v0 + o + x * 128, kIdN, x > 0);
           tc_commit(&B.o_full);
           tc_commit(&B.empty[st]);
+          tc_commit(&B.v_empty[st]);
         }
         __syncwarp();
         if (!ahead && i + 1 < n) {
@@ -440,18 +459,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     // ------------------------------------------------------------ weighted scores
     if constexpr (!STATE_ONLY) {
       const int w = wid & 3;
-      const float sign = reverse ? -1.f : 1.f;
       const uint32_t diag = reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane);  // columns kept of the lane's row
       for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
         const int m = min(kTcC, len - first_token(c));
         if (!warp_wait(&B.full[st], ph) || !warp_wait(&B.s_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
-        const float* G = dec_G(st);
-        const float gi = G[row];
+        const float* X = dec_X(st);
+        const float xi = X[row];
         const uint32_t sp = lanes + kTmS + (i & 1) * 128;
         // 32 columns at a time.  P's columns x .. x + 31 land on S's columns x / 2 .., always behind
         // what is still to be read; blocks on the far side of the diagonal are zero.  Off the diagonal
-        // e^{G_i - G_j} = e^{G_i - R} e^{R - G_j}, R the sum at the columns' border: one exponential a
+        // e^{X_j - X_i} = e^{R - X_i} e^{X_j - R}, R the value at the columns' border: one exponential a
         // row, and the columns' factors from the loading warp
 #pragma unroll 1
         for (int x = 0; x < 4; ++x) {
@@ -460,8 +478,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
             float s[32];
             tmem_ld32(sp + x * 32, s);
             if (x != w) {
-              const float2 rf = f2(ex2(sign * (gi - G[reverse ? x * 32 - 1 : x * 32 + 31])));
-              const float* cf = G + 2 * kTcC + (reverse ? x - 1 : x) * 32;
+              const float2 rf = f2(ex2(X[reverse ? x * 32 - 1 : x * 32 + 31] - xi));
+              const float* cf = X + kTcC + (reverse ? x - 1 : x) * 32;
               tc_wait_ld();
 #pragma unroll
               for (int j = 0; j < 32; j += 4) {
@@ -474,11 +492,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
               tc_wait_ld();
 #pragma unroll
               for (int j = 0; j < 32; j += 4) {
-                const float4 gj = *reinterpret_cast<const float4*>(G + x * 32 + j);
-                const float g4[4] = {gj.x, gj.y, gj.z, gj.w};
+                const float4 xj = *reinterpret_cast<const float4*>(X + x * 32 + j);
+                const float x4[4] = {xj.x, xj.y, xj.z, xj.w};
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                  const float e = s[j + r] * ex2_ordered(sign * (gi - g4[r]));
+                  const float e = s[j + r] * ex2_ordered(x4[r] - xi);
                   s[j + r] = diag & (1u << (j + r)) ? e : 0.f;
                 }
               }
@@ -508,7 +526,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       const int m = min(kTcC, len - first_token(c));
       if (!warp_wait(&B.full[st], ph)) break;
       unsigned char* k = smem + st * S::kStageBytes + S::kBoxes * kBox + row * 128;
-      unsigned char* v = smem + st * S::kStageBytes + 2 * S::kBoxes * kBox + row * 128;
+      unsigned char* v = smem + st * S::kStageBytes + S::kVAt + row * 128;
       if (row >= m) {  // behind the row's end: whatever was read there must not meet a product
 #pragma unroll 1
         for (int j = 0; j < 8; ++j) {
@@ -518,9 +536,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         }
       }
       __syncwarp();
-      const float2 w = f2(ex2(dec_G(st)[reverse ? row : kTcC + row]));
-      if (i > 0 && !warp_wait(&B.l_full, (i - 1) & 1)) break;  // the product over the buffer has ended
-#pragma unroll 1
+      const float2 w = f2(ex2(dec_X(st)[row]));
+      // the product over the buffer has ended
+      if (i >= S::kVps && !warp_wait(&B.vp_empty[S::kVps == 2 ? i & 1 : 0], (uint32_t)(i / S::kVps - 1) & 1)) break;
+      unsigned char* vp = smem + S::kVp + (S::kVps == 2 ? (i & 1) * 2 * kBox : 0);
+#pragma unroll 2
       for (int j = 0; j < 8; ++j) {
         const uint4 q = *reinterpret_cast<const uint4*>(v + ((j ^ (row & 7)) << 4));
         const uint32_t u[4] = {q.x, q.y, q.z, q.w};
@@ -531,30 +551,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
           x[2 * r] = f.x;
           x[2 * r + 1] = f.y;
         }
-        store_split<IT>(smem + S::kVp, smem + S::kVp + kBox, row, j, x);
+        store_split<IT>(vp, vp + kBox, row, j, x);
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&B.vp_full);
+      if (lane == 0) mbar_arrive(&B.vp_full[S::kVps == 2 ? i & 1 : 0]);
       if (++st == S::kStages) st = 0, ph ^= 1;
     }
   } else if (wg == 2) {
     // ------------------------------------------------------------ outputs
     if constexpr (!STATE_ONLY) {
       const int w4 = wid & 3;
-      const bool own_out = S::kOwnOut && !A.o_f32;  // fp32 tiles take Q's and K's room, 32 KB
+      const uint32_t tile0 = A.o_f32 ? 0 : S::kVAt;  // fp32 tiles, twice as large, take Q's and K's room
       const IT* p_at = A.dot ? static_cast<const IT*>(A.p) + (int64_t)b * A.pb + (int64_t)(head / A.rp) * A.ph + n0 : nullptr;
       float* dot_at = A.dot ? A.dot + (((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen : nullptr;
       const float2 sc = f2(A.scale);
       for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
         const int t0 = first_token(c), m = min(kTcC, len - t0), t = t0 + row;
         if (!warp_wait(&B.full[st], ph)) break;
-        const float2 w = f2(A.scale * ex2(dec_G(st)[reverse ? kTcC + row : row]));
+        const float2 w = f2(A.scale * ex2(*reinterpret_cast<volatile float*>(&B.total2[st]) - dec_X(st)[row]));
         const bool on = row < m;
-        if (own_out) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&B.empty[st]);
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(A.o_f32 ? &B.v_empty[st] : &B.empty[st]);
         // 16 columns at a time, the next ones of p under way
         const IT* p = p_at + (int64_t)t * A.pl;
         uint4 q0 = make_uint4(0, 0, 0, 0), q1 = q0;
@@ -565,9 +583,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         if (dot_at) load_p(0);
         if (!warp_wait(&B.o_full, i & 1)) break;
         tc_after();
-        if (elect_one()) tma_store_read();  // the tile before has left
-        __syncwarp();
-        const uint32_t tile_at = own_out ? S::kOut : st * S::kStageBytes;
+        const uint32_t tile_at = tile0 + st * S::kStageBytes;
         unsigned char* out = smem + tile_at + row * 128;
         float2 dot = f2(0.f);
 #pragma unroll 1
@@ -611,17 +627,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
             tma_store_4d(&P.map[pass][3], src, n0, head, t0 + w4 * 32, b);
             if (A.o_f32 && n0 + 32 < dv) tma_store_4d(&P.map[pass][3], src + kBox, n0 + 32, head, t0 + w4 * 32, b);
           }
-          if (!own_out) {
-            tma_store_read();
-            mbar_arrive(&B.empty[st]);
-          }
+          tma_store_read();
+          mbar_arrive(A.o_f32 ? &B.empty[st] : &B.v_empty[st]);
         }
         __syncwarp();
         if (dot_at && t < K.seqlen) dot_at[t] = on ? dot.x + dot.y : 0.f;
         if (++st == S::kStages) st = 0, ph ^= 1;
       }
-      if (elect_one()) tma_store_read();
-      __syncwarp();
       auto zero_row = [&](int t) {
         const int es = A.o_f32 ? 4 : 2;
         char* o = static_cast<char*>(A.o) + ((int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0) * es;
@@ -634,25 +646,49 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     }
   } else {
     // ------------------------------------------------------------ state: row `row` of H
-    const bool on = row < dk;
+    // Rows enter and leave the registers through the room of the 16-bit halves (256 bytes a row), each
+    // warp its own: short loops, and a warp's lanes side by side along a row in memory
     float h[kTcN];
+    float* rows = reinterpret_cast<float*>(smem + S::kH) + (wid & 3) * 32 * kTcN;
+    const int r0 = (wid & 3) * 32, rn = min(32, dk - r0);  // this warp's rows; <= 0: none
+    if (r0 < DK) {
+      // 8 loads under way at a time; one segment after the other
+      auto each = [&](auto&& f) {
+#pragma unroll 1
+        for (int e0 = lane; e0 < 32 * kTcN; e0 += 8 * 32) {
+          float x[8];
 #pragma unroll
-    for (int j = 0; j < kTcN; ++j) h[j] = 0.f;
-    if (!STATE_ONLY && on) {
-      if (A.s_in) {
-        const float* s = A.s_in + bh * block + (int64_t)row * A.s_row + (int64_t)n0 * A.s_col;
+          for (int u = 0; u < 8; ++u) {
+            const int e = e0 + 32 * u, r = e / kTcN, j = e % kTcN;
+            x[u] = r < rn && j < nv ? f(r, j) : 0.f;
+          }
 #pragma unroll
-        for (int j = 0; j < kTcN; ++j)
-          if (j < nv) h[j] = A.s_in_scale * s[(int64_t)j * A.s_col];
+          for (int u = 0; u < 8; ++u) {
+            const int e = e0 + 32 * u;
+            rows[e] = x[u];
+          }
+        }
+      };
+      const float* s0 = STATE_ONLY || A.s_in == nullptr ? nullptr
+                        : A.s_in + bh * block + (int64_t)r0 * A.s_row + (int64_t)n0 * A.s_col;
+      each([&](int r, int j) { return s0 ? A.s_in_scale * s0[(int64_t)r * A.s_row + (int64_t)j * A.s_col] : 0.f; });
+      if (!STATE_ONLY) {
+#pragma unroll 1
+        for (int q = 0; q < seg; ++q) {
+          const float d = expf(K.seg_decay[((int64_t)reverse * K.batch * K.heads + bh) * K.segs + q]);
+          const float* part = A.sum + ((int64_t)bh * K.segs + q) * block + (int64_t)r0 * dv + n0;
+          each([&](int r, int j) { return fmaf(d, rows[r * kTcN + j], part[(int64_t)r * dv + j]); });
+        }
       }
-      for (int r = 0; r < seg; ++r) {
-        const float d = expf(K.seg_decay[((int64_t)reverse * K.batch * K.heads + bh) * K.segs + r]);
-        const float* s = A.sum + ((int64_t)bh * K.segs + r) * block + (int64_t)row * dv + n0;
-#pragma unroll
-        for (int j = 0; j < kTcN; ++j)
-          if (j < nv) h[j] = fmaf(d, h[j], s[j]);
-      }
+      __syncwarp();
     }
+#pragma unroll
+    for (int j = 0; j < kTcN; j += 4) {
+      const float4 x = r0 < DK ? *reinterpret_cast<const float4*>(rows + lane * kTcN + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      h[j] = x.x, h[j + 1] = x.y, h[j + 2] = x.z, h[j + 3] = x.w;
+    }
+    // the halves of one warp lie in the rows of others
+    asm volatile("bar.sync 1, 128;" ::: "memory");
     unsigned char* hh = smem + S::kH;
     auto publish = [&]() {
       if (row < DK) {
@@ -697,17 +733,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       if (lane == 0) mbar_arrive(&B.l_empty);
       if (++st == S::kStages) st = 0, ph ^= 1;
     }
-    if (on && !*reinterpret_cast<volatile int*>(&B.abort)) {
-      if (STATE_ONLY) {
-        float* s = A.sum + ((int64_t)bh * K.segs + seg) * block + (int64_t)row * dv + n0;
+    // the last halves have been read (h_empty) before the rows take their room again
+    const int n = cn - c0;
+    bool ok = *reinterpret_cast<volatile int*>(&B.abort) == 0;
+    if (!STATE_ONLY && n > 0) ok = warp_wait(&B.h_empty, (n - 1) & 1) && ok;
+    float* to = STATE_ONLY ? A.sum + ((int64_t)bh * K.segs + seg) * block
+                           : (A.s_out && seg == K.segs - 1 ? A.s_out + bh * block : nullptr);
+    if (to && r0 < DK) {  // every warp that has rows comes here, one that gave up as well
+      asm volatile("bar.sync 1, %0;" ::"n"(DK) : "memory");
 #pragma unroll
-        for (int j = 0; j < kTcN; ++j)
-          if (j < nv) s[j] = h[j];
-      } else if (A.s_out && seg == K.segs - 1) {
-        float* s = A.s_out + bh * block + (int64_t)row * A.s_row + (int64_t)n0 * A.s_col;
-#pragma unroll
-        for (int j = 0; j < kTcN; ++j)
-          if (j < nv) s[(int64_t)j * A.s_col] = A.s_out_scale * h[j];
+      for (int j = 0; j < kTcN; j += 4)
+        *reinterpret_cast<float4*>(rows + lane * kTcN + j) = make_float4(h[j], h[j + 1], h[j + 2], h[j + 3]);
+      __syncwarp();
+      const float f = STATE_ONLY ? 1.f : A.s_out_scale;
+      const int64_t sr = STATE_ONLY ? dv : A.s_row, sc = STATE_ONLY ? 1 : A.s_col;
+#pragma unroll 1
+      for (int e = lane; e < 32 * kTcN; e += 32) {
+        const int r = e / kTcN, j = e % kTcN;
+        if (ok && r < rn && j < nv) to[(int64_t)(r0 + r) * sr + (int64_t)(n0 + j) * sc] = f * rows[e];
       }
     }
   }
