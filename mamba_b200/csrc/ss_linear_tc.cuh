@@ -80,16 +80,19 @@ __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sy
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-               "r"((uint32_t)add)
+// Operand descriptors: the low word holds the address (and the distance of 64-wide groups), the high word
+// is the same for all of them (8-row groups 1024 bytes apart, 128-byte swizzle)
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n setp.ne.u32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+               "r"((uint32_t)add), "n"(kDescHi)
                : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-               "r"((uint32_t)add)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  asm volatile("{\n .reg .pred p;\n .reg .b64 y;\n mov.b64 y, {%2, %5};\n setp.ne.u32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+               "r"((uint32_t)add), "n"(kDescHi)
                : "memory");
 }
 // 32 columns of this warp's 32 lanes
@@ -111,13 +114,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       : "memory");
 }
 
-// shared-memory operand descriptors, 128-byte swizzle: K-major (rows of 64 elements along K, 8-row
-// groups 1024 bytes apart) and MN-major (rows of 64 elements along M or N, one K a row; `lead` bytes
-// between groups of 64)
-__device__ __forceinline__ uint64_t desc_of(uint32_t addr, uint32_t lead) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
-}
+// low word of a shared-memory operand's descriptor: K-major (rows of 64 elements along K) or MN-major (rows
+// of 64 elements along M or N, one K a row; `lead` bytes between groups of 64)
+__device__ __forceinline__ uint32_t desc_of(uint32_t addr, uint32_t lead) { return (addr >> 4) | ((lead >> 4) << 16); }
 template <typename IT>
 __device__ __forceinline__ constexpr uint32_t idesc_of(int m, int n, bool a_mn, bool b_mn) {
   const uint32_t f = std::is_same<IT, __nv_bfloat16>::value ? 1u : 0u;
@@ -179,15 +178,15 @@ struct TcShape {
 struct TcBars {
   uint64_t full[3], empty[3], v_empty[3];
   uint64_t s_full[2], p_full[2];
-  uint64_t vp_full[2], vp_empty[2], l_full, l_empty, h_full, h_empty, o_full, o_empty, drain;
+  uint64_t vp_full[2], vp_empty[2], l_full, l_empty, h_full, h_empty, o_full[2], o_empty[2], drain;
   float total[3], total2[3];  // e^T of the stage's chunk, T log2 e
   uint32_t tmem;
   int abort;
 };
 
-// TMEM columns: two score buffers (the weighted scores overwrite the first half of theirs), outputs,
-// L of the high and of the low parts
-constexpr uint32_t kTmS = 0, kTmOi = 256, kTmOa = 320, kTmL = 384, kTmCols = 512;
+// TMEM columns: two score buffers (the weighted scores overwrite the first half of theirs, their product
+// with V the second), two of Q H, L of the high and of the low parts
+constexpr uint32_t kTmS = 0, kTmOa = 64, kTmOi = 256, kTmL = 384, kTmCols = 512;
 
 // try_wait that may suspend the thread for up to ~1 ms instead of coming back at once: a waiting warp
 // that polls takes issue slots from the ones that work
@@ -268,7 +267,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     for (int i = 0; i < 2; ++i) mbar_init(&B.vp_full[i], 4), mbar_init(&B.vp_empty[i], 1);
     mbar_init(&B.l_full, 1), mbar_init(&B.l_empty, 4);
     mbar_init(&B.h_full, 4), mbar_init(&B.h_empty, 1);
-    mbar_init(&B.o_full, 1), mbar_init(&B.o_empty, 4);
+    mbar_init(&B.o_full[0], 1), mbar_init(&B.o_full[1], 1), mbar_init(&B.o_empty[0], 4), mbar_init(&B.o_empty[1], 4);
     mbar_init(&B.drain, 1);
     B.abort = 0;
     mbar_fence_init();
@@ -373,18 +372,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     constexpr uint32_t kIdQK = idesc_of<IT>(128, kTcC, false, false), kIdN = idesc_of<IT>(128, kTcN, false, true),
                        kIdL = idesc_of<IT>(128, 2 * kTcN, true, true);
     // descriptors of the first stage; a step of 16 along K is 32 bytes (K-major) or 2048 (MN-major)
-    const uint64_t q0 = desc_of(base, 16), kk0 = desc_of(base + S::kBoxes * kBox, 16),
+    const uint32_t q0 = desc_of(base, 16), kk0 = desc_of(base + S::kBoxes * kBox, 16),
                    km0 = desc_of(base + S::kBoxes * kBox, kBox), v0 = desc_of(base + S::kVAt, kBox),
                    vp0 = desc_of(base + S::kVp, kBox), h0 = desc_of(base + S::kH, kBox);
     auto scores = [&](int st, int buf) {
-      const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4));
+      const uint32_t o = st * (S::kStageBytes >> 4);
       if (elect_one()) {
-        for (int x = 0; x < S::kBoxes; ++x)
-#pragma unroll 1
-          for (int k = 0; k < 4; ++k) {
-            const uint64_t at = o + x * (kBox >> 4) + k * 2;
-            mma_ss(tm + kTmS + buf * 128, q0 + at, kk0 + at, kIdQK, x + k > 0);
-          }
+#pragma unroll
+        for (int x = 0; x < DK / 16; ++x) {
+          const uint32_t at = (x >> 2) * (kBox >> 4) + (x & 3) * 2;
+          mma_ss(tm + kTmS + buf * 128, q0 + o + at, kk0 + o + at, kIdQK, x > 0);
+        }
         tc_commit(&B.s_full[buf]);
       }
       __syncwarp();
@@ -397,9 +395,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       // L = K^T [V'hi, V'lo]: a product of 64 columns takes as long as one of 128
       if (!warp_wait(&B.vp_full[S::kVps == 2 ? i & 1 : 0], (uint32_t)(i / S::kVps) & 1) || (i > 0 && !warp_wait(&B.l_empty, (i - 1) & 1))) break;
       tc_after();
-      const uint64_t o = (uint64_t)(st * (S::kStageBytes >> 4)), vp = vp0 + (S::kVps == 2 ? (i & 1) * 2 * (kBox >> 4) : 0);
+      const uint32_t o = st * (S::kStageBytes >> 4), vp = vp0 + (S::kVps == 2 ? (i & 1) * 2 * (kBox >> 4) : 0);
       if (elect_one()) {
-#pragma unroll 1
+#pragma unroll
         for (int x = 0; x < kTcC / 16; ++x) mma_ss(tm + kTmL, km0 + o + x * 128, vp + x * 128, kIdL, x > 0);
         tc_commit(&B.l_full);
         tc_commit(&B.vp_empty[S::kVps == 2 ? i & 1 : 0]);
@@ -409,20 +407,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       const int nst = st + 1 == S::kStages ? 0 : st + 1, nph = nst ? ph : ph ^ 1;
       if constexpr (!STATE_ONLY) {
         // Oi = Q H
-        if (!warp_wait(&B.h_full, i & 1) || (i > 0 && !warp_wait(&B.o_empty, (i - 1) & 1))) break;
+        if (!warp_wait(&B.h_full, i & 1)) break;
         tc_after();
         if (elect_one()) {
-#pragma unroll 1
+#pragma unroll
           for (int x = 0; x < 2 * DK / 16; ++x) {
             const int k = x % (DK / 16);
-            mma_ss(tm + kTmOi, q0 + o + (k >> 2) * (kBox >> 4) + (k & 3) * 2, h0 + x * 128, kIdN, x > 0);
+            mma_ss(tm + kTmOi + (i & 1) * kTcN, q0 + o + (k >> 2) * (kBox >> 4) + (k & 3) * 2, h0 + x * 128, kIdN, x > 0);
           }
           tc_commit(&B.h_empty);
         }
         __syncwarp();
-        // the next chunk's scores, into the buffer whose weighted scores were used a chunk ago (o_empty says
-        // so): now if the chunk is here, else after this chunk's last product, which must not wait for it
-        bool ahead = i + 1 < n && __all_sync(0xffffffffu, mbar_test_wait(&B.full[nst], nph));
+        // the next chunk's scores, into the buffer whose outputs were read (o_empty; those of Q H before them
+        // as well): now if chunk and buffer are there, else after this chunk's last product, which must not
+        // wait for them
+        bool ahead = i + 1 < n && __all_sync(0xffffffffu, mbar_test_wait(&B.full[nst], nph) &&
+                                                              (i == 0 || mbar_test_wait(&B.o_empty[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1)));
         if (ahead) {
           tc_after();
           scores(nst, (i + 1) & 1);
@@ -431,16 +431,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         if (!warp_wait(&B.p_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
         if (elect_one()) {
-#pragma unroll 1
+#pragma unroll
           for (int x = 0; x < kTcC / 16; ++x)
-            mma_ts(tm + kTmOa, tm + kTmS + (i & 1) * 128 + x * 8, v0 + o + x * 128, kIdN, x > 0);
-          tc_commit(&B.o_full);
+            mma_ts(tm + kTmOa + (i & 1) * 128, tm + kTmS + (i & 1) * 128 + x * 8, v0 + o + x * 128, kIdN, x > 0);
+          tc_commit(&B.o_full[i & 1]);
           tc_commit(&B.empty[st]);
           tc_commit(&B.v_empty[st]);
         }
         __syncwarp();
         if (!ahead && i + 1 < n) {
-          if (!warp_wait(&B.full[nst], nph)) break;
+          if (!warp_wait(&B.full[nst], nph) || (i > 0 && !warp_wait(&B.o_empty[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1))) break;
           tc_after();
           scores(nst, (i + 1) & 1);
         }
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
           q1 = on && 16 * x + 8 < nv ? *reinterpret_cast<const uint4*>(p + 16 * x + 8) : make_uint4(0, 0, 0, 0);
         };
         if (dot_at) load_p(0);
-        if (!warp_wait(&B.o_full, i & 1)) break;
+        if (!warp_wait(&B.o_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
         const uint32_t tile_at = tile0 + st * S::kStageBytes;
         unsigned char* out = smem + tile_at + row * 128;
@@ -589,8 +589,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
 #pragma unroll 1
         for (int x = 0; x < 4; ++x) {
           float o[16], oa[16];
-          tmem_ld16(lanes + kTmOi + x * 16, o);
-          tmem_ld16(lanes + kTmOa + x * 16, oa);
+          tmem_ld16(lanes + kTmOi + (i & 1) * kTcN + x * 16, o);
+          tmem_ld16(lanes + kTmOa + (i & 1) * 128 + x * 16, oa);
           const uint32_t u[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
           if (dot_at && x < 3) load_p(x + 1);
           tc_wait_ld();
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         }
         tc_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&B.o_empty);
+        if (lane == 0) mbar_arrive(&B.o_empty[i & 1]);
         fence_async_smem();
         __syncwarp();
         if (elect_one()) {
