@@ -56,10 +56,9 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t sr
                "r"(x), "r"(y), "r"(z), "r"(w), "r"(src)
                : "memory");
 }
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // every store of this thread has read its shared memory
-__device__ __forceinline__ void tma_store_read() {
-  asm volatile("cp.async.bulk.commit_group;\n cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
+__device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -156,21 +155,22 @@ __device__ __forceinline__ void store_split(unsigned char* hi, unsigned char* lo
   *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// Shared memory: stages of Q, K, V as TMA writes them; buffers of V' (hi, lo); H (hi, lo); per stage the
-// decays: X of every token and the column factors of three blocks; barriers.  Narrow heads have room for
-// three stages and for V' of the next chunk.  The output tile takes the room of its chunk's V on its
-// way to the TMA store (V is needed later in the stage's next chunk than Q and K are).
+// Shared memory: stages of Q, K, V as TMA writes them; V' (hi, lo); H (hi, lo); the output tile on its way to
+// the TMA store; per stage the decays: X of every token and the column factors of three blocks; barriers.
+// Wide heads have room for two stages and none for the output tile, which takes its chunk's V (needed later
+// in the stage's next chunk than Q and K).
 template <int DK>
 struct TcShape {
   static constexpr int kBoxes = DK / 64;
   static constexpr int kStages = DK == 128 ? 2 : 3;
-  static constexpr int kVps = DK == 128 ? 1 : 2;
+  static constexpr bool kOwnOut = DK == 64;
   static constexpr uint32_t kStageBytes = (2 * kBoxes + 1) * kBox;
   static constexpr uint32_t kVAt = 2 * kBoxes * kBox;
   static constexpr uint32_t kVp = kStages * kStageBytes;
-  static constexpr uint32_t kH = kVp + kVps * 2 * kBox;
+  static constexpr uint32_t kH = kVp + 2 * kBox;
+  static constexpr uint32_t kOut = kH + 2 * DK * 128;
   static constexpr uint32_t kDecStage = (kTcC + 96) * 4;
-  static constexpr uint32_t kDec = kH + 2 * DK * 128;
+  static constexpr uint32_t kDec = kOut + (kOwnOut ? kBox : 0);
   static constexpr uint32_t kBars = kDec + kStages * kDecStage;
   static constexpr uint32_t kBytes = kBars + 256;
 };
@@ -178,7 +178,7 @@ struct TcShape {
 struct TcBars {
   uint64_t full[3], empty[3], v_empty[3];
   uint64_t s_full[2], p_full[2];
-  uint64_t vp_full[2], vp_empty[2], l_full, l_empty, h_full, h_empty, o_full[2], o_empty[2], drain;
+  uint64_t vp_full, l_full, l_empty, h_full, h_empty, o_full[2], o_empty[2], drain;
   float total[3], total2[3];  // e^T of the stage's chunk, T log2 e
   uint32_t tmem;
   int abort;
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       mbar_init(&B.v_empty[i], STATE_ONLY ? 1 : 1 + 4);    // the products, the output tile that takes V's room
     }
     for (int i = 0; i < 2; ++i) mbar_init(&B.s_full[i], 1), mbar_init(&B.p_full[i], 4);
-    for (int i = 0; i < 2; ++i) mbar_init(&B.vp_full[i], 4), mbar_init(&B.vp_empty[i], 1);
+    mbar_init(&B.vp_full, 4);
     mbar_init(&B.l_full, 1), mbar_init(&B.l_empty, 4);
     mbar_init(&B.h_full, 4), mbar_init(&B.h_empty, 1);
     mbar_init(&B.o_full[0], 1), mbar_init(&B.o_full[1], 1), mbar_init(&B.o_empty[0], 4), mbar_init(&B.o_empty[1], 4);
@@ -393,14 +393,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       tc_after();
       if (!STATE_ONLY && i == 0) scores(0, 0);
       // L = K^T [V'hi, V'lo]: a product of 64 columns takes as long as one of 128
-      if (!warp_wait(&B.vp_full[S::kVps == 2 ? i & 1 : 0], (uint32_t)(i / S::kVps) & 1) || (i > 0 && !warp_wait(&B.l_empty, (i - 1) & 1))) break;
+      if (!warp_wait(&B.vp_full, i & 1) || (i > 0 && !warp_wait(&B.l_empty, (i - 1) & 1))) break;
       tc_after();
-      const uint32_t o = st * (S::kStageBytes >> 4), vp = vp0 + (S::kVps == 2 ? (i & 1) * 2 * (kBox >> 4) : 0);
+      const uint32_t o = st * (S::kStageBytes >> 4);
       if (elect_one()) {
 #pragma unroll
-        for (int x = 0; x < kTcC / 16; ++x) mma_ss(tm + kTmL, km0 + o + x * 128, vp + x * 128, kIdL, x > 0);
+        for (int x = 0; x < kTcC / 16; ++x) mma_ss(tm + kTmL, km0 + o + x * 128, vp0 + x * 128, kIdL, x > 0);
         tc_commit(&B.l_full);
-        tc_commit(&B.vp_empty[S::kVps == 2 ? i & 1 : 0]);
         if (STATE_ONLY) tc_commit(&B.empty[st]), tc_commit(&B.v_empty[st]);
       }
       __syncwarp();
@@ -537,9 +536,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       }
       __syncwarp();
       const float2 w = f2(ex2(dec_X(st)[row]));
-      // the product over the buffer has ended
-      if (i >= S::kVps && !warp_wait(&B.vp_empty[S::kVps == 2 ? i & 1 : 0], (uint32_t)(i / S::kVps - 1) & 1)) break;
-      unsigned char* vp = smem + S::kVp + (S::kVps == 2 ? (i & 1) * 2 * kBox : 0);
+      if (i > 0 && !warp_wait(&B.l_full, (i - 1) & 1)) break;  // the product over the buffer has ended
+      unsigned char* vp = smem + S::kVp;
 #pragma unroll 2
       for (int j = 0; j < 8; ++j) {
         const uint4 q = *reinterpret_cast<const uint4*>(v + ((j ^ (row & 7)) << 4));
@@ -555,14 +553,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&B.vp_full[S::kVps == 2 ? i & 1 : 0]);
+      if (lane == 0) mbar_arrive(&B.vp_full);
       if (++st == S::kStages) st = 0, ph ^= 1;
     }
   } else if (wg == 2) {
     // ------------------------------------------------------------ outputs
     if constexpr (!STATE_ONLY) {
       const int w4 = wid & 3;
-      const uint32_t tile0 = A.o_f32 ? 0 : S::kVAt;  // fp32 tiles, twice as large, take Q's and K's room
+      const bool own_out = S::kOwnOut && !A.o_f32;  // fp32 tiles, twice as large, take Q's and K's room
       const IT* p_at = A.dot ? static_cast<const IT*>(A.p) + (int64_t)b * A.pb + (int64_t)(head / A.rp) * A.ph + n0 : nullptr;
       float* dot_at = A.dot ? A.dot + (((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen : nullptr;
       const float2 sc = f2(A.scale);
@@ -572,7 +570,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         const float2 w = f2(A.scale * ex2(*reinterpret_cast<volatile float*>(&B.total2[st]) - dec_X(st)[row]));
         const bool on = row < m;
         __syncwarp();
-        if (lane == 0) mbar_arrive(A.o_f32 ? &B.v_empty[st] : &B.empty[st]);
+        if (lane == 0) {
+          mbar_arrive(A.o_f32 ? &B.v_empty[st] : &B.empty[st]);
+          if (own_out) mbar_arrive(&B.v_empty[st]);
+        }
         // 16 columns at a time, the next ones of p under way
         const IT* p = p_at + (int64_t)t * A.pl;
         uint4 q0 = make_uint4(0, 0, 0, 0), q1 = q0;
@@ -583,7 +584,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         if (dot_at) load_p(0);
         if (!warp_wait(&B.o_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
-        const uint32_t tile_at = tile0 + st * S::kStageBytes;
+        const uint32_t tile_at = own_out ? S::kOut : st * S::kStageBytes + (A.o_f32 ? 0 : S::kVAt);
+        if (own_out) {
+          if (elect_one()) tma_store_read();  // the tile before has left
+          __syncwarp();
+        }
         unsigned char* out = smem + tile_at + row * 128;
         float2 dot = f2(0.f);
 #pragma unroll 1
@@ -627,13 +632,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
             tma_store_4d(&P.map[pass][3], src, n0, head, t0 + w4 * 32, b);
             if (A.o_f32 && n0 + 32 < dv) tma_store_4d(&P.map[pass][3], src + kBox, n0 + 32, head, t0 + w4 * 32, b);
           }
-          tma_store_read();
-          mbar_arrive(A.o_f32 ? &B.empty[st] : &B.v_empty[st]);
+          if (own_out) {
+            tma_store_commit();
+          } else {
+            tma_store_commit();
+            tma_store_read();
+            mbar_arrive(A.o_f32 ? &B.empty[st] : &B.v_empty[st]);
+          }
         }
         __syncwarp();
         if (dot_at && t < K.seqlen) dot_at[t] = on ? dot.x + dot.y : 0.f;
         if (++st == S::kStages) st = 0, ph ^= 1;
       }
+      if (elect_one()) tma_store_read();
+      __syncwarp();
       auto zero_row = [&](int t) {
         const int es = A.o_f32 ? 4 : 2;
         char* o = static_cast<char*>(A.o) + ((int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0) * es;
