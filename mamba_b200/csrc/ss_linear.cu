@@ -85,6 +85,14 @@ Work work_of(const ss_linear_args& a, int backward) {
   return w;
 }
 
+cudaError_t launch_fold(const LinK& P, int passes, cudaStream_t st) {
+  int64_t block = 0;
+  for (int i = 0; i < passes; ++i) block = std::max<int64_t>(block, (int64_t)P.pass[i].dk * P.pass[i].dv);
+  const dim3 grid((unsigned)((block + 255) / 256), (unsigned)(P.batch * P.heads), (unsigned)passes);
+  linear_fold_kernel<<<grid, 256, 0, st>>>(P);
+  return cudaGetLastError();
+}
+
 template <typename IT>
 cudaError_t run_simt(const LinK& P, int passes, cudaStream_t st) {
   constexpr size_t smem = sizeof(LsSmem);
@@ -98,6 +106,7 @@ cudaError_t run_simt(const LinK& P, int passes, cudaStream_t st) {
   if (P.segs > 1) {
     sum_k<<<grid, kLsThreads, smem, st>>>(P);
     e = cudaGetLastError();
+    if (e == cudaSuccess) e = launch_fold(P, passes, st);
     if (e != cudaSuccess) return e;
   }
   main_k<<<grid, kLsThreads, smem, st>>>(P);
@@ -108,7 +117,7 @@ template <typename IT, int DK>
 cudaError_t launch_tc(const LinTcK& P, cudaStream_t st) {
   constexpr size_t smem = TcShape<DK>::kBytes;
   static_assert(smem <= 232448, "shared memory of a CTA");
-  static_assert(sizeof(TcBars) <= 256, "barriers");
+  static_assert(sizeof(TcBars) <= 512, "barriers");
   auto main_k = linear_tc_kernel<IT, DK, false>;
   auto sum_k = linear_tc_kernel<IT, DK, true>;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(main_k), smem);
@@ -118,6 +127,7 @@ cudaError_t launch_tc(const LinTcK& P, cudaStream_t st) {
   if (P.k.segs > 1) {
     sum_k<<<grid, kTcThreads, smem, st>>>(P);
     e = cudaGetLastError();
+    if (e == cudaSuccess) e = launch_fold(P.k, P.parts / P.tiles, st);
     if (e != cudaSuccess) return e;
   }
   main_k<<<grid, kTcThreads, smem, st>>>(P);

@@ -45,7 +45,7 @@ struct LinPass {
   int64_t pb, pl, ph;
   int rp;
   float* dot;
-  float* sum;          // segment states: [b * h][segment][dk * dv], nullable when there is one segment
+  float* sum;          // segments' own states, then the states before them: [b * h][segment][dk * dv]; null for one segment
 };
 
 constexpr int kLinMaxPasses = 3;
@@ -120,16 +120,13 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
   const int hi = tid / 16 * 8;                     // 8 x 4 tile of the state
   const int64_t block = (int64_t)dk * dv;
 
-  // the state before this segment: the initial state folded with the earlier segments' own states
+  // the state before this segment: the initial state, or what it and the earlier segments fold to
   for (int e = tid; e < kLinMaxDim * kLsN; e += kLsThreads) {
     const int i = e / kLsN, j = e % kLsN;
     float s = 0.f;
     if (!STATE_ONLY && i < dk && j < nv) {
-      if (A.s_in) s = A.s_in_scale * A.s_in[bh * block + (int64_t)i * A.s_row + (int64_t)(n0 + j) * A.s_col];
-      for (int r = 0; r < seg; ++r) {
-        const float d = expf(P.seg_decay[((int64_t)A.reverse * P.batch * P.heads + bh) * P.segs + r]);
-        s = fmaf(d, s, A.sum[((int64_t)bh * P.segs + r) * block + (int64_t)i * dv + n0 + j]);
-      }
+      if (P.segs > 1) s = A.sum[((int64_t)bh * P.segs + seg) * block + (int64_t)i * dv + n0 + j];
+      else if (A.s_in) s = A.s_in_scale * A.s_in[bh * block + (int64_t)i * A.s_row + (int64_t)(n0 + j) * A.s_col];
     }
     S.h[i][j] = s;
   }
@@ -307,6 +304,32 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
       const int i = e / nv, j = e % nv;
       A.s_out[bh * block + (int64_t)i * A.s_row + (int64_t)(n0 + j) * A.s_col] = A.s_out_scale * S.h[i][j];
     }
+  }
+}
+
+// The segments' own states -> the state before each segment, in place: a thread an entry, its segments in
+// order, 8 loads under way at a time.
+__global__ void __launch_bounds__(256) linear_fold_kernel(const __grid_constant__ LinK P) {
+  const LinPass& A = P.pass[blockIdx.z];
+  const int64_t block = (int64_t)A.dk * A.dv, bh = blockIdx.y;
+  __shared__ float decay[32];
+  if (threadIdx.x < P.segs - 1)
+    decay[threadIdx.x] = expf(P.seg_decay[((int64_t)A.reverse * P.batch * P.heads + bh) * P.segs + threadIdx.x]);
+  __syncthreads();
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= block) return;
+  float s = A.s_in ? A.s_in_scale * A.s_in[bh * block + e / A.dv * A.s_row + e % A.dv * A.s_col] : 0.f;
+  float* at = A.sum + bh * P.segs * block + e;
+  for (int q0 = 0; q0 < P.segs; q0 += 8) {
+    float x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[u] = q0 + u < P.segs - 1 ? at[(q0 + u) * block] : 0.f;  // the last one's own is not needed
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (q0 + u < P.segs) {
+        at[(q0 + u) * block] = s;
+        if (q0 + u < P.segs - 1) s = fmaf(decay[q0 + u], s, x[u]);
+      }
   }
 }
 

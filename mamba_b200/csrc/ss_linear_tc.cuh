@@ -14,6 +14,9 @@
 // (half a step) are accepted: an output is rounded to the same type anyway.  The state and the
 // weighted values would spread their rounding to every later token and to the fp32 final state, so
 // they are split: hi + lo keeps 16 (bf16) or 22 (fp16) bits, at two products of 64 columns each.
+// fp16 has a mantissa to spare and no range: its weighted scores are scaled by a power of two per row (from a
+// bound, the row's largest |q| times the chunk's largest |k| times dk), V' and H by one per chunk (from their
+// largest value), which the outputs and the state take back; bf16 needs none of that.
 // The dot products for the decays' gradient need it too: sums of q . dq - k . dk telescope only as far
 // as both runs round the same P alike and nothing else.
 //
@@ -172,7 +175,7 @@ struct TcShape {
   static constexpr uint32_t kDecStage = (kTcC + 96) * 4;
   static constexpr uint32_t kDec = kOut + (kOwnOut ? kBox : 0);
   static constexpr uint32_t kBars = kDec + kStages * kDecStage;
-  static constexpr uint32_t kBytes = kBars + 256;
+  static constexpr uint32_t kBytes = kBars + 512 + 256;  // and the rows' exponents (fp16)
 };
 
 struct TcBars {
@@ -182,6 +185,10 @@ struct TcBars {
   float total[3], total2[3];  // e^T of the stage's chunk, T log2 e
   uint32_t tmem;
   int abort;
+  // fp16: largest values of a chunk found by four warps, and the exponents they give
+  uint64_t max_full[3];
+  uint32_t max_of[3][4];
+  int v_exp[2], h_exp[4];
 };
 
 // TMEM columns: two score buffers (the weighted scores overwrite the first half of theirs, their product
@@ -228,6 +235,28 @@ __device__ __noinline__ bool tc_wait_slow(uint64_t* bar, uint32_t parity, volati
   return true;
 }
 
+// exponent of the power of two that brings values up to m to just below 2^15 (0 where there is nothing to bring)
+__device__ __forceinline__ int half_exp(float m) {
+  const int e = (int)(__float_as_uint(m) >> 23) & 255;
+  return e == 0 || e == 255 ? 0 : max(-100, min(100, 127 + 14 - e));
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// largest magnitude of a packed row's words (fp16 only)
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, const uint4& q) {
+  auto two = [](uint32_t a, uint32_t b) {
+    const __half2 x = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&x);
+  };
+  m = two(m, q.x & 0x7fff7fffu);
+  m = two(m, q.y & 0x7fff7fffu);
+  m = two(m, q.z & 0x7fff7fffu);
+  return two(m, q.w & 0x7fff7fffu);
+}
+__device__ __forceinline__ float max_of2(uint32_t m) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
+  return fmaxf(f.x, f.y);
+}
+
 template <typename IT, int DK, bool STATE_ONLY>
 __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_constant__ LinTcK P) {
   using S = TcShape<DK>;
@@ -269,6 +298,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     mbar_init(&B.h_full, 4), mbar_init(&B.h_empty, 1);
     mbar_init(&B.o_full[0], 1), mbar_init(&B.o_full[1], 1), mbar_init(&B.o_empty[0], 4), mbar_init(&B.o_empty[1], 4);
     mbar_init(&B.drain, 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&B.max_full[i], 4);
+      for (int j = 0; j < 4; ++j) B.max_of[i][j] = 0;
+    }
     B.abort = 0;
     mbar_fence_init();
   }
@@ -282,6 +315,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
   tc_after();
   const uint32_t tm = B.tmem;
   const uint32_t lanes = tm + ((uint32_t)(wid & 3) << 21);  // this warp's 32 lanes
+
+  // The largest m >= 0 of a chunk over the four warps of group `g`, into *m; false: gave up.  Slots go round:
+  // who passes the wait of chunk i knows that everyone has read chunk i - 1's.
+  auto group_max = [&](int g, int i, float* m) {
+    const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(*m));  // order of non-negative floats
+    if (lane == 0) {
+      atomicMax(&B.max_of[g][i & 3], w);
+      mbar_arrive(&B.max_full[g]);
+    }
+    if (!warp_wait(&B.max_full[g], i & 1)) return false;
+    *m = __uint_as_float(*reinterpret_cast<volatile uint32_t*>(&B.max_of[g][i & 3]));
+    if ((wid & 3) == 0 && lane == 0) *reinterpret_cast<volatile uint32_t*>(&B.max_of[g][(i + 2) & 3]) = 0;
+    return true;
+  };
+  signed char* row_exp = reinterpret_cast<signed char*>(smem + S::kBars + 512);  // [2][128]
+  constexpr bool kHalf = std::is_same<IT, __half>::value;
 
   if (wid == 16) {
     // ------------------------------------------------------------ loads
@@ -462,6 +511,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
         const int m = min(kTcC, len - first_token(c));
         if (!warp_wait(&B.full[st], ph) || !warp_wait(&B.s_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
+        float pw = 1.f;  // fp16: the row's scale
+        if constexpr (kHalf) {
+          uint32_t qm = 0, km = 0;
+#pragma unroll 1
+          for (int j = 0; j < DK / 8; ++j) {
+            const unsigned char* at = smem + st * S::kStageBytes + (j >> 3) * kBox + row * 128 + (j & 7) * 16;
+            qm = max_abs2(qm, *reinterpret_cast<const uint4*>(at));
+            km = max_abs2(km, *reinterpret_cast<const uint4*>(at + S::kBoxes * kBox));
+          }
+          float k = row < m ? max_of2(km) : 0.f;
+          if (!group_max(0, i, &k)) break;
+          const int e = half_exp(max_of2(qm) * k * DK);
+          row_exp[(i & 1) * 128 + row] = (signed char)e;
+          pw = pow2(e);
+        }
         tc_after();
         const float* X = dec_X(st);
         const float xi = X[row];
@@ -477,7 +541,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
             float s[32];
             tmem_ld32(sp + x * 32, s);
             if (x != w) {
-              const float2 rf = f2(ex2(X[reverse ? x * 32 - 1 : x * 32 + 31] - xi));
+              const float2 rf = f2(pw * ex2(X[reverse ? x * 32 - 1 : x * 32 + 31] - xi));
               const float* cf = X + kTcC + (reverse ? x - 1 : x) * 32;
               tc_wait_ld();
 #pragma unroll
@@ -495,7 +559,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
                 const float x4[4] = {xj.x, xj.y, xj.z, xj.w};
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                  const float e = s[j + r] * ex2_ordered(x4[r] - xi);
+                  const float e = s[j + r] * (kHalf ? pw * ex2_ordered(x4[r] - xi) : ex2_ordered(x4[r] - xi));
                   s[j + r] = diag & (1u << (j + r)) ? e : 0.f;
                 }
               }
@@ -535,8 +599,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         }
       }
       __syncwarp();
-      const float2 w = f2(ex2(dec_X(st)[row]));
+      float wv = ex2(dec_X(st)[row]);
+      int v_exp = 0;
+      if constexpr (kHalf) {
+        uint32_t vm = 0;
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) vm = max_abs2(vm, *reinterpret_cast<const uint4*>(v + j * 16));
+        float x = wv * max_of2(vm);
+        if (!group_max(1, i, &x)) break;
+        v_exp = half_exp(x);
+        wv *= pow2(v_exp);
+      }
+      const float2 w = f2(wv);
       if (i > 0 && !warp_wait(&B.l_full, (i - 1) & 1)) break;  // the product over the buffer has ended
+      if (kHalf && row == 0) *reinterpret_cast<volatile int*>(&B.v_exp[i & 1]) = v_exp;
       unsigned char* vp = smem + S::kVp;
 #pragma unroll 2
       for (int j = 0; j < 8; ++j) {
@@ -584,6 +660,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         if (dot_at) load_p(0);
         if (!warp_wait(&B.o_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
+        float2 wi = w, wa = sc;
+        if constexpr (kHalf) {
+          wi = mul2(wi, f2(pow2(-*reinterpret_cast<volatile int*>(&B.h_exp[i & 3]))));
+          wa = mul2(wa, f2(pow2(-row_exp[(i & 1) * 128 + row])));
+        }
         const uint32_t tile_at = own_out ? S::kOut : st * S::kStageBytes + (A.o_f32 ? 0 : S::kVAt);
         if (own_out) {
           if (elect_one()) tma_store_read();  // the tile before has left
@@ -601,7 +682,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
           tc_wait_ld();
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
-            const float2 r = fma2(w, make_float2(o[j], o[j + 1]), mul2(sc, make_float2(oa[j], oa[j + 1])));
+            const float2 r = fma2(wi, make_float2(o[j], o[j + 1]), mul2(wa, make_float2(oa[j], oa[j + 1])));
             o[j] = on ? r.x : 0.f, o[j + 1] = on ? r.y : 0.f;
           }
           if (A.o_f32) {
@@ -664,7 +745,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     float* rows = reinterpret_cast<float*>(smem + S::kH) + (wid & 3) * 32 * kTcN;
     const int r0 = (wid & 3) * 32, rn = min(32, dk - r0);  // this warp's rows; <= 0: none
     if (r0 < DK) {
-      // 8 loads under way at a time; one segment after the other
+      // 8 loads under way at a time
       auto each = [&](auto&& f) {
 #pragma unroll 1
         for (int e0 = lane; e0 < 32 * kTcN; e0 += 8 * 32) {
@@ -681,16 +762,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
           }
         }
       };
-      const float* s0 = STATE_ONLY || A.s_in == nullptr ? nullptr
-                        : A.s_in + bh * block + (int64_t)r0 * A.s_row + (int64_t)n0 * A.s_col;
-      each([&](int r, int j) { return s0 ? A.s_in_scale * s0[(int64_t)r * A.s_row + (int64_t)j * A.s_col] : 0.f; });
-      if (!STATE_ONLY) {
-#pragma unroll 1
-        for (int q = 0; q < seg; ++q) {
-          const float d = expf(K.seg_decay[((int64_t)reverse * K.batch * K.heads + bh) * K.segs + q]);
-          const float* part = A.sum + ((int64_t)bh * K.segs + q) * block + (int64_t)r0 * dv + n0;
-          each([&](int r, int j) { return fmaf(d, rows[r * kTcN + j], part[(int64_t)r * dv + j]); });
-        }
+      if (!STATE_ONLY && K.segs > 1) {  // folded from the initial state and the segments before
+        const float* s0 = A.sum + ((int64_t)bh * K.segs + seg) * block + (int64_t)r0 * dv + n0;
+        each([&](int r, int j) { return s0[(int64_t)r * dv + j]; });
+      } else {
+        const float* s0 = STATE_ONLY || A.s_in == nullptr ? nullptr
+                          : A.s_in + bh * block + (int64_t)r0 * A.s_row + (int64_t)n0 * A.s_col;
+        each([&](int r, int j) { return s0 ? A.s_in_scale * s0[(int64_t)r * A.s_row + (int64_t)j * A.s_col] : 0.f; });
       }
       __syncwarp();
     }
@@ -702,24 +780,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     // the halves of one warp lie in the rows of others
     asm volatile("bar.sync 1, 128;" ::: "memory");
     unsigned char* hh = smem + S::kH;
-    auto publish = [&]() {
+    auto publish = [&](int i) {
+      float2 hw = f2(1.f);
+      if constexpr (kHalf) {
+        float x = 0.f;
+#pragma unroll
+        for (int j = 0; j < kTcN; ++j) x = fmaxf(x, fabsf(h[j]));
+        if (row >= dk) x = 0.f;
+        if (!group_max(2, i, &x)) return false;
+        const int e = half_exp(x);
+        hw = f2(pow2(e));
+        if (row == 0) *reinterpret_cast<volatile int*>(&B.h_exp[i & 3]) = e;
+      }
       if (row < DK) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float x[8];
 #pragma unroll
-          for (int r = 0; r < 8; ++r) x[r] = h[8 * j + r];
+          for (int r = 0; r < 8; r += 2) {
+            const float2 t = kHalf ? mul2(hw, make_float2(h[8 * j + r], h[8 * j + r + 1]))
+                                   : make_float2(h[8 * j + r], h[8 * j + r + 1]);
+            x[r] = t.x, x[r + 1] = t.y;
+          }
           store_split<IT>(hh, hh + DK * 128, row, j, x);
         }
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.h_full);
+      return true;
     };
     for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
       if (!STATE_ONLY) {
         if (i > 0 && !warp_wait(&B.h_empty, (i - 1) & 1)) break;
-        publish();
+        if (!publish(i)) break;
       }
       if (!warp_wait(&B.full[st], ph)) break;
       const float d = *reinterpret_cast<volatile float*>(&B.total[st]);
@@ -727,6 +821,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
       if (lane == 0) mbar_arrive(&B.empty[st]);
       if (!warp_wait(&B.l_full, i & 1)) break;
       tc_after();
+      const float2 lw = f2(kHalf ? pow2(-*reinterpret_cast<volatile int*>(&B.v_exp[i & 1])) : 1.f);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         float l[16], lo[16];
@@ -735,8 +830,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
         tc_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-          const float2 r = fma2(f2(d), make_float2(h[x * 16 + j], h[x * 16 + j + 1]),
-                                add2(make_float2(l[j], l[j + 1]), make_float2(lo[j], lo[j + 1])));
+          float2 t = add2(make_float2(l[j], l[j + 1]), make_float2(lo[j], lo[j + 1]));
+          if (kHalf) t = mul2(lw, t);
+          const float2 r = fma2(f2(d), make_float2(h[x * 16 + j], h[x * 16 + j + 1]), t);
           h[x * 16 + j] = r.x, h[x * 16 + j + 1] = r.y;
         }
       }
