@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "../../include/mamba_b200_ss.h"
@@ -13,24 +14,29 @@ namespace {
 
 using namespace ssb;
 
-bool rows16(const void* p, int64_t stride, size_t es) {
-  return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((stride * (int64_t)es) & 15) == 0);
+// rows that start on a vector of 4 values
+bool rows4(const void* p, int64_t stride, size_t es) {
+  const uintptr_t m = 4 * es - 1;
+  return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & m) == 0 && ((uintptr_t)(stride * (int64_t)es) & m) == 0);
+}
+
+bool weights16(const ss_block_norm_args& a) {
+  return a.dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.post_weight) | reinterpret_cast<uintptr_t>(a.pre_weight) |
+                             reinterpret_cast<uintptr_t>(a.scale)) & 15) == 0;
 }
 
 struct Shape {
-  int nv, wpr;  // 16-byte vectors a lane, warps a row; nv 0: the row is too long
+  int nv, wpr;  // vectors a lane, warps a row
 };
 
-// A row in as few warps as its vectors allow: up to 4 a lane in the forward, 3 in the backward
-// (whose column sums take two more registers a value)
-Shape shape_of(int dim, size_t es, int most) {
-  const int vw = (int)(16 / es);
+// A row's warps: as few as hold it with 3 vectors of 4 values a lane, at most 8
+Shape shape_of(int dim) {
   for (int wpr : {1, 2, 4, 8}) {
-    const int need = (dim + 32 * wpr * vw - 1) / (32 * wpr * vw);
-    if (need <= most) return {need, wpr};
+    const int need = (dim + 128 * wpr - 1) / (128 * wpr);
+    if (need <= 3) return {need, wpr};
   }
-  const int need = (dim + 32 * 8 * vw - 1) / (32 * 8 * vw);
-  return need <= 8 ? Shape{need <= 4 ? 4 : need <= 6 ? 6 : 8, 8} : Shape{0, 8};
+  const int need = (dim + 1023) / 1024;
+  return {need <= 4 ? 4 : need <= 6 ? 6 : 8, 8};
 }
 
 int sm_count() {
@@ -68,22 +74,39 @@ int by_dtype(int io, F&& f) {
   }
 }
 
+// the kernel's MODE of a call
+int mode_of(const ss_block_norm_args& a, int vec, int wvec) {
+  if (!vec || !wvec || !a.post_weight || !a.pre_weight) return kBnAny;
+  if (!a.gate) return kBnPlain;
+  return a.activation == kActSilu ? kBnGated : kBnAny;
+}
+
 template <typename IT, int NV, int WPR>
 cudaError_t fwd(const BlockNormK& P, cudaStream_t st) {
-  constexpr size_t smem = sizeof(float) * 2 * NV * WPR * 32 * (16 / sizeof(IT));
-  auto kern = block_norm_fwd_kernel<IT, NV, WPR>;
-  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), smem + 256);  // and the static part
-  if (e != cudaSuccess) return e;
+  const int mode = mode_of(P.a, P.vec, P.wvec);
+  auto kern = mode == kBnGated ? block_norm_fwd_kernel<IT, NV, WPR, kBnGated>
+              : mode == kBnPlain ? block_norm_fwd_kernel<IT, NV, WPR, kBnPlain> : block_norm_fwd_kernel<IT, NV, WPR, kBnAny>;
+  // as many CTAs as are resident at once, each walking its share of the rows: a second wave of a third of
+  // them would take as long as the first
+  static std::atomic<int> resident[3];
+  int occ = resident[mode].load();
+  if (occ == 0) {
+    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, 32 * kBnWarps, 0);
+    if (e != cudaSuccess) return e;
+    resident[mode].store(occ = std::max(occ, 1));
+  }
   const int rpc = kBnWarps / WPR;
   const int64_t ctas = ((int64_t)P.a.rows + rpc - 1) / rpc;
-  kern<<<(unsigned)std::min<int64_t>(ctas, 4 * sm_count()), 32 * kBnWarps, smem, st>>>(P);
+  kern<<<(unsigned)std::min<int64_t>(ctas, (int64_t)occ * sm_count()), 32 * kBnWarps, 0, st>>>(P);
   return cudaGetLastError();
 }
 
 template <typename IT, int NV, int WPR>
 cudaError_t bwd(const BlockNormBwdK& P, cudaStream_t st) {
-  constexpr size_t smem = sizeof(float) * 2 * NV * WPR * 32 * (16 / sizeof(IT));
-  auto kern = block_norm_bwd_kernel<IT, NV, WPR>;
+  constexpr size_t smem = sizeof(float) * NV * WPR * 32 * kBv;
+  const int mode = P.a.dh ? mode_of(P.a.f, P.vec, P.wvec) : kBnAny;
+  auto kern = mode == kBnGated ? block_norm_bwd_kernel<IT, NV, WPR, kBnGated>
+              : mode == kBnPlain ? block_norm_bwd_kernel<IT, NV, WPR, kBnPlain> : block_norm_bwd_kernel<IT, NV, WPR, kBnAny>;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), smem + 256);  // and the static part
   if (e != cudaSuccess) return e;
   kern<<<(unsigned)bwd_ctas(P.a.f.rows, WPR), 32 * kBnWarps, smem, st>>>(P);
@@ -92,32 +115,26 @@ cudaError_t bwd(const BlockNormBwdK& P, cudaStream_t st) {
 
 }  // namespace
 
-#define SSB_BN_SHAPES(F, MOST)                                    \
-  if (s.wpr == 1) {                                               \
-    if (s.nv == 1) return F<IT, 1, 1>(P, st);                     \
-    if (s.nv == 2) return F<IT, 2, 1>(P, st);                     \
-    if (s.nv == 3) return F<IT, 3, 1>(P, st);                     \
-    return F<IT, MOST, 1>(P, st);                                 \
-  }                                                               \
-  if (s.wpr == 2) { SSB_BN_WIDE(F, MOST, 2) }                     \
-  if (s.wpr == 4) { SSB_BN_WIDE(F, MOST, 4) }                     \
-  if (s.nv <= 2) return F<IT, 2, 8>(P, st);                       \
-  if (s.nv <= 3) return F<IT, 3, 8>(P, st);                       \
-  if (s.nv <= 4) return F<IT, 4, 8>(P, st);                       \
-  if (s.nv <= 6) return F<IT, 6, 8>(P, st);                       \
+// a row that did not fit half as many warps has at least 2 vectors a lane
+#define SSB_BN_SHAPES(F)                                            \
+  if (s.wpr == 1) {                                                 \
+    if (s.nv == 1) return F<IT, 1, 1>(P, st);                       \
+    return s.nv == 2 ? F<IT, 2, 1>(P, st) : F<IT, 3, 1>(P, st);     \
+  }                                                                 \
+  if (s.wpr == 2) return s.nv <= 2 ? F<IT, 2, 2>(P, st) : F<IT, 3, 2>(P, st); \
+  if (s.wpr == 4) return s.nv <= 2 ? F<IT, 2, 4>(P, st) : F<IT, 3, 4>(P, st); \
+  if (s.nv <= 2) return F<IT, 2, 8>(P, st);                         \
+  if (s.nv <= 3) return F<IT, 3, 8>(P, st);                         \
+  if (s.nv <= 4) return F<IT, 4, 8>(P, st);                         \
+  if (s.nv <= 6) return F<IT, 6, 8>(P, st);                         \
   return F<IT, 8, 8>(P, st);
-
-// a row that did not fit half as many warps has at least 2 vectors a lane here
-#define SSB_BN_WIDE(F, MOST, WPR)                                 \
-  if (s.nv <= 2) return F<IT, 2, WPR>(P, st);                     \
-  if (s.nv == 3) return F<IT, 3, WPR>(P, st);                     \
-  return F<IT, MOST, WPR>(P, st);
 
 extern "C" {
 
 size_t ss_block_norm_work_elems(int64_t rows, int dim, int io_dtype) {
+  (void)io_dtype;
   if (rows < 1 || dim < 1 || dim > SS_MAX_BLOCK_NORM_DIM) return 0;
-  return (size_t)bwd_ctas(rows, shape_of(dim, io_dtype == SS_F32 ? 4 : 2, 3).wpr) * 2 * dim;
+  return (size_t)bwd_ctas(rows, shape_of(dim).wpr) * 2 * dim;
 }
 
 int ss_block_norm_fwd(const ss_block_norm_args* a, void* stream) {
@@ -130,14 +147,15 @@ int ss_block_norm_fwd(const ss_block_norm_args* a, void* stream) {
   const size_t es = a->io_dtype == SS_F32 ? 4 : 2;
   BlockNormK P;
   P.a = *a;
-  P.vec = a->dim % (int)(16 / es) == 0 && rows16(a->y, a->y_row_stride, es) &&
-          rows16(a->residual, a->residual_row_stride, es) && rows16(a->gate, a->gate_row_stride, es) &&
-          rows16(a->h, a->h_row_stride, es) && (!a->pre_weight || rows16(a->x, a->x_row_stride, es));
+  P.wvec = weights16(*a);
+  P.vec = a->dim % 4 == 0 && rows4(a->y, a->y_row_stride, es) &&
+          rows4(a->residual, a->residual_row_stride, es) && rows4(a->gate, a->gate_row_stride, es) &&
+          rows4(a->h, a->h_row_stride, es) && (!a->pre_weight || rows4(a->x, a->x_row_stride, es));
   cudaStream_t st = (cudaStream_t)stream;
   return by_dtype(a->io_dtype, [&](auto tag) -> cudaError_t {
     using IT = decltype(tag);
-    const Shape s = shape_of(a->dim, sizeof(IT), 4);
-    SSB_BN_SHAPES(fwd, 4)
+    const Shape s = shape_of(a->dim);
+    SSB_BN_SHAPES(fwd)
   });
 }
 
@@ -149,7 +167,7 @@ int ss_block_norm_bwd(const ss_block_norm_bwd_args* g, void* stream) {
   cudaStream_t st = (cudaStream_t)stream;
   const float ofs = a.unit_offset ? 1.f : 0.f;
   const size_t es = a.io_dtype == SS_F32 ? 4 : 2;
-  const Shape s = shape_of(a.dim, es, 3);
+  const Shape s = shape_of(a.dim);
   if (a.rows > 0) {
     if (!a.rstd || !g->dresidual || !g->dy || !g->work || (a.gate && !g->dgate) || (a.pre_weight && !g->dx))
       return SS_ERR_INVALID;
@@ -158,20 +176,21 @@ int ss_block_norm_bwd(const ss_block_norm_bwd_args* g, void* stream) {
       return SS_ERR_INVALID;
     BlockNormBwdK P;
     P.a = *g;
-    P.vec = a.dim % (int)(16 / es) == 0 && rows16(a.y, a.y_row_stride, es) &&
-            rows16(a.residual, a.residual_row_stride, es) && rows16(a.gate, a.gate_row_stride, es) &&
-            (!a.pre_weight || rows16(g->dx, g->dx_row_stride, es)) && rows16(g->dh, g->dh_row_stride, es) &&
-            rows16(g->dy, g->dy_row_stride, es) && rows16(g->dresidual, g->dresidual_row_stride, es) &&
-            (!a.gate || rows16(g->dgate, g->dgate_row_stride, es));
+    P.wvec = weights16(a);
+    P.vec = a.dim % 4 == 0 && rows4(a.y, a.y_row_stride, es) &&
+            rows4(a.residual, a.residual_row_stride, es) && rows4(a.gate, a.gate_row_stride, es) &&
+            (!a.pre_weight || rows4(g->dx, g->dx_row_stride, es)) && rows4(g->dh, g->dh_row_stride, es) &&
+            rows4(g->dy, g->dy_row_stride, es) && rows4(g->dresidual, g->dresidual_row_stride, es) &&
+            (!a.gate || rows4(g->dgate, g->dgate_row_stride, es));
     const int r = by_dtype(a.io_dtype, [&](auto tag) -> cudaError_t {
       using IT = decltype(tag);
-      SSB_BN_SHAPES(bwd, 3)
+      SSB_BN_SHAPES(bwd)
     });
     if (r != SS_OK) return r;
   }
   if (!g->dpost_weight && !g->dpre_weight && !g->dscale) return SS_OK;
   const dim3 grid((unsigned)((a.dim + 31) / 32), 2);
-  block_norm_cols_kernel<<<grid, 256, 0, st>>>(g->work, a.rows > 0 ? bwd_ctas(a.rows, s.wpr) : 0, a.dim, a.post_weight,
+  block_norm_cols_kernel<<<grid, 1024, 0, st>>>(g->work, a.rows > 0 ? bwd_ctas(a.rows, s.wpr) : 0, a.dim, a.post_weight,
                                                a.scale, a.scale_const, ofs, g->dpost_weight, g->dpre_weight, g->dscale);
   return record_cuda_status(cudaGetLastError());
 }

@@ -12,11 +12,13 @@
 //   X  = sum over rows of gh act(z) n:   dw_post = s X,   ds = (1 + w_post) X;   dw_pre = sum of dx h r_h
 //
 // Bound by the memory traffic: the rows stay in registers between the statistics and their use, so
-// every tensor moves once.  A row belongs to WPR warps (one up to 768 ... 1024 16-bit values, so
-// that its two reductions need no barrier), each lane holding NV 16-byte vectors of every tensor;
-// CTAs are persistent and keep the columns' factors in shared memory, and in the backward the two
-// column sums in registers until a CTA's rows are done.  The CTAs' sums meet in a second small
-// kernel in a fixed order, so the gradients of the weights do not vary between runs.
+// every tensor moves once.  A row belongs to WPR warps, each lane holding NV groups of 4 values of every
+// tensor (8 bytes of a 16-bit type, 16 of fp32): 12 values a lane keep the backward's rows, weights and
+// column sums in 128 registers, where the 24 of one warp to a row of 768 spilled (163 us a pass over
+// 16384 rows).  A row's warps meet at a barrier of their own.  A lane's columns are the same for all its
+// rows: their weights are loaded once, with the first row, and in the backward their two sums stay in
+// registers over the rows of a persistent CTA; the CTAs' sums meet in a second small kernel in a fixed
+// order, so the gradients of the weights do not vary between runs.
 #pragma once
 #include "ss_norm.cuh"
 
@@ -28,35 +30,50 @@ enum { kActNone = 0, kActSilu = 1, kActSigmoid = 2 };
 
 struct BlockNormK {
   ss_block_norm_args a;
-  int vec;
+  int vec, wvec;  // rows, weights: whole 16-byte vectors
 };
 
 struct BlockNormBwdK {
   ss_block_norm_bwd_args a;
-  int vec;
+  int vec, wvec;
 };
 
-// act(z) and its slope
-__device__ __forceinline__ void gate_act(int act, float z, float& f, float& df) {
-  const float sg = 1.f / (1.f + __expf(-z));
-  if (act == kActSilu) {
-    f = z * sg;
-    df = sg * fmaf(z, 1.f - sg, 1.f);
+// act(z) from the sigmoid of z, and its slope
+__device__ __forceinline__ float act_of(int act, float z, float sg) {
+  return act == kActSilu ? z * sg : act == kActSigmoid ? sg : z;
+}
+__device__ __forceinline__ float slope_of(int act, float z, float sg) {
+  return act == kActSilu ? sg * fmaf(z, 1.f - sg, 1.f) : act == kActSigmoid ? sg * (1.f - sg) : 1.f;
+}
+
+constexpr int kBv = 4;  // values of a vector
+
+// kBv weights of the columns from e0 on; `none` where there are no weights, 0 beyond the row
+__device__ __forceinline__ void load_weights(float (&w)[kBv], const float* p, int e0, int dim, float ofs, float none,
+                                             bool vec) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int k = 0; k < kBv; ++k) w[k] = none;
+  } else if (vec) {
+    const float4 x = e0 < dim ? __ldg(reinterpret_cast<const float4*>(p + e0)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    w[0] = x.x + ofs, w[1] = x.y + ofs, w[2] = x.z + ofs, w[3] = x.w + ofs;
   } else {
-    f = sg;
-    df = sg * (1.f - sg);
+#pragma unroll
+    for (int k = 0; k < kBv; ++k) w[k] = e0 + k < dim ? p[e0 + k] + ofs : 0.f;
   }
 }
 
-// sum over a row's WPR warps; `slot` alternates between uses so that one barrier a sum is enough
+template <typename IT> struct BnVec { using T = uint2; };
+template <> struct BnVec<float> { using T = uint4; };
+
+// sum over a row's WPR warps; `slot` alternates between uses, so that one barrier a sum is enough
 template <int WPR>
 __device__ __forceinline__ float row_sum(float v, float (*red)[kBnWarps], int slot) {
   v = warp_sum(v);
   if constexpr (WPR > 1) {
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, w0 = wid / WPR * WPR;
     if (lane == 0) red[slot][wid] = v;
-    __syncthreads();
-    const int w0 = wid / WPR * WPR;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + wid / WPR), "n"(32 * WPR) : "memory");
     v = 0.f;
 #pragma unroll
     for (int i = 0; i < WPR; ++i) v += red[slot][w0 + i];
@@ -64,233 +81,249 @@ __device__ __forceinline__ float row_sum(float v, float (*red)[kBnWarps], int sl
   return v;
 }
 
-// a row's vectors: lane `lane` of warp `part` holds elements ((j * WPR + part) * 32 + lane) * VW + k
+// a lane's first element of vector j of its row: warp `part` of WPR
+template <int WPR>
+__device__ __forceinline__ int bn_at(int j, int part, int lane) { return ((j * WPR + part) * 32 + lane) * kBv; }
+
+// streaming load of a vector, zeros where `on` is false; predicated inside, since a branch around the load
+// would wait for it before the next one is issued
+__device__ __forceinline__ uint2 ld_stream(const uint2* p, bool on) {
+  uint2 r;
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %3, 0;\n mov.u32 %0, 0;\n mov.u32 %1, 0;\n"
+               " @p ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n}\n"
+               : "=&r"(r.x), "=&r"(r.y) : "l"(p), "r"((uint32_t)on));
+  return r;
+}
+__device__ __forceinline__ uint4 ld_stream(const uint4* p, bool on) {
+  uint4 r;
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n mov.u32 %0, 0;\n mov.u32 %1, 0;\n mov.u32 %2, 0;\n mov.u32 %3, 0;\n"
+               " @p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n}\n"
+               : "=&r"(r.x), "=&r"(r.y), "=&r"(r.z), "=&r"(r.w) : "l"(p), "r"((uint32_t)on));
+  return r;
+}
+
 template <typename IT, int NV, int WPR>
-__device__ __forceinline__ void bn_load(uint4 (&q)[NV], const IT* row, int dim, int part, int lane, bool vec) {
-  constexpr int VW = 16 / sizeof(IT);
+__device__ __forceinline__ void bn_load(typename BnVec<IT>::T (&q)[NV], const IT* row, int dim, int part, int lane, bool vec) {
+  using V = typename BnVec<IT>::T;
+  if (vec) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int e0 = ((j * WPR + part) * 32 + lane) * VW;
-    if (vec) {
-      q[j] = e0 < dim ? ld_stream16(row + e0) : make_uint4(0u, 0u, 0u, 0u);
-    } else {
-      union { uint4 u; IT e[VW]; } pk;
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = bn_at<WPR>(j, part, lane);
+      q[j] = ld_stream(reinterpret_cast<const V*>(row + e0), e0 < dim);
+    }
+  } else {
 #pragma unroll
-      for (int k = 0; k < VW; ++k) pk.e[k] = (e0 + k < dim) ? row[e0 + k] : zero_v<IT>();
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = bn_at<WPR>(j, part, lane);
+      union { V u; IT e[kBv]; } pk;
+#pragma unroll
+      for (int k = 0; k < kBv; ++k) pk.e[k] = (e0 + k < dim) ? row[e0 + k] : zero_v<IT>();
       q[j] = pk.u;
     }
   }
 }
 
 template <typename IT>
-__device__ __forceinline__ void bn_store(IT* row, int e0, const float (&v)[16 / sizeof(IT)], int dim, bool vec) {
-  constexpr int VW = 16 / sizeof(IT);
+__device__ __forceinline__ void bn_store(IT* row, int e0, const float (&v)[kBv], int dim, bool vec) {
+  using V = typename BnVec<IT>::T;
   if (e0 >= dim) return;
   if (vec) {
-    uint4 pk;
-    IT* e = reinterpret_cast<IT*>(&pk);
+    union { V u; IT e[kBv]; } pk;
 #pragma unroll
-    for (int k = 0; k < VW; ++k) e[k] = from_f<IT>(v[k]);
-    *reinterpret_cast<uint4*>(row + e0) = pk;
+    for (int k = 0; k < kBv; ++k) pk.e[k] = from_f<IT>(v[k]);
+    *reinterpret_cast<V*>(row + e0) = pk.u;
   } else {
 #pragma unroll
-    for (int k = 0; k < VW; ++k)
+    for (int k = 0; k < kBv; ++k)
       if (e0 + k < dim) row[e0 + k] = from_f<IT>(v[k]);
   }
 }
 
 template <typename IT>
-__device__ __forceinline__ float lane_of(const uint4& q, int k) {
-  return to_f<IT>(reinterpret_cast<const IT*>(&q)[k]);
+__device__ __forceinline__ void unpack(float (&v)[kBv], const typename BnVec<IT>::T& q) {
+  union { typename BnVec<IT>::T u; IT e[kBv]; } pk;
+  pk.u = q;
+#pragma unroll
+  for (int k = 0; k < kBv; ++k) v[k] = to_f<IT>(pk.e[k]);
 }
 
-template <typename IT, int NV, int WPR>
+// MODE: 0 any call; 1 both norms, whole vectors (and dh in the backward), no gate; 2 the same with a SiLU
+// gate.  The common calls know at compile time what the others branch on for every vector (norm_train: 159
+// -> see below).
+enum { kBnAny = 0, kBnPlain = 1, kBnGated = 2 };
+
+template <typename IT, int NV, int WPR, int MODE>
 __global__ void __launch_bounds__(32 * kBnWarps) block_norm_fwd_kernel(const __grid_constant__ BlockNormK P) {
-  constexpr int VW = 16 / sizeof(IT);
-  constexpr int LEN = NV * WPR * 32 * VW;
+  using V = typename BnVec<IT>::T;
   constexpr int RPC = kBnWarps / WPR;  // rows of a CTA at a time
-  extern __shared__ __align__(16) float w_s[];  // [0, LEN): s (1 + w_post); [LEN, 2 LEN): 1 + w_pre
   __shared__ float red[2][kBnWarps];
   const ss_block_norm_args& a = P.a;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, part = wid % WPR;
   const int dim = a.dim;
-  const bool gate = a.gate != nullptr, post = a.post_weight != nullptr, pre = a.pre_weight != nullptr;
+  const bool gate = MODE ? MODE == kBnGated : a.gate != nullptr, post = MODE || a.post_weight != nullptr,
+             pre = MODE || a.pre_weight != nullptr, vec = MODE || P.vec, wvec = MODE || P.wvec;
+  const int act = MODE ? (int)kActSilu : a.activation;
   const float ofs = a.unit_offset ? 1.f : 0.f, inv = 1.f / (float)dim;
-  for (int e = threadIdx.x; e < LEN; e += blockDim.x) {
-    const bool on = e < dim;
-    w_s[e] = on ? (a.scale ? a.scale[e] : a.scale_const) * (post ? a.post_weight[e] + ofs : 1.f) : 0.f;
-    w_s[LEN + e] = on && pre ? a.pre_weight[e] + ofs : 0.f;
-  }
-  __syncthreads();
-  for (int64_t r0 = (int64_t)blockIdx.x * RPC; r0 < a.rows; r0 += (int64_t)gridDim.x * RPC) {
-    const int64_t row = r0 + wid / WPR;
-    const bool on = row < a.rows;  // the same for the row's warps; idle ones only join the barriers
-    uint4 yq[NV], rq[NV], zq[NV];
-    float h[NV][VW];
-    float ss = 0.f;
-    if (on) {
-      bn_load<IT, NV, WPR>(yq, (const IT*)a.y + row * a.y_row_stride, dim, part, lane, P.vec);
-      bn_load<IT, NV, WPR>(rq, (const IT*)a.residual + row * a.residual_row_stride, dim, part, lane, P.vec);
-      if (gate) bn_load<IT, NV, WPR>(zq, (const IT*)a.gate + row * a.gate_row_stride, dim, part, lane, P.vec);
-      if (post) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int k = 0; k < VW; ++k) {
-            const float y = lane_of<IT>(yq[j], k);
-            ss = fmaf(y, y, ss);
-          }
-      }
-    }
-    float ry = 1.f;
-    if (post) ry = rsqrtf(fmaf(row_sum<WPR>(ss, red, 0), inv, a.eps));
-    ss = 0.f;
-    if (on) {
+  float w[NV][kBv], wn[NV][kBv];  // s (1 + w_post), 1 + w_pre
+  for (int64_t first = (int64_t)blockIdx.x * RPC + wid / WPR, row = first; row < a.rows; row += (int64_t)gridDim.x * RPC) {
+    V yq[NV], rq[NV], zq[NV];
+    bn_load<IT, NV, WPR>(yq, (const IT*)a.y + row * a.y_row_stride, dim, part, lane, vec);
+    bn_load<IT, NV, WPR>(rq, (const IT*)a.residual + row * a.residual_row_stride, dim, part, lane, vec);
+    if (gate) bn_load<IT, NV, WPR>(zq, (const IT*)a.gate + row * a.gate_row_stride, dim, part, lane, vec);
+    if (row == first) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int e0 = ((j * WPR + part) * 32 + lane) * VW;
+        const int e0 = bn_at<WPR>(j, part, lane);
+        float sc[kBv];
+        load_weights(w[j], a.post_weight, e0, dim, ofs, 1.f, wvec);
+        load_weights(sc, a.scale, e0, dim, 0.f, a.scale_const, wvec);
+        load_weights(wn[j], a.pre_weight, e0, dim, ofs, 1.f, wvec);
 #pragma unroll
-        for (int k = 0; k < VW; ++k) {
-          float u = lane_of<IT>(yq[j], k) * ry * w_s[e0 + k];
-          if (gate) {
-            float f = lane_of<IT>(zq[j], k), df;
-            if (a.activation != kActNone) gate_act(a.activation, f, f, df);
-            u *= f;
-          }
-          h[j][k] = lane_of<IT>(rq[j], k) + u;
-          ss = fmaf(h[j][k], h[j][k], ss);
-        }
-        bn_store<IT>((IT*)a.h + row * a.h_row_stride, e0, h[j], dim, P.vec);
+        for (int k = 0; k < kBv; ++k) w[j][k] *= sc[k];
       }
+    }
+    float h[NV][kBv];
+    float ss = 0.f, ry = 1.f;
+    if (post) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float y[kBv];
+        unpack<IT>(y, yq[j]);
+#pragma unroll
+        for (int k = 0; k < kBv; ++k) ss = fmaf(y[k], y[k], ss);
+      }
+      ry = rsqrtf(fmaf(row_sum<WPR>(ss, red, 0), inv, a.eps));
+    }
+    ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float y[kBv], z[kBv];
+      unpack<IT>(y, yq[j]);
+      unpack<IT>(h[j], rq[j]);
+      if (gate) unpack<IT>(z, zq[j]);
+#pragma unroll
+      for (int k = 0; k < kBv; ++k) {
+        float u = y[k] * ry * w[j][k];
+        if (gate) u *= act_of(act, z[k], sigmoid_fast(z[k]));
+        h[j][k] += u;
+        ss = fmaf(h[j][k], h[j][k], ss);
+      }
+      bn_store<IT>((IT*)a.h + row * a.h_row_stride, bn_at<WPR>(j, part, lane), h[j], dim, vec);
     }
     float rh = 0.f;
     if (pre) {
       rh = rsqrtf(fmaf(row_sum<WPR>(ss, red, 1), inv, a.pre_eps));
-      if (on) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int e0 = ((j * WPR + part) * 32 + lane) * VW;
+      for (int j = 0; j < NV; ++j) {
 #pragma unroll
-          for (int k = 0; k < VW; ++k) h[j][k] *= rh * w_s[LEN + e0 + k];
-          bn_store<IT>((IT*)a.x + row * a.x_row_stride, e0, h[j], dim, P.vec);
-        }
+        for (int k = 0; k < kBv; ++k) h[j][k] *= rh * wn[j][k];
+        bn_store<IT>((IT*)a.x + row * a.x_row_stride, bn_at<WPR>(j, part, lane), h[j], dim, vec);
       }
     }
-    if (on && a.rstd && part == 0 && lane == 0) {
-      a.rstd[2 * row] = ry;
-      a.rstd[2 * row + 1] = rh;
-    }
+    if (a.rstd && part == 0 && lane == 0) *reinterpret_cast<float2*>(a.rstd + 2 * row) = make_float2(ry, rh);
     // one sum a row: without the other's barrier the next row's write could meet this row's reads
-    if (WPR > 1 && !(post && pre)) __syncthreads();
+    if (WPR > 1 && !(post && pre)) asm volatile("bar.sync %0, %1;" ::"r"(1 + wid / WPR), "n"(32 * WPR) : "memory");
   }
 }
 
-template <typename IT, int NV, int WPR>
-__global__ void __launch_bounds__(32 * kBnWarps) block_norm_bwd_kernel(const __grid_constant__ BlockNormBwdK P) {
-  constexpr int VW = 16 / sizeof(IT);
-  constexpr int LEN = NV * WPR * 32 * VW;
+template <typename IT, int NV, int WPR, int MODE>
+__global__ void __launch_bounds__(32 * kBnWarps, 2)
+    block_norm_bwd_kernel(const __grid_constant__ BlockNormBwdK P) {
+  using V = typename BnVec<IT>::T;
   constexpr int RPC = kBnWarps / WPR;
-  extern __shared__ __align__(16) float w_s[];  // factors as in the forward; then the rows' column sums
+  extern __shared__ __align__(16) float sums[];  // a column sum of the CTA's rows
   __shared__ float red[2][kBnWarps];
   const ss_block_norm_args& a = P.a.f;
   const ss_block_norm_bwd_args& g = P.a;
+  const bool has_dh = MODE || g.dh != nullptr;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, part = wid % WPR;
   const int dim = a.dim;
-  const bool gate = a.gate != nullptr, post = a.post_weight != nullptr, pre = a.pre_weight != nullptr;
+  const bool gate = MODE ? MODE == kBnGated : a.gate != nullptr, post = MODE || a.post_weight != nullptr,
+             pre = MODE || a.pre_weight != nullptr, vec = MODE || P.vec, wvec = MODE || P.wvec;
+  const int act = MODE ? (int)kActSilu : a.activation;
   const float ofs = a.unit_offset ? 1.f : 0.f, inv = 1.f / (float)dim;
-  for (int e = threadIdx.x; e < LEN; e += blockDim.x) {
-    const bool on = e < dim;
-    w_s[e] = on ? (a.scale ? a.scale[e] : a.scale_const) * (post ? a.post_weight[e] + ofs : 1.f) : 0.f;
-    w_s[LEN + e] = on && pre ? a.pre_weight[e] + ofs : 0.f;
+  float w[NV][kBv], wn[NV][kBv], sx[NV][kBv], sp[NV][kBv];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int e0 = bn_at<WPR>(j, part, lane);
+    float sc[kBv];
+    load_weights(w[j], a.post_weight, e0, dim, ofs, 1.f, wvec);
+    load_weights(sc, a.scale, e0, dim, 0.f, a.scale_const, wvec);
+    load_weights(wn[j], a.pre_weight, e0, dim, ofs, 1.f, wvec);
+#pragma unroll
+    for (int k = 0; k < kBv; ++k) w[j][k] *= sc[k], sx[j][k] = sp[j][k] = 0.f;
   }
-  float sx[NV][VW], sp[NV][VW];
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int k = 0; k < VW; ++k) sx[j][k] = sp[j][k] = 0.f;
-  __syncthreads();
-  for (int64_t r0 = (int64_t)blockIdx.x * RPC; r0 < a.rows; r0 += (int64_t)gridDim.x * RPC) {
-    const int64_t row = r0 + wid / WPR;
-    const bool on = row < a.rows;
-    uint4 yq[NV], rq[NV], zq[NV], xq[NV], hq[NV];
-    float ry = 1.f, rh = 0.f;
-    float h[NV][VW];  // h, then gh
+  for (int64_t row = (int64_t)blockIdx.x * RPC + wid / WPR; row < a.rows; row += (int64_t)gridDim.x * RPC) {
+    V yq[NV], rq[NV], zq[NV], xq[NV], hq[NV];
+    bn_load<IT, NV, WPR>(yq, (const IT*)a.y + row * a.y_row_stride, dim, part, lane, vec);
+    bn_load<IT, NV, WPR>(rq, (const IT*)a.residual + row * a.residual_row_stride, dim, part, lane, vec);
+    if (gate) bn_load<IT, NV, WPR>(zq, (const IT*)a.gate + row * a.gate_row_stride, dim, part, lane, vec);
+    if (pre) bn_load<IT, NV, WPR>(xq, (const IT*)g.dx + row * g.dx_row_stride, dim, part, lane, vec);
+    if (has_dh) bn_load<IT, NV, WPR>(hq, (const IT*)g.dh + row * g.dh_row_stride, dim, part, lane, vec);
+    const float2 rr = *reinterpret_cast<const float2*>(a.rstd + 2 * row);
+    const float ry = rr.x, rh = rr.y;
+    float h[NV][kBv];  // h, then u
     float dot = 0.f;
-    if (on) {
-      bn_load<IT, NV, WPR>(yq, (const IT*)a.y + row * a.y_row_stride, dim, part, lane, P.vec);
-      bn_load<IT, NV, WPR>(rq, (const IT*)a.residual + row * a.residual_row_stride, dim, part, lane, P.vec);
-      if (gate) bn_load<IT, NV, WPR>(zq, (const IT*)a.gate + row * a.gate_row_stride, dim, part, lane, P.vec);
-      if (pre) bn_load<IT, NV, WPR>(xq, (const IT*)g.dx + row * g.dx_row_stride, dim, part, lane, P.vec);
-      if (g.dh) bn_load<IT, NV, WPR>(hq, (const IT*)g.dh + row * g.dh_row_stride, dim, part, lane, P.vec);
-      ry = a.rstd[2 * row];
-      rh = a.rstd[2 * row + 1];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int e0 = ((j * WPR + part) * 32 + lane) * VW;
+    for (int j = 0; j < NV; ++j) {
+      float y[kBv], z[kBv], d[kBv];
+      unpack<IT>(y, yq[j]);
+      unpack<IT>(h[j], rq[j]);
+      if (gate) unpack<IT>(z, zq[j]);
+      if (pre) unpack<IT>(d, xq[j]);
 #pragma unroll
-        for (int k = 0; k < VW; ++k) {
-          float u = lane_of<IT>(yq[j], k) * ry * w_s[e0 + k];
-          if (gate) {
-            float f = lane_of<IT>(zq[j], k), df;
-            if (a.activation != kActNone) gate_act(a.activation, f, f, df);
-            u *= f;
-          }
-          h[j][k] = lane_of<IT>(rq[j], k) + u;
-          if (pre) {
-            const float d = lane_of<IT>(xq[j], k);
-            dot = fmaf(d * w_s[LEN + e0 + k], h[j][k], dot);
-            sp[j][k] = fmaf(d, h[j][k] * rh, sp[j][k]);
-          }
+      for (int k = 0; k < kBv; ++k) {
+        float u = y[k] * ry * w[j][k];
+        if (gate) u *= act_of(act, z[k], sigmoid_fast(z[k]));
+        h[j][k] += u;
+        if (pre) {
+          dot = fmaf(d[k] * wn[j][k], h[j][k], dot);
+          sp[j][k] = fmaf(d[k], h[j][k] * rh, sp[j][k]);
         }
       }
     }
     float c = 0.f;
     if (pre) c = row_sum<WPR>(dot, red, 0) * inv * rh * rh;
     dot = 0.f;
-    if (on) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int e0 = ((j * WPR + part) * 32 + lane) * VW;
-        float dz[VW];
+    for (int j = 0; j < NV; ++j) {
+      float y[kBv], z[kBv], d[kBv], gh[kBv], dz[kBv];
+      unpack<IT>(y, yq[j]);
+      if (gate) unpack<IT>(z, zq[j]);
+      if (pre) unpack<IT>(d, xq[j]);
+      if (has_dh) unpack<IT>(gh, hq[j]);
 #pragma unroll
-        for (int k = 0; k < VW; ++k) {
-          float gh = g.dh ? lane_of<IT>(hq[j], k) : 0.f;
-          if (pre) gh = fmaf(rh, fmaf(lane_of<IT>(xq[j], k), w_s[LEN + e0 + k], -h[j][k] * c), gh);
-          const float n = lane_of<IT>(yq[j], k) * ry, w = w_s[e0 + k];
-          float f = 1.f, df = 1.f;
-          if (gate) {
-            f = lane_of<IT>(zq[j], k);
-            if (a.activation != kActNone) gate_act(a.activation, f, f, df);
-          }
-          dz[k] = gh * w * n * df;
-          sx[j][k] = fmaf(gh * f, n, sx[j][k]);
-          dot = fmaf(gh * w * f, n, dot);
-          h[j][k] = gh;
+      for (int k = 0; k < kBv; ++k) {
+        if (!has_dh) gh[k] = 0.f;
+        if (pre) gh[k] = fmaf(rh, fmaf(d[k], wn[j][k], -h[j][k] * c), gh[k]);
+        const float n = y[k] * ry;
+        float f = 1.f;
+        if (gate) {
+          const float sg = sigmoid_fast(z[k]);
+          f = act_of(act, z[k], sg);
+          dz[k] = gh[k] * w[j][k] * n * slope_of(act, z[k], sg);
         }
-        bn_store<IT>((IT*)g.dresidual + row * g.dresidual_row_stride, e0, h[j], dim, P.vec);
-        if (gate) bn_store<IT>((IT*)g.dgate + row * g.dgate_row_stride, e0, dz, dim, P.vec);
+        sx[j][k] = fmaf(gh[k] * f, n, sx[j][k]);
+        h[j][k] = gh[k] * w[j][k] * f;
+        dot = fmaf(h[j][k], n, dot);
       }
+      const int e0 = bn_at<WPR>(j, part, lane);
+      bn_store<IT>((IT*)g.dresidual + row * g.dresidual_row_stride, e0, gh, dim, vec);
+      if (gate) bn_store<IT>((IT*)g.dgate + row * g.dgate_row_stride, e0, dz, dim, vec);
     }
     float m = 0.f;
     if (post) m = row_sum<WPR>(dot, red, 1) * inv;
-    if (on) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int e0 = ((j * WPR + part) * 32 + lane) * VW;
+    for (int j = 0; j < NV; ++j) {
+      if (post) {
+        float y[kBv];
+        unpack<IT>(y, yq[j]);
 #pragma unroll
-        for (int k = 0; k < VW; ++k) {
-          float f = 1.f, df;
-          if (gate) {
-            f = lane_of<IT>(zq[j], k);
-            if (a.activation != kActNone) gate_act(a.activation, f, f, df);
-          }
-          const float u = h[j][k] * w_s[e0 + k] * f;
-          h[j][k] = post ? ry * (u - lane_of<IT>(yq[j], k) * ry * m) : u;
-        }
-        bn_store<IT>((IT*)g.dy + row * g.dy_row_stride, e0, h[j], dim, P.vec);
+        for (int k = 0; k < kBv; ++k) h[j][k] = ry * (h[j][k] - y[k] * ry * m);
       }
+      bn_store<IT>((IT*)g.dy + row * g.dy_row_stride, bn_at<WPR>(j, part, lane), h[j], dim, vec);
     }
-    if (WPR > 1 && !(post && pre)) __syncthreads();
+    if (WPR > 1 && !(post && pre)) asm volatile("bar.sync %0, %1;" ::"r"(1 + wid / WPR), "n"(32 * WPR) : "memory");
   }
   // this CTA's column sums: its row groups in order, then to the workspace
   __syncthreads();
@@ -299,38 +332,38 @@ __global__ void __launch_bounds__(32 * kBnWarps) block_norm_bwd_kernel(const __g
     for (int r = 0; r < RPC; ++r) {
       if (wid / WPR == r) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int k = 0; k < VW; ++k) {
-            const int e = ((j * WPR + part) * 32 + lane) * VW + k;
-            const float v = s ? sp[j][k] : sx[j][k];
-            w_s[e] = r ? w_s[e] + v : v;
-          }
+        for (int j = 0; j < NV; ++j) {
+          const float4 v = s ? make_float4(sp[j][0], sp[j][1], sp[j][2], sp[j][3])
+                             : make_float4(sx[j][0], sx[j][1], sx[j][2], sx[j][3]);
+          float4* to = reinterpret_cast<float4*>(sums + bn_at<WPR>(j, part, lane));
+          const float4 x = r ? *to : make_float4(0.f, 0.f, 0.f, 0.f);
+          *to = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
+        }
       }
       __syncthreads();
     }
-    for (int e = threadIdx.x; e < dim; e += blockDim.x) out[s * dim + e] = w_s[e];
+    for (int e = threadIdx.x; e < dim; e += blockDim.x) out[s * dim + e] = sums[e];
     __syncthreads();
   }
 }
 
-// Column sums over the CTAs' partial sums: 32 columns and 8 slices of the CTAs per block, added in
+// Column sums over the CTAs' partial sums: 32 columns and 32 slices of the CTAs per block, added in
 // a fixed order.
-__global__ void __launch_bounds__(256) block_norm_cols_kernel(const float* work, int parts, int dim,
+__global__ void __launch_bounds__(1024) block_norm_cols_kernel(const float* work, int parts, int dim,
                                                               const float* post_weight, const float* scale,
                                                               float scale_const, float ofs, float* dpost, float* dpre,
                                                               float* dscale) {
-  __shared__ float red[8][33];
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + lane, which = blockIdx.y;
   float s = 0.f;
   if (col < dim)
-    for (int i = wid; i < parts; i += 8) s += work[((int64_t)i * 2 + which) * dim + col];
+    for (int i = wid; i < parts; i += 32) s += work[((int64_t)i * 2 + which) * dim + col];
   red[wid][lane] = s;
   __syncthreads();
   if (wid == 0 && col < dim) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += red[i][lane];
+    for (int i = 1; i < 32; ++i) s += red[i][lane];
     if (which) {
       if (dpre) dpre[col] = s;
     } else {
