@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -271,11 +272,9 @@ def lib():
                 L.ss_rmsnorm_fwd.argtypes = [ctypes.POINTER(RmsNormArgs), c_vp]
                 L.ss_rmsnorm_bwd.argtypes = [ctypes.POINTER(RmsNormBwdArgs), c_vp]
                 L.ss_mamba_step.argtypes = [ctypes.POINTER(MambaStepArgs), c_vp]
-                for f, st in (("ss_linear_fwd", LinearArgs), ("ss_linear_bwd", LinearBwdArgs),
-                              ("ss_linear_step", LinearStepArgs), ("ss_block_norm_fwd", BlockNormArgs),
-                              ("ss_block_norm_bwd", BlockNormBwdArgs), ("ss_beam_select", BeamArgs),
-                              ("ss_reorder", ReorderArgs)):
-                    getattr(L, f).argtypes = [ctypes.POINTER(st), c_vp]
+                for f in ("ss_linear_fwd", "ss_linear_bwd", "ss_linear_step", "ss_block_norm_fwd", "ss_block_norm_bwd",
+                          "ss_beam_select", "ss_reorder"):
+                    getattr(L, f).argtypes = [c_vp, c_vp]  # a struct's address, or its packed bytes
                     getattr(L, f).restype = c_int
                 L.ss_linear_work_bytes.argtypes = [ctypes.POINTER(LinearArgs), c_int]
                 L.ss_block_norm_work_elems.argtypes = [c_i64, c_int, c_int]
@@ -342,6 +341,38 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 def stream_of(device: torch.device) -> int:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     return _raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+_CODES = {c_int: "i", c_i64: "q", c_vp: "P", ctypes.c_float: "f"}
+
+
+def _codes(st):
+    for _, t in st._fields_:
+        if issubclass(t, ctypes.Structure):
+            yield from _codes(t)
+        elif issubclass(t, ctypes.Array):
+            yield str(t._length_) + _CODES[t._type_]
+        else:
+            yield _CODES[t]
+
+
+def packer(st):
+    """A function of a struct's values, in order (pointers as integers, 0 for null), that returns its bytes: a
+    fraction of the time that building the ctypes struct takes, which a single-token call feels."""
+    return struct.Struct("@" + "".join(_codes(st))).pack
+
+
+def launch(name: str, packed: bytes, device: torch.device) -> None:
+    """Call the library's function `name` with packed arguments on `device`'s current stream."""
+    f = getattr(_lib or lib(), name)
+    idx = device.index
+    if idx == torch._C._cuda_getDevice():
+        rc = f(packed, stream_of(device))
+    else:
+        with torch.cuda.device(idx):
+            rc = f(packed, stream_of(device))
+    if rc:
+        check(rc, name)
 
 
 def device_status(device, reset: bool = True) -> int:

@@ -10,7 +10,9 @@ from . import _lib as L
 from .selective_scan_interface import _cuda_device
 
 
-@torch.no_grad()
+_pack_beam, _pack_reorder = L.packer(L.BeamArgs), L.packer(L.ReorderArgs)
+
+
 def beam_select(logits, scores, num_select=None, finished=None, eos_token_id=None):
     """The num_select best continuations of every batch row.
 
@@ -44,27 +46,24 @@ def beam_select(logits, scores, num_select=None, finished=None, eos_token_id=Non
         finished = finished.contiguous()
     io = L.dtype_code(logits.dtype)
     x = logits if (logits.stride(-1) == 1 or vocab == 1) and min(logits.stride()) >= 0 else logits.contiguous()
-    s = scores.to(torch.float32).contiguous()
+    s = scores if scores.dtype == torch.float32 and scores.is_contiguous() else scores.to(torch.float32).contiguous()
     out = torch.empty((b, k), dtype=torch.float32, device=dev)
-    parents, tokens = (torch.empty((b, k), dtype=torch.int64, device=dev) for _ in range(2))
-    n = int(L.lib().ss_beam_work_bytes(b, w, vocab, k))
-    work = torch.empty(n, dtype=torch.uint8, device=dev)
-    args = L.BeamArgs(b, w, vocab, k, io, eos, x.data_ptr(), x.stride(0), x.stride(1), s.data_ptr(), L.ptr(finished),
-                      out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), work.data_ptr())
-    with torch.cuda.device(dev):
-        L.check(L.lib().ss_beam_select(args, L.stream_of(dev)), "ss_beam_select")
+    parents = torch.empty((b, k), dtype=torch.int64, device=dev)
+    tokens = torch.empty((b, k), dtype=torch.int64, device=dev)
+    work = torch.empty(int(L.lib().ss_beam_work_bytes(b, w, vocab, k)), dtype=torch.uint8, device=dev)
+    L.launch("ss_beam_select", _pack_beam(b, w, vocab, k, io, eos, x.data_ptr(), x.stride(0), x.stride(1), s.data_ptr(),
+                                          0 if finished is None else finished.data_ptr(), out.data_ptr(),
+                                          parents.data_ptr(), tokens.data_ptr(), work.data_ptr()), dev)
     return out, parents, tokens
 
 
-@torch.no_grad()
 def reorder_states(states, parents):
     """Put per-beam rows in their new order, in place: for every tensor of ``states`` ((batch * beams, ...)
     contiguous, rows of a multiple of 4 bytes) and every batch row, row w becomes what row
     parents[:, w] was.  parents: (batch, beams) int64 (its beams may be a slice of a wider result of
     ``beam_select``).  A parent outside the beams leaves its row as it was, and the next
     ``check_device_status`` raises.  Tensors that share memory are refused."""
-    states = list(states)
-    dev = _cuda_device(parents, *states)
+    _cuda_device(parents)
     if parents.dim() != 2 or parents.dtype != torch.int64:
         raise ValueError(f"parents must be (batch, beams) int64, got {parents.dtype} {tuple(parents.shape)}")
     b, w = parents.shape
@@ -72,24 +71,27 @@ def reorder_states(states, parents):
         raise ValueError("parents must name at least one beam")
     if w > L.MAX_BEAMS:
         raise NotImplementedError(f"{w} beams are more than {L.MAX_BEAMS}")
-    rows = []
+    total, dev, rows = b * w, parents.get_device(), []
     for t in states:
-        if t.dim() < 1 or t.shape[0] != b * w or not t.is_contiguous():
-            raise ValueError(f"a state must have {b * w} contiguous rows, got {tuple(t.shape)}")
-        n = t.numel() // max(t.shape[0], 1) * t.element_size()
-        if n % 4:
-            raise NotImplementedError(f"rows of {n} bytes (a multiple of 4 is supported)")
-        if n and b:
+        if t.get_device() != dev:
+            raise RuntimeError(f"tensors on different devices: {parents.device} and {t.device}")
+        if t.dim() < 1 or t.size(0) != total or not t.is_contiguous():
+            raise ValueError(f"a state must have {total} contiguous rows, got {tuple(t.shape)}")
+        n = t.nbytes
+        if n:
+            if n % (4 * total):
+                raise NotImplementedError(f"rows of {n / total} bytes (a multiple of 4 is supported)")
             rows.append((t.data_ptr(), n))
     rows.sort()
-    for (p, n), (q, _) in zip(rows, rows[1:]):
-        if p + n * b * w > q:
+    end = 0
+    for at, n in rows:
+        if at < end:
             raise ValueError("states must not share memory")
+        end = at + n
     p = parents if parents.stride(1) == 1 or w == 1 else parents.contiguous()
-    with torch.cuda.device(dev):
-        for i in range(0, len(rows), L.MAX_REORDER):
-            part = rows[i:i + L.MAX_REORDER]
-            args = L.ReorderArgs(b, w, len(part), p.data_ptr(), p.stride(0) if b > 1 else w)
-            args.data[:len(part)] = [q for q, _ in part]
-            args.row_bytes[:len(part)] = [n for _, n in part]
-            L.check(L.lib().ss_reorder(args, L.stream_of(dev)), "ss_reorder")
+    for i in range(0, len(rows), L.MAX_REORDER):
+        part = rows[i:i + L.MAX_REORDER]
+        none = (0,) * (L.MAX_REORDER - len(part))
+        L.launch("ss_reorder", _pack_reorder(b, w, len(part), p.data_ptr(), p.stride(0) if b > 1 else w,
+                                             *[at for at, _ in part], *none, *[n // total for _, n in part], *none),
+                 parents.device)

@@ -16,6 +16,7 @@ and head,
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -25,12 +26,21 @@ from . import _lib as L
 from .selective_scan_interface import _cuda_device
 
 
-def _unit(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+_pack_fwd, _pack_bwd, _pack_step = (L.packer(st) for st in (L.LinearArgs, L.LinearBwdArgs, L.LinearStepArgs))
+_NONE4 = (0, 0, 0, 0)
 
 
-def _strides(t):
+def _as(t, dtype):
+    return t if t.dtype == dtype else t.to(dtype)
+
+
+def _at(t):
+    """Address and the strides but the innermost."""
     return t.data_ptr(), *t.stride()[:-1]
+
+
+def _p(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _decay(log_decay, io):
@@ -44,24 +54,24 @@ def _scale(scale, key_dim):
     return s
 
 
-def _check_heads(q, k, v, lead):
-    """q, k: (*lead, key_heads, key_dim), v: (*lead, heads, value_dim)."""
-    n = len(lead) + 2
-    names = "(batch, seqlen, heads, dim)" if n == 4 else "(batch, heads, dim)"
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != n:
-            raise ValueError(f"{name} must be {names}, got shape {tuple(t.shape)}")
-        if tuple(t.shape[:-2]) != tuple(lead):
-            raise ValueError(f"q, k and v must share their leading shape: {name} has {tuple(t.shape)}")
-    if q.shape != k.shape:
-        raise ValueError(f"q and k must have the same shape, got {tuple(q.shape)} and {tuple(k.shape)}")
-    heads, key_heads = v.shape[-2], k.shape[-2]
-    if key_heads < 1 or heads < 1 or heads % key_heads:
-        raise ValueError(f"the heads of v ({heads}) must be a multiple of those of q and k ({key_heads})")
-    if min(k.shape[-1], v.shape[-1]) < 1:
+def _check_heads(q, k, v, n):
+    """q, k: (..., key_heads, key_dim), v: (..., heads, value_dim), n axes each.  Returns their sizes."""
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != n or len(ks) != n or len(vs) != n:
+        names = "(batch, seqlen, heads, dim)" if n == 4 else "(batch, heads, dim)"
+        raise ValueError(f"q, k and v must be {names}, got {tuple(qs)}, {tuple(ks)} and {tuple(vs)}")
+    if qs != ks:
+        raise ValueError(f"q and k must have the same shape, got {tuple(qs)} and {tuple(ks)}")
+    if ks[:-2] != vs[:-2]:
+        raise ValueError(f"q, k and v must share their leading shape, got {tuple(ks)} and {tuple(vs)}")
+    (hk, dk), (h, dv) = ks[-2:], vs[-2:]
+    if hk < 1 or h < 1 or h % hk:
+        raise ValueError(f"the heads of v ({h}) must be a multiple of those of q and k ({hk})")
+    if dk < 1 or dv < 1:
         raise ValueError("head sizes must be at least 1")
-    if max(k.shape[-1], v.shape[-1]) > L.MAX_LINEAR_DIM:
-        raise NotImplementedError(f"head sizes above {L.MAX_LINEAR_DIM}: {k.shape[-1]}, {v.shape[-1]}")
+    if dk > L.MAX_LINEAR_DIM or dv > L.MAX_LINEAR_DIM:
+        raise NotImplementedError(f"head sizes above {L.MAX_LINEAR_DIM}: {dk}, {dv}")
+    return h, hk, dk, dv
 
 
 def _check_state(t, shape, name):
@@ -69,101 +79,116 @@ def _check_state(t, shape, name):
         raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
 
 
-class _Call:
-    """Validated, normalised operands of one sequence call."""
+@functools.lru_cache(maxsize=1024)
+def _work_bytes(sizes, io, decay, backward):
+    args = L.LinearArgs(*sizes, io, decay)
+    return int(L.lib().ss_linear_work_bytes(args, backward))
 
-    def __init__(self, q, k, v, log_decay, scale, initial_state, seq_lens):
-        self.device = _cuda_device(q, k, v, log_decay, initial_state, seq_lens)
-        io = v.dtype
-        L.dtype_code(io)
-        _check_heads(q, k, v, tuple(v.shape[:2]) if v.dim() == 4 else (0, 0))
-        self.b, self.l, self.h, self.dv = v.shape
-        self.hk, self.dk = k.shape[2:]
-        self.io, self.scale = io, _scale(scale, self.dk)
-        if tuple(log_decay.shape) not in ((self.h,), (self.b, self.l, self.h)):
-            raise ValueError(f"log_decay must be ({self.h},) or {(self.b, self.l, self.h)}, got {tuple(log_decay.shape)}")
-        self.q, self.k, self.v = (_unit(t if t.dtype == io else t.to(io)) for t in (q, k, v))
-        self.g = _decay(log_decay, io)
-        if self.g.dim() == 3 and self.g.stride(0) == 0 and self.g.stride(1) == 0:
-            self.g = self.g.contiguous()  # an expanded tensor still has a gradient for every token
-        self.state = None
-        if initial_state is not None:
-            _check_state(initial_state, (self.b, self.h, self.dk, self.dv), "initial_state")
-            self.state = initial_state.to(torch.float32).contiguous()
-        self.lens = None
-        if seq_lens is not None:
-            if tuple(seq_lens.shape) != (self.b,) or seq_lens.is_floating_point() or seq_lens.dtype == torch.bool:
-                raise ValueError(f"seq_lens must be ({self.b},) integers, got {seq_lens.dtype} {tuple(seq_lens.shape)}")
-            self.lens = seq_lens.clamp(0, self.l).to(torch.int32).contiguous() if seq_lens.dtype != torch.int32 \
-                else seq_lens.contiguous()
 
-    def args(self, o=None, state_out=None):
-        g = (0, 0, self.g.stride(0)) if self.g.dim() == 1 else self.g.stride()
-        return L.LinearArgs(
-            self.b, self.l, self.h, self.hk, self.dk, self.dv, L.dtype_code(self.io), L.dtype_code(self.g.dtype),
-            self.scale, *_strides(self.q), *_strides(self.k), *_strides(self.v), self.g.data_ptr(), *g,
-            L.ptr(self.lens), L.ptr(self.state), L.ptr(state_out), *((None, 0, 0, 0) if o is None else _strides(o)),
-            None)
+def _work(c, backward, device):
+    n = _work_bytes(c[:6], c[6], c[7], backward)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
-    def work(self, args, backward):
-        n = int(L.lib().ss_linear_work_bytes(args, int(backward)))
-        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
 
-    def forward(self, want_final):
-        o = torch.empty((self.b, self.l, self.h, self.dv), dtype=self.io, device=self.device)
-        final = None
-        if want_final:
-            final = torch.empty((self.b, self.h, self.dk, self.dv), dtype=torch.float32, device=self.device)
-        args = self.args(o, final)
-        work = self.work(args, False)
-        args.work = L.ptr(work)
-        with torch.cuda.device(self.device):
-            L.check(L.lib().ss_linear_fwd(args, L.stream_of(self.device)), "ss_linear_fwd")
-            L.maybe_check_status(self.device, "ss_linear_fwd")
-        return o, final
+def _whole(t):
+    """t with rows of whole 16-byte units, as the tensor-core kernel's copies need them: itself where it has them."""
+    if t.shape[-1] % 8:
+        return torch.nn.functional.pad(t, (0, -t.shape[-1] % 8))
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+        n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
-    def backward(self, dout, dfinal, final, want_decay, want_state):
-        new = lambda t, dtype=None: torch.empty(t.shape, dtype=dtype or t.dtype, device=self.device)  # noqa: E731
-        dout = _unit(dout if dout.dtype == self.io else dout.to(self.io))
-        dfinal = None if dfinal is None else dfinal.to(torch.float32).contiguous()
-        dq, dk, dv = new(self.q), new(self.k), new(self.v)
-        dg = new(self.g) if want_decay else None
-        ds = torch.empty((self.b, self.h, self.dk, self.dv), dtype=torch.float32, device=self.device) \
-            if want_state else None
-        args = L.LinearBwdArgs(self.args(None, final), *_strides(dout), L.ptr(dfinal), *_strides(dq), *_strides(dk),
-                               *_strides(dv), L.ptr(dg), L.ptr(ds), None)
-        work = self.work(args.f, True)
-        args.work = L.ptr(work)
-        with torch.cuda.device(self.device):
-            L.check(L.lib().ss_linear_bwd(args, L.stream_of(self.device)), "ss_linear_bwd")
-            L.maybe_check_status(self.device, "ss_linear_bwd")
-        return dq, dk, dv, dg, ds
+
+def _prepare(q, k, v, log_decay, scale, initial_state, seq_lens):
+    """Validated, normalised operands: (tensors, (sizes, type codes, scale)), tensors q, k, v, log_decay,
+    initial_state, seq_lens."""
+    _cuda_device(q, k, v, log_decay, initial_state, seq_lens)
+    io = v.dtype
+    io_code = L.dtype_code(io)
+    h, hk, dk, dv = _check_heads(q, k, v, 4)
+    b, l = v.shape[:2]
+    scale = _scale(scale, dk)
+    if tuple(log_decay.shape) not in ((h,), (b, l, h)):
+        raise ValueError(f"log_decay must be ({h},) or {(b, l, h)}, got {tuple(log_decay.shape)}")
+    q, k, v = _as(q, io), _as(k, io), _as(v, io)
+    if q.stride(-1) != 1 or k.stride(-1) != 1 or v.stride(-1) != 1:
+        q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+    g = _decay(log_decay, io)
+    if g.dim() == 3 and g.stride(0) == 0 and g.stride(1) == 0:
+        g = g.contiguous()  # an expanded tensor still has a gradient for every token
+    if initial_state is not None:
+        _check_state(initial_state, (b, h, dk, dv), "initial_state")
+        initial_state = _as(initial_state, torch.float32).contiguous()
+    if seq_lens is not None:
+        if tuple(seq_lens.shape) != (b,) or seq_lens.is_floating_point() or seq_lens.dtype == torch.bool:
+            raise ValueError(f"seq_lens must be ({b},) integers, got {seq_lens.dtype} {tuple(seq_lens.shape)}")
+        if seq_lens.dtype != torch.int32:
+            seq_lens = seq_lens.clamp(0, l).to(torch.int32)
+        seq_lens = seq_lens.contiguous()
+    return (q, k, v, g, initial_state, seq_lens), (b, l, h, hk, dk, dv, io_code, L.dtype_code(g.dtype), scale)
+
+
+def _inputs(t, c, state_out):
+    """The leading fields of ss_linear_args."""
+    q, k, v, g, state, lens = t
+    gs = (0, 0, g.stride(0)) if g.dim() == 1 else g.stride()
+    return (*c, *_at(q), *_at(k), *_at(v), g.data_ptr(), *gs, _p(lens), _p(state), _p(state_out))
+
+
+def _forward(t, c, want_final):
+    b, l, h, _, dk, dv = c[:6]
+    v = t[2]
+    dev = v.device
+    o = torch.empty((b, l, h, dv), dtype=v.dtype, device=dev)
+    final = torch.empty((b, h, dk, dv), dtype=torch.float32, device=dev) if want_final else None
+    work = _work(c, 0, dev)
+    L.launch("ss_linear_fwd", _pack_fwd(*_inputs(t, c, final), *_at(o), _p(work)), dev)
+    L.maybe_check_status(dev, "ss_linear_fwd")
+    return o, final
+
+
+def _backward(t, c, dout, dfinal, final, want_decay, want_state):
+    q, k, v, g = t[:4]
+    dev, new = v.device, torch.empty
+    dout = _as(dout, v.dtype)
+    if v.dtype != torch.float32:
+        dout = _whole(dout)
+    elif dout.stride(-1) != 1:
+        dout = dout.contiguous()
+    if dfinal is not None:
+        dfinal = _as(dfinal, torch.float32).contiguous()
+    dq, dk, dv = (new(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
+    dg = new(g.shape, dtype=g.dtype, device=dev) if want_decay else None
+    ds = new((c[0], c[2], c[4], c[5]), dtype=torch.float32, device=dev) if want_state else None
+    work = _work(c, 1, dev)
+    L.launch("ss_linear_bwd", _pack_bwd(*_inputs(t, c, final), *_NONE4, 0, *_at(dout), _p(dfinal), *_at(dq), *_at(dk),
+                                        *_at(dv), _p(dg), _p(ds), _p(work)), dev)
+    L.maybe_check_status(dev, "ss_linear_bwd")
+    return dq, dk, dv, dg, ds
 
 
 class LinearAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, scale, initial_state, seq_lens, want_final):
-        c = _Call(q, k, v, log_decay, scale, initial_state, seq_lens)
-        o, final = c.forward(want_final)
+        t, c = _prepare(q, k, v, log_decay, scale, initial_state, seq_lens)
+        o, final = _forward(t, c, want_final)
         ctx.set_materialize_grads(False)
         # the final state is needed again for the decays' gradient through it
-        ctx.save_for_backward(c.q, c.k, c.v, c.g, c.state, c.lens, final)
-        ctx.scale = c.scale
-        ctx.dtypes = tuple(None if t is None else t.dtype for t in (q, k, v, log_decay, initial_state))
+        ctx.save_for_backward(*t, final)
+        ctx.call = c
+        ctx.dtypes = tuple(None if x is None else x.dtype for x in (q, k, v, log_decay, initial_state))
         return (o, final) if want_final else o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dfinal=None):
-        q, k, v, g, state, lens, final = ctx.saved_tensors
+        *t, final = ctx.saved_tensors
         if dout is None and dfinal is None:
             return (None,) * 8
-        c = _Call(q, k, v, g, ctx.scale, state, lens)
         if dout is None:
-            dout = torch.zeros_like(v)
-        grads = c.backward(dout, dfinal, final, ctx.needs_input_grad[3], ctx.needs_input_grad[5])
-        dq, dk, dv, dg, ds = (t if t is None or t.dtype == d else t.to(d)
-                              for t, d in zip(grads, ctx.dtypes))
+            dout = torch.zeros_like(t[2])
+        grads = _backward(t, ctx.call, dout, dfinal, final, ctx.needs_input_grad[3], ctx.needs_input_grad[5])
+        dq, dk, dv, dg, ds = (x if x is None else _as(x, d) for x, d in zip(grads, ctx.dtypes))
         return dq, dk, dv, dg, None, ds, None, None
 
 
@@ -178,35 +203,57 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, seq_
     seq_lens: (batch,) integers; the tokens behind a row's length are ignored (whatever they hold),
     their outputs and gradients are zero.  Returns o (batch, seqlen, heads, value_dim) in v's dtype,
     and with return_final_state the state after each row's last token, fp32.
-    float32, bfloat16 and float16; the state is fp32 throughout."""
-    return LinearAttentionFn.apply(q, k, v, log_decay, scale, initial_state, seq_lens, bool(return_final_state))
+
+    float32, bfloat16 and float16; the state is fp32 throughout.  16-bit inputs run on the tensor cores; for
+    that, inputs whose rows are not whole 16-byte units (head sizes off a multiple of 8, odd strides) are
+    copied first."""
+    want = bool(return_final_state)
+    cut = None
+    if v.dtype in (torch.bfloat16, torch.float16) and v.is_cuda and v.dim() == 4 and v.numel():
+        dk, dv = k.shape[-1], v.shape[-1]
+        if (dk % 8 or dv % 8) and q.shape == k.shape and min(dk, dv) > 0:
+            scale = _scale(scale, dk)
+            cut = dk, dv
+            if initial_state is not None and tuple(initial_state.shape) == (v.shape[0], v.shape[2], dk, dv):
+                initial_state = torch.nn.functional.pad(initial_state, (0, -dv % 8, 0, -dk % 8))
+        q, k, v = _whole(_as(q, v.dtype)), _whole(_as(k, v.dtype)), _whole(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                    or (initial_state is not None and initial_state.requires_grad)):
+        out = LinearAttentionFn.apply(q, k, v, log_decay, scale, initial_state, seq_lens, want)
+        o, final = out if want else (out, None)
+    else:
+        o, final = _forward(*_prepare(q, k, v, log_decay, scale, initial_state, seq_lens), want)
+    if cut:
+        o = o[..., :cut[1]].contiguous()
+        final = final[..., :cut[0], :cut[1]].contiguous() if want else None
+    return (o, final) if want else o
 
 
-@torch.no_grad()
 def linear_attention_step(state, q, k, v, log_decay, scale=None):
     """One token of ``linear_attention_fn``; updates ``state`` (batch, heads, key_dim, value_dim) fp32 in
     place.  q, k: (batch, key_heads, key_dim); v: (batch, heads, value_dim); log_decay: (batch, heads)
-    or (heads,).  Returns o (batch, heads, value_dim) in v's dtype."""
+    or (heads,).  Returns o (batch, heads, value_dim) in v's dtype.  Not differentiable."""
     dev = _cuda_device(state, q, k, v, log_decay)
     io = v.dtype
-    L.dtype_code(io)
-    _check_heads(q, k, v, tuple(v.shape[:1]) if v.dim() == 3 else (0,))
-    b, h, dv = v.shape
-    hk, dk = k.shape[1:]
+    io_code = L.dtype_code(io)
+    h, hk, dk, dv = _check_heads(q, k, v, 3)
+    b, n = v.shape[0], h * dk * dv
     _check_state(state, (b, h, dk, dv), "state")
-    if state.dtype != torch.float32 or not state[:1].is_contiguous() or (b > 1 and state.stride(0) < h * dk * dv):
+    ss = state.stride()
+    if state.dtype != torch.float32 or (b > 1 and ss[0] < n) or (
+            ss[1:] != (dk * dv, dv, 1) and not state[:1].is_contiguous()):
         raise ValueError("state must be float32 with contiguous (heads, key_dim, value_dim) rows")
     if tuple(log_decay.shape) not in ((h,), (b, h)):
         raise ValueError(f"log_decay must be ({h},) or {(b, h)}, got {tuple(log_decay.shape)}")
-    q, k, v = (_unit(t if t.dtype == io else t.to(io)) for t in (q, k, v))
+    q, k, v = _as(q, io), _as(k, io), _as(v, io)
+    if q.stride(-1) != 1 or k.stride(-1) != 1 or v.stride(-1) != 1:
+        q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
     g = _decay(log_decay, io)
     gs = (0, g.stride(0)) if g.dim() == 1 else g.stride()
     o = torch.empty((b, h, dv), dtype=io, device=dev)
-    args = L.LinearStepArgs(b, h, hk, dk, dv, L.dtype_code(io), L.dtype_code(g.dtype), _scale(scale, dk),
-                            state.data_ptr(), state.stride(0) if b > 1 else h * dk * dv, *_strides(q), *_strides(k),
-                            *_strides(v), g.data_ptr(), *gs, *_strides(o))
-    with torch.cuda.device(dev):
-        L.check(L.lib().ss_linear_step(args, L.stream_of(dev)), "ss_linear_step")
+    L.launch("ss_linear_step", _pack_step(b, h, hk, dk, dv, io_code, L.dtype_code(g.dtype), _scale(scale, dk),
+                                          state.data_ptr(), ss[0] if b > 1 else n, *_at(q), *_at(k), *_at(v),
+                                          g.data_ptr(), *gs, o.data_ptr(), h * dv, dv), dev)
     return o
 
 

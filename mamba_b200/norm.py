@@ -97,67 +97,89 @@ def rms_norm(norm, x, residual=None, prenorm=False):
 _ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
 
 
+_pack_block_fwd, _pack_block_bwd = (L.packer(st) for st in (L.BlockNormArgs, L.BlockNormBwdArgs))
+
+
+def _row_at(t):
+    """Address and row stride of a (rows, dim) tensor."""
+    return (0, 0) if t is None else (t.data_ptr(), t.stride(0))
+
+
+def _block_rows(t, dtype, dim):
+    if t is None or (t.dtype == dtype and t.dim() == 2 and t.stride(1) == 1):
+        return t
+    return _rows(t if t.dtype == dtype else t.to(dtype), dim)
+
+
+def _f32(t):
+    return t if t is None or (t.dtype == torch.float32 and t.is_contiguous()) else t.to(torch.float32).contiguous()
+
+
+def _block_args(rows, cols, call, h=None, x=None, rstd=None):
+    (y, residual, gate), (post, pre, scale) = rows, cols
+    io, activation, eps, pre_eps, unit, const = call
+    return (*y.shape, io, unit, activation, eps, pre_eps, const, *_row_at(y), *_row_at(residual), *_row_at(gate),
+            L.ptr(post) or 0, L.ptr(pre) or 0, L.ptr(scale) or 0, *_row_at(h), *_row_at(x), L.ptr(rstd) or 0)
+
+
+def _block_forward(y, residual, post, pre, gate, scale, call, train):
+    """Returns (x | None, h, rows, columns, rstd | None)."""
+    dev = _cuda_device(y, residual, post, pre, gate, scale)
+    dim, io = y.shape[-1], y.dtype
+    rows = [_block_rows(t, io, dim) for t in (y, residual, gate)]
+    cols = [_f32(t) for t in (post, pre, scale)]
+    n = rows[0].shape[0]
+    h = torch.empty((n, dim), dtype=io, device=dev)
+    x = torch.empty((n, dim), dtype=io, device=dev) if pre is not None else None
+    rstd = torch.empty((n, 2), dtype=torch.float32, device=dev) if train else None
+    L.launch("ss_block_norm_fwd", _pack_block_fwd(*_block_args(rows, cols, call, h, x, rstd)), dev)
+    if y.dim() != 2:
+        h = h.reshape(y.shape)
+        x = x if x is None else x.reshape(y.shape)
+    return x, h, rows, cols, rstd
+
+
 class BlockNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, residual, post_weight, pre_weight, gate, scale, scale_const, activation, eps, pre_eps,
-                unit_offset):
-        _cuda_device(y, residual, post_weight, pre_weight, gate, scale)
-        dim, io = y.shape[-1], y.dtype
-        L.dtype_code(io)
-        rows = [None if t is None else _rows(t if t.dtype == io else t.to(io), dim) for t in (y, residual, gate)]
-        cols = [None if t is None else t.to(torch.float32).contiguous() for t in (post_weight, pre_weight, scale)]
-        n = rows[0].shape[0]
+    def forward(ctx, y, residual, post_weight, pre_weight, gate, scale, call):
+        x, h, rows, cols, rstd = _block_forward(y, residual, post_weight, pre_weight, gate, scale, call, True)
+        ctx.save_for_backward(*rows, *cols, rstd)
         ctx.set_materialize_grads(False)
-        ctx.meta = (y.shape, activation, float(eps), float(pre_eps), bool(unit_offset), float(scale_const))
+        ctx.call, ctx.shape = call, y.shape
         ctx.dtypes = tuple(None if t is None else t.dtype
                            for t in (y, residual, post_weight, pre_weight, gate, scale))
-        new = lambda *s, dtype=io: torch.empty(s, dtype=dtype, device=y.device)  # noqa: E731
-        h = new(n, dim)
-        x = new(n, dim) if pre_weight is not None else None
-        rstd = new(n, 2, dtype=torch.float32)
-        ctx.save_for_backward(*rows, *cols, rstd)
-        args = BlockNormFn._args(ctx, rows, cols, rstd, h, x)
-        with torch.cuda.device(y.device):
-            L.check(L.lib().ss_block_norm_fwd(args, L.stream_of(y.device)), "ss_block_norm_fwd")
-        h = h.reshape(y.shape)
-        return h if x is None else (x.reshape(y.shape), h)
-
-    @staticmethod
-    def _args(ctx, rows, cols, rstd, h=None, x=None):
-        (y, residual, gate), (post, pre, scale) = rows, cols
-        shape, activation, eps, pre_eps, unit, const = ctx.meta
-        at = lambda t: (None, 0) if t is None else (t.data_ptr(), t.stride(0))  # noqa: E731
-        return L.BlockNormArgs(y.shape[0], shape[-1], L.dtype_code(y.dtype), int(unit), activation, eps, pre_eps, const,
-                               *at(y), *at(residual), *at(gate), L.ptr(post), L.ptr(pre), L.ptr(scale), *at(h), *at(x),
-                               rstd.data_ptr())
+        return h if x is None else (x, h)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
         *rows, post, pre, scale, rstd = ctx.saved_tensors
         y, residual, gate = rows
-        n, dim, io = y.shape[0], ctx.meta[0][-1], y.dtype
+        (n, dim), io, dev = y.shape, y.dtype, y.device
         dx, dh = grads if pre is not None else (None, grads[0])
         if dx is None and dh is None:
-            return (None,) * 11
+            return (None,) * 7
         if pre is not None and dx is None:
             dx = torch.zeros_like(y)
-        dx, dh = (None if t is None else _rows(t if t.dtype == io else t.to(io), dim) for t in (dx, dh))
-        new = lambda t: None if t is None else torch.empty((n, dim), dtype=io, device=y.device)  # noqa: E731
+        dx, dh = _block_rows(dx, io, dim), _block_rows(dh, io, dim)
+        new = lambda t: None if t is None else torch.empty((n, dim), dtype=io, device=dev)  # noqa: E731
         dy, dres, dgate = new(y), new(residual), new(gate)
-        col = lambda t: None if t is None else torch.empty(dim, dtype=torch.float32, device=y.device)  # noqa: E731
-        dpost, dpre, dscale = col(post), col(pre), col(scale)
-        work = torch.empty(int(L.lib().ss_block_norm_work_elems(n, dim, L.dtype_code(io))), dtype=torch.float32,
-                           device=y.device)
-        at = lambda t: (None, 0) if t is None else (t.data_ptr(), t.stride(0))  # noqa: E731
-        args = L.BlockNormBwdArgs(BlockNormFn._args(ctx, rows, (post, pre, scale), rstd), *at(dx), *at(dh), *at(dy), *at(dres),
-                                  *at(dgate), L.ptr(dpost), L.ptr(dpre), L.ptr(dscale), work.data_ptr())
-        with torch.cuda.device(y.device):
-            L.check(L.lib().ss_block_norm_bwd(args, L.stream_of(y.device)), "ss_block_norm_bwd")
-        shape = ctx.meta[0]
-        out = [None if t is None else t.reshape(shape) for t in (dy, dres)] + [dpost, dpre]
-        out += [None if dgate is None else dgate.reshape(shape), dscale]
-        return (*(t if t is None or t.dtype == d else t.to(d) for t, d in zip(out, ctx.dtypes)),) + (None,) * 5
+        # the columns' gradients and the scratch of their sums in one buffer
+        m = int(L.lib().ss_block_norm_work_elems(n, dim, ctx.call[0]))
+        k = sum(t is not None for t in (post, pre, scale))
+        buf = torch.empty(m + k * dim, dtype=torch.float32, device=dev)
+        at, cols = m, []
+        for t in (post, pre, scale):
+            cols.append(None if t is None else buf[at:at + dim])
+            at += 0 if t is None else dim
+        dpost, dpre, dscale = cols
+        L.launch("ss_block_norm_bwd", _pack_block_bwd(
+            *_block_args(rows, (post, pre, scale), ctx.call, rstd=rstd), *_row_at(dx), *_row_at(dh), *_row_at(dy),
+            *_row_at(dres), *_row_at(dgate), L.ptr(dpost) or 0, L.ptr(dpre) or 0, L.ptr(dscale) or 0, buf.data_ptr()), dev)
+        if len(ctx.shape) != 2:
+            dy, dres, dgate = (t if t is None else t.reshape(ctx.shape) for t in (dy, dres, dgate))
+        return (*(t if t is None or t.dtype == d else t.to(d)
+                  for t, d in zip((dy, dres, dpost, dpre, dgate, dscale), ctx.dtypes)), None)
 
 
 def block_norm_fn(y, residual, post_weight=None, pre_weight=None, gate=None, residual_scale=None, activation="silu",
@@ -172,9 +194,10 @@ def block_norm_fn(y, residual, post_weight=None, pre_weight=None, gate=None, res
     pre_weight (dim,): the norm before the next block.  Norms scale by 1 + weight (unit_offset) or
     weight.  Everything is computed in fp32 and rounded once, x from the unrounded h.  dim is at most
     8192.  Returns (x, h), or h alone without pre_weight; differentiable in every tensor."""
-    if residual.shape != y.shape or (gate is not None and gate.shape != y.shape):
+    shape = y.shape
+    if residual.shape != shape or (gate is not None and gate.shape != shape):
         raise ValueError("residual and gate must have the shape of y")
-    dim = y.shape[-1] if y.dim() else 0
+    dim = shape[-1] if len(shape) else 0
     if dim < 1:
         raise ValueError("y must have a last dimension of at least 1")
     if dim > L.MAX_BLOCK_NORM_DIM:
@@ -186,5 +209,10 @@ def block_norm_fn(y, residual, post_weight=None, pre_weight=None, gate=None, res
             raise ValueError(f"{name} must be ({dim},), got {tuple(t.shape)}")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation {activation!r} (one of {list(_ACTIVATIONS)})")
-    return BlockNormFn.apply(y, residual, post_weight, pre_weight, gate, scale, const, _ACTIVATIONS[activation], eps,
-                             eps if pre_eps is None else pre_eps, unit_offset)
+    call = (L.dtype_code(y.dtype), _ACTIVATIONS[activation], float(eps), float(eps if pre_eps is None else pre_eps),
+            int(bool(unit_offset)), const)
+    tensors = y, residual, post_weight, pre_weight, gate, scale
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return BlockNormFn.apply(*tensors, call)
+    x, h, *_ = _block_forward(*tensors, call, False)
+    return h if x is None else (x, h)

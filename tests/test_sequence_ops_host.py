@@ -157,7 +157,7 @@ def test_workspace_sizes():
     assert lib.ss_beam_work_bytes(0, 4, 100, 4) == 0 and lib.ss_beam_work_bytes(1, 4, 100, 0) == 0
     assert lib.ss_beam_work_bytes(1, 4, 100, 4) == 4 * (16 + 4 * 8)      # one slice a beam
     assert lib.ss_block_norm_work_elems(0, 768, L.SS_BF16) == 0
-    assert lib.ss_block_norm_work_elems(5, 768, L.SS_BF16) == 2 * 768    # one CTA
+    assert lib.ss_block_norm_work_elems(5, 768, L.SS_BF16) == 2 * 2 * 768  # two CTAs of four rows
     assert lib.ss_linear_work_bytes(ctypes.byref(_linear_args(batch=-1)), 0) == 0
     # many heads: one segment, nothing but the backward's row sums and the groups' parts
     a = _linear_args(batch=64, heads=8, key_heads=4)
