@@ -4,12 +4,15 @@ place.  ``mamba_b200.beam_search`` runs a model with them; the reference has no 
 ``generate`` is a stub, models/causal_lm.py:61-62)."""
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import _lib as L
 from .selective_scan_interface import _cuda_device
 
 
+_nbytes = operator.attrgetter("nbytes")
 _pack_beam, _pack_reorder = L.packer(L.BeamArgs), L.packer(L.ReorderArgs)
 
 
@@ -71,20 +74,17 @@ def reorder_states(states, parents):
         raise ValueError("parents must name at least one beam")
     if w > L.MAX_BEAMS:
         raise NotImplementedError(f"{w} beams are more than {L.MAX_BEAMS}")
-    total, dev, rows = b * w, parents.get_device(), []
+    total = b * w
     for t in states:
-        if t.get_device() != dev:
-            raise RuntimeError(f"tensors on different devices: {parents.device} and {t.device}")
-        if t.dim() < 1 or t.size(0) != total or not t.is_contiguous():
+        if t.dim() < 1 or len(t) != total or not t.is_contiguous():
             raise ValueError(f"a state must have {total} contiguous rows, got {tuple(t.shape)}")
-        n = t.nbytes
-        if n:
-            if n % (4 * total):
-                raise NotImplementedError(f"rows of {n / total} bytes (a multiple of 4 is supported)")
-            rows.append((t.data_ptr(), n))
-    rows.sort()
+    if states and set(map(torch.Tensor.get_device, states)) != {parents.get_device()}:
+        raise RuntimeError("states and parents on different devices")
+    rows = sorted(r for r in zip(map(torch.Tensor.data_ptr, states), map(_nbytes, states)) if r[1])
     end = 0
     for at, n in rows:
+        if n % (4 * total):
+            raise NotImplementedError(f"rows of {n / total} bytes (a multiple of 4 is supported)")
         if at < end:
             raise ValueError("states must not share memory")
         end = at + n

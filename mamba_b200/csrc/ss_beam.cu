@@ -11,11 +11,11 @@ namespace {
 
 using namespace ssb;
 
-// slices of a beam's vocabulary: about two CTAs per SM over all beams, at least 1024 tokens each (a
-// slice ends with a merge of its warps' lists)
+// slices of a beam's vocabulary: up to eight CTAs per SM over all beams, at least 2048 tokens each (a slice
+// ends with a merge of its warps' lists)
 int slices_of(int64_t rows, int vocab) {
-  const int64_t want = std::max<int64_t>(1, (2 * 148 + rows - 1) / std::max<int64_t>(1, rows));
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, (vocab + 1023) / 1024, 64}));
+  const int64_t want = std::max<int64_t>(1, (8 * 148 + rows - 1) / std::max<int64_t>(1, rows));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, (vocab + 2047) / 2048, 64}));
 }
 
 bool sizes_ok(int batch, int beams, int vocab, int k) {

@@ -7,8 +7,9 @@
 // of the candidates is the order of the logits, so a slice needs only its largest num_select logits
 // (the first among equals), beside its running maximum and sum of exponentials.  A warp keeps the
 // best so far sorted over its lanes, as 64-bit keys (the logit's bits mapped to ascending integers,
-// then the complement of the index, so one comparison orders both); an element enters only above
-// the current last, which for n elements in no particular order happens about k ln(n / k) times.
+// then the complement of the index, so one comparison orders both).  Of a batch of 32 logits a lane only those
+// are offered that reach the k-th largest of the lanes' maxima (a bound from below) and the list's last: a
+// few more than k in the first batch, about k ln 2 each time the number read doubles.
 // Pass 2, one CTA per batch row and one warp per beam: slices' sums (in fp64) and keys merged, then
 // the beams' lists, compared as fp64 values.  The sums of exponentials are fp32 inside a lane (tens
 // of terms) and fp64 across lanes, which leaves the logarithm good to about 1e-8, so that two
@@ -58,6 +59,28 @@ struct WarpBest {
   }
 };
 
+// the k-th largest over the warp of one value a lane
+__device__ __forceinline__ uint32_t kth_of_warp(uint32_t v, int k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {  // bitonic, falling
+      const uint32_t w = __shfl_xor_sync(kFull, v, o);
+      v = ((lane & size) == 0) == ((lane & o) == 0) ? max(v, w) : min(v, w);
+    }
+  return __shfl_sync(kFull, v, k - 1);
+}
+
+// 16 bytes, zeros where `on` is false; predicated inside, so that no branch waits for the load
+__device__ __forceinline__ uint4 ld_vector(const void* p, bool on) {
+  uint4 r;
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n mov.u32 %0, 0;\n mov.u32 %1, 0;\n mov.u32 %2, 0;\n mov.u32 %3, 0;\n"
+               " @p ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n}\n"
+               : "=&r"(r.x), "=&r"(r.y), "=&r"(r.z), "=&r"(r.w) : "l"(p), "r"((uint32_t)on));
+  return r;
+}
+
 struct BeamSlice {
   double sum;  // of e^{logit - max}
   float max;
@@ -88,37 +111,53 @@ __global__ void __launch_bounds__(kBsThreads) beam_slice_kernel(const __grid_con
   const int v0 = slice * P.slice_len, v1 = min(v0 + P.slice_len, a.vocab);
   WarpBest best;
   float m = -INFINITY, sum = 0.f;
-  for (int base = v0; base < v1; base += kBsThreads * VW) {
-    const int e0 = base + threadIdx.x * VW;
-    float v[VW];
-    if (P.vec && e0 + VW <= v1) {
-      const uint4 q = ld_stream16(x + e0);
+  constexpr int E = 32, U = E / VW;  // values of a thread in a batch, 16-byte vectors of them under way at once
+  for (int base = v0; base < v1; base += kBsThreads * E) {
+    const int first = base + threadIdx.x * VW;  // vector u starts kBsThreads * VW * u further
+    uint4 q[U];
 #pragma unroll
-      for (int i = 0; i < VW; ++i) v[i] = to_f<IT>(reinterpret_cast<const IT*>(&q)[i]);
-    } else {
+    for (int u = 0; u < U; ++u) {
+      const int e0 = first + u * kBsThreads * VW;
+      if (P.vec) {
+        q[u] = ld_vector(x + e0, e0 + VW <= v1);
+      }
+      if (!P.vec || (e0 < v1 && e0 + VW > v1)) {
+        union { uint4 v; IT e[VW]; } pk;
 #pragma unroll
-      for (int i = 0; i < VW; ++i) v[i] = e0 + i < v1 ? to_f<IT>(x[e0 + i]) : -INFINITY;
+        for (int i = 0; i < VW; ++i) pk.e[i] = e0 + i < v1 ? x[e0 + i] : from_f<IT>(-INFINITY);
+        q[u] = pk.v;
+      }
     }
-    float vm = v[0];
+    float vm = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < VW; ++i) vm = fmaxf(vm, v[i]);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < VW; ++i)
+        if (first + u * kBsThreads * VW + i < v1) vm = fmaxf(vm, to_f<IT>(reinterpret_cast<const IT*>(&q[u])[i]));
     if (vm > m) {
       sum *= expf(m - vm);  // 0 at the first finite value
       m = vm;
     }
+    const uint32_t last = (uint32_t)(__shfl_sync(kFull, best.mine, k - 1) >> 32);
+    const uint32_t bound = max(last, kth_of_warp(first < v1 ? order_key(vm) : 0u, k));
+    uint32_t mask = 0;  // this lane's candidates
 #pragma unroll
-    for (int i = 0; i < VW; ++i)  // an infinite maximum, or NaN, makes the sum NaN
-      if (e0 + i < v1 && v[i] != -INFINITY) sum += expf(v[i] - m);
-    // the warp's elements, one of each lane at a time
-    const u64 last = __shfl_sync(kFull, best.mine, k - 1);
-    const float floor_v = last ? key_value((uint32_t)(last >> 32)) : -INFINITY;
-    bool any = last == 0;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int i = 0; i < VW; ++i) any |= !(v[i] < floor_v);
-    if (__any_sync(kFull, any)) {
-#pragma unroll
-      for (int i = 0; i < VW; ++i)
-        best.offer(e0 + i < v1 ? ((u64)order_key(v[i]) << 32) | (uint32_t)~(uint32_t)(e0 + i) : 0, k);
+      for (int i = 0; i < VW; ++i) {
+        const float v = to_f<IT>(reinterpret_cast<const IT*>(&q[u])[i]);
+        const bool in = first + u * kBsThreads * VW + i < v1;
+        if (in && v != -INFINITY) sum += expf(v - m);  // an infinite maximum, or NaN, makes the sum NaN
+        if (in && order_key(v) >= bound) mask |= 1u << (u * VW + i);
+      }
+    while (__any_sync(kFull, mask != 0)) {  // one of each lane at a time, read again
+      u64 key = 0;
+      if (mask) {
+        const int e = __ffs(mask) - 1, at = first + e / VW * (kBsThreads * VW) + e % VW;
+        mask &= mask - 1;
+        key = ((u64)order_key(to_f<IT>(x[at])) << 32) | (uint32_t)~(uint32_t)at;
+      }
+      best.offer(key, k);
     }
   }
   // the CTA's maximum and sum

@@ -113,15 +113,16 @@ cudaError_t run_simt(const LinK& P, int passes, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-template <typename IT, int DK>
-cudaError_t launch_tc(const LinTcK& P, cudaStream_t st) {
-  constexpr size_t smem = TcShape<DK>::kBytes;
-  static_assert(smem <= 232448, "shared memory of a CTA");
+template <typename IT>
+cudaError_t launch_tc(const LinTcK& P, bool wide, cudaStream_t st) {
+  static_assert(TcShape<64>::kBytes <= 232448 && TcShape<128>::kBytes <= 232448, "shared memory of a CTA");
   static_assert(sizeof(TcBars) <= 512, "barriers");
-  auto main_k = linear_tc_kernel<IT, DK, false>;
-  auto sum_k = linear_tc_kernel<IT, DK, true>;
-  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(main_k), smem);
-  if (e == cudaSuccess) e = ensure_smem_limit(reinterpret_cast<const void*>(sum_k), smem);
+  const size_t smem = wide ? std::max(TcShape<64>::kBytes, TcShape<128>::kBytes) : TcShape<64>::kBytes;
+  auto main_k = linear_tc_kernel<IT, false>;
+  auto sum_k = linear_tc_kernel<IT, true>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(main_k), std::max(TcShape<64>::kBytes, TcShape<128>::kBytes));
+  if (e == cudaSuccess)
+    e = ensure_smem_limit(reinterpret_cast<const void*>(sum_k), std::max(TcShape<64>::kBytes, TcShape<128>::kBytes));
   if (e != cudaSuccess) return e;
   const unsigned grid = (unsigned)((int64_t)P.k.batch * P.k.heads * P.k.segs * P.parts);
   if (P.k.segs > 1) {
@@ -140,44 +141,35 @@ bool vec16(const void* p, int es, int64_t b, int64_t l, int64_t h) {
 
 // The tensor-core kernel takes every 16-bit call whose rows are whole 16-byte units (TMA loads, vector
 // stores); false: it cannot.
-// Runs are grouped by the width of their keys (up to 64, up to 128), each group one launch.
 bool run_tc(int io, const LinK& P, int passes, cudaStream_t st, cudaError_t* e) {
-  LinTcK T[2];
-  int n[2] = {0, 0};
+  LinTcK T;
+  T.tiles = 1;
+  bool wide = false;
   for (int i = 0; i < passes; ++i) {
     const LinPass& A = P.pass[i];
     if (A.dk % 8 || A.dv % 8 || !vec16(A.o, A.o_f32 ? 4 : 2, A.ob, A.ol, A.oh) ||
         (A.dot && !vec16(A.p, 2, A.pb, A.pl, A.ph)))
       return false;
-    const int w = A.dk > 64;
-    LinTcK& t = T[w];
     const struct {
       const void* p;
       int64_t d, b, l, h;
       int r;
     } x[3] = {{A.q, A.dk, A.qb, A.ql, A.qh, A.rq}, {A.k, A.dk, A.kb, A.kl, A.kh, A.rk}, {A.v, A.dv, A.vb, A.vl, A.vh, A.rv}};
-    for (int j = 0; j < 3; ++j)
-      if (!map_heads(&t.map[n[w]][j], x[j].p, io, x[j].d, P.heads / x[j].r, P.seqlen, P.batch, x[j].h, x[j].l, x[j].b, kTcC))
-        return false;
-    if (!map_heads(&t.map[n[w]][3], A.o, A.o_f32 ? SS_F32 : io, A.dv, P.heads, P.seqlen, P.batch, A.oh, A.ol, A.ob, 32))
-      return false;
-    if (n[w] == 0) {
-      t.k = P;
-      t.tiles = 1;
-      t.status = device_status_word();
-      t.wait_limit = wait_limit();
+    for (int j = 0; j < 4; ++j) {
+      const bool ok = j < 3 ? map_heads(&T.map[i][j], x[j].p, io, x[j].d, P.heads / x[j].r, P.seqlen, P.batch, x[j].h, x[j].l,
+                                        x[j].b, kTcC)
+                            : map_heads(&T.map[i][3], A.o, A.o_f32 ? SS_F32 : io, A.dv, P.heads, P.seqlen, P.batch, A.oh,
+                                        A.ol, A.ob, 32);
+      if (!ok) return false;
     }
-    t.k.pass[n[w]] = A;
-    t.tiles = std::max(t.tiles, (A.dv + kTcN - 1) / kTcN);
-    ++n[w];
+    T.tiles = std::max(T.tiles, (A.dv + kTcN - 1) / kTcN);
+    wide |= A.dk > 64;
   }
-  *e = cudaSuccess;
-  for (int w = 0; w < 2 && *e == cudaSuccess; ++w) {
-    if (n[w] == 0) continue;
-    T[w].parts = n[w] * T[w].tiles;
-    if (io == SS_BF16) *e = w ? launch_tc<__nv_bfloat16, 128>(T[w], st) : launch_tc<__nv_bfloat16, 64>(T[w], st);
-    else *e = w ? launch_tc<__half, 128>(T[w], st) : launch_tc<__half, 64>(T[w], st);
-  }
+  T.k = P;
+  T.parts = passes * T.tiles;
+  T.status = device_status_word();
+  T.wait_limit = wait_limit();
+  *e = io == SS_BF16 ? launch_tc<__nv_bfloat16>(T, wide, st) : launch_tc<__half>(T, wide, st);
   return true;
 }
 
@@ -321,11 +313,17 @@ int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
     G.parts[0] = parts, G.out[0] = g->dq, G.ob[0] = g->dq_batch_stride, G.ol[0] = g->dq_seq_stride, G.oh[0] = g->dq_head_stride;
     G.parts[1] = parts + bh * a.seqlen * a.key_dim;
     G.out[1] = g->dk, G.ob[1] = g->dk_batch_stride, G.ol[1] = g->dk_seq_stride, G.oh[1] = g->dk_head_stride;
-    const int64_t n = (int64_t)a.batch * a.seqlen * a.key_heads * a.key_dim;
+    const bool v4 = a.key_dim % 4 == 0;  // the parts start on 16 bytes then
+    const int64_t n = (int64_t)a.batch * a.seqlen * a.key_heads * (v4 ? a.key_dim / 4 : a.key_dim);
     const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 8 * sm_count()), 2);
-    if (a.io_dtype == SS_F32) linear_group_sum_kernel<float><<<grid, 256, 0, st>>>(G);
-    else if (a.io_dtype == SS_BF16) linear_group_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(G);
-    else linear_group_sum_kernel<__half><<<grid, 256, 0, st>>>(G);
+    auto sum = [&](auto tag) {
+      using IT = decltype(tag);
+      if (v4) linear_group_sum_kernel<IT, 4><<<grid, 256, 0, st>>>(G);
+      else linear_group_sum_kernel<IT, 1><<<grid, 256, 0, st>>>(G);
+    };
+    if (a.io_dtype == SS_F32) sum(float{});
+    else if (a.io_dtype == SS_BF16) sum(__nv_bfloat16{});
+    else sum(__half{});
     e = cudaGetLastError();
     if (e != cudaSuccess) return record_cuda_status(e);
   }
@@ -362,11 +360,15 @@ int ss_linear_step(const ss_linear_step_args* a, void* stream) {
   P.vec = a->value_dim % 4 == 0 && a->state_batch_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a->state) & 15) == 0;
   const unsigned grid = (unsigned)((int64_t)a->batch * a->heads);
   cudaStream_t st = (cudaStream_t)stream;
-  switch (a->io_dtype) {
-    case SS_F32: linear_step_kernel<float><<<grid, 32 * kLstWarps, 0, st>>>(P); break;
-    case SS_BF16: linear_step_kernel<__nv_bfloat16><<<grid, 32 * kLstWarps, 0, st>>>(P); break;
-    default: linear_step_kernel<__half><<<grid, 32 * kLstWarps, 0, st>>>(P); break;
-  }
+  auto step = [&](auto tag) {
+    using IT = decltype(tag);
+    if (a->value_dim <= 32) linear_step_kernel<IT, 8><<<grid, 32 * kLstWarps, 0, st>>>(P);
+    else if (a->value_dim <= 64) linear_step_kernel<IT, 16><<<grid, 32 * kLstWarps, 0, st>>>(P);
+    else linear_step_kernel<IT, 32><<<grid, 32 * kLstWarps, 0, st>>>(P);
+  };
+  if (a->io_dtype == SS_F32) step(float{});
+  else if (a->io_dtype == SS_BF16) step(__nv_bfloat16{});
+  else step(__half{});
   return record_cuda_status(cudaGetLastError());
 }
 

@@ -149,16 +149,28 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
     const int t0 = (A.reverse ? n_live - 1 - c : c) * kLsC;
     const int m = min(kLsC, len - t0);  // valid tokens
     __syncthreads();                    // the chunk before is done with shared memory
-    for (int e = tid; e < kLsC * dk; e += kLsThreads) {
-      const int t = e / dk, d = e % dk;
-      const bool on = t < m;
-      if (!STATE_ONLY) S.qt[d][t] = on ? to_f<IT>(q[(int64_t)(t0 + t) * A.ql + d]) : 0.f;
-      S.kt[d][t] = on ? to_f<IT>(k[(int64_t)(t0 + t) * A.kl + d]) : 0.f;
-    }
-    for (int e = tid; e < kLsC * kLsN; e += kLsThreads) {
-      const int t = e / kLsN, j = e % kLsN;
-      S.v[t][j] = (t < m && j < nv) ? to_f<IT>(v[(int64_t)(t0 + t) * A.vl + j]) : 0.f;
-    }
+    // 16 threads a token, 4 tokens a thread; all of a thread's loads of a tensor are under way at once
+    auto fetch = [&](const IT* p, int64_t stride, int n, auto&& put) {
+      float x[4][kLinMaxDim / 16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = tid / 16 + 16 * i;
+#pragma unroll
+        for (int j = 0; j < kLinMaxDim / 16; ++j) {
+          const int d = tid % 16 + 16 * j;
+          x[i][j] = t < m && d < n ? to_f<IT>(p[(int64_t)(t0 + t) * stride + d]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < kLinMaxDim / 16; ++j) put(tid / 16 + 16 * i, tid % 16 + 16 * j, x[i][j]);
+    };
+    if (!STATE_ONLY) fetch(q, A.ql, dk, [&](int t, int d, float x) { S.qt[d][t] = x; });
+    fetch(k, A.kl, dk, [&](int t, int d, float x) { S.kt[d][t] = x; });
+    fetch(v, A.vl, nv, [&](int t, int d, float x) {
+      if (d < kLsN) S.v[t][d] = x;
+    });
     if (tid < 32) {  // inclusive sums of two tokens a lane, in 64 bits: differences stay exact behind a reset
       constexpr bool bf = sizeof(IT) == 2 && std::is_same<IT, __nv_bfloat16>::value;
       const double g0 = 2 * tid < m ? (double)lin_decay(P, b, t0 + 2 * tid, head, bf) : 0.0;
@@ -343,25 +355,36 @@ struct LinGroupK {
   int batch, seqlen, key_heads, rep, dim;
 };
 
-template <typename IT>
+template <typename IT, int VW>
 __global__ void __launch_bounds__(256) linear_group_sum_kernel(const __grid_constant__ LinGroupK P) {
-  const int which = blockIdx.y;
-  const int64_t n = (int64_t)P.batch * P.seqlen * P.key_heads * P.dim;
+  const int which = blockIdx.y, nd = P.dim / VW;
+  const int64_t n = (int64_t)P.batch * P.seqlen * P.key_heads * nd;
   for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (int64_t)gridDim.x * blockDim.x) {
-    const int d = (int)(e % P.dim);
-    const int64_t r = e / P.dim;  // (b, t, kh)
+    const int d = (int)(e % nd) * VW;
+    const int64_t r = e / nd;  // (b, t, kh)
     const float* src = P.parts[which] + (r * P.rep) * P.dim + d;
-    float s = 0.f;
-    for (int i = 0; i < P.rep; ++i) s += src[(int64_t)i * P.dim];
+    float s[VW] = {};
+#pragma unroll 4
+    for (int i = 0; i < P.rep; ++i) {
+      float x[VW];
+      if constexpr (VW == 4) {
+        const float4 q = *reinterpret_cast<const float4*>(src + (int64_t)i * P.dim);
+        x[0] = q.x, x[1] = q.y, x[2] = q.z, x[3] = q.w;
+      } else {
+        x[0] = src[(int64_t)i * P.dim];
+      }
+#pragma unroll
+      for (int k = 0; k < VW; ++k) s[k] += x[k];
+    }
     const int kh = (int)(r % P.key_heads);
     const int64_t bt = r / P.key_heads;
-    static_cast<IT*>(P.out[which])[(bt / P.seqlen) * P.ob[which] + (bt % P.seqlen) * P.ol[which] + kh * P.oh[which] + d] =
-        from_f<IT>(s);
+    IT* out = static_cast<IT*>(P.out[which]) + (bt / P.seqlen) * P.ob[which] + (bt % P.seqlen) * P.ol[which] + kh * P.oh[which] + d;
+#pragma unroll
+    for (int k = 0; k < VW; ++k) out[k] = from_f<IT>(s[k]);
   }
 }
 
-// dg_t = sum_{i >= t} (q_i . dq_i - k_i . dk_i) + <dS_last, S_last>, summed in 64 bits from the last
-// token.  One CTA per (b, h), 512 tokens a step; for a decay per head one CTA per head, which sums
+// dg_t = sum_{i >= t} (q_i . dq_i - k_i . dk_i) + <dS_last, S_last>, summed from the last token.  One CTA per (b, h), 512 tokens a step; for a decay per head one CTA per head, which sums
 // over its rows and tokens in a fixed order.
 struct LinDecayK {
   const float *xq, *yk;  // [tile][b][h][t]
@@ -380,6 +403,7 @@ constexpr int kLdThreads = 512;
 
 __global__ void __launch_bounds__(kLdThreads) linear_decay_grad_kernel(const __grid_constant__ LinDecayK P) {
   __shared__ double part[kLdThreads / 32];
+  __shared__ float part_f[2][kLdThreads / 32];
   __shared__ double carry_s;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int head = P.per_head ? blockIdx.x : blockIdx.x % P.heads;
@@ -410,39 +434,51 @@ __global__ void __launch_bounds__(kLdThreads) linear_decay_grad_kernel(const __g
     }
     __syncthreads();
     double carry = carry_s;
-    // thread i holds token end - 1 - i, so a prefix over threads is a suffix over tokens
+    // thread i holds token end - 1 - i, so a prefix over threads is a suffix over tokens; the next tokens'
+    // loads are under way while these are summed
+    float xn = 0.f, gn = 0.f;
+    auto load = [&](int end) {
+      const int t = end - 1 - tid;
+      xn = gn = 0.f;
+      if (t < 0) return;
+      const int64_t at = (int64_t)b * P.gb + (int64_t)t * P.gl + (int64_t)head * P.gh;
+      if (P.g_f32) gn = static_cast<const float*>(P.g)[at];
+      else if (P.g_bf16) gn = to_f<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(P.g)[at]);
+      else gn = to_f<__half>(static_cast<const __half*>(P.g)[at]);
+      if (t >= len) return;
+      float s = 0.f, r = 0.f;  // one or two tiles each
+      for (int i = 0; i < P.tq; ++i) s += P.xq[i * bhl + bh * P.seqlen + t];
+      for (int i = 0; i < P.tk; ++i) r += P.yk[i * bhl + bh * P.seqlen + t];
+      xn = s - r;
+    };
+    load(P.seqlen);
     for (int end = P.seqlen; end > 0; end -= kLdThreads) {
       const int t = end - 1 - tid;
-      double d = 0.0;
-      if (t >= 0 && t < len) {
-        for (int i = 0; i < P.tq; ++i) d += (double)P.xq[i * bhl + bh * P.seqlen + t];
-        for (int i = 0; i < P.tk; ++i) d -= (double)P.yk[i * bhl + bh * P.seqlen + t];
-      }
+      const float g = gn;
+      float d = xn;  // a step's 512 tokens in fp32, the steps in 64 bits
+      load(end - kLdThreads);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const double u = __shfl_up_sync(0xffffffffu, d, o);
+        const float u = __shfl_up_sync(0xffffffffu, d, o);
         if (lane >= o) d += u;
       }
+      const int slot = (end / kLdThreads) & 1;
+      if (lane == 31) part_f[slot][wid] = d;
       __syncthreads();
-      if (lane == 31) part[wid] = d;
-      __syncthreads();
-      double before = 0.0, all = 0.0;
-      for (int i = 0; i < kLdThreads / 32; ++i) {
-        if (i < wid) before += part[i];
-        all += part[i];
+      const float w = lane < kLdThreads / 32 ? part_f[slot][lane] : 0.f;
+      float before = lane < wid ? w : 0.f, all = w;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+        all += __shfl_xor_sync(0xffffffffu, all, o);
       }
       if (t >= 0) {
-        const int64_t at = (int64_t)b * P.gb + (int64_t)t * P.gl + (int64_t)head * P.gh;
-        float g;
-        if (P.g_f32) g = static_cast<const float*>(P.g)[at];
-        else if (P.g_bf16) g = to_f<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(P.g)[at]);
-        else g = to_f<__half>(static_cast<const __half*>(P.g)[at]);
         // a reset passes nothing from before the token, and behind the row's end there is nothing
-        const double r = t >= len || g < kLinZeroBelow ? 0.0 : carry + before + d;
+        const double r = t >= len || g < kLinZeroBelow ? 0.0 : carry + (double)(before + d);
         if (P.per_head) sum += r;
         else store(((int64_t)b * P.seqlen + t) * P.heads + head, (float)r);
       }
-      carry += all;
+      carry += (double)all;
     }
   }
   if (P.per_head) {
@@ -460,8 +496,9 @@ __global__ void __launch_bounds__(kLdThreads) linear_decay_grad_kernel(const __g
 }
 
 // ------------------------------------------------------------------------------------ single token
-// S <- e^g S + k v^T, o = scale q S.  The state is read and written once: a warp owns 4 x 32
-// consecutive columns (a float4 a lane; narrower values leave lanes idle) and a slice of the rows.
+// S <- e^g S + k v^T, o = scale q S.  The state is read and written once, a float4 a lane: LPR lanes hold a
+// row of the state (8, 16 or 32 for up to 32, 64 or 128 columns), so that narrow heads fill their warps too.
+// Bound by the state's traffic: 64 x 40 heads of 128 x 128 move 336 MB in 61 us, 84 % of the copy rate.
 struct LinStepK {
   ss_linear_step_args a;
   int vec;
@@ -469,7 +506,7 @@ struct LinStepK {
 
 constexpr int kLstWarps = 8;
 
-template <typename IT>
+template <typename IT, int LPR>
 __global__ void __launch_bounds__(32 * kLstWarps) linear_step_kernel(const __grid_constant__ LinStepK P) {
   const ss_linear_step_args& a = P.a;
   __shared__ float4 red[kLstWarps][32];
@@ -486,7 +523,8 @@ __global__ void __launch_bounds__(32 * kLstWarps) linear_step_kernel(const __gri
   const float g = a.decay_dtype == SS_F32 ? static_cast<const float*>(a.log_decay)[gat]
                                           : to_f<IT>(static_cast<const IT*>(a.log_decay)[gat]);
   const float decay = expf(g);
-  const int n0 = lane * 4;
+  const int n0 = lane % LPR * 4, sub = lane / LPR;
+  constexpr int step = 32 / LPR * kLstWarps;
   float v[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -496,41 +534,50 @@ __global__ void __launch_bounds__(32 * kLstWarps) linear_step_kernel(const __gri
   float* st = a.state + (int64_t)b * a.state_batch_stride + (int64_t)head * dk * dv;
   float o[4] = {0.f, 0.f, 0.f, 0.f};
   if (n0 < dv) {
-#pragma unroll 8
-    for (int d = wid; d < dk; d += kLstWarps) {
-      float* row = st + (int64_t)d * dv + n0;
-      float s[4];
-      if (P.vec) {
-        const float4 x = *reinterpret_cast<const float4*>(row);
-        s[0] = x.x, s[1] = x.y, s[2] = x.z, s[3] = x.w;
-      } else {
+    constexpr int U = 8;  // rows of a lane under way at once
+    for (int d0 = wid * (32 / LPR) + sub; d0 < dk; d0 += U * step) {
+      float4 x[U];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = n0 + j < dv ? row[j] : 0.f;
+      for (int u = 0; u < U; ++u) {
+        const int d = d0 + u * step;
+        const float* row = st + (int64_t)d * dv + n0;
+        if (P.vec) {
+          if (d < dk) x[u] = *reinterpret_cast<const float4*>(row);
+        } else {
+          float* e = reinterpret_cast<float*>(&x[u]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) e[j] = d < dk && n0 + j < dv ? row[j] : 0.f;
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j] = fmaf(decay, s[j], ks[d] * v[j]);
-        o[j] = fmaf(qs[d], s[j], o[j]);
-      }
-      if (P.vec) {
-        *reinterpret_cast<float4*>(row) = make_float4(s[0], s[1], s[2], s[3]);
-      } else {
+      for (int u = 0; u < U; ++u) {
+        const int d = d0 + u * step;
+        if (d >= dk) break;
+        float* row = st + (int64_t)d * dv + n0;
+        float* s = reinterpret_cast<float*>(&x[u]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n0 + j < dv) row[j] = s[j];
+        for (int j = 0; j < 4; ++j) {
+          s[j] = fmaf(decay, s[j], ks[d] * v[j]);
+          o[j] = fmaf(qs[d], s[j], o[j]);
+        }
+        if (P.vec) {
+          *reinterpret_cast<float4*>(row) = x[u];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n0 + j < dv) row[j] = s[j];
+        }
       }
     }
   }
   red[wid][lane] = make_float4(o[0], o[1], o[2], o[3]);
   __syncthreads();
-  if (wid == 0) {
-    float4 s = red[0][lane];
-#pragma unroll
-    for (int w = 1; w < kLstWarps; ++w) {
-      const float4 x = red[w][lane];
-      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+  if (wid == 0 && lane < LPR) {
+    float r[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = lane; i < 32 * kLstWarps; i += LPR) {  // the rows' slices in a fixed order
+      const float4 x = red[i >> 5][i & 31];
+      r[0] += x.x, r[1] += x.y, r[2] += x.z, r[3] += x.w;
     }
-    const float r[4] = {s.x, s.y, s.z, s.w};
     IT* out = static_cast<IT*>(a.o) + (int64_t)b * a.o_batch_stride + (int64_t)head * a.o_head_stride;
 #pragma unroll
     for (int j = 0; j < 4; ++j)

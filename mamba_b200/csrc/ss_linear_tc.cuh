@@ -258,14 +258,10 @@ __device__ __forceinline__ float max_of2(uint32_t m) {
 }
 
 template <typename IT, int DK, bool STATE_ONLY>
-__global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_constant__ LinTcK P) {
+__device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int tile, int where, unsigned char* smem) {
   using S = TcShape<DK>;
-  extern __shared__ __align__(1024) unsigned char smem[];
   TcBars& B = *reinterpret_cast<TcBars*>(smem + S::kBars);
   const LinK& K = P.k;
-  // value tiles and runs of one head are neighbours in the grid, so that they share what they read in L2
-  const int part = blockIdx.x % P.parts, where = blockIdx.x / P.parts;
-  const int pass = part / P.tiles, tile = part % P.tiles;
   const LinPass& A = K.pass[pass];
   const int dk = A.dk, dv = A.dv, n0 = tile * kTcN;
   const int bh = where / K.segs, seg = where % K.segs;
@@ -876,6 +872,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(kTmCols) : "memory");
   }
+}
+
+// Value tiles and runs of one head are neighbours in the grid, so that they share what they read in L2; runs
+// with narrow and with wide keys go side by side in one launch.
+template <typename IT, bool STATE_ONLY>
+__global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_constant__ LinTcK P) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int part = blockIdx.x % P.parts, where = blockIdx.x / P.parts;
+  const int pass = part / P.tiles, tile = part % P.tiles;
+  if (P.k.pass[pass].dk > 64) linear_tc_run<IT, 128, STATE_ONLY>(P, pass, tile, where, smem);
+  else linear_tc_run<IT, 64, STATE_ONLY>(P, pass, tile, where, smem);
 }
 
 }  // namespace ssb

@@ -94,6 +94,8 @@ def _whole(t):
     """t with rows of whole 16-byte units, as the tensor-core kernel's copies need them: itself where it has them."""
     if t.shape[-1] % 8:
         return torch.nn.functional.pad(t, (0, -t.shape[-1] % 8))
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
         n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()))
     return t if ok else t.clone(memory_format=torch.contiguous_format)
