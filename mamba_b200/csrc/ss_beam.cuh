@@ -128,28 +128,34 @@ __global__ void __launch_bounds__(kBsThreads) beam_slice_kernel(const __grid_con
         q[u] = pk.v;
       }
     }
+    const bool full = base + kBsThreads * E <= v1;  // the whole CTA's batch lies in the slice
     float vm = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < VW; ++i)
-        if (first + u * kBsThreads * VW + i < v1) vm = fmaxf(vm, to_f<IT>(reinterpret_cast<const IT*>(&q[u])[i]));
+      for (int i = 0; i < VW; ++i)  // what was read behind the slice's end is 0
+        if (full || first + u * kBsThreads * VW + i < v1) vm = fmaxf(vm, to_f<IT>(reinterpret_cast<const IT*>(&q[u])[i]));
     if (vm > m) {
       sum *= expf(m - vm);  // 0 at the first finite value
       m = vm;
     }
-    const uint32_t last = (uint32_t)(__shfl_sync(kFull, best.mine, k - 1) >> 32);
-    const uint32_t bound = max(last, kth_of_warp(first < v1 ? order_key(vm) : 0u, k));
+    uint32_t bound = (uint32_t)(__shfl_sync(kFull, best.mine, k - 1) >> 32);
+    if (base == v0) bound = kth_of_warp(first < v1 ? order_key(vm) : 0u, k);  // the list is empty
+    const float floor_v = bound ? key_value(bound) : -INFINITY;
+    const float mm = m == -INFINITY ? 0.f : m;
     uint32_t mask = 0;  // this lane's candidates
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < VW; ++i) {
         const float v = to_f<IT>(reinterpret_cast<const IT*>(&q[u])[i]);
-        const bool in = first + u * kBsThreads * VW + i < v1;
-        if (in && v != -INFINITY) sum += expf(v - m);  // an infinite maximum, or NaN, makes the sum NaN
-        if (in && order_key(v) >= bound) mask |= 1u << (u * VW + i);
+        if (full || first + u * kBsThreads * VW + i < v1) {
+          (i & 1 ? s1 : s0) += expf(v - mm);  // an infinite maximum, or NaN, makes the sum NaN
+          if (!(v < floor_v)) mask |= 1u << (u * VW + i);
+        }
       }
+    sum += s0 + s1;
     while (__any_sync(kFull, mask != 0)) {  // one of each lane at a time, read again
       u64 key = 0;
       if (mask) {
