@@ -16,13 +16,13 @@ Public operators (all CUDA-only, backed by libmamba_b200_ss.so):
   beam_select, reorder_states          a beam-search step: the best continuations, and the beams'
                                        states in their new order in place
   causal_lm_forward                    a CausalLM's forward through the fused block and norm
-  generate, Decoder                    prefill + cached single-token decode (CUDA-graph step)
+  generate, beam_search, Decoder       prefill + cached single-token decode (CUDA-graph step)
   check_device_status                  raise if a kernel's bounded wait gave up since the last check
   set_status_check                     check after every scan call (debugging; synchronises)
 """
 from ._lib import check_device_status, set_status_check
 from .beam import beam_select, reorder_states
-from .decode import Decoder, generate
+from .decode import Decoder, beam_search, generate
 from .inner import MambaInnerFn, mamba_inner_fn, mamba_simple_forward
 from .lm import causal_lm_forward
 from .linear_attention import LinearAttentionFn, linear_attention_fn, linear_attention_step
@@ -31,6 +31,7 @@ from .selective_scan_interface import SelectiveScanFn, selective_scan_fn, select
 
 __all__ = ["SelectiveScanFn", "selective_scan_fn", "selective_state_update", "MambaInnerFn", "mamba_inner_fn",
            "mamba_simple_forward", "linear_attention_fn", "LinearAttentionFn", "linear_attention_step", "beam_select",
-           "reorder_states", "block_norm_fn", "rms_norm_fn", "rms_norm", "causal_lm_forward", "generate", "Decoder",
+           "reorder_states", "block_norm_fn", "rms_norm_fn", "rms_norm", "causal_lm_forward", "generate", "beam_search",
+           "Decoder",
            "check_device_status", "set_status_check"]
 __version__ = "0.1.0"

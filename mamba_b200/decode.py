@@ -1,12 +1,13 @@
 """Decoding for MambaSimple models: a prompt prefill that leaves per-layer states, single-token
-steps that continue from them, and ``generate`` for CausalLM-shaped models.
+steps that continue from them, and ``generate`` and ``beam_search`` for CausalLM-shaped models.
 
 The reference has no decode path: ``CausalLM.generate`` is a stub (models/causal_lm.py:61-62)
 and ``MambaSimple`` has no step, so continuing a sequence there means re-running the whole
 forward over it for every new token.  Here a block keeps two states per sequence:
 
 * conv state (batch, d_inner, K-1) fp32 — the last K-1 inputs of its causal convolution;
-* SSM state  (batch, d_inner, d_state) fp32 — h of the selective scan,
+* SSM state  (batch, d_inner, d_state) fp32 — h of the selective scan
+  (a layer with a ``linear_attn`` mixer: its state (batch, heads, key_dim, value_dim) fp32),
 
 and a new token costs the block's input and output projections plus one fused mixer kernel
 (``ss_mamba_step``: the conv step, the x and delta projections, the SSM step and the SiLU(z)
@@ -18,15 +19,23 @@ step is one graph launch rather than a dozen kernel launches per layer from Pyth
 
 Models are duck-typed on the reference's structure (models/causal_lm.py:20-58): ``embedding``,
 ``layers`` (each with ``norm``, ``mamba``), ``norm``, ``lm_head``; each ``mamba`` has
-MambaSimple's parameter names (modules/mamba_simple.py:33-85).  Dropout is not applied
-(inference).
+MambaSimple's parameter names (modules/mamba_simple.py:33-85); layers may hold a ``linear_attn``
+mixer, a ``post_norm``, a ``gate_proj`` and a ``residual_scale`` instead (see lm.py).  Dropout is not
+applied (inference).
+
+``beam_search`` keeps the beams as rows of the decoder's batch: after each selection
+(``beam_select``) the layers' states are put in the beams' new order in place (``reorder_states``), so
+the captured step goes on at the same addresses.
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib as L
+from .beam import beam_select, reorder_states
 from .inner import mamba_inner_prefill
+from .linear_attention import linear_attention_block_step, linear_attention_prefill
+from .lm import branch_parts, join_residual
 from .norm import rms_norm_fn
 from .selective_scan_interface import _cuda_device
 
@@ -94,57 +103,109 @@ def mamba_simple_step(block, hidden, conv_state, ssm_state, params: _BlockParams
     return block.output_proj(y)
 
 
+class _MambaLayer:
+    """A MambaSimple mixer and its states for a batch."""
+
+    def __init__(self, mixer, batch, dev):
+        self.mixer, self.params = mixer, _BlockParams(mixer)
+        p = self.params
+        self.states = [torch.zeros(batch, p.d, p.K - 1, device=dev), torch.zeros(batch, p.d, p.n, device=dev)]
+
+    def prefill(self, x):
+        y, *states = mamba_simple_prefill(self.mixer, x, self.params)
+        return y, states
+
+    def step(self, x):
+        return mamba_simple_step(self.mixer, x, *self.states, self.params)
+
+
+class _LinearLayer:
+    """A linear-attention mixer and its state for a batch."""
+
+    def __init__(self, mixer, batch, dev):
+        self.mixer = mixer
+        heads, key_heads = mixer.num_heads, mixer.num_key_heads
+        self.states = [torch.zeros(batch, heads, mixer.k_proj.weight.shape[0] // key_heads,
+                                   mixer.v_proj.weight.shape[0] // heads, device=dev)]
+
+    def prefill(self, x):
+        y, state = linear_attention_prefill(self.mixer, x)
+        return y, [state]
+
+    def step(self, x):
+        return linear_attention_block_step(self.mixer, x, *self.states)
+
+
 class Decoder:
     """Incremental decoding of a CausalLM-shaped model for a fixed batch size.
 
     ``prefill(input_ids)`` runs the prompt and returns the last position's logits;
-    ``step(token_ids)`` feeds one token per sequence and returns the next logits (fp32).
+    ``step(token_ids)`` feeds one token per sequence and returns the next logits (fp32);
+    ``reorder(parents)`` puts the states of beams in a new order.
     With ``cuda_graph`` the step is captured on first use and replayed afterwards."""
 
     def __init__(self, model, batch: int, cuda_graph: bool = True):
         self.model = model
         self.batch = batch
-        self.params = [_BlockParams(layer.mamba) for layer in model.layers]
-        # fp32 norm weights, cast once (a per-call cast would be one more kernel per layer and step)
-        self.norms = [(layer.norm.weight.detach().float().contiguous(), layer.norm.eps) for layer in model.layers]
-        self.final_norm = (model.norm.weight.detach().float().contiguous(), model.norm.eps)
         dev = model.lm_head.weight.device
-        self.conv_states = [torch.zeros(batch, p.d, p.K - 1, device=dev) for p in self.params]
-        self.ssm_states = [torch.zeros(batch, p.d, p.n, device=dev) for p in self.params]
+        self.mixers = [_LinearLayer(layer.linear_attn, batch, dev) if getattr(layer, "linear_attn", None) is not None
+                       else _MambaLayer(layer.mamba, batch, dev) for layer in model.layers]
+        self.states = [s for m in self.mixers for s in m.states]
+        # fp32 norm weights, cast once (a per-call cast would be one more kernel per layer and step)
+        norms = [layer.norm for layer in model.layers] + [model.norm]
+        self.norms = [(n.weight.detach().float().contiguous(), n.eps) for n in norms]
+        self.parts = [branch_parts(layer, n) for layer, n in zip(model.layers, norms[1:])]
         self.cuda_graph = cuda_graph
         self.graph = None
         self.tok = torch.zeros(batch, dtype=torch.long, device=dev)
         self.logits = None
 
-    @torch.no_grad()
-    def prefill(self, input_ids):
-        if input_ids.shape[0] != self.batch:
-            raise ValueError(f"batch {input_ids.shape[0]} != decoder batch {self.batch}")
-        m = self.model
-        h = m.embedding(input_ids)
-        res = y = None
-        for i, layer in enumerate(m.layers):
-            # the residual add of the previous block fused with this block's RMSNorm
-            x, res = self._norm(i, h if res is None else y, res)
-            y, cs, ss = mamba_simple_prefill(layer.mamba, x, self.params[i])
-            self.conv_states[i].copy_(cs)
-            self.ssm_states[i].copy_(ss)
-        w, eps = self.final_norm
-        return m.lm_head(rms_norm_fn(y[:, -1], w, res[:, -1], eps)).float()
+    # the per-layer states of MambaSimple layers, as lists over the layers
+    @property
+    def conv_states(self):
+        return [m.states[0] for m in self.mixers if isinstance(m, _MambaLayer)]
 
-    def _norm(self, i, x, res):
-        w, eps = self.norms[i]
-        return rms_norm_fn(x, w, res, eps, True, True)
+    @property
+    def ssm_states(self):
+        return [m.states[1] for m in self.mixers if isinstance(m, _MambaLayer)]
+
+    @torch.no_grad()
+    def prefill(self, input_ids, repeat: int = 1):
+        """Runs a prompt (batch / repeat, L); each row's states go to ``repeat`` rows of the batch (its beams).
+        Returns the last position's logits (batch / repeat, vocab)."""
+        if input_ids.shape[0] * repeat != self.batch:
+            raise ValueError(f"batch {input_ids.shape[0]} x {repeat} != decoder batch {self.batch}")
+
+        def mixer(m, x):
+            y, states = m.prefill(x)
+            for own, new in zip(m.states, states):
+                own.unflatten(0, (-1, repeat)).copy_(new[:, None])
+            return y
+
+        return self._run(self.model.embedding(input_ids), mixer)
+
+    def _run(self, h, mixer):
+        """Logits from embeddings (batch, [L,] d_model): the last position's where there are several."""
+        w, eps = self.norms[0]
+        x, res = rms_norm_fn(h, w, None, eps, True, True)
+        last = len(self.mixers) - 1
+        for i, m in enumerate(self.mixers):
+            y = mixer(m, x)
+            if i == last and y.dim() == 3:
+                x, y, res = x[:, -1], y[:, -1], res[:, -1]
+            w, eps = self.norms[i + 1]
+            if i == last and self.parts[i] is None:
+                x = rms_norm_fn(y, w, res, eps)
+            else:  # the residual add of this block fused with the next norm
+                x, res = join_residual(self.parts[i], x, y, res, w, eps)
+        return self.model.lm_head(x).float()
 
     def _step_eager(self, tok):
-        m = self.model
-        h = m.embedding(tok)
-        res = y = None
-        for i, layer in enumerate(m.layers):
-            x, res = self._norm(i, h if res is None else y, res)
-            y = mamba_simple_step(layer.mamba, x, self.conv_states[i], self.ssm_states[i], self.params[i])
-        w, eps = self.final_norm
-        return m.lm_head(rms_norm_fn(y, w, res, eps)).float()
+        return self._run(self.model.embedding(tok), lambda m, x: m.step(x))
+
+    def reorder(self, parents):
+        """parents (batch / beams, beams) int64: row w of a prompt's beams becomes what row parents[:, w] was."""
+        reorder_states(self.states, parents)
 
     @torch.no_grad()
     def step(self, token_ids):
@@ -158,7 +219,7 @@ class Decoder:
 
     def _capture(self):
         # warm-up on a side stream (library handles, cuBLAS workspaces), states saved around it
-        saved = [t.clone() for t in self.conv_states + self.ssm_states]
+        saved = [t.clone() for t in self.states]
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -168,7 +229,7 @@ class Decoder:
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self.logits = self._step_eager(self.tok)
-        for t, v in zip(self.conv_states + self.ssm_states, saved):
+        for t, v in zip(self.states, saved):
             t.copy_(v)
 
 
@@ -197,3 +258,46 @@ def generate(model, input_ids, max_new_tokens: int = 50, temperature: float = 1.
         if i + 1 < max_new_tokens:
             logits = dec.step(tok)
     return torch.cat(out, 1)
+
+
+@torch.no_grad()
+def beam_search(model, input_ids, num_beams: int, max_new_tokens: int = 50, eos_token_id: int | None = None,
+                length_penalty: float = 1.0, cuda_graph: bool = True):
+    """The most probable continuation found with ``num_beams`` beams for every sequence of ``input_ids``
+    (batch, L).  A beam that emits eos_token_id is finished and keeps its place and its score, its row
+    filled with eos_token_id.  The beams of a prompt are ranked by score / length ** length_penalty, length
+    counting new tokens up to the first eos.  Returns (ids (batch, L + T) of the best beam, its ranking
+    score (batch,)), T <= max_new_tokens (less when every beam has finished)."""
+    if num_beams < 1:
+        raise ValueError(f"num_beams {num_beams}")
+    b, l = input_ids.shape
+    if max_new_tokens < 1:
+        return input_ids, torch.zeros(b, device=input_ids.device)
+    w, dev = num_beams, input_ids.device
+    dec = Decoder(model, b * w, cuda_graph=cuda_graph)
+    logits = dec.prefill(input_ids, repeat=w)
+    # the first step chooses among one beam's tokens: the others are copies of it
+    scores = torch.full((b, w), float("-inf"), device=dev)
+    scores[:, 0] = 0.0
+    logits = logits[:, None].expand(b, w, logits.shape[-1])
+    done = torch.zeros(b, w, dtype=torch.bool, device=dev)
+    length = torch.zeros(b, w, dtype=torch.long, device=dev)
+    ids = input_ids[:, None].expand(b, w, l)
+    for i in range(max_new_tokens):
+        marks = (None, None) if eos_token_id is None else (done, eos_token_id)
+        scores, parents, tokens = beam_select(logits, scores, None, *marks)
+        ids = torch.cat([ids.gather(1, parents[..., None].expand_as(ids)), tokens[..., None]], -1)
+        done, length = done.gather(1, parents), length.gather(1, parents)
+        length = length + (~done)
+        if eos_token_id is not None:
+            done = done | (tokens == eos_token_id)
+            if bool(done.all()):
+                break
+        if i + 1 < max_new_tokens:
+            if i > 0:  # after the prompt every beam has the same states
+                dec.reorder(parents)
+            logits = dec.step(tokens.flatten()).unflatten(0, (b, w))
+    rank = scores / length.clamp(min=1).float() ** length_penalty
+    best = rank.argmax(-1)
+    rows = torch.arange(b, device=dev)
+    return ids[rows, best], rank[rows, best]
