@@ -35,21 +35,25 @@ bool dtypes_ok(int io, int decay) {
   return (io == SS_F32 || io == SS_BF16 || io == SS_F16) && (decay == SS_F32 || decay == io);
 }
 
-// Segments that run side by side: enough CTAs for the GPU when batch x heads are few, at least two
-// chunks each (a segment's own state costs a pass over its keys and values), at most 32 (every
-// segment folds the states of those before it).
+// Segments that run side by side: enough CTAs for the GPU when batch x heads are few, at least two chunks
+// each, at most 32.  A segment's own state costs about half of what its outputs cost, and the first segment
+// neither needs nor waits for the states of the others: it starts beside their first pass (a programmatic
+// launch) and is half as long again (1 x 16384 x 16 heads of 128 x 128: 165 us with equal segments).
 struct Split {
-  int segs, chunks;
+  int segs, first, chunks;
 };
 
 Split split_of(const ss_linear_args& a, int chunk, int passes, int tiles) {
-  const int64_t n = (a.seqlen + chunk - 1) / chunk;
+  const int n = (a.seqlen + chunk - 1) / chunk;
   const int64_t ctas = (int64_t)a.batch * a.heads * passes * tiles;
-  int64_t segs = 1;
-  if (ctas > 0 && ctas < 148) segs = std::max<int64_t>(1, std::min<int64_t>({148 / ctas, n / 2, 32}));
-  Split s;
-  s.chunks = (int)std::max<int64_t>(1, (n + segs - 1) / segs);
-  s.segs = (int)std::max<int64_t>(1, (n + s.chunks - 1) / s.chunks);
+  int segs = 1;
+  if (ctas > 0 && ctas < 148) segs = (int)std::max<int64_t>(1, std::min<int64_t>({148 / ctas, n / 2, 32}));
+  Split s{1, std::max(n, 1), std::max(n, 1)};
+  if (segs > 1) {
+    s.chunks = std::max(1, (2 * n + 2 * segs) / (2 * segs + 1));  // n / (segs + 1/2)
+    s.first = std::min(n - 1, std::max(s.chunks, n - (segs - 1) * s.chunks));
+    s.segs = 1 + (n - s.first + s.chunks - 1) / s.chunks;
+  }
   return s;
 }
 
@@ -66,7 +70,7 @@ Work work_of(const ss_linear_args& a, int backward) {
   const int passes = backward ? 3 : 1;
   const int tiles = backward ? std::max(tiles_of(a.key_dim), tiles_of(a.value_dim)) : tiles_of(a.value_dim);
   w.simt = split_of(a, kLsC, passes, tiles);
-  w.tc = a.io_dtype == SS_F32 ? Split{1, 1} : split_of(a, kTcC, passes, tiles);
+  w.tc = a.io_dtype == SS_F32 ? Split{1, 1, 1} : split_of(a, kTcC, passes, tiles);
   const int segs = a.io_dtype == SS_F32 ? w.simt.segs : std::max(w.simt.segs, w.tc.segs);
   const size_t bh = (size_t)a.batch * a.heads;
   auto take = [&](size_t n) {
@@ -85,12 +89,27 @@ Work work_of(const ss_linear_args& a, int backward) {
   return w;
 }
 
+// a launch that may start before the kernel ahead of it in the stream has ended (it waits where it has to)
+template <typename K>
+cudaError_t launch_early(void (*kern)(K), dim3 grid, int threads, size_t smem, const K& P, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, P);
+}
+
 cudaError_t launch_fold(const LinK& P, int passes, cudaStream_t st) {
   int64_t block = 0;
   for (int i = 0; i < passes; ++i) block = std::max<int64_t>(block, (int64_t)P.pass[i].dk * P.pass[i].dv);
   const dim3 grid((unsigned)((block + 255) / 256), (unsigned)(P.batch * P.heads), (unsigned)passes);
-  linear_fold_kernel<<<grid, 256, 0, st>>>(P);
-  return cudaGetLastError();
+  return launch_early(linear_fold_kernel, grid, 256, 0, P, st);
 }
 
 template <typename IT>
@@ -108,31 +127,53 @@ cudaError_t run_simt(const LinK& P, int passes, cudaStream_t st) {
     e = cudaGetLastError();
     if (e == cudaSuccess) e = launch_fold(P, passes, st);
     if (e != cudaSuccess) return e;
+    return launch_early(main_k, grid, kLsThreads, smem, P, st);
   }
   main_k<<<grid, kLsThreads, smem, st>>>(P);
   return cudaGetLastError();
 }
 
-template <typename IT>
-cudaError_t launch_tc(const LinTcK& P, bool wide, cudaStream_t st) {
-  static_assert(TcShape<64>::kBytes <= 232448 && TcShape<128>::kBytes <= 232448, "shared memory of a CTA");
+// one launch over passes [pass0, pass0 + n) of T
+template <typename IT, int MODE>
+cudaError_t launch_tc(LinTcK& T, int pass0, int n, bool early, cudaStream_t st) {
+  constexpr size_t most = std::max(TcShape<64>::kBytes, TcShape<128>::kBytes);
+  static_assert(most <= 232448, "shared memory of a CTA");
   static_assert(sizeof(TcBars) <= 512, "barriers");
-  const size_t smem = wide ? std::max(TcShape<64>::kBytes, TcShape<128>::kBytes) : TcShape<64>::kBytes;
-  auto main_k = linear_tc_kernel<IT, false>;
-  auto sum_k = linear_tc_kernel<IT, true>;
-  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(main_k), std::max(TcShape<64>::kBytes, TcShape<128>::kBytes));
-  if (e == cudaSuccess)
-    e = ensure_smem_limit(reinterpret_cast<const void*>(sum_k), std::max(TcShape<64>::kBytes, TcShape<128>::kBytes));
+  auto kern = linear_tc_kernel<IT, MODE>;
+  const cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), most);
   if (e != cudaSuccess) return e;
-  const unsigned grid = (unsigned)((int64_t)P.k.batch * P.k.heads * P.k.segs * P.parts);
-  if (P.k.segs > 1) {
-    sum_k<<<grid, kTcThreads, smem, st>>>(P);
-    e = cudaGetLastError();
-    if (e == cudaSuccess) e = launch_fold(P.k, P.parts / P.tiles, st);
-    if (e != cudaSuccess) return e;
+  T.pass0 = pass0;
+  T.tiles = 1;
+  bool wide = false;
+  for (int i = pass0; i < pass0 + n; ++i) {
+    T.tiles = std::max(T.tiles, (T.k.pass[i].dv + kTcN - 1) / kTcN);
+    wide |= T.k.pass[i].dk > 64;
   }
-  main_k<<<grid, kTcThreads, smem, st>>>(P);
+  T.parts = n * T.tiles;
+  const dim3 grid((unsigned)((int64_t)T.k.batch * T.k.heads * T.k.segs * T.parts));
+  const size_t smem = wide ? most : (size_t)TcShape<64>::kBytes;
+  if (early) return launch_early(kern, grid, kTcThreads, smem, T, st);
+  kern<<<grid, kTcThreads, smem, st>>>(T);
   return cudaGetLastError();
+}
+
+// The passes' segments and fold, then the gradients with dot products (the first `grads`), then the others.
+// Every launch but the first may start while the one ahead of it runs: its first segments need nothing of it.
+template <typename IT>
+cudaError_t launch_all(LinTcK& T, int passes, int grads, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
+  bool early = false;
+  if (T.k.segs > 1) {
+    e = launch_tc<IT, kTcState>(T, 0, passes, false, st);
+    if (e == cudaSuccess) e = launch_fold(T.k, passes, st);
+    early = true;
+  }
+  if (e == cudaSuccess && grads > 0) {
+    e = launch_tc<IT, kTcGrad>(T, 0, grads, early, st);
+    early = true;
+  }
+  if (e == cudaSuccess && grads < passes) e = launch_tc<IT, kTcOut>(T, grads, passes - grads, early, st);
+  return e;
 }
 
 bool vec16(const void* p, int es, int64_t b, int64_t l, int64_t h) {
@@ -143,8 +184,7 @@ bool vec16(const void* p, int es, int64_t b, int64_t l, int64_t h) {
 // stores); false: it cannot.
 bool run_tc(int io, const LinK& P, int passes, cudaStream_t st, cudaError_t* e) {
   LinTcK T;
-  T.tiles = 1;
-  bool wide = false;
+  int grads = 0;
   for (int i = 0; i < passes; ++i) {
     const LinPass& A = P.pass[i];
     if (A.dk % 8 || A.dv % 8 || !vec16(A.o, A.o_f32 ? 4 : 2, A.ob, A.ol, A.oh) ||
@@ -162,24 +202,22 @@ bool run_tc(int io, const LinK& P, int passes, cudaStream_t st, cudaError_t* e) 
                                         A.ol, A.ob, 32);
       if (!ok) return false;
     }
-    T.tiles = std::max(T.tiles, (A.dv + kTcN - 1) / kTcN);
-    wide |= A.dk > 64;
+    grads += A.dot || A.o_f32;  // they come first
   }
   T.k = P;
-  T.parts = passes * T.tiles;
   T.status = device_status_word();
   T.wait_limit = wait_limit();
-  *e = io == SS_BF16 ? launch_tc<__nv_bfloat16>(T, wide, st) : launch_tc<__half>(T, wide, st);
+  *e = io == SS_BF16 ? launch_all<__nv_bfloat16>(T, passes, grads, st) : launch_all<__half>(T, passes, grads, st);
   return true;
 }
 
 cudaError_t run_passes(int io, LinK& P, const Work& w, int passes, cudaStream_t st) {
   if (io != SS_F32 && P.seqlen > 0) {
-    P.segs = w.tc.segs, P.seg_chunks = w.tc.chunks;
+    P.segs = w.tc.segs, P.seg_first = w.tc.first, P.seg_chunks = w.tc.chunks;
     cudaError_t e;
     if (run_tc(io, P, passes, st, &e)) return e;
   }
-  P.segs = w.simt.segs, P.seg_chunks = w.simt.chunks;
+  P.segs = w.simt.segs, P.seg_first = w.simt.first, P.seg_chunks = w.simt.chunks;
   switch (io) {
     case SS_F32: return run_simt<float>(P, passes, st);
     case SS_BF16: return run_simt<__nv_bfloat16>(P, passes, st);

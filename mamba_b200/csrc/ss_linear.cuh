@@ -58,7 +58,7 @@ struct LinK {
   const int* lens;     // nullable
   float* seg_decay;    // [direction][b * h][segment]: the segment's total log decay
   int batch, seqlen, heads;
-  int segs, seg_chunks;  // segments of the sequence, chunks of each
+  int segs, seg_first, seg_chunks;  // segments of the sequence, chunks of the first and of each other
 };
 
 // log decays below this act as a reset: e^x is 0 in fp32 already, and sums of -1e4 stay exact
@@ -106,12 +106,15 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
   const int dk = A.dk, dv = A.dv;
   if (n0 >= dv) return;
   const int nv = min(kLsN, dv - n0);
-  const int bh = blockIdx.x / P.segs, seg = blockIdx.x % P.segs;
+  const int bh = blockIdx.x % (P.batch * P.heads), seg = blockIdx.x / (P.batch * P.heads);
+  if (STATE_ONLY) griddep_launch_dependents();
+  else if (seg > 0) griddep_wait();  // the first segment needs nothing of the passes before
   if (STATE_ONLY && seg == P.segs - 1) return;  // nothing follows the last segment
   const int b = bh / P.heads, head = bh % P.heads;
   const int len = P.lens ? max(0, min(P.lens[b], P.seqlen)) : P.seqlen;
   const int n_chunks = (P.seqlen + kLsC - 1) / kLsC, n_live = (len + kLsC - 1) / kLsC;
-  const int c0 = seg * P.seg_chunks, c1 = min(c0 + P.seg_chunks, n_chunks);
+  const int c0 = seg ? P.seg_first + (seg - 1) * P.seg_chunks : 0,
+            c1 = min(seg ? c0 + P.seg_chunks : P.seg_first, n_chunks);
   const IT* q = static_cast<const IT*>(A.q) + (int64_t)b * A.qb + (int64_t)(head / A.rq) * A.qh;
   const IT* k = static_cast<const IT*>(A.k) + (int64_t)b * A.kb + (int64_t)(head / A.rk) * A.kh;
   const IT* v = static_cast<const IT*>(A.v) + (int64_t)b * A.vb + (int64_t)(head / A.rv) * A.vh + n0;
@@ -125,7 +128,7 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
     const int i = e / kLsN, j = e % kLsN;
     float s = 0.f;
     if (!STATE_ONLY && i < dk && j < nv) {
-      if (P.segs > 1) s = A.sum[((int64_t)bh * P.segs + seg) * block + (int64_t)i * dv + n0 + j];
+      if (seg > 0) s = A.sum[((int64_t)bh * P.segs + seg) * block + (int64_t)i * dv + n0 + j];
       else if (A.s_in) s = A.s_in_scale * A.s_in[bh * block + (int64_t)i * A.s_row + (int64_t)(n0 + j) * A.s_col];
     }
     S.h[i][j] = s;
@@ -322,6 +325,8 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
 // The segments' own states -> the state before each segment, in place: a thread an entry, its segments in
 // order, 8 loads under way at a time.
 __global__ void __launch_bounds__(256) linear_fold_kernel(const __grid_constant__ LinK P) {
+  griddep_launch_dependents();  // the main pass's first segments need no fold; the others wait for it
+  griddep_wait();
   const LinPass& A = P.pass[blockIdx.z];
   const int64_t block = (int64_t)A.dk * A.dv, bh = blockIdx.y;
   __shared__ float decay[32];

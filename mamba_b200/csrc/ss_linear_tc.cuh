@@ -6,19 +6,19 @@
 //   S   = Q K^T                 128 x 128 x dk    operands as TMA wrote them (K-major, 128-byte swizzle)
 //   P   = S * e^{G_i - G_j}     masked, rounded to 16 bits into TMEM, the A operand of the next product
 //   Oa  = P V                   128 x 64 x 128    V as the MN-major B operand
-//   Oi  = Q Hhi + Q Hlo         128 x 64 x dk     the state before the chunk, split into two 16-bit parts
+//   Oi  = Q Hhi [+ Q Hlo]       128 x 64 x dk     the state before the chunk, in one or two 16-bit parts
 //   L   = K^T V'hi + K^T V'lo   dk x 64 x 128     V' = e^{T - G_j} v_j, split likewise; K as MN-major A
 //   o   = scale (e^{G_i} Oi + Oa),   H <- e^T H + L   (H in fp32 registers, one row a thread)
 //
-// Rounding: Q, K and V enter as they are.  The weighted scores P are the one place where 16 bits
-// (half a step) are accepted: an output is rounded to the same type anyway.  The state and the
-// weighted values would spread their rounding to every later token and to the fp32 final state, so
-// they are split: hi + lo keeps 16 (bf16) or 22 (fp16) bits, at two products of 64 columns each.
+// Rounding: Q, K and V enter as they are.  Each of an output's two sums has one factor rounded to 16 bits
+// (half a step): the weighted scores P, and the state H.  An output is rounded to the same type anyway, so
+// its error grows by at most sqrt 2.  The weighted values are split: hi + lo keeps 16 (bf16) or 22 (fp16)
+// bits, since their rounding would spread to every later token and to the fp32 final state.  Where the dot
+// products for the decays' gradient are wanted, H is split as well: the sums of q . dq - k . dk telescope
+// only as far as both runs round the same P alike and nothing else.
 // fp16 has a mantissa to spare and no range: its weighted scores are scaled by a power of two per row (from a
 // bound, the row's largest |q| times the chunk's largest |k| times dk), V' and H by one per chunk (from their
 // largest value), which the outputs and the state take back; bf16 needs none of that.
-// The dot products for the decays' gradient need it too: sums of q . dq - k . dk telescope only as far
-// as both runs round the same P alike and nothing else.
 //
 // What bounds it: a chunk moves 128 x (2 dk + 128) x 2 bytes through TMA; two value tiles of one head
 // run side by side, so keys and queries come from L2 the second time.
@@ -39,7 +39,7 @@ constexpr uint32_t kBox = kTcC * 128;  // one TMA box: 128 rows of 128 bytes
 
 struct LinTcK {
   LinK k;
-  int tiles, parts;      // value tiles of the widest pass; passes x tiles
+  int pass0, tiles, parts;  // first pass of the launch, value tiles of its widest, passes x tiles
   int* status;
   long long wait_limit;
   alignas(64) CUtensorMap map[kLinMaxPasses][4];  // q, k, v, o of each pass
@@ -257,20 +257,28 @@ __device__ __forceinline__ float max_of2(uint32_t m) {
   return fmaxf(f.x, f.y);
 }
 
-template <typename IT, int DK, bool STATE_ONLY>
+// What a run writes: the segments' own states; outputs; outputs in parts or with their dot products (gradients
+// of q and k)
+enum { kTcState = 0, kTcOut = 1, kTcGrad = 2 };
+
+template <typename IT, int DK, int MODE>
 __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int tile, int where, unsigned char* smem) {
   using S = TcShape<DK>;
+  constexpr bool STATE_ONLY = MODE == kTcState;
+  constexpr bool split_h = MODE == kTcGrad;  // H enters Q H in two parts
   TcBars& B = *reinterpret_cast<TcBars*>(smem + S::kBars);
   const LinK& K = P.k;
   const LinPass& A = K.pass[pass];
   const int dk = A.dk, dv = A.dv, n0 = tile * kTcN;
-  const int bh = where / K.segs, seg = where % K.segs;
+  const int bh = where % (K.batch * K.heads), seg = where / (K.batch * K.heads);
+  if (!STATE_ONLY && seg > 0) griddep_wait();  // the first segment needs nothing of the passes before
   if (n0 >= dv || (STATE_ONLY && seg == K.segs - 1)) return;
   const int nv = min(kTcN, dv - n0);
   const int b = bh / K.heads, head = bh % K.heads;
   const int len = K.lens ? max(0, min(K.lens[b], K.seqlen)) : K.seqlen;
   const int n_chunks = (K.seqlen + kTcC - 1) / kTcC, n_live = (len + kTcC - 1) / kTcC;
-  const int c0 = seg * K.seg_chunks, c1 = min(c0 + K.seg_chunks, n_chunks), cn = min(c1, n_live);
+  const int c0 = seg ? K.seg_first + (seg - 1) * K.seg_chunks : 0,
+            c1 = min(seg ? c0 + K.seg_chunks : K.seg_first, n_chunks), cn = min(c1, n_live);
   const bool reverse = A.reverse != 0;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, wg = wid >> 2, row = tid & 127;
   auto first_token = [&](int c) { return (reverse ? n_live - 1 - c : c) * kTcC; };
@@ -455,9 +463,13 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
         tc_after();
         if (elect_one()) {
 #pragma unroll
-          for (int x = 0; x < 2 * DK / 16; ++x) {
-            const int k = x % (DK / 16);
-            mma_ss(tm + kTmOi + (i & 1) * kTcN, q0 + o + (k >> 2) * (kBox >> 4) + (k & 3) * 2, h0 + x * 128, kIdN, x > 0);
+          for (int x = 0; x < DK / 16; ++x)
+            mma_ss(tm + kTmOi + (i & 1) * kTcN, q0 + o + (x >> 2) * (kBox >> 4) + (x & 3) * 2, h0 + x * 128, kIdN, x > 0);
+          if constexpr (split_h) {
+#pragma unroll
+            for (int x = 0; x < DK / 16; ++x)
+              mma_ss(tm + kTmOi + (i & 1) * kTcN, q0 + o + (x >> 2) * (kBox >> 4) + (x & 3) * 2,
+                     h0 + (DK / 16 + x) * 128, kIdN, true);
           }
           tc_commit(&B.h_empty);
         }
@@ -631,10 +643,12 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
   } else if (wg == 2) {
     // ------------------------------------------------------------ outputs
     if constexpr (!STATE_ONLY) {
+      const bool o_f32 = MODE == kTcGrad && A.o_f32;
       const int w4 = wid & 3;
-      const bool own_out = S::kOwnOut && !A.o_f32;  // fp32 tiles, twice as large, take Q's and K's room
+      // wide heads: the room of H's low part where that is not used; fp32 tiles, twice as large, take Q's and K's
+      const bool own_out = (S::kOwnOut || !split_h) && !o_f32;
       const IT* p_at = A.dot ? static_cast<const IT*>(A.p) + (int64_t)b * A.pb + (int64_t)(head / A.rp) * A.ph + n0 : nullptr;
-      float* dot_at = A.dot ? A.dot + (((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen : nullptr;
+      float* dot_at = MODE == kTcGrad && A.dot ? A.dot + (((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen : nullptr;
       const float2 sc = f2(A.scale);
       for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
         const int t0 = first_token(c), m = min(kTcC, len - t0), t = t0 + row;
@@ -643,7 +657,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
         const bool on = row < m;
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(A.o_f32 ? &B.v_empty[st] : &B.empty[st]);
+          mbar_arrive(o_f32 ? &B.v_empty[st] : &B.empty[st]);
           if (own_out) mbar_arrive(&B.v_empty[st]);
         }
         // 16 columns at a time, the next ones of p under way
@@ -661,7 +675,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
           wi = mul2(wi, f2(pow2(-*reinterpret_cast<volatile int*>(&B.h_exp[i & 3]))));
           wa = mul2(wa, f2(pow2(-row_exp[(i & 1) * 128 + row])));
         }
-        const uint32_t tile_at = own_out ? S::kOut : st * S::kStageBytes + (A.o_f32 ? 0 : S::kVAt);
+        const uint32_t tile_at = own_out ? (S::kOwnOut ? S::kOut : S::kH + DK * 128) : st * S::kStageBytes + (o_f32 ? 0 : S::kVAt);
         if (own_out) {
           if (elect_one()) tma_store_read();  // the tile before has left
           __syncwarp();
@@ -681,7 +695,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
             const float2 r = fma2(wi, make_float2(o[j], o[j + 1]), mul2(wa, make_float2(oa[j], oa[j + 1])));
             o[j] = on ? r.x : 0.f, o[j + 1] = on ? r.y : 0.f;
           }
-          if (A.o_f32) {
+          if (o_f32) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               *reinterpret_cast<float4*>(out + (x >> 1) * kBox + ((((x & 1) * 4 + j) ^ (row & 7)) << 4)) =
@@ -707,14 +721,14 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
           if (t0 + w4 * 32 < K.seqlen) {
             const uint32_t src = smem_u32(smem) + tile_at + w4 * 32 * 128;
             tma_store_4d(&P.map[pass][3], src, n0, head, t0 + w4 * 32, b);
-            if (A.o_f32 && n0 + 32 < dv) tma_store_4d(&P.map[pass][3], src + kBox, n0 + 32, head, t0 + w4 * 32, b);
+            if (o_f32 && n0 + 32 < dv) tma_store_4d(&P.map[pass][3], src + kBox, n0 + 32, head, t0 + w4 * 32, b);
           }
           if (own_out) {
             tma_store_commit();
           } else {
             tma_store_commit();
             tma_store_read();
-            mbar_arrive(A.o_f32 ? &B.empty[st] : &B.v_empty[st]);
+            mbar_arrive(o_f32 ? &B.empty[st] : &B.v_empty[st]);
           }
         }
         __syncwarp();
@@ -724,7 +738,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       if (elect_one()) tma_store_read();
       __syncwarp();
       auto zero_row = [&](int t) {
-        const int es = A.o_f32 ? 4 : 2;
+        const int es = o_f32 ? 4 : 2;
         char* o = static_cast<char*>(A.o) + ((int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0) * es;
 #pragma unroll 1
         for (int j = 0; j < nv * es; j += 16) *reinterpret_cast<uint4*>(o + j) = make_uint4(0, 0, 0, 0);
@@ -758,7 +772,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
           }
         }
       };
-      if (!STATE_ONLY && K.segs > 1) {  // folded from the initial state and the segments before
+      if (!STATE_ONLY && seg > 0) {  // folded from the initial state and the segments before
         const float* s0 = A.sum + ((int64_t)bh * K.segs + seg) * block + (int64_t)r0 * dv + n0;
         each([&](int r, int j) { return s0[(int64_t)r * dv + j]; });
       } else {
@@ -798,7 +812,12 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
                                    : make_float2(h[8 * j + r], h[8 * j + r + 1]);
             x[r] = t.x, x[r + 1] = t.y;
           }
-          store_split<IT>(hh, hh + DK * 128, row, j, x);
+          if constexpr (split_h) {
+            store_split<IT>(hh, hh + DK * 128, row, j, x);
+          } else {
+            *reinterpret_cast<uint4*>(hh + row * 128 + ((j ^ (row & 7)) << 4)) =
+                make_uint4(pack2<IT>(x[0], x[1]), pack2<IT>(x[2], x[3]), pack2<IT>(x[4], x[5]), pack2<IT>(x[6], x[7]));
+          }
         }
       }
       fence_async_smem();
@@ -837,14 +856,12 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       if (lane == 0) mbar_arrive(&B.l_empty);
       if (++st == S::kStages) st = 0, ph ^= 1;
     }
-    // the last halves have been read (h_empty) before the rows take their room again
-    const int n = cn - c0;
-    bool ok = *reinterpret_cast<volatile int*>(&B.abort) == 0;
-    if (!STATE_ONLY && n > 0) ok = warp_wait(&B.h_empty, (n - 1) & 1) && ok;
+    // the last product over V' has ended (l_full): the rows leave through its room
+    rows = reinterpret_cast<float*>(smem + S::kVp) + (wid & 3) * 32 * kTcN;
+    const bool ok = *reinterpret_cast<volatile int*>(&B.abort) == 0;
     float* to = STATE_ONLY ? A.sum + ((int64_t)bh * K.segs + seg) * block
                            : (A.s_out && seg == K.segs - 1 ? A.s_out + bh * block : nullptr);
-    if (to && r0 < DK) {  // every warp that has rows comes here, one that gave up as well
-      asm volatile("bar.sync 1, %0;" ::"n"(DK) : "memory");
+    if (to && r0 < DK) {
 #pragma unroll
       for (int j = 0; j < kTcN; j += 4)
         *reinterpret_cast<float4*>(rows + lane * kTcN + j) = make_float4(h[j], h[j + 1], h[j + 2], h[j + 3]);
@@ -875,14 +892,16 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
 }
 
 // Value tiles and runs of one head are neighbours in the grid, so that they share what they read in L2; runs
-// with narrow and with wide keys go side by side in one launch.
-template <typename IT, bool STATE_ONLY>
+// with narrow and with wide keys go side by side in one launch.  One kernel a mode: together they spilled and
+// fought over the instruction cache (8 x 2048 x 24 heads of 64, gradients: 322 us in one launch).
+template <typename IT, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_constant__ LinTcK P) {
   extern __shared__ __align__(1024) unsigned char smem[];
   const int part = blockIdx.x % P.parts, where = blockIdx.x / P.parts;
-  const int pass = part / P.tiles, tile = part % P.tiles;
-  if (P.k.pass[pass].dk > 64) linear_tc_run<IT, 128, STATE_ONLY>(P, pass, tile, where, smem);
-  else linear_tc_run<IT, 64, STATE_ONLY>(P, pass, tile, where, smem);
+  const int pass = P.pass0 + part / P.tiles, tile = part % P.tiles;
+  griddep_launch_dependents();
+  if (P.k.pass[pass].dk > 64) linear_tc_run<IT, 128, MODE>(P, pass, tile, where, smem);
+  else linear_tc_run<IT, 64, MODE>(P, pass, tile, where, smem);
 }
 
 }  // namespace ssb
