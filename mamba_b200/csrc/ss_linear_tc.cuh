@@ -657,17 +657,20 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
         const bool on = row < m;
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(o_f32 ? &B.v_empty[st] : &B.empty[st]);
+          if (!o_f32) mbar_arrive(&B.empty[st]);
           if (own_out) mbar_arrive(&B.v_empty[st]);
         }
-        // 16 columns at a time, the next ones of p under way
-        const IT* p = p_at + (int64_t)t * A.pl;
-        uint4 q0 = make_uint4(0, 0, 0, 0), q1 = q0;
-        auto load_p = [&](int x) {
-          q0 = on && 16 * x < nv ? *reinterpret_cast<const uint4*>(p + 16 * x) : make_uint4(0, 0, 0, 0);
-          q1 = on && 16 * x + 8 < nv ? *reinterpret_cast<const uint4*>(p + 16 * x + 8) : make_uint4(0, 0, 0, 0);
-        };
-        if (dot_at) load_p(0);
+        // the rows of p that go with the outputs, 8 lanes a row; they pass through shared memory, since a lane
+        // that read its own row would touch 32 lines an instruction
+        uint4 pq[8];
+        if (dot_at) {
+          const IT* p = p_at + (int64_t)(t0 + w4 * 32 + (lane >> 3)) * A.pl + (lane & 7) * 8;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const bool in = w4 * 32 + 4 * k + (lane >> 3) < m && (lane & 7) * 8 < nv;
+            pq[k] = in ? *reinterpret_cast<const uint4*>(p + (int64_t)4 * k * A.pl) : make_uint4(0, 0, 0, 0);
+          }
+        }
         if (!warp_wait(&B.o_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
         float2 wi = w, wa = sc;
@@ -681,14 +684,27 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
           __syncwarp();
         }
         unsigned char* out = smem + tile_at + row * 128;
+        const unsigned char* prow = o_f32 ? smem + st * S::kStageBytes + S::kVAt + row * 128 : out;  // V has been used
+        if (dot_at) {
+          unsigned char* to = const_cast<unsigned char*>(prow) - row * 128;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int r = w4 * 32 + 4 * k + (lane >> 3);
+            *reinterpret_cast<uint4*>(to + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = pq[k];
+          }
+          __syncwarp();
+        }
         float2 dot = f2(0.f);
 #pragma unroll 1
         for (int x = 0; x < 4; ++x) {
           float o[16], oa[16];
           tmem_ld16(lanes + kTmOi + (i & 1) * kTcN + x * 16, o);
           tmem_ld16(lanes + kTmOa + (i & 1) * 128 + x * 16, oa);
-          const uint32_t u[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
-          if (dot_at && x < 3) load_p(x + 1);
+          uint4 q0, q1;
+          if (dot_at) {
+            q0 = *reinterpret_cast<const uint4*>(prow + (((2 * x) ^ (row & 7)) << 4));
+            q1 = *reinterpret_cast<const uint4*>(prow + (((2 * x + 1) ^ (row & 7)) << 4));
+          }
           tc_wait_ld();
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
@@ -708,13 +724,17 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
                              pack2<IT>(o[8 * j + 4], o[8 * j + 5]), pack2<IT>(o[8 * j + 6], o[8 * j + 7]));
           }
           if (dot_at) {
+            const uint32_t u[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
             for (int j = 0; j < 8; ++j) dot = fma2(make_float2(o[2 * j], o[2 * j + 1]), unpack2<IT>(u[j]), dot);
           }
         }
         tc_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&B.o_empty[i & 1]);
+        if (lane == 0) {
+          mbar_arrive(&B.o_empty[i & 1]);
+          if (o_f32) mbar_arrive(&B.v_empty[st]);
+        }
         fence_async_smem();
         __syncwarp();
         if (elect_one()) {
