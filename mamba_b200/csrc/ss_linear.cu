@@ -172,7 +172,14 @@ cudaError_t launch_all(LinTcK& T, int passes, int grads, cudaStream_t st) {
     e = launch_tc<IT, kTcGrad>(T, 0, grads, early, st);
     early = true;
   }
-  if (e == cudaSuccess && grads < passes) e = launch_tc<IT, kTcOut>(T, grads, passes - grads, early, st);
+  if (e == cudaSuccess && grads < passes) {
+    bool state = false;  // fp16 keeps 22 bits in two parts and needs no other kernel
+    for (int i = grads; i < passes; ++i) state |= T.k.pass[i].s_out != nullptr && std::is_same<IT, __nv_bfloat16>::value;
+    if constexpr (std::is_same<IT, __nv_bfloat16>::value) {
+      if (state) return launch_tc<IT, kTcOutState>(T, grads, passes - grads, early, st);
+    }
+    e = launch_tc<IT, kTcOut>(T, grads, passes - grads, early, st);
+  }
   return e;
 }
 

@@ -7,7 +7,7 @@
 //   P   = S * e^{G_i - G_j}     masked, rounded to 16 bits into TMEM, the A operand of the next product
 //   Oa  = P V                   128 x 64 x 128    V as the MN-major B operand
 //   Oi  = Q Hhi [+ Q Hlo]       128 x 64 x dk     the state before the chunk, in one or two 16-bit parts
-//   L   = K^T V'hi + K^T V'lo   dk x 64 x 128     V' = e^{T - G_j} v_j, split likewise; K as MN-major A
+//   L   = K^T V'hi + K^T V'lo   dk x 64 x 128     V' = e^{T - G_j} v_j in two or three parts; K as MN-major A
 //   o   = scale (e^{G_i} Oi + Oa),   H <- e^T H + L   (H in fp32 registers, one row a thread)
 //
 // Rounding: Q, K and V enter as they are.  Each of an output's two sums has one factor rounded to 16 bits
@@ -143,19 +143,25 @@ __device__ __forceinline__ float2 unpack2(uint32_t p) {
   else
     return __half22float2(*reinterpret_cast<__half2*>(&p));
 }
-// 8 values of a row split into hi + lo and stored at 16-byte chunk j of row r of two swizzled tiles
+// 8 values of a row split into hi + lo [+ what is left] and stored at 16-byte chunk j of row r of swizzled tiles
 template <typename IT>
-__device__ __forceinline__ void store_split(unsigned char* hi, unsigned char* lo, int r, int j, const float (&v)[8]) {
-  uint32_t h[4], l[4];
+__device__ __forceinline__ void store_split(unsigned char* hi, unsigned char* lo, unsigned char* rest, int r, int j,
+                                            const float (&v)[8]) {
+  uint32_t h[4], l[4], t[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     h[i] = pack2<IT>(v[2 * i], v[2 * i + 1]);
     const float2 d = fma2(unpack2<IT>(h[i]), f2(-1.f), make_float2(v[2 * i], v[2 * i + 1]));
     l[i] = pack2<IT>(d.x, d.y);
+    if (rest) {
+      const float2 e = fma2(unpack2<IT>(l[i]), f2(-1.f), d);
+      t[i] = pack2<IT>(e.x, e.y);
+    }
   }
   const int at = r * 128 + ((j ^ (r & 7)) << 4);
   *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
   *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+  if (rest) *reinterpret_cast<uint4*>(rest + at) = make_uint4(t[0], t[1], t[2], t[3]);
 }
 
 // Shared memory: stages of Q, K, V as TMA writes them; V' (hi, lo); H (hi, lo); the output tile on its way to
@@ -259,13 +265,18 @@ __device__ __forceinline__ float max_of2(uint32_t m) {
 
 // What a run writes: the segments' own states; outputs; outputs in parts or with their dot products (gradients
 // of q and k)
-enum { kTcState = 0, kTcOut = 1, kTcGrad = 2 };
+// of q and k); outputs and a final state that is returned
+enum { kTcState = 0, kTcOut = 1, kTcGrad = 2, kTcOutState = 3 };
 
 template <typename IT, int DK, int MODE>
 __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int tile, int where, unsigned char* smem) {
   using S = TcShape<DK>;
   constexpr bool STATE_ONLY = MODE == kTcState;
   constexpr bool split_h = MODE == kTcGrad;  // H enters Q H in two parts
+  // bf16 states that leave the kernel: V' in three parts (24 bits; two are good to 2.4e-6 of a state's norm,
+  // three to 2e-7), the third where the output tile would go
+  constexpr bool third = std::is_same<IT, __nv_bfloat16>::value && (MODE == kTcState || MODE == kTcOutState);
+  constexpr uint32_t kThird = STATE_ONLY ? S::kH : S::kOwnOut ? S::kOut : S::kH + DK * 128;
   TcBars& B = *reinterpret_cast<TcBars*>(smem + S::kBars);
   const LinK& K = P.k;
   const LinPass& A = K.pass[pass];
@@ -452,6 +463,12 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       if (elect_one()) {
 #pragma unroll
         for (int x = 0; x < kTcC / 16; ++x) mma_ss(tm + kTmL, km0 + o + x * 128, vp0 + x * 128, kIdL, x > 0);
+        if constexpr (third) {  // onto the low part's columns
+#pragma unroll
+          for (int x = 0; x < kTcC / 16; ++x)
+            mma_ss(tm + kTmL + kTcN, km0 + o + x * 128, desc_of(base + kThird, kBox) + x * 128,
+                   idesc_of<IT>(128, kTcN, true, true), true);
+        }
         tc_commit(&B.l_full);
         if (STATE_ONLY) tc_commit(&B.empty[st]), tc_commit(&B.v_empty[st]);
       }
@@ -593,6 +610,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
     }
   } else if (wg == 1) {
     // ------------------------------------------------------------ weighted values
+    if constexpr (third && !STATE_ONLY) asm volatile("bar.sync 1, 256;" ::: "memory");  // the state has left the room
     for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
       const int m = min(kTcC, len - first_token(c));
       if (!warp_wait(&B.full[st], ph)) break;
@@ -633,7 +651,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
           x[2 * r] = f.x;
           x[2 * r + 1] = f.y;
         }
-        store_split<IT>(vp, vp + kBox, row, j, x);
+        store_split<IT>(vp, vp + kBox, third ? smem + kThird : nullptr, row, j, x);
       }
       fence_async_smem();
       __syncwarp();
@@ -646,7 +664,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       const bool o_f32 = MODE == kTcGrad && A.o_f32;
       const int w4 = wid & 3;
       // wide heads: the room of H's low part where that is not used; fp32 tiles, twice as large, take Q's and K's
-      const bool own_out = (S::kOwnOut || !split_h) && !o_f32;
+      const bool own_out = (S::kOwnOut || !split_h) && !third && !o_f32;
       const IT* p_at = A.dot ? static_cast<const IT*>(A.p) + (int64_t)b * A.pb + (int64_t)(head / A.rp) * A.ph + n0 : nullptr;
       float* dot_at = MODE == kTcGrad && A.dot ? A.dot + (((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen : nullptr;
       const float2 sc = f2(A.scale);
@@ -774,7 +792,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
     float h[kTcN];
     float* rows = reinterpret_cast<float*>(smem + S::kH) + (wid & 3) * 32 * kTcN;
     const int r0 = (wid & 3) * 32, rn = min(32, dk - r0);  // this warp's rows; <= 0: none
-    if (r0 < DK) {
+    if (!STATE_ONLY && r0 < DK) {
       // 8 loads under way at a time
       auto each = [&](auto&& f) {
 #pragma unroll 1
@@ -804,11 +822,12 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
     }
 #pragma unroll
     for (int j = 0; j < kTcN; j += 4) {
-      const float4 x = r0 < DK ? *reinterpret_cast<const float4*>(rows + lane * kTcN + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 x = !STATE_ONLY && r0 < DK ? *reinterpret_cast<const float4*>(rows + lane * kTcN + j)
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
       h[j] = x.x, h[j + 1] = x.y, h[j + 2] = x.z, h[j + 3] = x.w;
     }
-    // the halves of one warp lie in the rows of others
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    // the halves of one warp lie in the rows of others, and so may V's third part
+    if constexpr (!STATE_ONLY) asm volatile("bar.sync 1, %0;" ::"n"(third ? 256 : 128) : "memory");
     unsigned char* hh = smem + S::kH;
     auto publish = [&](int i) {
       float2 hw = f2(1.f);
@@ -833,7 +852,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
             x[r] = t.x, x[r + 1] = t.y;
           }
           if constexpr (split_h) {
-            store_split<IT>(hh, hh + DK * 128, row, j, x);
+            store_split<IT>(hh, hh + DK * 128, nullptr, row, j, x);
           } else {
             *reinterpret_cast<uint4*>(hh + row * 128 + ((j ^ (row & 7)) << 4)) =
                 make_uint4(pack2<IT>(x[0], x[1]), pack2<IT>(x[2], x[3]), pack2<IT>(x[4], x[5]), pack2<IT>(x[6], x[7]));
