@@ -187,14 +187,14 @@ struct TcShape {
 struct TcBars {
   uint64_t full[3], empty[3], v_empty[3];
   uint64_t s_full[2], p_full[2];
-  uint64_t vp_full, l_full, l_empty, h_full, h_empty, o_full[2], o_empty[2], drain;
+  uint64_t vp_full[2], vp_empty[2], l_full, l_empty, h_full, h_empty, o_full[2], o_empty[2], drain;
   float total[3], total2[3];  // e^T of the stage's chunk, T log2 e
   uint32_t tmem;
   int abort;
   // fp16: largest values of a chunk found by four warps, and the exponents they give
   uint64_t max_full[3];
   uint32_t max_of[3][4];
-  int v_exp[2], h_exp[4];
+  int v_exp[4], h_exp[4];
 };
 
 // TMEM columns: two score buffers (the weighted scores overwrite the first half of theirs, their product
@@ -277,6 +277,10 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
   // three to 2e-7), the third where the output tile would go
   constexpr bool third = std::is_same<IT, __nv_bfloat16>::value && (MODE == kTcState || MODE == kTcOutState);
   constexpr uint32_t kThird = STATE_ONLY ? S::kH : S::kOwnOut ? S::kOut : S::kH + DK * 128;
+  // buffers of V': a state's run, which loads no Q, keeps a second one where the stages' Q would be (its parts
+  // one after the other with wide keys, a stage apart with narrow ones)
+  constexpr int kVps = STATE_ONLY ? 2 : 1;
+  constexpr uint32_t kVp2Lead = DK == 128 ? kBox : S::kStageBytes, kVp2Third = DK == 128 ? S::kStageBytes : 2 * S::kStageBytes;
   TcBars& B = *reinterpret_cast<TcBars*>(smem + S::kBars);
   const LinK& K = P.k;
   const LinPass& A = K.pass[pass];
@@ -308,7 +312,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       mbar_init(&B.v_empty[i], STATE_ONLY ? 1 : 1 + 4);    // the products, the output tile that takes V's room
     }
     for (int i = 0; i < 2; ++i) mbar_init(&B.s_full[i], 1), mbar_init(&B.p_full[i], 4);
-    mbar_init(&B.vp_full, 4);
+    for (int i = 0; i < 2; ++i) mbar_init(&B.vp_full[i], STATE_ONLY ? 12 : 4), mbar_init(&B.vp_empty[i], 1);
     mbar_init(&B.l_full, 1), mbar_init(&B.l_empty, 4);
     mbar_init(&B.h_full, 4), mbar_init(&B.h_empty, 1);
     mbar_init(&B.o_full[0], 1), mbar_init(&B.o_full[1], 1), mbar_init(&B.o_empty[0], 4), mbar_init(&B.o_empty[1], 4);
@@ -457,18 +461,19 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       tc_after();
       if (!STATE_ONLY && i == 0) scores(0, 0);
       // L = K^T [V'hi, V'lo]: a product of 64 columns takes as long as one of 128
-      if (!warp_wait(&B.vp_full, i & 1) || (i > 0 && !warp_wait(&B.l_empty, (i - 1) & 1))) break;
+      if (!warp_wait(&B.vp_full[kVps == 2 ? i & 1 : 0], (uint32_t)(i / kVps) & 1) || (i > 0 && !warp_wait(&B.l_empty, (i - 1) & 1))) break;
       tc_after();
-      const uint32_t o = st * (S::kStageBytes >> 4);
+      const uint32_t o = st * (S::kStageBytes >> 4), vp = kVps == 2 && (i & 1) ? desc_of(base, kVp2Lead) : vp0;
       if (elect_one()) {
 #pragma unroll
-        for (int x = 0; x < kTcC / 16; ++x) mma_ss(tm + kTmL, km0 + o + x * 128, vp0 + x * 128, kIdL, x > 0);
+        for (int x = 0; x < kTcC / 16; ++x) mma_ss(tm + kTmL, km0 + o + x * 128, vp + x * 128, kIdL, x > 0);
         if constexpr (third) {  // onto the low part's columns
+          const uint32_t v3 = kVps == 2 && (i & 1) ? desc_of(base + kVp2Third, kBox) : desc_of(base + kThird, kBox);
 #pragma unroll
           for (int x = 0; x < kTcC / 16; ++x)
-            mma_ss(tm + kTmL + kTcN, km0 + o + x * 128, desc_of(base + kThird, kBox) + x * 128,
-                   idesc_of<IT>(128, kTcN, true, true), true);
+            mma_ss(tm + kTmL + kTcN, km0 + o + x * 128, v3 + x * 128, idesc_of<IT>(128, kTcN, true, true), true);
         }
+        tc_commit(&B.vp_empty[kVps == 2 ? i & 1 : 0]);
         tc_commit(&B.l_full);
         if (STATE_ONLY) tc_commit(&B.empty[st]), tc_commit(&B.v_empty[st]);
       }
@@ -528,7 +533,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
     while (!mbar_try_wait(&B.drain, 0) && clock64() - t0 < kWaitCycles) {
     }
     __syncwarp();
-  } else if (wg == 0) {
+  } else if (!STATE_ONLY && wg == 0) {
     // ------------------------------------------------------------ weighted scores
     if constexpr (!STATE_ONLY) {
       const int w = wid & 3;
@@ -608,8 +613,10 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
         if (++st == S::kStages) st = 0, ph ^= 1;
       }
     }
-  } else if (wg == 1) {
+  } else if (STATE_ONLY ? wg < 3 : wg == 1) {
     // ------------------------------------------------------------ weighted values
+    // a state's run shares them among the three groups that have nothing else to do, by columns
+    const int j0 = STATE_ONLY ? 3 * wg : 0, j1 = STATE_ONLY ? min(j0 + 3, 8) : 8;
     if constexpr (third && !STATE_ONLY) asm volatile("bar.sync 1, 256;" ::: "memory");  // the state has left the room
     for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
       const int m = min(kTcC, len - first_token(c));
@@ -632,16 +639,19 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
 #pragma unroll 1
         for (int j = 0; j < 8; ++j) vm = max_abs2(vm, *reinterpret_cast<const uint4*>(v + j * 16));
         float x = wv * max_of2(vm);
-        if (!group_max(1, i, &x)) break;
+        if (!group_max(STATE_ONLY ? wg : 1, i, &x)) break;
         v_exp = half_exp(x);
         wv *= pow2(v_exp);
       }
       const float2 w = f2(wv);
-      if (i > 0 && !warp_wait(&B.l_full, (i - 1) & 1)) break;  // the product over the buffer has ended
-      if (kHalf && row == 0) *reinterpret_cast<volatile int*>(&B.v_exp[i & 1]) = v_exp;
-      unsigned char* vp = smem + S::kVp;
+      // the product over the buffer has ended
+      if (i >= kVps && !warp_wait(&B.vp_empty[kVps == 2 ? i & 1 : 0], (uint32_t)(i / kVps - 1) & 1)) break;
+      if (kHalf && row == 0 && wg == 1) *reinterpret_cast<volatile int*>(&B.v_exp[i & 3]) = v_exp;
+      const bool second = kVps == 2 && (i & 1);
+      unsigned char *vp = second ? smem : smem + S::kVp, *lo = vp + (second ? kVp2Lead : kBox),
+                    *rest = third ? smem + (second ? kVp2Third : kThird) : nullptr;
 #pragma unroll 2
-      for (int j = 0; j < 8; ++j) {
+      for (int j = j0; j < j1; ++j) {
         const uint4 q = *reinterpret_cast<const uint4*>(v + ((j ^ (row & 7)) << 4));
         const uint32_t u[4] = {q.x, q.y, q.z, q.w};
         float x[8];
@@ -651,14 +661,14 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
           x[2 * r] = f.x;
           x[2 * r + 1] = f.y;
         }
-        store_split<IT>(vp, vp + kBox, third ? smem + kThird : nullptr, row, j, x);
+        store_split<IT>(vp, lo, rest, row, j, x);
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&B.vp_full);
+      if (lane == 0) mbar_arrive(&B.vp_full[kVps == 2 ? i & 1 : 0]);
       if (++st == S::kStages) st = 0, ph ^= 1;
     }
-  } else if (wg == 2) {
+  } else if (!STATE_ONLY && wg == 2) {
     // ------------------------------------------------------------ outputs
     if constexpr (!STATE_ONLY) {
       const bool o_f32 = MODE == kTcGrad && A.o_f32;
@@ -875,7 +885,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       if (lane == 0) mbar_arrive(&B.empty[st]);
       if (!warp_wait(&B.l_full, i & 1)) break;
       tc_after();
-      const float2 lw = f2(kHalf ? pow2(-*reinterpret_cast<volatile int*>(&B.v_exp[i & 1])) : 1.f);
+      const float2 lw = f2(kHalf ? pow2(-*reinterpret_cast<volatile int*>(&B.v_exp[i & 3])) : 1.f);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         float l[16], lo[16];
