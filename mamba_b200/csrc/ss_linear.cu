@@ -248,7 +248,7 @@ int check_fwd(const ss_linear_args& a) {
   if (!sizes_ok(a)) return SS_ERR_INVALID;
   if (!dtypes_ok(a.io_dtype, a.decay_dtype)) return SS_ERR_UNSUPPORTED;
   if (a.key_dim > SS_MAX_LINEAR_DIM || a.value_dim > SS_MAX_LINEAR_DIM) return SS_ERR_UNSUPPORTED;
-  if ((int64_t)a.batch * a.heads > (1 << 24)) return SS_ERR_UNSUPPORTED;
+  if ((int64_t)a.batch * a.heads > (1 << 24) || a.seqlen > (1 << 30)) return SS_ERR_UNSUPPORTED;  // 32-bit token indexes
   if (!std::isfinite(a.scale) || a.scale == 0.f) return SS_ERR_INVALID;
   const bool empty = a.batch == 0 || a.seqlen == 0;
   if (!empty && (!a.q || !a.k || !a.v || !a.log_decay)) return SS_ERR_INVALID;

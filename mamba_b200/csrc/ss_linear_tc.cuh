@@ -264,7 +264,6 @@ __device__ __forceinline__ float max_of2(uint32_t m) {
 }
 
 // What a run writes: the segments' own states; outputs; outputs in parts or with their dot products (gradients
-// of q and k)
 // of q and k); outputs and a final state that is returned
 enum { kTcState = 0, kTcOut = 1, kTcGrad = 2, kTcOutState = 3 };
 
@@ -281,6 +280,9 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
   // one after the other with wide keys, a stage apart with narrow ones)
   constexpr int kVps = STATE_ONLY ? 2 : 1;
   constexpr uint32_t kVp2Lead = DK == 128 ? kBox : S::kStageBytes, kVp2Third = DK == 128 ? S::kStageBytes : 2 * S::kStageBytes;
+  // and its three groups with nothing else to do build V' together, by columns (74 -> 70 us over 16384 tokens of
+  // 16 heads of 128 x 128; fp16, with a maximum over all columns to find first: 27 us by one group, 34 by three)
+  constexpr bool kShare = STATE_ONLY && std::is_same<IT, __nv_bfloat16>::value;
   TcBars& B = *reinterpret_cast<TcBars*>(smem + S::kBars);
   const LinK& K = P.k;
   const LinPass& A = K.pass[pass];
@@ -312,7 +314,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       mbar_init(&B.v_empty[i], STATE_ONLY ? 1 : 1 + 4);    // the products, the output tile that takes V's room
     }
     for (int i = 0; i < 2; ++i) mbar_init(&B.s_full[i], 1), mbar_init(&B.p_full[i], 4);
-    for (int i = 0; i < 2; ++i) mbar_init(&B.vp_full[i], STATE_ONLY ? 12 : 4), mbar_init(&B.vp_empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&B.vp_full[i], kShare ? 12 : 4), mbar_init(&B.vp_empty[i], 1);
     mbar_init(&B.l_full, 1), mbar_init(&B.l_empty, 4);
     mbar_init(&B.h_full, 4), mbar_init(&B.h_empty, 1);
     mbar_init(&B.o_full[0], 1), mbar_init(&B.o_full[1], 1), mbar_init(&B.o_empty[0], 4), mbar_init(&B.o_empty[1], 4);
@@ -613,10 +615,9 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
         if (++st == S::kStages) st = 0, ph ^= 1;
       }
     }
-  } else if (STATE_ONLY ? wg < 3 : wg == 1) {
+  } else if (kShare ? wg < 3 : wg == 1) {
     // ------------------------------------------------------------ weighted values
-    // a state's run shares them among the three groups that have nothing else to do, by columns
-    const int j0 = STATE_ONLY ? 3 * wg : 0, j1 = STATE_ONLY ? min(j0 + 3, 8) : 8;
+    const int j0 = kShare ? 3 * wg : 0, j1 = kShare ? min(j0 + 3, 8) : 8;
     if constexpr (third && !STATE_ONLY) asm volatile("bar.sync 1, 256;" ::: "memory");  // the state has left the room
     for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
       const int m = min(kTcC, len - first_token(c));
@@ -639,14 +640,14 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
 #pragma unroll 1
         for (int j = 0; j < 8; ++j) vm = max_abs2(vm, *reinterpret_cast<const uint4*>(v + j * 16));
         float x = wv * max_of2(vm);
-        if (!group_max(STATE_ONLY ? wg : 1, i, &x)) break;
+        if (!group_max(1, i, &x)) break;
         v_exp = half_exp(x);
         wv *= pow2(v_exp);
       }
       const float2 w = f2(wv);
       // the product over the buffer has ended
       if (i >= kVps && !warp_wait(&B.vp_empty[kVps == 2 ? i & 1 : 0], (uint32_t)(i / kVps - 1) & 1)) break;
-      if (kHalf && row == 0 && wg == 1) *reinterpret_cast<volatile int*>(&B.v_exp[i & 3]) = v_exp;
+      if (kHalf && row == 0) *reinterpret_cast<volatile int*>(&B.v_exp[i & 3]) = v_exp;
       const bool second = kVps == 2 && (i & 1);
       unsigned char *vp = second ? smem : smem + S::kVp, *lo = vp + (second ? kVp2Lead : kBox),
                     *rest = third ? smem + (second ? kVp2Third : kThird) : nullptr;
@@ -795,7 +796,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       for (int c = max(cn, c0); c < c1; ++c)  // chunks behind the row's end
         if (c * kTcC + row < K.seqlen) zero_row(c * kTcC + row);
     }
-  } else {
+  } else if (wg == 3) {
     // ------------------------------------------------------------ state: row `row` of H
     // Rows enter and leave the registers through the room of the 16-bit halves (256 bytes a row), each
     // warp its own: short loops, and a warp's lanes side by side along a row in memory
@@ -951,6 +952,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_c
   griddep_launch_dependents();
   if (P.k.pass[pass].dk > 64) linear_tc_run<IT, 128, MODE>(P, pass, tile, where, smem);
   else linear_tc_run<IT, 64, MODE>(P, pass, tile, where, smem);
+  griddep_wait();  // blocks that had nothing to wait for do not end before the launches ahead of theirs
 }
 
 }  // namespace ssb

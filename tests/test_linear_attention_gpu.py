@@ -207,6 +207,45 @@ def test_long_sequence_is_its_halves(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,l,h,hk,dk,dv,lens", [(1, 4100, 1, 1, 128, 128, None), (1, 3333, 2, 1, 64, 128, None),
+                                                 (2, 2600, 2, 2, 128, 64, [2600, 1301]), (3, 2050, 1, 1, 48, 40, [0, 2050, 300])])
+def test_many_chunks_in_segments(dtype, b, l, h, hk, dk, dv, lens):
+    """Few heads and many chunks a segment, decays that reach across segments, against the recurrence."""
+    check(make(b, l, h, hk, dk, dv, dtype, state=True, bias=5.0, lens=lens, seed=l))
+
+
+@pytest.mark.parametrize("sizes", [(1.0, 1.0, 1.0), (100.0, 60.0, 1e-3), (1e-3, 1e-4, 100.0), (1e-2, 100.0, 1e-3),
+                                   (200.0, 1e-2, 1e-2)])
+def test_range_of_fp16(sizes):
+    """Scores far above and below what fp16 holds (6.1e-5 is its smallest normal number, 65504 its largest),
+    of inputs that it holds; the outputs' scale is chosen so that they are normal numbers again.  The tolerance
+    has fp16's smallest step (2^-24, half of it a rounding) beside the relative one: inputs of 1e-4 already
+    carry that step, results below 2^-14 are rounded by it, and gradients reach down there."""
+    from mamba_b200 import linear_attention_fn
+
+    t = make(2, 300, 2, 1, 64, 64, torch.float16, seed=31)
+    for n, x in zip(("q", "k", "v"), sizes):
+        t[n] = (t[n].float() * x).half()
+    scale = 0.1 / (sizes[0] * sizes[1] * sizes[2])
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g")]
+    o, f = linear_attention_fn(*leaves, scale=scale, return_final_state=True)
+    want_o, want_f, _ = reference(t, scale, False)
+    mag_o, mag_f, _ = reference(t, scale, False, absolute=True)
+    soft = 2 * HALF[torch.float16] + 2.0 ** -17
+    close("o", o, want_o, mag_o + 2.0 ** -15, torch.float16, soft)
+    close("final", f, want_f, mag_f, torch.float16, 2.0 ** -14)
+    # seeds that keep the gradients in range: dq is about 1 / q of o.do, and so on
+    do = (t["do"].float() * min(1.0, *sizes)).half()
+    grads = torch.autograd.grad(o, leaves, do)
+    ref = [x.detach().double().requires_grad_() for x in leaves]
+    want = torch.autograd.grad(linear_ref(*ref, scale)[0], ref, do.double())
+    pos = [x.detach().double().abs().requires_grad_() for x in leaves[:3]]
+    mags = torch.autograd.grad(linear_ref(*pos, leaves[3].detach().double(), scale)[0], pos, do.double().abs())
+    for name, got, w, m in zip(("dq", "dk", "dv"), grads, want, mags):
+        close(name, got, w, m + 2.0 ** -15, torch.float16, soft)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_results_do_not_vary(dtype):
     from mamba_b200 import linear_attention_fn
 
