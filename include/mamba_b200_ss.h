@@ -266,7 +266,8 @@ typedef struct ss_mamba_step_args {
  * heads is a multiple of key_heads; head j uses q and k of key head j / (heads / key_heads).
  * key_dim and value_dim are at most SS_MAX_LINEAR_DIM.  The innermost axis of q, k, v, o has stride 1.
  * A log decay of -infinity resets the state.  With seq_lens, tokens t >= seq_lens[b] (clamped to
- * [0, seqlen]) are not read into anything and their o is zero. */
+ * [0, seqlen]) are not read into anything and their o is zero.  seqlen is at most 2^30, scale a normal
+ * number. */
 typedef struct ss_linear_args {
   int batch, seqlen, heads, key_heads, key_dim, value_dim;
   int io_dtype;             /* dtype of q, k, v, o                                        */
@@ -297,7 +298,7 @@ typedef struct ss_linear_bwd_args {
   void* dlog_decay;         /* nullable; decay_dtype, packed: (batch, seqlen, heads), or (heads) when
                                f's batch and seq decay strides are 0                       */
   float* dstate_in;         /* nullable; packed                                            */
-  void* work;               /* ss_linear_work_bytes(&f, 1) bytes                           */
+  void* work;               /* 16-byte aligned, ss_linear_work_bytes(&f, 1) bytes           */
 } ss_linear_bwd_args;
 
 /* One token: state <- exp(log_decay) state + k v^T; o = scale * q state. */
@@ -354,7 +355,8 @@ typedef struct ss_block_norm_bwd_args {
  *   finished beam: its score at eos_token, -infinity elsewhere
  * and the num_select largest of (beams x vocab), the lowest index first among equals.  A candidate
  * that is not a number, and every candidate of a beam whose score is NaN or +infinity, counts as
- * -infinity.  Candidates are compared in fp64. */
+ * -infinity.  Candidates are compared in fp64.  beams and num_select are at most SS_MAX_BEAMS, beams * vocab
+ * at most 2^30. */
 typedef struct ss_beam_args {
   int batch, beams, vocab, num_select, io_dtype;
   int eos_token;                                             /* used with finished            */

@@ -375,6 +375,14 @@ def launch(name: str, packed: bytes, device: torch.device) -> None:
         check(rc, name)
 
 
+def written(tensors) -> None:
+    """Mark tensors that a kernel updates in place, so that a backward which has saved one of them raises."""
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:  # inference tensors among them: they have no version, and no backward saves them
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
 def device_status(device, reset: bool = True) -> int:
     """Error bits raised by kernels on `device` (STATUS_BITS)."""
     import torch

@@ -75,6 +75,8 @@ def reorder_states(states, parents):
     if w > L.MAX_BEAMS:
         raise NotImplementedError(f"{w} beams are more than {L.MAX_BEAMS}")
     total = b * w
+    if not isinstance(states, (list, tuple)):
+        states = list(states)
     # whole columns of checks at a time: a model's dozens of states pass in a few microseconds
     if min(map(torch.Tensor.dim, states), default=1) < 1 or not set(map(_rows_of, states)) <= {total} or not all(
             map(torch.Tensor.is_contiguous, states)):
@@ -84,12 +86,13 @@ def reorder_states(states, parents):
     rows = sorted(r for r in zip(map(torch.Tensor.data_ptr, states), map(_nbytes, states)) if r[1])
     end = 0
     for at, n in rows:
-        if n % (4 * total):
-            raise NotImplementedError(f"rows of {n / total} bytes (a multiple of 4 is supported)")
+        if n % (4 * total) or at % 4:
+            raise NotImplementedError(f"rows of {n / total} bytes at address {at} (multiples of 4 are supported)")
         if at < end:
             raise ValueError("states must not share memory")
         end = at + n
     p = parents if parents.stride(1) == 1 or w == 1 else parents.contiguous()
+    L.written(states)
     for i in range(0, len(rows), L.MAX_REORDER):
         part = rows[i:i + L.MAX_REORDER]
         none = (0,) * (L.MAX_REORDER - len(part))

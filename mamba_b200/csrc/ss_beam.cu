@@ -50,11 +50,13 @@ int ss_beam_select(const ss_beam_args* a, void* stream) {
   if (a == nullptr) return SS_ERR_INVALID;
   if (!sizes_ok(a->batch, a->beams, a->vocab, a->num_select)) return SS_ERR_INVALID;
   if (a->io_dtype != SS_F32 && a->io_dtype != SS_BF16 && a->io_dtype != SS_F16) return SS_ERR_UNSUPPORTED;
-  if (a->beams > SS_MAX_BEAMS || a->num_select > 32 || (int64_t)a->beams * a->vocab >= 2147483647LL)
+  if (a->beams > SS_MAX_BEAMS || a->num_select > 32 || (int64_t)a->beams * a->vocab > (1 << 30))
     return SS_ERR_UNSUPPORTED;
   if (a->finished && (a->eos_token < 0 || a->eos_token >= a->vocab)) return SS_ERR_INVALID;
   if (a->batch == 0) return SS_OK;
-  if (!a->logits || !a->scores || !a->out_scores || !a->parents || !a->tokens || !a->work) return SS_ERR_INVALID;
+  if (!a->logits || !a->scores || !a->out_scores || !a->parents || !a->tokens || !a->work ||
+      (reinterpret_cast<uintptr_t>(a->work) & 15))
+    return SS_ERR_INVALID;
   if (a->logits_batch_stride < 0 || a->logits_beam_stride < 0) return SS_ERR_INVALID;
   const int64_t rows = (int64_t)a->batch * a->beams;
   const size_t es = a->io_dtype == SS_F32 ? 4 : 2;

@@ -25,6 +25,9 @@ bool weights16(const ss_block_norm_args& a) {
                              reinterpret_cast<uintptr_t>(a.scale)) & 15) == 0;
 }
 
+// the two roots of a row move as one 8-byte word
+bool pairs(const float* rstd) { return (reinterpret_cast<uintptr_t>(rstd) & 7) == 0; }
+
 struct Shape {
   int nv, wpr;  // vectors a lane, warps a row
 };
@@ -142,7 +145,7 @@ int ss_block_norm_fwd(const ss_block_norm_args* a, void* stream) {
   const int rc = check(*a);
   if (rc != SS_OK) return rc;
   if (a->rows == 0) return SS_OK;
-  if (!a->h || a->h_row_stride < a->dim) return SS_ERR_INVALID;
+  if (!a->h || a->h_row_stride < a->dim || !pairs(a->rstd)) return SS_ERR_INVALID;
   if (a->pre_weight && (!a->x || a->x_row_stride < a->dim)) return SS_ERR_INVALID;
   const size_t es = a->io_dtype == SS_F32 ? 4 : 2;
   BlockNormK P;
@@ -169,7 +172,7 @@ int ss_block_norm_bwd(const ss_block_norm_bwd_args* g, void* stream) {
   const size_t es = a.io_dtype == SS_F32 ? 4 : 2;
   const Shape s = shape_of(a.dim);
   if (a.rows > 0) {
-    if (!a.rstd || !g->dresidual || !g->dy || !g->work || (a.gate && !g->dgate) || (a.pre_weight && !g->dx))
+    if (!a.rstd || !pairs(a.rstd) || !g->dresidual || !g->dy || !g->work || (a.gate && !g->dgate) || (a.pre_weight && !g->dx))
       return SS_ERR_INVALID;
     if (g->dy_row_stride < a.dim || g->dresidual_row_stride < a.dim || (a.gate && g->dgate_row_stride < a.dim) ||
         (a.pre_weight && g->dx_row_stride < a.dim) || (g->dh && g->dh_row_stride < a.dim))

@@ -243,13 +243,15 @@ LinK problem(const ss_linear_args& a, const Work& w, void* work) {
   return P;
 }
 
+bool work_ok(const Work& w, const void* p) { return !w.bytes || (p && (reinterpret_cast<uintptr_t>(p) & 15) == 0); }
+
 // status of the arguments that both directions share (a zero batch may carry null pointers)
 int check_fwd(const ss_linear_args& a) {
   if (!sizes_ok(a)) return SS_ERR_INVALID;
   if (!dtypes_ok(a.io_dtype, a.decay_dtype)) return SS_ERR_UNSUPPORTED;
   if (a.key_dim > SS_MAX_LINEAR_DIM || a.value_dim > SS_MAX_LINEAR_DIM) return SS_ERR_UNSUPPORTED;
   if ((int64_t)a.batch * a.heads > (1 << 24) || a.seqlen > (1 << 30)) return SS_ERR_UNSUPPORTED;  // 32-bit token indexes
-  if (!std::isfinite(a.scale) || a.scale == 0.f) return SS_ERR_INVALID;
+  if (!std::isnormal(a.scale)) return SS_ERR_INVALID;  // its reciprocal is needed too
   const bool empty = a.batch == 0 || a.seqlen == 0;
   if (!empty && (!a.q || !a.k || !a.v || !a.log_decay)) return SS_ERR_INVALID;
   return SS_OK;
@@ -272,7 +274,7 @@ int ss_linear_fwd(const ss_linear_args* a, void* stream) {
   if (a->seqlen > 0 && !a->o) return SS_ERR_INVALID;
   if (a->seqlen == 0 && !a->state_out) return SS_OK;
   const Work w = work_of(*a, 0);
-  if (w.bytes && !a->work) return SS_ERR_INVALID;
+  if (!work_ok(w, a->work)) return SS_ERR_INVALID;
   LinK P = problem(*a, w, a->work);
   LinPass& A = P.pass[0];
   const int rep = a->heads / a->key_heads;
@@ -298,7 +300,7 @@ int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
   if (a.seqlen > 0 && (!g->dout || !g->dq || !g->dk || !g->dv)) return SS_ERR_INVALID;
   if (g->dstate_out && g->dlog_decay && !a.state_out) return SS_ERR_INVALID;
   const Work w = work_of(a, 1);
-  if (w.bytes && !g->work) return SS_ERR_INVALID;
+  if (!work_ok(w, g->work)) return SS_ERR_INVALID;
   char* base = static_cast<char*>(g->work);
   LinK P = problem(a, w, base);
   const int rep = a.heads / a.key_heads;

@@ -154,11 +154,15 @@ class Decoder:
         # fp32 norm weights, cast once (a per-call cast would be one more kernel per layer and step)
         norms = [layer.norm for layer in model.layers] + [model.norm]
         self.norms = [(n.weight.detach().float().contiguous(), n.eps) for n in norms]
-        self.parts = [branch_parts(layer, n) for layer, n in zip(model.layers, norms[1:])]
+        self.parts = [self._cast(branch_parts(layer, n)) for layer, n in zip(model.layers, norms[1:])]
         self.cuda_graph = cuda_graph
         self.graph = None
         self.tok = torch.zeros(batch, dtype=torch.long, device=dev)
         self.logits = None
+
+    @staticmethod
+    def _cast(parts):
+        return parts and tuple(t.detach().float().contiguous() if isinstance(t, torch.Tensor) else t for t in parts)
 
     # the per-layer states of MambaSimple layers, as lists over the layers
     @property

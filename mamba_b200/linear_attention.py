@@ -141,7 +141,7 @@ def _forward(t, c, want_final):
     b, l, h, _, dk, dv = c[:6]
     v = t[2]
     dev = v.device
-    o = torch.empty((b, l, h, dv), dtype=v.dtype, device=dev)
+    o = torch.empty_like(v, memory_format=torch.contiguous_format)
     final = torch.empty((b, h, dk, dv), dtype=torch.float32, device=dev) if want_final else None
     work = _work(c, 0, dev)
     L.launch("ss_linear_fwd", _pack_fwd(*_inputs(t, c, final), *_at(o), _p(work)), dev)
@@ -151,7 +151,8 @@ def _forward(t, c, want_final):
 
 def _backward(t, c, dout, dfinal, final, want_decay, want_state):
     q, k, v, g = t[:4]
-    dev, new = v.device, torch.empty
+    dev = v.device
+    new = functools.partial(torch.empty_like, memory_format=torch.contiguous_format)
     dout = _as(dout, v.dtype)
     if v.dtype != torch.float32:
         dout = _whole(dout)
@@ -159,9 +160,9 @@ def _backward(t, c, dout, dfinal, final, want_decay, want_state):
         dout = dout.contiguous()
     if dfinal is not None:
         dfinal = _as(dfinal, torch.float32).contiguous()
-    dq, dk, dv = (new(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
-    dg = new(g.shape, dtype=g.dtype, device=dev) if want_decay else None
-    ds = new((c[0], c[2], c[4], c[5]), dtype=torch.float32, device=dev) if want_state else None
+    dq, dk, dv = new(q), new(k), new(v)
+    dg = new(g) if want_decay else None
+    ds = new(t[4]) if want_state else None
     work = _work(c, 1, dev)
     L.launch("ss_linear_bwd", _pack_bwd(*_inputs(t, c, final), *_NONE4, 0, *_at(dout), _p(dfinal), *_at(dq), *_at(dk),
                                         *_at(dv), _p(dg), _p(ds), _p(work)), dev)
@@ -252,10 +253,11 @@ def linear_attention_step(state, q, k, v, log_decay, scale=None):
         q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
     g = _decay(log_decay, io)
     gs = (0, g.stride(0)) if g.dim() == 1 else g.stride()
-    o = torch.empty((b, h, dv), dtype=io, device=dev)
+    o = torch.empty_like(v, memory_format=torch.contiguous_format)
     L.launch("ss_linear_step", _pack_step(b, h, hk, dk, dv, io_code, L.dtype_code(g.dtype), _scale(scale, dk),
                                           state.data_ptr(), ss[0] if b > 1 else n, *_at(q), *_at(k), *_at(v),
                                           g.data_ptr(), *gs, o.data_ptr(), h * dv, dv), dev)
+    L.written((state,))
     return o
 
 

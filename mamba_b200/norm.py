@@ -15,6 +15,8 @@ pass each way.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -101,14 +103,24 @@ _pack_block_fwd, _pack_block_bwd = (L.packer(st) for st in (L.BlockNormArgs, L.B
 
 
 def _row_at(t):
-    """Address and row stride of a (rows, dim) tensor."""
-    return (0, 0) if t is None else (t.data_ptr(), t.stride(0))
+    """Address and row stride of a (rows, dim) tensor, or of a packed (..., dim) one."""
+    return (0, 0) if t is None else (t.data_ptr(), t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else t.shape[-1])
+
+
+def _like(t):
+    return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=1024)
+def _block_work(n, dim, io):
+    return int(L.lib().ss_block_norm_work_elems(n, dim, io))
 
 
 def _block_rows(t, dtype, dim):
-    if t is None or (t.dtype == dtype and t.dim() == 2 and t.stride(1) == 1):
+    if t is None or (t.dtype == dtype and t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= dim):
         return t
-    return _rows(t if t.dtype == dtype else t.to(dtype), dim)
+    t = _rows(t if t.dtype == dtype else t.to(dtype), dim)
+    return t if t.stride(0) >= dim else t.contiguous()  # rows that share memory
 
 
 def _f32(t):
@@ -128,14 +140,10 @@ def _block_forward(y, residual, post, pre, gate, scale, call, train):
     dim, io = y.shape[-1], y.dtype
     rows = [_block_rows(t, io, dim) for t in (y, residual, gate)]
     cols = [_f32(t) for t in (post, pre, scale)]
-    n = rows[0].shape[0]
-    h = torch.empty((n, dim), dtype=io, device=dev)
-    x = torch.empty((n, dim), dtype=io, device=dev) if pre is not None else None
-    rstd = torch.empty((n, 2), dtype=torch.float32, device=dev) if train else None
+    h = _like(y)
+    x = None if pre is None else _like(y)
+    rstd = torch.empty((rows[0].shape[0], 2), dtype=torch.float32, device=dev) if train else None
     L.launch("ss_block_norm_fwd", _pack_block_fwd(*_block_args(rows, cols, call, h, x, rstd)), dev)
-    if y.dim() != 2:
-        h = h.reshape(y.shape)
-        x = x if x is None else x.reshape(y.shape)
     return x, h, rows, cols, rstd
 
 
@@ -162,20 +170,12 @@ class BlockNormFn(torch.autograd.Function):
         if pre is not None and dx is None:
             dx = torch.zeros_like(y)
         dx, dh = _block_rows(dx, io, dim), _block_rows(dh, io, dim)
-        new = lambda t: None if t is None else torch.empty((n, dim), dtype=io, device=dev)  # noqa: E731
-        dy, dres, dgate = new(y), new(residual), new(gate)
-        # the columns' gradients and the scratch of their sums in one buffer
-        m = int(L.lib().ss_block_norm_work_elems(n, dim, ctx.call[0]))
-        k = sum(t is not None for t in (post, pre, scale))
-        buf = torch.empty(m + k * dim, dtype=torch.float32, device=dev)
-        at, cols = m, []
-        for t in (post, pre, scale):
-            cols.append(None if t is None else buf[at:at + dim])
-            at += 0 if t is None else dim
-        dpost, dpre, dscale = cols
+        dy, dres, dgate = _like(y), _like(residual), _like(gate)
+        work = torch.empty(_block_work(n, dim, ctx.call[0]), dtype=torch.float32, device=dev)
+        dpost, dpre, dscale = _like(post), _like(pre), _like(scale)
         L.launch("ss_block_norm_bwd", _pack_block_bwd(
             *_block_args(rows, (post, pre, scale), ctx.call, rstd=rstd), *_row_at(dx), *_row_at(dh), *_row_at(dy),
-            *_row_at(dres), *_row_at(dgate), L.ptr(dpost) or 0, L.ptr(dpre) or 0, L.ptr(dscale) or 0, buf.data_ptr()), dev)
+            *_row_at(dres), *_row_at(dgate), L.ptr(dpost) or 0, L.ptr(dpre) or 0, L.ptr(dscale) or 0, work.data_ptr()), dev)
         if len(ctx.shape) != 2:
             dy, dres, dgate = (t if t is None else t.reshape(ctx.shape) for t in (dy, dres, dgate))
         return (*(t if t is None or t.dtype == d else t.to(d)

@@ -91,6 +91,25 @@ def test_strided_and_misaligned_rows(dtype):
     run((6, 96), dtype, seed=6, view=lambda v: torch.cat([v[:, :1], v], -1)[:, 1:])
 
 
+def test_a_row_of_any_stride_and_rows_that_share_memory():
+    from mamba_b200 import block_norm_fn
+
+    g = torch.Generator().manual_seed(6)
+    y, res, w = (torch.randn(*s, generator=g).cuda() for s in ((40, 1), (40,), (40,)))
+    a = block_norm_fn(y.t(), res[None], w, w)              # one row, strides (1, 1)
+    b = block_norm_fn(y.t().contiguous(), res[None], w, w)
+    c = block_norm_fn(y.flatten(), res, w, w)              # no row axis at all
+    for i in range(2):
+        assert torch.equal(a[i], b[i]) and torch.equal(c[i], b[i][0])
+    leaf = res.clone().requires_grad_()
+    rows = torch.randn(5, 40, generator=g).cuda()
+    h = block_norm_fn(rows, leaf.expand(5, 40), w)         # one residual row for all
+    assert torch.equal(h, block_norm_fn(rows, res.repeat(5, 1), w))
+    dh = torch.randn(5, 40, generator=g).cuda()
+    (d,) = torch.autograd.grad(h, [leaf], dh)
+    assert torch.allclose(d, dh.sum(0), rtol=0, atol=1e-5)  # five fp32 terms of about 1
+
+
 def test_expanded_gate_and_its_gradient():
     from mamba_b200 import block_norm_fn
 

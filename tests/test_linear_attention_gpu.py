@@ -354,6 +354,59 @@ def test_step_on_strided_state_rows():
     assert torch.equal(cache[:, 1:3], packed) and bool((cache[:, [0, 3, 4]] == 7).all())
 
 
+def test_gradients_of_an_empty_sequence():
+    from mamba_b200 import linear_attention_fn
+
+    for dtype in DTYPES:
+        t = make(2, 0, 2, 1, 16, 16, dtype, state=True)
+        leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g", "s0")]
+        o, f = linear_attention_fn(*leaves[:4], 0.5, leaves[4], None, True)
+        grads = torch.autograd.grad([o, f], leaves, [t["do"], t["dF"]])
+        assert all(g.shape == x.shape for g, x in zip(grads, leaves))
+        # the state passes through; its gradient carries the scale and its reciprocal, exact at a power of two
+        assert torch.equal(grads[4], t["dF"])
+
+
+def test_a_state_that_a_backward_needs_cannot_be_stepped():
+    from mamba_b200 import linear_attention_fn, linear_attention_step
+
+    t = make(1, 20, 2, 2, 16, 16, torch.float32, seed=25)
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g")]
+    o, f = linear_attention_fn(*leaves, return_final_state=True)
+    with torch.no_grad():
+        linear_attention_step(f, t["q"][:, 0], t["k"][:, 0], t["v"][:, 0], t["g"][:, 0])
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(o.sum() + f.sum(), leaves)
+    with torch.inference_mode():
+        s = torch.zeros(1, 2, 16, 16, device="cuda")
+        linear_attention_step(s, t["q"][:, 0], t["k"][:, 0], t["v"][:, 0], t["g"][:, 0])
+        assert float(s.abs().max()) > 0
+
+
+def test_two_streams_at_once():
+    from mamba_b200 import linear_attention_fn
+
+    ts = [make(1, 2000, 2, 1, 64, 64, torch.bfloat16, state=True, seed=26 + i) for i in range(2)]
+
+    def once(t):
+        leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g", "s0")]
+        o, f = linear_attention_fn(*leaves[:4], None, leaves[4], None, True)
+        return [o, f, *torch.autograd.grad([o, f], leaves, [t["do"], t["dF"]])]
+
+    want = [once(t) for t in ts]
+    streams = [torch.cuda.Stream() for _ in ts]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for t, s in zip(ts, streams):
+            with torch.cuda.stream(s):
+                got.append(once(t))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        for a, b in zip(g, want[i % 2]):
+            assert torch.equal(a, b)
+
+
 def test_runs_on_another_stream_and_in_a_graph():
     from mamba_b200 import linear_attention_fn
 

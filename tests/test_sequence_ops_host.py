@@ -112,7 +112,8 @@ _S = torch.zeros(6, 4)
     ([torch.zeros(6, 3, dtype=torch.float16)], torch.zeros(2, 3, dtype=torch.int64), NotImplementedError),
     ([_S], torch.zeros(2, 3, dtype=torch.int32), ValueError), ([_S], torch.zeros(6, dtype=torch.int64), ValueError),
     ([_S], torch.zeros(2, 0, dtype=torch.int64), ValueError), ([_S, _S], torch.zeros(2, 3, dtype=torch.int64), ValueError),
-    ([torch.zeros(33, 4)], torch.zeros(1, 33, dtype=torch.int64), NotImplementedError)])
+    ([torch.zeros(33, 4)], torch.zeros(1, 33, dtype=torch.int64), NotImplementedError),
+    ([torch.zeros(13, dtype=torch.float16)[1:].view(6, 2)], torch.zeros(2, 3, dtype=torch.int64), NotImplementedError)])
 def test_reorder_refuses(on_cpu, states, parents, error):
     with pytest.raises(error):
         mamba_b200.reorder_states(states, parents)
@@ -132,7 +133,8 @@ def _linear_args(**kw):
 @pytest.mark.parametrize("kw,status", [
     (dict(batch=-1), 1), (dict(heads=3), 1), (dict(key_heads=0), 1), (dict(key_dim=0), 1), (dict(scale=0.0), 1),
     (dict(scale=float("inf")), 1), (dict(q=None), 1), (dict(log_decay=None), 1), (dict(o=None), 1), (dict(key_dim=129), 2),
-    (dict(value_dim=129), 2), (dict(io_dtype=7), 2), (dict(decay_dtype=L.SS_F16), 2), (dict(batch=0), 0)])
+    (dict(value_dim=129), 2), (dict(io_dtype=7), 2), (dict(decay_dtype=L.SS_F16), 2), (dict(batch=0), 0),
+    (dict(scale=1e-40), 1), (dict(seqlen=2 ** 30 + 1), 2), (dict(work=0x1008), 1), (dict(work=None), 1)])
 def test_c_boundary_of_linear_attention(kw, status):
     assert L.lib().ss_linear_fwd(ctypes.byref(_linear_args(**kw)), None) == status
 
@@ -150,6 +152,19 @@ def test_c_boundary_missing_gradients():
     b = L.BlockNormBwdArgs()
     b.f.rows, b.f.dim, b.f.y, b.f.residual, b.f.y_row_stride, b.f.residual_row_stride = 2, 8, 0x1000, 0x1000, 8, 8
     assert L.lib().ss_block_norm_bwd(ctypes.byref(b), None) == L.SS_ERR_INVALID
+
+
+def test_c_boundary_alignment_and_limits():
+    b = L.BlockNormArgs()
+    b.rows, b.dim, b.y_row_stride, b.residual_row_stride, b.h_row_stride = 2, 8, 8, 8, 8
+    b.y = b.residual = b.h = 0x1000
+    b.rstd = 0x1004
+    assert L.lib().ss_block_norm_fwd(ctypes.byref(b), None) == L.SS_ERR_INVALID
+    s = L.BeamArgs(1, 1, 2 ** 30 + 1, 1, L.SS_F16, 0, 0x1000, 2 ** 30 + 1, 2 ** 30 + 1, 0x1000, None, 0x1000, 0x1000, 0x1000,
+                   0x1000)
+    assert L.lib().ss_beam_select(ctypes.byref(s), None) == L.SS_ERR_UNSUPPORTED
+    s.vocab, s.work = 100, 0x1008
+    assert L.lib().ss_beam_select(ctypes.byref(s), None) == L.SS_ERR_INVALID
 
 
 def test_workspace_sizes():
