@@ -43,11 +43,11 @@ struct Split {
   int segs, first, chunks;
 };
 
-Split split_of(const ss_linear_args& a, int chunk, int passes, int tiles) {
+Split split_of(const ss_linear_args& a, int chunk, int passes, int tiles, int slots) {
   const int n = (a.seqlen + chunk - 1) / chunk;
   const int64_t ctas = (int64_t)a.batch * a.heads * passes * tiles;
   int segs = 1;
-  if (ctas > 0 && ctas < 148) segs = (int)std::max<int64_t>(1, std::min<int64_t>({148 / ctas, n / 2, 32}));
+  if (ctas > 0 && ctas < slots) segs = (int)std::max<int64_t>(1, std::min<int64_t>({slots / ctas, n / 2, 32}));
   Split s{1, std::max(n, 1), std::max(n, 1)};
   if (segs > 1) {
     s.chunks = std::max(1, (2 * n + 2 * segs) / (2 * segs + 1));  // n / (segs + 1/2)
@@ -69,8 +69,8 @@ Work work_of(const ss_linear_args& a, int backward) {
   Work w;
   const int passes = backward ? 3 : 1;
   const int tiles = backward ? std::max(tiles_of(a.key_dim), tiles_of(a.value_dim)) : tiles_of(a.value_dim);
-  w.simt = split_of(a, kLsC, passes, tiles);
-  w.tc = a.io_dtype == SS_F32 ? Split{1, 1, 1} : split_of(a, kTcC, passes, tiles);
+  w.simt = split_of(a, kLsC, passes, tiles, std::max(a.key_dim, a.value_dim) > kLsN ? 148 : 2 * 148);
+  w.tc = a.io_dtype == SS_F32 ? Split{1, 1, 1} : split_of(a, kTcC, passes, tiles, 148);
   const int segs = a.io_dtype == SS_F32 ? w.simt.segs : std::max(w.simt.segs, w.tc.segs);
   const size_t bh = (size_t)a.batch * a.heads;
   auto take = [&](size_t n) {
@@ -112,16 +112,15 @@ cudaError_t launch_fold(const LinK& P, int passes, cudaStream_t st) {
   return launch_early(linear_fold_kernel, grid, 256, 0, P, st);
 }
 
-template <typename IT>
+template <typename IT, int DMAX>
 cudaError_t run_simt(const LinK& P, int passes, cudaStream_t st) {
-  constexpr size_t smem = sizeof(LsSmem);
-  auto main_k = linear_simt_kernel<IT, false>;
-  auto sum_k = linear_simt_kernel<IT, true>;
+  constexpr size_t smem = sizeof(LsSmem<DMAX>);
+  auto main_k = linear_simt_kernel<IT, DMAX, false>;
+  auto sum_k = linear_simt_kernel<IT, DMAX, true>;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(main_k), smem);
   if (e == cudaSuccess) e = ensure_smem_limit(reinterpret_cast<const void*>(sum_k), smem);
   if (e != cudaSuccess) return e;
-  const int kt = (kLinMaxDim + kLsN - 1) / kLsN;
-  const dim3 grid((unsigned)((int64_t)P.batch * P.heads * P.segs), (unsigned)(passes * kt));
+  const dim3 grid((unsigned)((int64_t)P.batch * P.heads * P.segs), (unsigned)(passes * (DMAX / kLsN)));
   if (P.segs > 1) {
     sum_k<<<grid, kLsThreads, smem, st>>>(P);
     e = cudaGetLastError();
@@ -225,10 +224,12 @@ cudaError_t run_passes(int io, LinK& P, const Work& w, int passes, cudaStream_t 
     if (run_tc(io, P, passes, st, &e)) return e;
   }
   P.segs = w.simt.segs, P.seg_first = w.simt.first, P.seg_chunks = w.simt.chunks;
+  bool wide = false;
+  for (int i = 0; i < passes; ++i) wide |= P.pass[i].dk > 64 || P.pass[i].dv > 64;
   switch (io) {
-    case SS_F32: return run_simt<float>(P, passes, st);
-    case SS_BF16: return run_simt<__nv_bfloat16>(P, passes, st);
-    default: return run_simt<__half>(P, passes, st);
+    case SS_F32: return wide ? run_simt<float, 128>(P, passes, st) : run_simt<float, 64>(P, passes, st);
+    case SS_BF16: return run_simt<__nv_bfloat16, 128>(P, passes, st);
+    default: return run_simt<__half, 128>(P, passes, st);
   }
 }
 

@@ -76,30 +76,35 @@ __device__ __forceinline__ float lin_decay(const LinK& P, int b, int t, int h, b
 
 // ------------------------------------------------------------------ fp32 units, any size and stride
 // One CTA per (segment, batch row and head, 64 value columns, pass); chunks of 64 tokens in shared
-// memory as fp32, each thread a 4 x 4 tile of every product.  This path serves fp32 I/O, where
-// 16-bit tensor-core operands would lose half the mantissa.
+// memory as fp32, each thread of a group of 128 an 8 x 4 tile of a product (4 x 4 tiles wait for shared memory
+// twice as long).  One group makes the scores while the other multiplies with the state, both take half of
+// the tokens in P V, then one updates the state while the other writes the outputs.  This path serves fp32 I/O, where
+// 16-bit tensor-core operands would lose half the mantissa.  A chunk is a chain of short steps with
+// barriers between them, so heads of at most DMAX = 64 run two CTAs on an SM (and are cut into twice the
+// segments); wider ones fill its shared memory alone.
 constexpr int kLsC = 64;          // tokens of a chunk
 constexpr int kLsN = 64;          // value columns of a CTA
 constexpr int kLsThreads = 256;
 constexpr int kLsLd = 68;         // row stride (floats): 16-byte aligned, rows 4 banks apart
 constexpr int kLinMaxDim = 128;
 
+template <int DMAX>
 struct LsSmem {
-  float qt[kLinMaxDim][kLsLd];  // [d][token]
-  float kt[kLinMaxDim][kLsLd];
+  float qt[DMAX][kLsLd];        // [d][token]
+  float kt[DMAX][kLsLd];
   float v[kLsC][kLsLd];         // [token][column]
-  float h[kLinMaxDim][kLsLd];   // [d][column]
+  float h[DMAX][kLsLd];         // [d][column]
   float at[kLsC][kLsLd];        // weighted scores, [j][i]
   double G[kLsC];
   float w_out[kLsC], w_upd[kLsC];
   double total;
 };
 
-template <typename IT, bool STATE_ONLY>
-__global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_constant__ LinK P) {
+template <typename IT, int DMAX, bool STATE_ONLY>
+__global__ void __launch_bounds__(kLsThreads, 128 / DMAX) linear_simt_kernel(const __grid_constant__ LinK P) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  LsSmem& S = *reinterpret_cast<LsSmem*>(smem_raw);
-  const int tiles = (kLinMaxDim + kLsN - 1) / kLsN;
+  LsSmem<DMAX>& S = *reinterpret_cast<LsSmem<DMAX>*>(smem_raw);
+  constexpr int tiles = DMAX / kLsN;
   const LinPass& A = P.pass[blockIdx.y / tiles];
   const int tile = blockIdx.y % tiles;
   const int n0 = tile * kLsN;
@@ -119,12 +124,15 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
   const IT* k = static_cast<const IT*>(A.k) + (int64_t)b * A.kb + (int64_t)(head / A.rk) * A.kh;
   const IT* v = static_cast<const IT*>(A.v) + (int64_t)b * A.vb + (int64_t)(head / A.rv) * A.vh + n0;
   const int tid = threadIdx.x;
-  const int ti = tid / 16 * 4, tj = tid % 16 * 4;  // 4 x 4 tile of a 64 x 64 product
-  const int hi = tid / 16 * 8;                     // 8 x 4 tile of the state
+  const bool second = tid >= kLsThreads / 2;       // the group that makes the outputs
+  const int ti = (tid / 16 & 7) * 8, tj = tid % 16 * 4;  // 8 x 4 tile of a group's 64 x 64 product
   const int64_t block = (int64_t)dk * dv;
+  // outputs as vectors of 4 fp32 values
+  const bool o_vec = (A.o_f32 || sizeof(IT) == 4) && dv % 4 == 0 && (reinterpret_cast<uintptr_t>(A.o) & 15) == 0 &&
+                     ((A.ob | A.ol | A.oh) & 3) == 0;
 
   // the state before this segment: the initial state, or what it and the earlier segments fold to
-  for (int e = tid; e < kLinMaxDim * kLsN; e += kLsThreads) {
+  for (int e = tid; e < DMAX * kLsN; e += kLsThreads) {
     const int i = e / kLsN, j = e % kLsN;
     float s = 0.f;
     if (!STATE_ONLY && i < dk && j < nv) {
@@ -134,6 +142,34 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
     S.h[i][j] = s;
   }
   double seg_total = 0.0;
+
+  // A chunk's inputs in registers, 16 threads a token and 4 tokens a thread: all of them under way at once, and
+  // the next chunk's while this one is computed
+  float xq[4][STATE_ONLY ? 1 : DMAX / 16], xk[4][DMAX / 16], xv[4][kLsN / 16], xg[2];
+  auto first_token = [&](int c) { return (A.reverse ? n_live - 1 - c : c) * kLsC; };
+  auto load = [&](int c) {
+    const int t0 = first_token(c), m = c < min(c1, n_live) ? min(kLsC, len - t0) : 0;
+    auto fetch = [&](auto& x, const IT* p, int64_t stride, int n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = tid / 16 + 16 * i;
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(x[0]) / sizeof(float)); ++j) {
+          const int d = tid % 16 + 16 * j;
+          x[i][j] = t < m && d < n ? to_f<IT>(p[(int64_t)(t0 + t) * stride + d]) : 0.f;
+        }
+      }
+    };
+    if constexpr (!STATE_ONLY) fetch(xq, q, A.ql, dk);
+    fetch(xk, k, A.kl, dk);
+    fetch(xv, v, A.vl, nv);
+    constexpr bool bf = std::is_same<IT, __nv_bfloat16>::value;
+    if (tid < 32)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) xg[r] = 2 * tid + r < m ? lin_decay(P, b, t0 + 2 * tid + r, head, bf) : 0.f;
+  };
+  constexpr bool kAhead = DMAX > 64;  // beside a second CTA the registers are worth more
+  if (kAhead) load(c0);
 
   for (int c = c0; c < (STATE_ONLY ? min(c1, n_live) : c1); ++c) {
     if (!STATE_ONLY && c >= n_live) {  // behind the row's end: zero outputs
@@ -149,35 +185,23 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
         A.dot[(((int64_t)tile * P.batch + b) * P.heads + head) * P.seqlen + c * kLsC + tid] = 0.f;
       continue;
     }
-    const int t0 = (A.reverse ? n_live - 1 - c : c) * kLsC;
+    const int t0 = first_token(c);
     const int m = min(kLsC, len - t0);  // valid tokens
+    if (!kAhead) load(c);
     __syncthreads();                    // the chunk before is done with shared memory
-    // 16 threads a token, 4 tokens a thread; all of a thread's loads of a tensor are under way at once
-    auto fetch = [&](const IT* p, int64_t stride, int n, auto&& put) {
-      float x[4][kLinMaxDim / 16];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = tid / 16 + 16 * i;
+    for (int i = 0; i < 4; ++i) {
+      const int t = tid / 16 + 16 * i, d = tid % 16;
 #pragma unroll
-        for (int j = 0; j < kLinMaxDim / 16; ++j) {
-          const int d = tid % 16 + 16 * j;
-          x[i][j] = t < m && d < n ? to_f<IT>(p[(int64_t)(t0 + t) * stride + d]) : 0.f;
-        }
+      for (int j = 0; j < DMAX / 16; ++j) {
+        if constexpr (!STATE_ONLY) S.qt[d + 16 * j][t] = xq[i][j];
+        S.kt[d + 16 * j][t] = xk[i][j];
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < kLinMaxDim / 16; ++j) put(tid / 16 + 16 * i, tid % 16 + 16 * j, x[i][j]);
-    };
-    if (!STATE_ONLY) fetch(q, A.ql, dk, [&](int t, int d, float x) { S.qt[d][t] = x; });
-    fetch(k, A.kl, dk, [&](int t, int d, float x) { S.kt[d][t] = x; });
-    fetch(v, A.vl, nv, [&](int t, int d, float x) {
-      if (d < kLsN) S.v[t][d] = x;
-    });
+      for (int j = 0; j < kLsN / 16; ++j) S.v[t][d + 16 * j] = xv[i][j];
+    }
     if (tid < 32) {  // inclusive sums of two tokens a lane, in 64 bits: differences stay exact behind a reset
-      constexpr bool bf = sizeof(IT) == 2 && std::is_same<IT, __nv_bfloat16>::value;
-      const double g0 = 2 * tid < m ? (double)lin_decay(P, b, t0 + 2 * tid, head, bf) : 0.0;
-      const double g1 = 2 * tid + 1 < m ? (double)lin_decay(P, b, t0 + 2 * tid + 1, head, bf) : 0.0;
+      const double g0 = xg[0], g1 = xg[1];
       double s = g0 + g1;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -197,100 +221,127 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
       if (tid == 0) S.total = T;
     }
     __syncthreads();
+    if (kAhead) load(c + 1);
     seg_total += S.total;
     if constexpr (!STATE_ONLY) {
-      // scores, weighted by the decay between the two tokens
-      float acc[4][4] = {};
-      for (int d = 0; d < dk; ++d) {
-        const float4 x = *reinterpret_cast<const float4*>(&S.qt[d][ti]);
-        const float4 y = *reinterpret_cast<const float4*>(&S.kt[d][tj]);
-        const float xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
+      // acc += a[n][ti ..] b[n][tj ..] over n in [n0, n1), both multiples of 8
+      float acc[8][4] = {};
+      auto product = [&](const float (*a)[kLsLd], const float (*b)[kLsLd], int n0, int n1) {
+        for (int n = n0; n < n1; n += 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int r = 0; r < 4; ++r) {
+            const float4 x = *reinterpret_cast<const float4*>(&a[n + r][ti]), z = *reinterpret_cast<const float4*>(&a[n + r][ti + 4]);
+            const float4 y = *reinterpret_cast<const float4*>(&b[n + r][tj]);
+            const float xa[8] = {x.x, x.y, x.z, x.w, z.x, z.y, z.z, z.w}, ya[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xa[i], ya[j], acc[i][j]);
-      }
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = ti + i, s = tj + j;
-          const bool on = A.reverse ? s >= r : s <= r;
-          const double d = A.reverse ? S.G[s] - S.G[r] : S.G[r] - S.G[s];
-          S.at[s][r] = on && s < m ? acc[i][j] * expf((float)d) : 0.f;
+              for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xa[i], ya[j], acc[i][j]);
+          }
         }
-      // e^{G_i} q_i H
-      float o[4][4] = {};
-      for (int d = 0; d < dk; ++d) {
-        const float4 x = *reinterpret_cast<const float4*>(&S.qt[d][ti]);
-        const float4 y = *reinterpret_cast<const float4*>(&S.h[d][tj]);
-        const float xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
+      };
+      const int dk8 = (dk + 7) & ~7;  // rows behind dk are zero
+      if (second) {  // e^{G_i} q_i H
+        product(S.qt, S.h, 0, dk8);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) o[i][j] = fmaf(xa[i], ya[j], o[i][j]);
+          for (int j = 0; j < 4; ++j) acc[i][j] *= S.w_out[ti + i];
+      } else {  // scores, weighted by the decay between the two tokens
+        product(S.qt, S.kt, 0, dk8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int n = tj + j;
+          const double g = S.G[n];
+          float w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = ti + i;
+            const bool on = A.reverse ? n >= r : n <= r;
+            const double d = A.reverse ? g - S.G[r] : S.G[r] - g;
+            w[i] = on && n < m ? acc[i][j] * expf((float)d) : 0.f;
+          }
+          *reinterpret_cast<float4*>(&S.at[n][ti]) = make_float4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<float4*>(&S.at[n][ti + 4]) = make_float4(w[4], w[5], w[6], w[7]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
       }
+      __syncthreads();  // scores written, H and q read
+      // each group's half of the tokens; a warp's 16 rows need none on the far side of the diagonal
+      const int r16 = ti & ~15, half = second ? kLsC / 2 : 0;
+      product(S.at, S.v, A.reverse ? max(half, r16) : half, A.reverse ? half + kLsC / 2 : min(half + kLsC / 2, r16 + 16));
+      float(*part)[kLsLd] = S.qt;
+      if (!second) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] *= S.w_out[ti + i];
-      __syncthreads();  // scores written, H read
-      for (int s = 0; s < kLsC; ++s) {
-        const float4 x = *reinterpret_cast<const float4*>(&S.at[s][ti]);
-        const float4 y = *reinterpret_cast<const float4*>(&S.v[s][tj]);
-        const float xa[4] = {x.x, x.y, x.z, x.w}, ya[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[i][j] = fmaf(xa[i], ya[j], o[i][j]);
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<float4*>(&part[ti + i][tj]) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
       }
+      __syncthreads();
+      if (second) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = t0 + ti + i;
-        const bool on = ti + i < m;
-        float dot = 0.f;
-        if (t < P.seqlen) {
-          const int64_t at = (int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0 + tj;
+        for (int i = 0; i < 8; ++i) {
+          const int t = t0 + ti + i;
+          const bool on = ti + i < m;
+          float dot = 0.f;
+          if (t < P.seqlen) {
+            const float4 x = *reinterpret_cast<const float4*>(&part[ti + i][tj]);
+            const float xa[4] = {x.x, x.y, x.z, x.w};
+            const int64_t at = (int64_t)b * A.ob + (int64_t)t * A.ol + (int64_t)head * A.oh + n0 + tj;
+            float r[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (tj + j < nv) {
-              const float r = on ? A.scale * o[i][j] : 0.f;
-              if (A.o_f32) static_cast<float*>(A.o)[at + j] = r;
-              else static_cast<IT*>(A.o)[at + j] = from_f<IT>(r);
-              if (A.dot && on)
-                dot = fmaf(r, to_f<IT>(static_cast<const IT*>(A.p)[(int64_t)b * A.pb + (int64_t)t * A.pl +
-                                                                   (int64_t)(head / A.rp) * A.ph + n0 + tj + j]), dot);
+            for (int j = 0; j < 4; ++j) r[j] = on ? A.scale * (acc[i][j] + xa[j]) : 0.f;
+            if (o_vec) {
+              if (tj < nv) *reinterpret_cast<float4*>(static_cast<float*>(A.o) + at) = make_float4(r[0], r[1], r[2], r[3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (tj + j < nv) {
+                  if (A.o_f32) static_cast<float*>(A.o)[at + j] = r[j];
+                  else static_cast<IT*>(A.o)[at + j] = from_f<IT>(r[j]);
+                }
             }
-        }
-        if (A.dot) {
+            if (A.dot && on) {
+              const IT* p = static_cast<const IT*>(A.p) + (int64_t)b * A.pb + (int64_t)t * A.pl + (int64_t)(head / A.rp) * A.ph + n0 + tj;
 #pragma unroll
-          for (int s = 8; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-          if (tid % 16 == 0 && t < P.seqlen)
-            A.dot[(((int64_t)tile * P.batch + b) * P.heads + head) * P.seqlen + t] = dot;
+              for (int j = 0; j < 4; ++j)
+                if (tj + j < nv) dot = fmaf(r[j], to_f<IT>(p[j]), dot);
+            }
+          }
+          if (A.dot) {
+#pragma unroll
+            for (int w = 8; w > 0; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
+            if (tid % 16 == 0 && t < P.seqlen)
+              A.dot[(((int64_t)tile * P.batch + b) * P.heads + head) * P.seqlen + t] = dot;
+          }
         }
       }
     }
-    // H <- e^T H + sum_j w_j k_j v_j^T: each thread updates its own 8 x 4 entries
+    // H <- e^T H + sum_j w_j k_j v_j^T, R x 4 entries a thread: the first group's part of it while the second
+    // writes the outputs; a state alone is shared evenly
+    constexpr int R = STATE_ONLY && DMAX == 64 ? 4 : 8;
+    const int hi = R == 4 ? tid / 16 * 4 : ti + (second ? 64 : 0);
     if (hi < dk) {
       const float d = expf((float)S.total);
-      float h[8][4];
+      float h[R][4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < R; ++i) {
         const float4 x = *reinterpret_cast<const float4*>(&S.h[hi + i][tj]);
         h[i][0] = d * x.x, h[i][1] = d * x.y, h[i][2] = d * x.z, h[i][3] = d * x.w;
       }
-      for (int s = 0; s < m; s += 4) {
+      for (int n = 0; n < m; n += 4) {
         float4 y[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          y[r] = *reinterpret_cast<const float4*>(&S.v[s + r][tj]);
-          const float w = S.w_upd[s + r];
+          y[r] = *reinterpret_cast<const float4*>(&S.v[n + r][tj]);
+          const float w = S.w_upd[n + r];
           y[r].x *= w, y[r].y *= w, y[r].z *= w, y[r].w *= w;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (hi + i >= dk) break;
-          const float4 x = *reinterpret_cast<const float4*>(&S.kt[hi + i][s]);
+        for (int i = 0; i < R; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>(&S.kt[hi + i][n]);
           const float xa[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -302,7 +353,7 @@ __global__ void __launch_bounds__(kLsThreads) linear_simt_kernel(const __grid_co
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < R; ++i)
         *reinterpret_cast<float4*>(&S.h[hi + i][tj]) = make_float4(h[i][0], h[i][1], h[i][2], h[i][3]);
     }
   }
