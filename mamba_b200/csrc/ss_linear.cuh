@@ -95,7 +95,7 @@ struct LsSmem {
   float v[kLsC][kLsLd];         // [token][column]
   float h[DMAX][kLsLd];         // [d][column]
   float at[kLsC][kLsLd];        // weighted scores, [j][i]
-  double G[kLsC];
+  float gh[kLsC], gl[kLsC];     // G log2 e in two parts
   float w_out[kLsC], w_upd[kLsC];
   double total;
 };
@@ -213,7 +213,9 @@ __global__ void __launch_bounds__(kLsThreads, 128 / DMAX) linear_simt_kernel(con
       for (int r = 0; r < 2; ++r) {
         const double G = r ? s : s - g1;
         const int t = 2 * tid + r;
-        S.G[t] = G;
+        const double g2 = G * 1.4426950408889634;
+        S.gh[t] = (float)g2;
+        S.gl[t] = (float)(g2 - (double)(float)g2);
         const float a = expf((float)G), z = expf((float)(T - G));
         S.w_out[t] = A.reverse ? z : a;
         S.w_upd[t] = t < m ? (A.reverse ? a : z) : 0.f;
@@ -252,14 +254,14 @@ __global__ void __launch_bounds__(kLsThreads, 128 / DMAX) linear_simt_kernel(con
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int n = tj + j;
-          const double g = S.G[n];
+          const float gh = S.gh[n], gl = S.gl[n];
           float w[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int r = ti + i;
             const bool on = A.reverse ? n >= r : n <= r;
-            const double d = A.reverse ? g - S.G[r] : S.G[r] - g;
-            w[i] = on && n < m ? acc[i][j] * expf((float)d) : 0.f;
+            const float d = (S.gh[r] - gh) + (S.gl[r] - gl);  // the difference of the sums, rounded once
+            w[i] = on && n < m ? acc[i][j] * ex2(A.reverse ? -d : d) : 0.f;
           }
           *reinterpret_cast<float4*>(&S.at[n][ti]) = make_float4(w[0], w[1], w[2], w[3]);
           *reinterpret_cast<float4*>(&S.at[n][ti + 4]) = make_float4(w[4], w[5], w[6], w[7]);
