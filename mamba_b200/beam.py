@@ -83,10 +83,13 @@ def reorder_states(states, parents):
         raise ValueError(f"a state must have {total} contiguous rows, got {[tuple(t.shape) for t in states]}")
     if states and set(map(torch.Tensor.get_device, states)) != {parents.get_device()}:
         raise RuntimeError("states and parents on different devices")
-    rows = sorted(r for r in zip(map(torch.Tensor.data_ptr, states), map(_nbytes, states)) if r[1])
-    end = 0
+    sizes = list(map(_nbytes, states))
+    rows = sorted(zip(map(torch.Tensor.data_ptr, states), sizes))
+    if 0 in sizes:
+        rows = [r for r in rows if r[1]]
+    end, step = 0, 4 * total
     for at, n in rows:
-        if n % (4 * total) or at % 4:
+        if n % step or at % 4:
             raise NotImplementedError(f"rows of {n / total} bytes at address {at} (multiples of 4 are supported)")
         if at < end:
             raise ValueError("states must not share memory")

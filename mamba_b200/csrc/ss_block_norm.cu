@@ -56,6 +56,9 @@ int bwd_ctas(int64_t rows, int wpr) {
   return (int)std::max<int64_t>(1, std::min<int64_t>((rows + rpc - 1) / rpc, 2 * 148));
 }
 
+// rows that would overlap (the stride of a single row is not used)
+bool short_rows(const ss_block_norm_args& a, int64_t stride) { return a.rows > 1 && stride < a.dim; }
+
 int check(const ss_block_norm_args& a) {
   if (a.rows < 0 || a.dim < 1 || !(a.eps >= 0.f) || !(a.pre_eps >= 0.f) || !std::isfinite(a.scale_const)) return SS_ERR_INVALID;
   if (a.io_dtype != SS_F32 && a.io_dtype != SS_BF16 && a.io_dtype != SS_F16) return SS_ERR_UNSUPPORTED;
@@ -63,8 +66,8 @@ int check(const ss_block_norm_args& a) {
   if (a.dim > SS_MAX_BLOCK_NORM_DIM) return SS_ERR_UNSUPPORTED;
   if (a.rows == 0) return SS_OK;
   if (!a.y || !a.residual) return SS_ERR_INVALID;
-  if (a.y_row_stride < a.dim || a.residual_row_stride < a.dim) return SS_ERR_INVALID;
-  if (a.gate && a.gate_row_stride != 0 && a.gate_row_stride < a.dim) return SS_ERR_INVALID;
+  if (short_rows(a, a.y_row_stride) || short_rows(a, a.residual_row_stride)) return SS_ERR_INVALID;
+  if (a.gate && a.gate_row_stride != 0 && short_rows(a, a.gate_row_stride)) return SS_ERR_INVALID;
   return SS_OK;
 }
 
@@ -145,8 +148,8 @@ int ss_block_norm_fwd(const ss_block_norm_args* a, void* stream) {
   const int rc = check(*a);
   if (rc != SS_OK) return rc;
   if (a->rows == 0) return SS_OK;
-  if (!a->h || a->h_row_stride < a->dim || !pairs(a->rstd)) return SS_ERR_INVALID;
-  if (a->pre_weight && (!a->x || a->x_row_stride < a->dim)) return SS_ERR_INVALID;
+  if (!a->h || short_rows(*a, a->h_row_stride) || !pairs(a->rstd)) return SS_ERR_INVALID;
+  if (a->pre_weight && (!a->x || short_rows(*a, a->x_row_stride))) return SS_ERR_INVALID;
   const size_t es = a->io_dtype == SS_F32 ? 4 : 2;
   BlockNormK P;
   P.a = *a;
@@ -174,8 +177,9 @@ int ss_block_norm_bwd(const ss_block_norm_bwd_args* g, void* stream) {
   if (a.rows > 0) {
     if (!a.rstd || !pairs(a.rstd) || !g->dresidual || !g->dy || !g->work || (a.gate && !g->dgate) || (a.pre_weight && !g->dx))
       return SS_ERR_INVALID;
-    if (g->dy_row_stride < a.dim || g->dresidual_row_stride < a.dim || (a.gate && g->dgate_row_stride < a.dim) ||
-        (a.pre_weight && g->dx_row_stride < a.dim) || (g->dh && g->dh_row_stride < a.dim))
+    if (short_rows(a, g->dy_row_stride) || short_rows(a, g->dresidual_row_stride) ||
+        (a.gate && short_rows(a, g->dgate_row_stride)) || (a.pre_weight && short_rows(a, g->dx_row_stride)) ||
+        (g->dh && short_rows(a, g->dh_row_stride)))
       return SS_ERR_INVALID;
     BlockNormBwdK P;
     P.a = *g;

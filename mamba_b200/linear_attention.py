@@ -170,6 +170,20 @@ def _backward(t, c, dout, dfinal, final, want_decay, want_state):
     return dq, dk, dv, dg, ds
 
 
+def _backward_of(ctx, dout, dfinal=None):
+    *t, final = ctx.saved_tensors
+    if dout is None and dfinal is None:
+        return (None,) * 8
+    if dout is None:
+        dout = torch.zeros_like(t[2])
+    grads = _backward(t, ctx.call, dout, dfinal, final, ctx.needs_input_grad[3], ctx.needs_input_grad[5])
+    dq, dk, dv, dg, ds = (x if x is None else _as(x, d) for x, d in zip(grads, ctx.dtypes))
+    return dq, dk, dv, dg, None, ds, None, None
+
+
+_backward_once = once_differentiable(_backward_of)
+
+
 class LinearAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, scale, initial_state, seq_lens, want_final):
@@ -183,16 +197,9 @@ class LinearAttentionFn(torch.autograd.Function):
         return (o, final) if want_final else o
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dout, dfinal=None):
-        *t, final = ctx.saved_tensors
-        if dout is None and dfinal is None:
-            return (None,) * 8
-        if dout is None:
-            dout = torch.zeros_like(t[2])
-        grads = _backward(t, ctx.call, dout, dfinal, final, ctx.needs_input_grad[3], ctx.needs_input_grad[5])
-        dq, dk, dv, dg, ds = (x if x is None else _as(x, d) for x, d in zip(grads, ctx.dtypes))
-        return dq, dk, dv, dg, None, ds, None, None
+    def backward(ctx, *grads):
+        # create_graph: the gradients may be used, not differentiated again
+        return (_backward_once if torch.is_grad_enabled() else _backward_of)(ctx, *grads)
 
 
 def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, seq_lens=None, return_final_state=False):

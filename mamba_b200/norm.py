@@ -103,8 +103,8 @@ _pack_block_fwd, _pack_block_bwd = (L.packer(st) for st in (L.BlockNormArgs, L.B
 
 
 def _row_at(t):
-    """Address and row stride of a (rows, dim) tensor, or of a packed (..., dim) one."""
-    return (0, 0) if t is None else (t.data_ptr(), t.stride(0) if t.dim() == 2 and t.shape[0] > 1 else t.shape[-1])
+    """Address and row stride of a (rows, dim) tensor."""
+    return (0, 0) if t is None else (t.data_ptr(), t.stride(0))
 
 
 def _like(t):
@@ -127,24 +127,61 @@ def _f32(t):
     return t if t is None or (t.dtype == torch.float32 and t.is_contiguous()) else t.to(torch.float32).contiguous()
 
 
-def _block_args(rows, cols, call, h=None, x=None, rstd=None):
+def _block_args(rows, cols, call, h, x, rstd):
+    """The fields of ss_block_norm_args; h, x (packed) and rstd are addresses."""
     (y, residual, gate), (post, pre, scale) = rows, cols
     io, activation, eps, pre_eps, unit, const = call
-    return (*y.shape, io, unit, activation, eps, pre_eps, const, *_row_at(y), *_row_at(residual), *_row_at(gate),
-            L.ptr(post) or 0, L.ptr(pre) or 0, L.ptr(scale) or 0, *_row_at(h), *_row_at(x), L.ptr(rstd) or 0)
+    n, dim = y.shape
+    return (n, dim, io, unit, activation, eps, pre_eps, const, y.data_ptr(), y.stride(0), residual.data_ptr(),
+            residual.stride(0), *_row_at(gate), _address(post), _address(pre), _address(scale), h, dim, x, dim, rstd)
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _block_forward(y, residual, post, pre, gate, scale, call, train):
     """Returns (x | None, h, rows, columns, rstd | None)."""
     dev = _cuda_device(y, residual, post, pre, gate, scale)
     dim, io = y.shape[-1], y.dtype
-    rows = [_block_rows(t, io, dim) for t in (y, residual, gate)]
-    cols = [_f32(t) for t in (post, pre, scale)]
+    rows = _block_rows(y, io, dim), _block_rows(residual, io, dim), _block_rows(gate, io, dim)
+    cols = _f32(post), _f32(pre), _f32(scale)
     h = _like(y)
     x = None if pre is None else _like(y)
     rstd = torch.empty((rows[0].shape[0], 2), dtype=torch.float32, device=dev) if train else None
-    L.launch("ss_block_norm_fwd", _pack_block_fwd(*_block_args(rows, cols, call, h, x, rstd)), dev)
+    L.launch("ss_block_norm_fwd", _pack_block_fwd(*_block_args(rows, cols, call, h.data_ptr(), _address(x), _address(rstd))),
+             dev)
     return x, h, rows, cols, rstd
+
+
+def _block_backward(ctx, *grads):
+    y, residual, gate, post, pre, scale, rstd = ctx.saved_tensors
+    (n, dim), io, dev = y.shape, y.dtype, y.device
+    dx, dh = grads if pre is not None else (None, grads[0])
+    if dx is None and dh is None:
+        return (None,) * 7
+    if pre is not None and dx is None:
+        dx = torch.zeros_like(y)
+    dx, dh = _block_rows(dx, io, dim), _block_rows(dh, io, dim)
+    dy, dres, dgate = _like(y), _like(residual), _like(gate)
+    work = torch.empty(_block_work(n, dim, ctx.call[0]), dtype=torch.float32, device=dev)
+    dpost, dpre, dscale = _like(post), _like(pre), _like(scale)
+    L.launch("ss_block_norm_bwd", _pack_block_bwd(
+        *_block_args((y, residual, gate), (post, pre, scale), ctx.call, 0, 0, rstd.data_ptr()), *_row_at(dx), *_row_at(dh),
+        dy.data_ptr(), dim, dres.data_ptr(), dim, _address(dgate), dim, _address(dpost), _address(dpre), _address(dscale),
+        work.data_ptr()), dev)
+    grads = dy, dres, dpost, dpre, dgate, dscale
+    if ctx.casts is not None:
+        grads = (t if t is None else _as_leaf(t, *c) for t, c in zip(grads, ctx.casts))
+    return (*grads, None)
+
+
+def _as_leaf(t, shape, dtype):
+    t = t if t.shape == shape else t.reshape(shape)
+    return t if t.dtype == dtype else t.to(dtype)
+
+
+_block_backward_once = once_differentiable(_block_backward)
 
 
 class BlockNormFn(torch.autograd.Function):
@@ -153,33 +190,16 @@ class BlockNormFn(torch.autograd.Function):
         x, h, rows, cols, rstd = _block_forward(y, residual, post_weight, pre_weight, gate, scale, call, True)
         ctx.save_for_backward(*rows, *cols, rstd)
         ctx.set_materialize_grads(False)
-        ctx.call, ctx.shape = call, y.shape
-        ctx.dtypes = tuple(None if t is None else t.dtype
-                           for t in (y, residual, post_weight, pre_weight, gate, scale))
+        ctx.call = call
+        # what came in another shape or type than it is saved in
+        had, kept = (y, residual, post_weight, pre_weight, gate, scale), (*rows[:2], *cols[:2], rows[2], cols[2])
+        ctx.casts = None if all(a is b for a, b in zip(had, kept)) else [None if t is None else (t.shape, t.dtype) for t in had]
         return h if x is None else (x, h)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
-        *rows, post, pre, scale, rstd = ctx.saved_tensors
-        y, residual, gate = rows
-        (n, dim), io, dev = y.shape, y.dtype, y.device
-        dx, dh = grads if pre is not None else (None, grads[0])
-        if dx is None and dh is None:
-            return (None,) * 7
-        if pre is not None and dx is None:
-            dx = torch.zeros_like(y)
-        dx, dh = _block_rows(dx, io, dim), _block_rows(dh, io, dim)
-        dy, dres, dgate = _like(y), _like(residual), _like(gate)
-        work = torch.empty(_block_work(n, dim, ctx.call[0]), dtype=torch.float32, device=dev)
-        dpost, dpre, dscale = _like(post), _like(pre), _like(scale)
-        L.launch("ss_block_norm_bwd", _pack_block_bwd(
-            *_block_args(rows, (post, pre, scale), ctx.call, rstd=rstd), *_row_at(dx), *_row_at(dh), *_row_at(dy),
-            *_row_at(dres), *_row_at(dgate), L.ptr(dpost) or 0, L.ptr(dpre) or 0, L.ptr(dscale) or 0, work.data_ptr()), dev)
-        if len(ctx.shape) != 2:
-            dy, dres, dgate = (t if t is None else t.reshape(ctx.shape) for t in (dy, dres, dgate))
-        return (*(t if t is None or t.dtype == d else t.to(d)
-                  for t, d in zip((dy, dres, dpost, dpre, dgate, dscale), ctx.dtypes)), None)
+        # create_graph: the gradients may be used, not differentiated again
+        return (_block_backward_once if torch.is_grad_enabled() else _block_backward)(ctx, *grads)
 
 
 def block_norm_fn(y, residual, post_weight=None, pre_weight=None, gate=None, residual_scale=None, activation="silu",

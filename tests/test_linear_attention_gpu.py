@@ -383,6 +383,21 @@ def test_a_state_that_a_backward_needs_cannot_be_stepped():
         assert float(s.abs().max()) > 0
 
 
+def test_a_second_derivative_is_refused():
+    from mamba_b200 import block_norm_fn, linear_attention_fn
+
+    t = make(1, 20, 2, 2, 16, 16, torch.float32, seed=29)
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g")]
+    y, w = torch.randn(3, 16, device="cuda").requires_grad_(), torch.zeros(16, device="cuda")
+    for out, xs in ((linear_attention_fn(*leaves), leaves), (block_norm_fn(y, y.detach(), w), [y])):
+        plain = torch.autograd.grad(out.square().sum(), xs, retain_graph=True)
+        grads = torch.autograd.grad(out.square().sum(), xs, create_graph=True)
+        for a, b in zip(plain, grads):
+            assert torch.equal(a, b)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(grads[0].sum(), xs)
+
+
 def test_two_streams_at_once():
     from mamba_b200 import linear_attention_fn
 
