@@ -70,6 +70,15 @@ template <> __device__ __forceinline__ __half from_f<__half>(float x) { return _
 
 template <typename T> __device__ __forceinline__ T zero_v() { return from_f<T>(0.f); }
 
+// 16 bytes, zeros where `on` is false; predicated inside, so that no branch waits for the load
+__device__ __forceinline__ uint4 ld_vector(const void* p, bool on) {
+  uint4 r;
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n mov.u32 %0, 0;\n mov.u32 %1, 0;\n mov.u32 %2, 0;\n mov.u32 %3, 0;\n"
+               " @p ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n}\n"
+               : "=&r"(r.x), "=&r"(r.y), "=&r"(r.z), "=&r"(r.w) : "l"(p), "r"((uint32_t)on));
+  return r;
+}
+
 // ---- transcendental helpers (hardware approximations, as the reference's fast-math build) --
 __device__ __forceinline__ float ex2(float x) {
   float y;

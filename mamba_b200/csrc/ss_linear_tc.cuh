@@ -679,6 +679,17 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       const IT* p_at = A.dot ? static_cast<const IT*>(A.p) + (int64_t)b * A.pb + (int64_t)(head / A.rp) * A.ph + n0 : nullptr;
       float* dot_at = MODE == kTcGrad && A.dot ? A.dot + (((int64_t)tile * K.batch + b) * K.heads + head) * K.seqlen : nullptr;
       const float2 sc = f2(A.scale);
+      // the rows of p that go with a chunk's outputs, 8 lanes a row: loaded a chunk ahead, then passed through
+      // shared memory, since a lane that read its own row would touch 32 lines an instruction
+      uint4 pq[8];
+      auto load_p = [&](int c) {
+        const int t0 = first_token(c), m = min(kTcC, len - t0);
+        const IT* p = p_at + (int64_t)(t0 + w4 * 32 + (lane >> 3)) * A.pl + (lane & 7) * 8;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          pq[k] = ld_vector(p + (int64_t)4 * k * A.pl, w4 * 32 + 4 * k + (lane >> 3) < m && (lane & 7) * 8 < nv);
+      };
+      if (dot_at && c0 < cn) load_p(c0);
       for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
         const int t0 = first_token(c), m = min(kTcC, len - t0), t = t0 + row;
         if (!warp_wait(&B.full[st], ph)) break;
@@ -688,17 +699,6 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
         if (lane == 0) {
           if (!o_f32) mbar_arrive(&B.empty[st]);
           if (own_out) mbar_arrive(&B.v_empty[st]);
-        }
-        // the rows of p that go with the outputs, 8 lanes a row; they pass through shared memory, since a lane
-        // that read its own row would touch 32 lines an instruction
-        uint4 pq[8];
-        if (dot_at) {
-          const IT* p = p_at + (int64_t)(t0 + w4 * 32 + (lane >> 3)) * A.pl + (lane & 7) * 8;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const bool in = w4 * 32 + 4 * k + (lane >> 3) < m && (lane & 7) * 8 < nv;
-            pq[k] = in ? *reinterpret_cast<const uint4*>(p + (int64_t)4 * k * A.pl) : make_uint4(0, 0, 0, 0);
-          }
         }
         if (!warp_wait(&B.o_full[i & 1], (uint32_t)(i >> 1) & 1)) break;
         tc_after();
@@ -722,6 +722,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
             *reinterpret_cast<uint4*>(to + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = pq[k];
           }
           __syncwarp();
+          if (c + 1 < cn) load_p(c + 1);
         }
         float2 dot = f2(0.f);
 #pragma unroll 1
