@@ -20,8 +20,15 @@
 // bound, the row's largest |q| times the chunk's largest |k| times dk), V' and H by one per chunk (from their
 // largest value), which the outputs and the state take back; bf16 needs none of that.
 //
-// What bounds it: a chunk moves 128 x (2 dk + 128) x 2 bytes through TMA; two value tiles of one head
-// run side by side, so keys and queries come from L2 the second time.
+// What bounds it: neither memory nor the tensor cores, but the hand-overs between the roles.  A chunk with keys
+// of 64 takes about 2.3 us a CTA (a gradient: 4400 cycles, of them 4000 in the warps that make the outputs),
+// its products 1500 cycles; a load that was issued early arrives after 3000.  Measured:
+//   8 x 2048 tokens, 24 heads of 64 x 64, bf16       75 us forward (201 MB, 2.7 TB/s), 250 us backward
+//   1 x 16384 tokens, 16 heads of 128 x 128, bf16    179 us forward with the final state (270 MB, 1.5 TB/s)
+//   4 x 1999 tokens, 16 heads, 4 of keys, fp16       95 us forward, 313 us backward
+// Tried and slower: the outputs of gradients shared with the scores' warps (273 against 250 us: a chunk's scores
+// then wait for the outputs before them), 32 columns of outputs at a time (295 us: it spills).
+// Two value tiles of one head run side by side, so keys and queries come from L2 the second time.
 // Roles (19 warps): 0-3 scores, 4-7 weighted values, 8-11 outputs, 12-15 state, 16 loads, 17 matrix
 // instructions, 18 decays.  The only chain from chunk to chunk is H: L -> state warps -> Q H.
 #pragma once
@@ -944,7 +951,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
 
 // Value tiles and runs of one head are neighbours in the grid, so that they share what they read in L2; runs
 // with narrow and with wide keys go side by side in one launch.  One kernel a mode: together they spilled and
-// fought over the instruction cache (8 x 2048 x 24 heads of 64, gradients: 322 us in one launch).
+// fought over the instruction cache (8 x 2048 tokens of 24 heads of 64, gradients: 322 us in one launch, 250 in two).
 template <typename IT, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1) linear_tc_kernel(const __grid_constant__ LinTcK P) {
   extern __shared__ __align__(1024) unsigned char smem[];
