@@ -17,8 +17,11 @@
 // column sums in 128 registers, where the 24 of one warp to a row of 768 spilled (163 us a pass over
 // 16384 rows).  A row's warps meet at a barrier of their own.  A lane's columns are the same for all its
 // rows: their weights are loaded once, with the first row, and in the backward their two sums stay in
-// registers over the rows of a persistent CTA; the CTAs' sums meet in a second small kernel in a fixed
+// registers over the rows of a persistent CTA; the CTAs' sums meet in a second small kernel (4 us) in a fixed
 // order, so the gradients of the weights do not vary between runs.
+// Measured: 16384 rows of 768, bf16, gated: forward 28 us (126 MB, 4.4 TB/s, 68 % of the copy rate), backward
+// 65 us (201 MB, 3.1 TB/s, 47 %: at two CTAs an SM the loads under way are too few); 4099 rows of 2560, fp32:
+// forward 33 us (168 MB, 5.1 TB/s), backward 51 us (252 MB, 4.9 TB/s).
 #pragma once
 #include "ss_norm.cuh"
 
@@ -148,8 +151,8 @@ __device__ __forceinline__ void unpack(float (&v)[kBv], const typename BnVec<IT>
 }
 
 // MODE: 0 any call; 1 both norms, whole vectors (and dh in the backward), no gate; 2 the same with a SiLU
-// gate.  The common calls know at compile time what the others branch on for every vector (norm_train: 159
-// -> see below).
+// gate.  The common calls know at compile time what the others branch on for every vector (16384 rows of 768
+// with a gate, bf16: forward 45 -> 28 us, backward 100 -> 65 us).
 enum { kBnAny = 0, kBnPlain = 1, kBnGated = 2 };
 
 template <typename IT, int NV, int WPR, int MODE>

@@ -35,22 +35,25 @@ bool dtypes_ok(int io, int decay) {
   return (io == SS_F32 || io == SS_BF16 || io == SS_F16) && (decay == SS_F32 || decay == io);
 }
 
-// Segments that run side by side: enough CTAs for the GPU when batch x heads are few, at least two chunks
-// each, at most 32.  A segment's own state costs about half of what its outputs cost, and the first segment
-// neither needs nor waits for the states of the others: it starts beside their first pass (a programmatic
-// launch) and is half as long again (1 x 16384 x 16 heads of 128 x 128: 165 us with equal segments).
+// Segments that run side by side: enough CTAs for the GPU (`slots`) when batch x heads are few, at least two
+// chunks each, at most 32.  A segment's own state costs half to four fifths of what its outputs cost, and the
+// first segment neither needs nor waits for the states of the others.  Where two CTAs share an SM (narrow fp32
+// heads) it starts beside their first pass (a programmatic launch) and is half as long again: 8 x 1024 tokens of
+// 12 heads of 64 take 151 us, 161 in equal segments.  Where a CTA fills its SM there is no room beside it, and
+// the segments are equal: 1 x 16384 tokens of 16 heads of 128 x 128 in bf16 take 151 us, 179 with a longer first.
 struct Split {
   int segs, first, chunks;
 };
 
-Split split_of(const ss_linear_args& a, int chunk, int passes, int tiles, int slots) {
+Split split_of(const ss_linear_args& a, int chunk, int passes, int tiles, bool two) {
   const int n = (a.seqlen + chunk - 1) / chunk;
   const int64_t ctas = (int64_t)a.batch * a.heads * passes * tiles;
+  const int slots = two ? 2 * 148 : 148;
   int segs = 1;
   if (ctas > 0 && ctas < slots) segs = (int)std::max<int64_t>(1, std::min<int64_t>({slots / ctas, n / 2, 32}));
   Split s{1, std::max(n, 1), std::max(n, 1)};
   if (segs > 1) {
-    s.chunks = std::max(1, (2 * n + 2 * segs) / (2 * segs + 1));  // n / (segs + 1/2)
+    s.chunks = two ? std::max(1, (2 * n + 2 * segs) / (2 * segs + 1)) : (n + segs - 1) / segs;  // n / (segs + 1/2)
     s.first = std::min(n - 1, std::max(s.chunks, n - (segs - 1) * s.chunks));
     s.segs = 1 + (n - s.first + s.chunks - 1) / s.chunks;
   }
@@ -69,8 +72,8 @@ Work work_of(const ss_linear_args& a, int backward) {
   Work w;
   const int passes = backward ? 3 : 1;
   const int tiles = backward ? std::max(tiles_of(a.key_dim), tiles_of(a.value_dim)) : tiles_of(a.value_dim);
-  w.simt = split_of(a, kLsC, passes, tiles, std::max(a.key_dim, a.value_dim) > kLsN ? 148 : 2 * 148);
-  w.tc = a.io_dtype == SS_F32 ? Split{1, 1, 1} : split_of(a, kTcC, passes, tiles, 148);
+  w.simt = split_of(a, kLsC, passes, tiles, std::max(a.key_dim, a.value_dim) <= kLsN);
+  w.tc = a.io_dtype == SS_F32 ? Split{1, 1, 1} : split_of(a, kTcC, passes, tiles, false);
   const int segs = a.io_dtype == SS_F32 ? w.simt.segs : std::max(w.simt.segs, w.tc.segs);
   const size_t bh = (size_t)a.batch * a.heads;
   auto take = [&](size_t n) {
@@ -157,7 +160,7 @@ cudaError_t launch_tc(LinTcK& T, int pass0, int n, bool early, cudaStream_t st) 
 }
 
 // The passes' segments and fold, then the gradients with dot products (the first `grads`), then the others.
-// Every launch but the first may start while the one ahead of it runs: its first segments need nothing of it.
+// Every launch but the first may start while the one ahead of it ends: its first segments need nothing of it.
 template <typename IT>
 cudaError_t launch_all(LinTcK& T, int passes, int grads, cudaStream_t st) {
   cudaError_t e = cudaSuccess;

@@ -24,7 +24,7 @@
 // of 64 takes about 2.3 us a CTA (a gradient: 4400 cycles, of them 4000 in the warps that make the outputs),
 // its products 1500 cycles; a load that was issued early arrives after 3000.  Measured:
 //   8 x 2048 tokens, 24 heads of 64 x 64, bf16       75 us forward (201 MB, 2.7 TB/s), 250 us backward
-//   1 x 16384 tokens, 16 heads of 128 x 128, bf16    179 us forward with the final state (270 MB, 1.5 TB/s)
+//   1 x 16384 tokens, 16 heads of 128 x 128, bf16    151 us forward (268 MB, 1.8 TB/s), 168 with the final state
 //   4 x 1999 tokens, 16 heads, 4 of keys, fp16       95 us forward, 313 us backward
 // Tried and slower: the outputs of gradients shared with the scores' warps (273 against 250 us: a chunk's scores
 // then wait for the outputs before them), 32 columns of outputs at a time (295 us: it spills).
