@@ -267,7 +267,8 @@ typedef struct ss_mamba_step_args {
  * key_dim and value_dim are at most SS_MAX_LINEAR_DIM.  The innermost axis of q, k, v, o has stride 1.
  * A log decay of -infinity resets the state.  With seq_lens, tokens t >= seq_lens[b] (clamped to
  * [0, seqlen]) are not read into anything and their o is zero.  seqlen is at most 2^30, scale a normal
- * number. */
+ * number.  Outputs must not overlap inputs.  A token that holds an infinity or NaN reaches the outputs of
+ * earlier tokens of its chunk (of 64 or 128) too. */
 typedef struct ss_linear_args {
   int batch, seqlen, heads, key_heads, key_dim, value_dim;
   int io_dtype;             /* dtype of q, k, v, o                                        */
@@ -318,7 +319,8 @@ typedef struct ss_linear_step_args {
  *   n = post_weight ? y * rsqrt(mean(y^2) + eps) * w(post_weight) : y       w(p) = unit_offset ? 1 + p : p
  *   h = residual + scale * act(gate) * n          (the next residual stream)
  *   x = h * rsqrt(mean(h^2) + pre_eps) * w(pre_weight)   from the unrounded h; only with pre_weight
- * activation: 0 none, 1 SiLU, 2 sigmoid.  A gate row stride of 0 uses one gate row for all rows. */
+ * activation: 0 none, 1 SiLU, 2 sigmoid.  A gate row stride of 0 uses one gate row for all rows.  Outputs must not
+ * overlap inputs; rstd is 8-byte aligned. */
 typedef struct ss_block_norm_args {
   int rows, dim, io_dtype, unit_offset, activation;
   float eps, pre_eps;                                        /* of the norm of y, and of h    */

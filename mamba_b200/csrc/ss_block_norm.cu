@@ -109,10 +109,11 @@ cudaError_t fwd(const BlockNormK& P, cudaStream_t st) {
 
 template <typename IT, int NV, int WPR>
 cudaError_t bwd(const BlockNormBwdK& P, cudaStream_t st) {
-  constexpr size_t smem = sizeof(float) * NV * WPR * 32 * kBv;
   const int mode = P.a.dh ? mode_of(P.a.f, P.vec, P.wvec) : kBnAny;
   auto kern = mode == kBnGated ? block_norm_bwd_kernel<IT, NV, WPR, kBnGated>
               : mode == kBnPlain ? block_norm_bwd_kernel<IT, NV, WPR, kBnPlain> : block_norm_bwd_kernel<IT, NV, WPR, kBnAny>;
+  const size_t smem = sizeof(float) * NV * WPR * 32 * kBv +  // column sums; the next row's vectors
+                      (mode == kBnAny ? 0 : (sizeof(IT) == 2 ? 2 : 1) * (mode == kBnGated ? 5 : 4) * NV * sizeof(typename BnVec<IT>::T) * 32 * kBnWarps);
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), smem + 256);  // and the static part
   if (e != cudaSuccess) return e;
   kern<<<(unsigned)bwd_ctas(P.a.f.rows, WPR), 32 * kBnWarps, smem, st>>>(P);

@@ -19,9 +19,9 @@
 // rows: their weights are loaded once, with the first row, and in the backward their two sums stay in
 // registers over the rows of a persistent CTA; the CTAs' sums meet in a second small kernel (4 us) in a fixed
 // order, so the gradients of the weights do not vary between runs.
-// Measured: 16384 rows of 768, bf16, gated: forward 28 us (126 MB, 4.4 TB/s, 68 % of the copy rate), backward
-// 65 us (201 MB, 3.1 TB/s, 47 %: at two CTAs an SM the loads under way are too few); 4099 rows of 2560, fp32:
-// forward 33 us (168 MB, 5.1 TB/s), backward 51 us (252 MB, 4.9 TB/s).
+// Measured: 16384 rows of 768, bf16, gated: forward 27 us (126 MB, 4.7 TB/s, 72 % of the copy rate), backward
+// 43 us (201 MB, 4.6 TB/s, 71 %; 65 us with each row loaded when its turn comes); 4099 rows of 2560, fp32:
+// forward 32 us (168 MB, 5.3 TB/s), backward 45 us (252 MB, 5.6 TB/s; 51 us).
 #pragma once
 #include "ss_norm.cuh"
 
@@ -126,6 +126,15 @@ __device__ __forceinline__ void bn_load(typename BnVec<IT>::T (&q)[NV], const IT
   }
 }
 
+// asynchronous copy of a vector into shared memory, zeros where `on` is false
+template <typename V>
+__device__ __forceinline__ void bn_fetch(V* to, const void* from, bool on) {
+  if constexpr (sizeof(V) == 8)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(on ? 8 : 0) : "memory");
+  else
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+
 template <typename IT>
 __device__ __forceinline__ void bn_store(IT* row, int e0, const float (&v)[kBv], int dim, bool vec) {
   using V = typename BnVec<IT>::T;
@@ -152,7 +161,7 @@ __device__ __forceinline__ void unpack(float (&v)[kBv], const typename BnVec<IT>
 
 // MODE: 0 any call; 1 both norms, whole vectors (and dh in the backward), no gate; 2 the same with a SiLU
 // gate.  The common calls know at compile time what the others branch on for every vector (16384 rows of 768
-// with a gate, bf16: forward 45 -> 28 us, backward 100 -> 65 us).
+// with a gate, bf16: forward 45 -> 28 us, backward 100 -> 65 us, and 43 with the rows fetched ahead).
 enum { kBnAny = 0, kBnPlain = 1, kBnGated = 2 };
 
 template <typename IT, int NV, int WPR, int MODE>
@@ -256,24 +265,68 @@ __global__ void __launch_bounds__(32 * kBnWarps, 2)
 #pragma unroll
     for (int k = 0; k < kBv; ++k) w[j][k] *= sc[k], sx[j][k] = sp[j][k] = 0.f;
   }
-  for (int64_t row = (int64_t)blockIdx.x * RPC + wid / WPR; row < a.rows; row += (int64_t)gridDim.x * RPC) {
+  // The common calls fetch the next row while this one is computed: a thread's own vectors, into its own room.
+  // 16-bit rows have two rooms and are read again for each use (63 us with one room, from registers that spill);
+  // fp32 rows, with room for one, move into registers
+  constexpr bool kRooms = MODE != 0 && sizeof(IT) == 2;
+  constexpr int kTensors = MODE == kBnGated ? 5 : 4;
+  V* room = reinterpret_cast<V*>(sums + NV * WPR * 32 * kBv) + threadIdx.x;
+  V *here = room, *there = room + (kRooms ? kTensors * NV * 32 * kBnWarps : 0);
+  auto slot = [&](V* in, int t, int j) { return in + (t * NV + j) * 32 * kBnWarps; };
+  auto fetch = [&](V* in, int64_t row) {
+    auto one = [&](int t, const void* p, int64_t stride) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int e0 = bn_at<WPR>(j, part, lane);
+        bn_fetch(slot(in, t, j), (const IT*)p + row * stride + (e0 < dim ? e0 : 0), e0 < dim);
+      }
+    };
+    if (row < a.rows) {
+      one(0, a.y, a.y_row_stride);
+      one(1, a.residual, a.residual_row_stride);
+      one(2, g.dx, g.dx_row_stride);
+      one(3, g.dh, g.dh_row_stride);
+      if (gate) one(4, a.gate, a.gate_row_stride);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int64_t first = (int64_t)blockIdx.x * RPC + wid / WPR, hop = (int64_t)gridDim.x * RPC;
+  if constexpr (MODE != 0) fetch(here, first);
+  for (int64_t row = first; row < a.rows; row += hop) {
     V yq[NV], rq[NV], zq[NV], xq[NV], hq[NV];
-    bn_load<IT, NV, WPR>(yq, (const IT*)a.y + row * a.y_row_stride, dim, part, lane, vec);
-    bn_load<IT, NV, WPR>(rq, (const IT*)a.residual + row * a.residual_row_stride, dim, part, lane, vec);
-    if (gate) bn_load<IT, NV, WPR>(zq, (const IT*)a.gate + row * a.gate_row_stride, dim, part, lane, vec);
-    if (pre) bn_load<IT, NV, WPR>(xq, (const IT*)g.dx + row * g.dx_row_stride, dim, part, lane, vec);
-    if (has_dh) bn_load<IT, NV, WPR>(hq, (const IT*)g.dh + row * g.dh_row_stride, dim, part, lane, vec);
     const float2 rr = *reinterpret_cast<const float2*>(a.rstd + 2 * row);
+    if constexpr (kRooms) {
+      fetch(there, row + hop);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else if constexpr (MODE != 0) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        yq[j] = *slot(here, 0, j), rq[j] = *slot(here, 1, j), xq[j] = *slot(here, 2, j), hq[j] = *slot(here, 3, j);
+        if (gate) zq[j] = *slot(here, 4, j);
+      }
+      fetch(here, row + hop);
+    } else {
+      bn_load<IT, NV, WPR>(yq, (const IT*)a.y + row * a.y_row_stride, dim, part, lane, vec);
+      bn_load<IT, NV, WPR>(rq, (const IT*)a.residual + row * a.residual_row_stride, dim, part, lane, vec);
+      if (gate) bn_load<IT, NV, WPR>(zq, (const IT*)a.gate + row * a.gate_row_stride, dim, part, lane, vec);
+      if (pre) bn_load<IT, NV, WPR>(xq, (const IT*)g.dx + row * g.dx_row_stride, dim, part, lane, vec);
+      if (has_dh) bn_load<IT, NV, WPR>(hq, (const IT*)g.dh + row * g.dh_row_stride, dim, part, lane, vec);
+    }
     const float ry = rr.x, rh = rr.y;
+    auto take = [&](float (&v)[kBv], int t, const V& q, int j) {
+      if constexpr (kRooms) unpack<IT>(v, *slot(here, t, j));
+      else unpack<IT>(v, q);
+    };
     float h[NV][kBv];  // h, then u
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float y[kBv], z[kBv], d[kBv];
-      unpack<IT>(y, yq[j]);
-      unpack<IT>(h[j], rq[j]);
-      if (gate) unpack<IT>(z, zq[j]);
-      if (pre) unpack<IT>(d, xq[j]);
+      take(y, 0, yq[j], j);
+      take(h[j], 1, rq[j], j);
+      if (gate) take(z, 4, zq[j], j);
+      if (pre) take(d, 2, xq[j], j);
 #pragma unroll
       for (int k = 0; k < kBv; ++k) {
         float u = y[k] * ry * w[j][k];
@@ -291,10 +344,10 @@ __global__ void __launch_bounds__(32 * kBnWarps, 2)
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float y[kBv], z[kBv], d[kBv], gh[kBv], dz[kBv];
-      unpack<IT>(y, yq[j]);
-      if (gate) unpack<IT>(z, zq[j]);
-      if (pre) unpack<IT>(d, xq[j]);
-      if (has_dh) unpack<IT>(gh, hq[j]);
+      take(y, 0, yq[j], j);
+      if (gate) take(z, 4, zq[j], j);
+      if (pre) take(d, 2, xq[j], j);
+      if (has_dh) take(gh, 3, hq[j], j);
 #pragma unroll
       for (int k = 0; k < kBv; ++k) {
         if (!has_dh) gh[k] = 0.f;
@@ -320,11 +373,15 @@ __global__ void __launch_bounds__(32 * kBnWarps, 2)
     for (int j = 0; j < NV; ++j) {
       if (post) {
         float y[kBv];
-        unpack<IT>(y, yq[j]);
+        take(y, 0, yq[j], j);
 #pragma unroll
         for (int k = 0; k < kBv; ++k) h[j][k] = ry * (h[j][k] - y[k] * ry * m);
       }
       bn_store<IT>((IT*)g.dy + row * g.dy_row_stride, bn_at<WPR>(j, part, lane), h[j], dim, vec);
+    }
+    if constexpr (kRooms) {
+      V* t = here;
+      here = there, there = t;
     }
     if (WPR > 1 && !(post && pre)) asm volatile("bar.sync %0, %1;" ::"r"(1 + wid / WPR), "n"(32 * WPR) : "memory");
   }

@@ -214,7 +214,8 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, seq_
     their outputs and gradients are zero.  Returns o (batch, seqlen, heads, value_dim) in v's dtype,
     and with return_final_state the state after each row's last token, fp32.
 
-    float32, bfloat16 and float16; the state is fp32 throughout.  16-bit inputs run on the tensor cores; for
+    float32, bfloat16 and float16; the state is fp32 throughout.  Tokens are summed in chunks, so one that holds
+    an infinity or NaN reaches the outputs of up to 127 tokens before it.  16-bit inputs run on the tensor cores; for
     that, inputs whose rows are not whole 16-byte units (head sizes off a multiple of 8, odd strides) are
     copied first."""
     want = bool(return_final_state)

@@ -86,6 +86,15 @@ def test_many_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("gate", [True, False])
+@pytest.mark.parametrize("rows,dim", [(5003, 128), (5001, 260), (2500, 512), (1300, 1100), (1301, 1536), (700, 2048), (700, 2564),
+                                      (700, 4096), (650, 5000), (601, 8192)])
+def test_several_rows_a_warp(dtype, gate, rows, dim):
+    """Every kernel's row loop: the next row is fetched while one is computed, and the last has no next."""
+    run((rows, dim), dtype, gate=gate, seed=dim)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_strided_and_misaligned_rows(dtype):
     run((6, 96), dtype, seed=5, view=lambda v: torch.cat([v, v], -1)[:, :96])
     run((6, 96), dtype, seed=6, view=lambda v: torch.cat([v[:, :1], v], -1)[:, 1:])
