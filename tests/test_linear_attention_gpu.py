@@ -297,6 +297,79 @@ def test_only_the_final_state_is_used():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hk", [4, 2, 1])
+def test_gradients_without_the_decays(dtype, hk):
+    """A fixed decay (no gradient asked for), own and shared key heads, one leaf at a time."""
+    from mamba_b200 import linear_attention_fn
+
+    t = make(2, 150, 4, hk, 64, 64, dtype, state=True, seed=32 + hk)
+    all_of = [t[n].detach().requires_grad_() for n in ("q", "k", "v")]
+    together = torch.autograd.grad(linear_attention_fn(*all_of, t["g"], 0.3, t["s0"]), all_of, t["do"])
+    _, _, want = reference(t, 0.3, False)
+    _, _, mags = reference(t, 0.3, False, absolute=True)
+    soft = 2.0 ** -17 if dtype == torch.float32 else 2 * HALF[dtype] + 2.0 ** -17
+    for i, name in enumerate(("dq", "dk", "dv")):
+        close(name, together[i], want[i], mags[i], dtype, soft)
+        args = [x.requires_grad_(j == i) for j, x in enumerate(t[n].detach().clone() for n in ("q", "k", "v"))]
+        (alone,) = torch.autograd.grad(linear_attention_fn(*args, t["g"], 0.3, t["s0"]), [args[i]], t["do"])
+        assert torch.equal(alone, together[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_broadcast_output_gradients(dtype):
+    """The gradient of a sum (all strides zero) and of a sum over heads."""
+    from mamba_b200 import linear_attention_fn
+
+    t = make(2, 70, 4, 2, 32, 32, dtype, seed=36)
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g")]
+    o = linear_attention_fn(*leaves)
+    for do in (torch.ones((), device="cuda", dtype=dtype).expand_as(o), t["do"][:, :, :1].expand_as(o)):
+        a = torch.autograd.grad(o, leaves, do, retain_graph=True)
+        b = torch.autograd.grad(o, leaves, do.contiguous(), retain_graph=True)
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dk,dv,per_head", [(33, 57, False), (128, 100, True)])
+def test_rows_off_16_bytes_on_the_fp32_units(dtype, dk, dv, per_head):
+    """LinearAttentionFn takes its operands as they are: 16-bit rows that TMA cannot copy."""
+    from mamba_b200 import LinearAttentionFn
+
+    t = make(2, 150, 4, 2, dk, dv, dtype, per_head=per_head, state=True, lens=[150, 77], seed=37)
+    leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g", "s0")]
+    o, f = LinearAttentionFn.apply(*leaves[:4], 0.3, leaves[4], t["lens"], True)
+    grads = torch.autograd.grad([o, f], leaves, [t["do"], t["dF"]])
+    want_o, want_f, want = reference(t, 0.3, True)
+    mag_o, mag_f, mags = reference(t, 0.3, True, absolute=True)
+    close("o", o, want_o, mag_o, dtype, 2.0 ** -17)
+    close("final", f, want_f, mag_f, dtype, 2.0 ** -17)
+    for i, name in ((0, "dq"), (1, "dk"), (2, "dv"), (4, "dinitial_state")):
+        close(name, grads[i], want[i], mags[i], dtype, 2.0 ** -17)
+    close("dlog_decay", grads[3], want[3], decay_magnitude(t, 0.3, mags, mag_f, True), dtype, 2.0 ** -17)
+
+
+def test_offsets_beyond_32_bits():
+    """A cache of more than 2^31 state entries (8.7 GB): the last row steps and moves as it does alone."""
+    from mamba_b200 import linear_attention_step, reorder_states
+
+    b, h, d = 3302, 40, 128
+    state = torch.empty(b, h, d, d, device="cuda")
+    assert state.numel() > 2 ** 31
+    state[-2:] = torch.randn(2, h, d, d, device="cuda")
+    state[:-2] = 0.0
+    alone = state[-2:].clone()
+    q, k, v = (torch.randn(b, h, d, device="cuda") for _ in range(3))
+    g = -torch.rand(h, device="cuda")
+    o = linear_attention_step(state, q, k, v, g)
+    assert torch.equal(o[-2:], linear_attention_step(alone, q[-2:], k[-2:], v[-2:], g)) and torch.equal(state[-2:], alone)
+    reorder_states([state], torch.tensor([[1, 0]], device="cuda").expand(b // 2, 2).contiguous())
+    assert torch.equal(state[-2:], alone.flip(0))
+    del state
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_empty_calls(dtype):
     from mamba_b200 import linear_attention_fn
 
