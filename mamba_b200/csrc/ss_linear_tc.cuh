@@ -811,7 +811,8 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
     float h[kTcN];
     float* rows = reinterpret_cast<float*>(smem + S::kH) + (wid & 3) * 32 * kTcN;
     const int r0 = (wid & 3) * 32, rn = min(32, dk - r0);  // this warp's rows; <= 0: none
-    if (!STATE_ONLY && r0 < DK) {
+    const bool from = !STATE_ONLY && r0 < DK && (seg > 0 || A.s_in != nullptr);  // else from zeros
+    if (from) {
       // 8 loads under way at a time
       auto each = [&](auto&& f) {
 #pragma unroll 1
@@ -829,20 +830,18 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
           }
         }
       };
-      if (!STATE_ONLY && seg > 0) {  // folded from the initial state and the segments before
+      if (seg > 0) {  // folded from the initial state and the segments before
         const float* s0 = A.sum + ((int64_t)bh * K.segs + seg) * block + (int64_t)r0 * dv + n0;
         each([&](int r, int j) { return s0[(int64_t)r * dv + j]; });
       } else {
-        const float* s0 = STATE_ONLY || A.s_in == nullptr ? nullptr
-                          : A.s_in + bh * block + (int64_t)r0 * A.s_row + (int64_t)n0 * A.s_col;
-        each([&](int r, int j) { return s0 ? A.s_in_scale * s0[(int64_t)r * A.s_row + (int64_t)j * A.s_col] : 0.f; });
+        const float* s0 = A.s_in + bh * block + (int64_t)r0 * A.s_row + (int64_t)n0 * A.s_col;
+        each([&](int r, int j) { return A.s_in_scale * s0[(int64_t)r * A.s_row + (int64_t)j * A.s_col]; });
       }
       __syncwarp();
     }
 #pragma unroll
     for (int j = 0; j < kTcN; j += 4) {
-      const float4 x = !STATE_ONLY && r0 < DK ? *reinterpret_cast<const float4*>(rows + lane * kTcN + j)
-                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 x = from ? *reinterpret_cast<const float4*>(rows + lane * kTcN + j) : make_float4(0.f, 0.f, 0.f, 0.f);
       h[j] = x.x, h[j + 1] = x.y, h[j + 2] = x.z, h[j + 3] = x.w;
     }
     // the halves of one warp lie in the rows of others, and so may V's third part

@@ -92,7 +92,6 @@ def test_strided_logits():
     wide[..., 33:233] = logits
     check(wide.cuda()[..., 33:233], scores, 5)
     check(logits.cuda().transpose(0, 1).contiguous().transpose(0, 1), scores, 5)
-    assert True
 
 
 @pytest.mark.parametrize("w", [1, 2, 4, 5, 8, 16, 32])
