@@ -68,6 +68,8 @@ struct Work {
   Split simt, tc;
 };
 
+size_t dot_bytes(int io) { return io == SS_F32 ? sizeof(LinDot<float>) : sizeof(LinDot<__half>); }
+
 Work work_of(const ss_linear_args& a, int backward) {
   Work w;
   const int passes = backward ? 3 : 1;
@@ -86,7 +88,7 @@ Work work_of(const ss_linear_args& a, int backward) {
     w.seg_decay = take(sizeof(float) * 2 * bh * segs);
   }
   if (backward) {
-    w.dots = take(sizeof(float) * 2 * tiles_of(a.key_dim) * bh * a.seqlen);
+    w.dots = take(dot_bytes(a.io_dtype) * 2 * tiles_of(a.key_dim) * bh * a.seqlen);
     if (a.heads != a.key_heads) w.parts = take(sizeof(float) * 2 * bh * a.seqlen * a.key_dim);
   }
   return w;
@@ -310,7 +312,8 @@ int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
   const int rep = a.heads / a.key_heads;
   const int64_t bh = (int64_t)a.batch * a.heads, block = (int64_t)a.key_dim * a.value_dim;
   const int tq = tiles_of(a.key_dim);
-  float* dots = g->dlog_decay ? reinterpret_cast<float*>(base + w.dots) : nullptr;
+  char* dots = g->dlog_decay ? base + w.dots : nullptr;
+  const int64_t dots_of_one = (int64_t)dot_bytes(a.io_dtype) * tq * bh * a.seqlen;
   float* parts = w.parts >= 0 ? reinterpret_cast<float*>(base + w.parts) : nullptr;
   float* sums = w.sums >= 0 ? reinterpret_cast<float*>(base + w.sums) : nullptr;
   struct T {
@@ -341,7 +344,7 @@ int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
       A.o = out, A.ob = b, A.ol = l, A.oh = h;
     }
     if (dots) {
-      A.dot = dots + (int64_t)i * tq * bh * a.seqlen;
+      A.dot = reinterpret_cast<float*>(dots + i * dots_of_one);
       A.p = p.p, A.pb = p.b, A.pl = p.l, A.ph = p.h, A.rp = p.rep;
     }
   };
@@ -380,7 +383,7 @@ int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
   }
   if (g->dlog_decay) {
     LinDecayK D{};
-    D.xq = dots, D.yk = dots + (int64_t)tq * bh * a.seqlen, D.tq = D.tk = tq;
+    D.xq = dots, D.yk = dots + dots_of_one, D.tq = D.tk = tq;
     if (g->dstate_out) D.d_last = g->dstate_out, D.last = a.state_out;
     D.block = block;
     D.g = a.log_decay, D.dg = g->dlog_decay;
@@ -389,7 +392,9 @@ int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
     D.gb = a.decay_batch_stride, D.gl = a.decay_seq_stride, D.gh = a.decay_head_stride;
     D.lens = a.seq_lens;
     D.batch = a.batch, D.seqlen = a.seqlen, D.heads = a.heads;
-    linear_decay_grad_kernel<<<(unsigned)(D.per_head ? a.heads : bh), kLdThreads, 0, st>>>(D);
+    const unsigned ctas = (unsigned)(D.per_head ? a.heads : bh);
+    if (a.io_dtype == SS_F32) linear_decay_grad_kernel<LinDot<float>><<<ctas, kLdThreads, 0, st>>>(D);
+    else linear_decay_grad_kernel<LinDot<__half>><<<ctas, kLdThreads, 0, st>>>(D);
     e = cudaGetLastError();
   }
   return record_cuda_status(e);

@@ -40,13 +40,16 @@ struct LinPass {
   float* s_out;        // final state, nullable
   float s_out_scale;
   int s_row, s_col;
-  // dot[tile][b][h][t] = sum over the tile's output columns of p[.., t, ..] * o (before rounding)
+  // dot[tile][b][h][t] = sum over the tile's output columns of p[.., t, ..] * o (before rounding); for fp32 I/O
+  // these are doubles (LinDot), since the decays' gradient is what is left of them when they cancel
   const void* p;
   int64_t pb, pl, ph;
   int rp;
   float* dot;
   float* sum;          // segments' own states, then the states before them: [b * h][segment][dk * dv]; null for one segment
 };
+
+template <typename IT> using LinDot = typename std::conditional<sizeof(IT) == 4, double, float>::type;
 
 constexpr int kLinMaxPasses = 3;
 
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(kLsThreads, 128 / DMAX) linear_simt_kernel(con
         }
       }
       if (A.dot && tid < kLsC && c * kLsC + tid < P.seqlen)
-        A.dot[(((int64_t)tile * P.batch + b) * P.heads + head) * P.seqlen + c * kLsC + tid] = 0.f;
+        reinterpret_cast<LinDot<IT>*>(A.dot)[(((int64_t)tile * P.batch + b) * P.heads + head) * P.seqlen + c * kLsC + tid] = 0;
       continue;
     }
     const int t0 = first_token(c);
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(kLsThreads, 128 / DMAX) linear_simt_kernel(con
         for (int i = 0; i < 8; ++i) {
           const int t = t0 + ti + i;
           const bool on = ti + i < m;
-          float dot = 0.f;
+          LinDot<IT> dot = 0;
           if (t < P.seqlen) {
             const float4 x = *reinterpret_cast<const float4*>(&part[ti + i][tj]);
             const float xa[4] = {x.x, x.y, x.z, x.w};
@@ -311,14 +314,14 @@ __global__ void __launch_bounds__(kLsThreads, 128 / DMAX) linear_simt_kernel(con
               const IT* p = static_cast<const IT*>(A.p) + (int64_t)b * A.pb + (int64_t)t * A.pl + (int64_t)(head / A.rp) * A.ph + n0 + tj;
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                if (tj + j < nv) dot = fmaf(r[j], to_f<IT>(p[j]), dot);
+                if (tj + j < nv) dot += (LinDot<IT>)r[j] * (LinDot<IT>)to_f<IT>(p[j]);
             }
           }
           if (A.dot) {
 #pragma unroll
             for (int w = 8; w > 0; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
             if (tid % 16 == 0 && t < P.seqlen)
-              A.dot[(((int64_t)tile * P.batch + b) * P.heads + head) * P.seqlen + t] = dot;
+              reinterpret_cast<LinDot<IT>*>(A.dot)[(((int64_t)tile * P.batch + b) * P.heads + head) * P.seqlen + t] = dot;
           }
         }
       }
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(256) linear_group_sum_kernel(const __grid_cons
 // (b, h), 512 tokens a step; for a decay per head one CTA per head, which sums over its rows and tokens in a
 // fixed order.  Bound by the latency of its steps: 14 us for 192 rows of 2048 tokens (5 MB).
 struct LinDecayK {
-  const float *xq, *yk;  // [tile][b][h][t]
+  const void *xq, *yk;   // [tile][b][h][t], the kernel's T
   int tq, tk;            // tiles of each
   const float *d_last, *last;  // nullable (b, h, dk * dv)
   int64_t block;
@@ -464,9 +467,10 @@ struct LinDecayK {
 
 constexpr int kLdThreads = 512;
 
+template <typename T>
 __global__ void __launch_bounds__(kLdThreads) linear_decay_grad_kernel(const __grid_constant__ LinDecayK P) {
   __shared__ double part[kLdThreads / 32];
-  __shared__ float part_f[2][kLdThreads / 32];
+  __shared__ T part_t[2][kLdThreads / 32];
   __shared__ double carry_s;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int head = P.per_head ? blockIdx.x : blockIdx.x % P.heads;
@@ -499,37 +503,38 @@ __global__ void __launch_bounds__(kLdThreads) linear_decay_grad_kernel(const __g
     double carry = carry_s;
     // thread i holds token end - 1 - i, so a prefix over threads is a suffix over tokens; the next tokens'
     // loads are under way while these are summed
-    float xn = 0.f, gn = 0.f;
+    T xn = 0;
+    float gn = 0.f;
     auto load = [&](int end) {
       const int t = end - 1 - tid;
-      xn = gn = 0.f;
+      xn = 0, gn = 0.f;
       if (t < 0) return;
       const int64_t at = (int64_t)b * P.gb + (int64_t)t * P.gl + (int64_t)head * P.gh;
       if (P.g_f32) gn = static_cast<const float*>(P.g)[at];
       else if (P.g_bf16) gn = to_f<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(P.g)[at]);
       else gn = to_f<__half>(static_cast<const __half*>(P.g)[at]);
       if (t >= len) return;
-      float s = 0.f, r = 0.f;  // one or two tiles each
-      for (int i = 0; i < P.tq; ++i) s += P.xq[i * bhl + bh * P.seqlen + t];
-      for (int i = 0; i < P.tk; ++i) r += P.yk[i * bhl + bh * P.seqlen + t];
+      T s = 0, r = 0;  // one or two tiles each
+      for (int i = 0; i < P.tq; ++i) s += static_cast<const T*>(P.xq)[i * bhl + bh * P.seqlen + t];
+      for (int i = 0; i < P.tk; ++i) r += static_cast<const T*>(P.yk)[i * bhl + bh * P.seqlen + t];
       xn = s - r;
     };
     load(P.seqlen);
     for (int end = P.seqlen; end > 0; end -= kLdThreads) {
       const int t = end - 1 - tid;
       const float g = gn;
-      float d = xn;  // a step's 512 tokens in fp32, the steps in 64 bits
+      T d = xn;  // a step's 512 tokens in T, the steps in 64 bits
       load(end - kLdThreads);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const float u = __shfl_up_sync(0xffffffffu, d, o);
+        const T u = __shfl_up_sync(0xffffffffu, d, o);
         if (lane >= o) d += u;
       }
       const int slot = (end / kLdThreads) & 1;
-      if (lane == 31) part_f[slot][wid] = d;
+      if (lane == 31) part_t[slot][wid] = d;
       __syncthreads();
-      const float w = lane < kLdThreads / 32 ? part_f[slot][lane] : 0.f;
-      float before = lane < wid ? w : 0.f, all = w;
+      const T w = lane < kLdThreads / 32 ? part_t[slot][lane] : T(0);
+      T before = lane < wid ? w : T(0), all = w;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         before += __shfl_xor_sync(0xffffffffu, before, o);
