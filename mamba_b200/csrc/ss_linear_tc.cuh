@@ -23,9 +23,9 @@
 // What bounds it: neither memory nor the tensor cores, but the hand-overs between the roles.  A chunk with keys
 // of 64 takes about 2.3 us a CTA (a gradient: 4400 cycles, of them 4000 in the warps that make the outputs),
 // its products 1500 cycles; a load that was issued early arrives after 3000.  Measured:
-//   8 x 2048 tokens, 24 heads of 64 x 64, bf16       75 us forward (201 MB, 2.7 TB/s), 250 us backward
+//   8 x 2048 tokens, 24 heads of 64 x 64, bf16       76 us forward (201 MB, 2.6 TB/s), 247 us backward
 //   1 x 16384 tokens, 16 heads of 128 x 128, bf16    151 us forward (268 MB, 1.8 TB/s), 168 with the final state
-//   4 x 1999 tokens, 16 heads, 4 of keys, fp16       95 us forward, 313 us backward
+//   4 x 1999 tokens, 16 heads, 4 of keys, fp16       91 us forward, 308 us backward
 // Tried and slower: the outputs of gradients shared with the scores' warps (273 against 250 us: a chunk's scores
 // then wait for the outputs before them), 32 columns of outputs at a time (295 us: it spills).
 // Two value tiles of one head run side by side, so keys and queries come from L2 the second time.
