@@ -302,7 +302,11 @@ int ss_linear_bwd(const ss_linear_bwd_args* g, void* stream) {
   const ss_linear_args& a = g->f;
   const int rc = check_fwd(a);
   if (rc != SS_OK) return rc;
-  if (a.batch == 0) return SS_OK;
+  if (a.batch == 0) {  // the one result that no rows leave something of: a decay per head, whose gradient is zero
+    if (!g->dlog_decay || a.decay_batch_stride || a.decay_seq_stride) return SS_OK;
+    const size_t es = a.decay_dtype == SS_F32 ? 4 : 2;
+    return record_cuda_status(cudaMemsetAsync(g->dlog_decay, 0, es * a.heads, (cudaStream_t)stream));
+  }
   if (a.seqlen > 0 && (!g->dout || !g->dq || !g->dk || !g->dv)) return SS_ERR_INVALID;
   if (g->dstate_out && g->dlog_decay && !a.state_out) return SS_ERR_INVALID;
   const Work w = work_of(a, 1);

@@ -538,3 +538,20 @@ def test_training_step_in_a_graph():
     graph.replay()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,l", [(0, 5), (2, 0)])
+def test_decays_of_heads_have_a_zero_gradient_without_tokens(dtype, b, l):
+    """No rows, or no tokens: the gradient of one decay per head is not empty, and is zero (exactly; the
+    allocator is left with NaN where the call finds its memory)."""
+    from mamba_b200 import linear_attention_fn
+
+    for decay_dtype in {torch.float32, dtype}:
+        t = make(b, l, 4, 2, 16, 16, dtype, per_head=True, state=True)
+        leaves = [t["g"].to(decay_dtype).requires_grad_(), t["s0"].requires_grad_()]
+        o, f = linear_attention_fn(t["q"], t["k"], t["v"], leaves[0], 0.5, leaves[1], None, True)
+        held = [torch.full((n,), float("nan"), device="cuda") for n in (1, 4, 64, 128, 256) for _ in range(8)]
+        del held
+        dg, ds = torch.autograd.grad([o, f], leaves, [t["do"], t["dF"]])
+        assert dg.dtype == decay_dtype and torch.equal(dg, torch.zeros_like(leaves[0])) and torch.equal(ds, t["dF"])
