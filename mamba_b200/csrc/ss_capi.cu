@@ -103,6 +103,14 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// The driver's call needs a current context, which a thread that has made no runtime call of its own yet does not
+// have (autograd's threads: without this, their first call found no tensor map and took a kernel that needs none)
+void bind_context() {
+  static thread_local bool bound = false;
+  int dev = 0;
+  if (!bound) bound = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+}
+
 CUtensorMapDataType tm_type(int dt) {
   return dt == SS_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                       : (dt == SS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
@@ -117,6 +125,7 @@ bool map3(CUtensorMap* m, const void* base, int dt, uint64_t d0, uint64_t d1, ui
   if (fn == nullptr || base == nullptr || (reinterpret_cast<uintptr_t>(base) & 15) || (s1 & 15) || (s2 & 15) ||
       ((b0 * es) & 15) || s1 >= (1ull << 40) || s2 >= (1ull << 40))
     return false;
+  bind_context();
   cuuint64_t dims[3] = {d0, d1, d2};
   cuuint64_t strides[2] = {s1, s2};
   cuuint32_t box[3] = {b0, b1, 1};
@@ -141,6 +150,7 @@ bool ssb::map_heads(CUtensorMap* m, const void* p, int dtype, int64_t dim, int64
     if (b <= 0 || (b & 15) || b >= (1ll << 40)) return false;
     strides[i] = (cuuint64_t)b;
   }
+  bind_context();
   cuuint32_t box[4] = {(cuuint32_t)(128 / es), 1, (cuuint32_t)rows, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   return fn(m, tm_type(dtype), 4, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,

@@ -555,3 +555,32 @@ def test_decays_of_heads_have_a_zero_gradient_without_tokens(dtype, b, l):
         del held
         dg, ds = torch.autograd.grad([o, f], leaves, [t["do"], t["dF"]])
         assert dg.dtype == decay_dtype and torch.equal(dg, torch.zeros_like(leaves[0])) and torch.equal(ds, t["dF"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_new_thread_runs_the_same_kernels(dtype):
+    """The first call that a thread makes (as autograd's do), every buffer at hand already: forward and backward
+    give the bits of any other call."""
+    import threading
+
+    from mamba_b200 import linear_attention_fn
+
+    t = make(1, 150, 2, 1, 64, 64, dtype, state=True, seed=41)
+    got = []
+
+    def once():
+        with torch.no_grad():
+            o, f = linear_attention_fn(t["q"], t["k"], t["v"], t["g"], None, t["s0"], None, True)
+        leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "g", "s0")]
+        out = linear_attention_fn(*leaves[:4], None, leaves[4], None, True)
+        got.append([o, f, *torch.autograd.grad(list(out), leaves, [t["do"], t["dF"]])])
+
+    once()
+    once()
+    torch.cuda.synchronize()
+    del got[0]  # its memory serves the next call
+    thread = threading.Thread(target=once)
+    thread.start()
+    thread.join()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
