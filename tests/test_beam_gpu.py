@@ -150,3 +150,21 @@ def test_selection_and_reordering_in_a_graph():
     state.copy_(start)
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(state, after)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,w,vocab,k", [(1, 2, 50, 4), (2, 3, 6000, 32), (3, 2, 7, 9)])
+def test_candidates_that_are_equal_though_their_logits_are_not(dtype, b, w, vocab, k):
+    """Logits whose difference is lost beside the sum of exponentials, or beside the beam's score: such candidates
+    are equal in fp64, and go by index like any others."""
+    tiny = torch.rand(b, w, vocab, generator=torch.Generator().manual_seed(vocab)) * 1e-20
+    if dtype != torch.float16:  # whose smallest number is 6e-8
+        check(tiny.to(dtype), -torch.arange(1.0, w + 1).expand(b, w), k)
+        tiny[..., 3] = 1.0
+        check(tiny.to(dtype), -torch.arange(1.0, w + 1).expand(b, w), k)
+    logits, _ = make(b, w, vocab, dtype, 9)
+    for low in (-3e38, -1e30, 1e25):
+        check(logits, torch.full((b, w), low), k)
+        scores = torch.full((b, w), low)
+        scores[:, 0] = -4.0
+        check(logits, scores, k)
