@@ -220,14 +220,17 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, seq_
     copied first."""
     want = bool(return_final_state)
     cut = None
-    if v.dtype in (torch.bfloat16, torch.float16) and v.is_cuda and v.dim() == 4 and v.numel():
-        dk, dv = k.shape[-1], v.shape[-1]
-        if (dk % 8 or dv % 8) and q.shape == k.shape and min(dk, dv) > 0:
-            scale = _scale(scale, dk)
-            cut = dk, dv
-            if initial_state is not None and tuple(initial_state.shape) == (v.shape[0], v.shape[2], dk, dv):
-                initial_state = torch.nn.functional.pad(initial_state, (0, -dv % 8, 0, -dk % 8))
-        q, k, v = _whole(_as(q, v.dtype)), _whole(_as(k, v.dtype)), _whole(v)
+    if v.dtype in (torch.bfloat16, torch.float16):
+        _cuda_device(q, k, v, log_decay, initial_state, seq_lens)
+        h, _, dk, dv = _check_heads(q, k, v, 4)  # of what the caller passed, not of the padded copies
+        if v.numel():
+            if dk % 8 or dv % 8:
+                scale = _scale(scale, dk)
+                cut = dk, dv
+                if initial_state is not None:
+                    _check_state(initial_state, (v.shape[0], h, dk, dv), "initial_state")
+                    initial_state = torch.nn.functional.pad(initial_state, (0, -dv % 8, 0, -dk % 8))
+            q, k, v = _whole(_as(q, v.dtype)), _whole(_as(k, v.dtype)), _whole(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
                                     or (initial_state is not None and initial_state.requires_grad)):
         out = LinearAttentionFn.apply(q, k, v, log_decay, scale, initial_state, seq_lens, want)

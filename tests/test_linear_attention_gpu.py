@@ -584,3 +584,15 @@ def test_a_new_thread_runs_the_same_kernels(dtype):
     thread.join()
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dq,dk,dv,state", [(60, 64, 64, None), (33, 40, 57, None), (33, 33, 57, (40, 64)), (64, 64, 57, (64, 64))])
+def test_shapes_that_padding_would_hide(dtype, dq, dk, dv, state):
+    """Operands and states of another size than their counterparts', equal to it in multiples of 8, are refused."""
+    from mamba_b200 import linear_attention_fn
+
+    z = lambda d: torch.zeros(1, 20, 2, d, dtype=dtype, device="cuda")  # noqa: E731
+    s = None if state is None else torch.zeros(1, 2, *state, device="cuda")
+    with pytest.raises(ValueError):
+        linear_attention_fn(z(dq), z(dk), z(dv), torch.zeros(2, device="cuda"), initial_state=s, return_final_state=True)

@@ -178,3 +178,26 @@ def test_workspace_sizes():
     a = _linear_args(batch=64, heads=8, key_heads=4)
     assert lib.ss_linear_work_bytes(ctypes.byref(a), 0) == 0
     assert lib.ss_linear_work_bytes(ctypes.byref(a), 1) >= 2 * 64 * 8 * 300 * 4 * (1 + 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q,k,v,state", [((1, 5, 2, 60), (1, 5, 2, 64), (1, 5, 2, 64), None),
+                                         ((1, 5, 2, 33), (1, 5, 2, 40), (1, 5, 2, 57), None),
+                                         ((1, 5, 2, 33), (1, 5, 2, 33), (1, 5, 2, 57), (1, 2, 40, 64)),
+                                         ((1, 5, 2, 64), (1, 5, 2, 64), (1, 5, 2, 57), (1, 2, 64, 64)),
+                                         ((1, 5, 2, 33), (1, 5, 2, 33), (1, 5, 2, 57), (1, 2, 33, 64)),
+                                         ((1, 4, 2, 33), (1, 4, 2, 33), (1, 5, 2, 57), None),
+                                         ((1, 5, 3, 33), (1, 5, 3, 33), (1, 5, 2, 57), None),
+                                         ((1, 5, 2, 33), (1, 5, 2, 33), (1, 5, 57), None)])
+def test_shapes_that_padding_would_hide(on_cpu, dtype, q, k, v, state):
+    """Head sizes that come to the same multiple of 8: refused by the sizes that were passed, in every type."""
+    q, k, v = (torch.zeros(*s, dtype=dtype) for s in (q, k, v))
+    with pytest.raises(ValueError):
+        mamba_b200.linear_attention_fn(q, k, v, torch.zeros(2), initial_state=None if state is None else torch.zeros(*state))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_limits_of_head_sizes_name_what_was_passed(on_cpu, dtype):
+    q, v = torch.zeros(1, 5, 2, 130, dtype=dtype), torch.zeros(1, 5, 2, 16, dtype=dtype)
+    with pytest.raises(NotImplementedError, match="130"):
+        mamba_b200.linear_attention_fn(q, q, v, torch.zeros(2))
