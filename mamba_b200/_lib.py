@@ -12,6 +12,7 @@ import struct
 import threading
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libmamba_b200_ss.so")
@@ -373,6 +374,12 @@ def launch(name: str, packed: bytes, device: torch.device) -> None:
             rc = f(packed, stream_of(device))
     if rc:
         check(rc, name)
+
+
+def differentiated(tensors) -> bool:
+    """Whether a call goes through its autograd function: where a tensor wants a gradient, and inside a level of
+    forward-mode differentiation, which the function refuses (passed by, it would leave a derivative of zero)."""
+    return _forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
 def written(tensors) -> None:

@@ -231,8 +231,7 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, seq_
                     _check_state(initial_state, (v.shape[0], h, dk, dv), "initial_state")
                     initial_state = torch.nn.functional.pad(initial_state, (0, -dv % 8, 0, -dk % 8))
             q, k, v = _whole(_as(q, v.dtype)), _whole(_as(k, v.dtype)), _whole(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
-                                    or (initial_state is not None and initial_state.requires_grad)):
+    if L.differentiated((q, k, v, log_decay, initial_state)):
         out = LinearAttentionFn.apply(q, k, v, log_decay, scale, initial_state, seq_lens, want)
         o, final = out if want else (out, None)
     else:

@@ -232,7 +232,7 @@ def block_norm_fn(y, residual, post_weight=None, pre_weight=None, gate=None, res
     call = (L.dtype_code(y.dtype), _ACTIVATIONS[activation], float(eps), float(eps if pre_eps is None else pre_eps),
             int(bool(unit_offset)), const)
     tensors = y, residual, post_weight, pre_weight, gate, scale
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if L.differentiated(tensors):
         return BlockNormFn.apply(*tensors, call)
     x, h, *_ = _block_forward(*tensors, call, False)
     return h if x is None else (x, h)

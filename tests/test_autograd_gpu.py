@@ -87,3 +87,34 @@ def test_mixed_input_dtypes_get_gradients_of_their_own_dtype():
         if t[k] is not None:
             got["d" + k] = t[k].grad.float() if k in ("A", "delta") else t[k].grad
     compare(got, oracle_case(ref_in), torch.bfloat16)
+
+
+def _forward_mode_calls():
+    import mamba_b200 as M
+
+    r = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    q, k, v, g, s0 = r(1, 20, 2, 16), r(1, 20, 2, 16), r(1, 20, 2, 16), -r(1, 20, 2).abs(), r(1, 2, 16, 16)
+    y, res, w = r(3, 16), r(3, 16), r(16)
+    linear = lambda *t: M.linear_attention_fn(*t[:4], initial_state=t[4], return_final_state=True)  # noqa: E731
+    norm = lambda *t: M.block_norm_fn(t[0], t[1], t[2], t[3], gate=t[4], residual_scale=t[5])  # noqa: E731
+    return [(linear, [q, k, v, g, s0]), (linear, [t.bfloat16() for t in (q, k, v, g)] + [s0]),
+            (norm, [y, res, w, w.clone(), r(3, 16), r(16)])]
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_derivatives_are_refused(grad_mode):
+    """The sequence operators have no forward-mode derivative: a tangent on any operand raises, where an output
+    without one would be a derivative of zero.  Inside a level without tangents, and after it, calls run."""
+    import torch.autograd.forward_ad as forward_ad
+
+    for f, tensors in _forward_mode_calls():
+        want = f(*tensors)
+        for i in range(len(tensors)):
+            with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(tensors)]
+                with pytest.raises((NotImplementedError, RuntimeError), match="forward|jvp"):
+                    f(*dual)
+        with forward_ad.dual_level():
+            got = f(*tensors)
+        for a, b, c in zip(want, got, f(*tensors)):
+            assert torch.equal(a, b) and torch.equal(a, c) and not c.requires_grad

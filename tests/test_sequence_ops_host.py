@@ -201,3 +201,15 @@ def test_limits_of_head_sizes_name_what_was_passed(on_cpu, dtype):
     q, v = torch.zeros(1, 5, 2, 130, dtype=dtype), torch.zeros(1, 5, 2, 16, dtype=dtype)
     with pytest.raises(NotImplementedError, match="130"):
         mamba_b200.linear_attention_fn(q, q, v, torch.zeros(2))
+
+
+def test_what_goes_through_the_autograd_functions():
+    import torch.autograd.forward_ad as forward_ad
+
+    plain, leaf = torch.zeros(2), torch.zeros(2).requires_grad_()
+    assert not L.differentiated((plain, None)) and L.differentiated((None, leaf))
+    with torch.no_grad():
+        assert not L.differentiated((leaf,))
+        with forward_ad.dual_level():
+            assert L.differentiated((plain,))
+    assert not L.differentiated((plain,))
