@@ -190,8 +190,9 @@ class LinearAttentionFn(torch.autograd.Function):
         t, c = _prepare(q, k, v, log_decay, scale, initial_state, seq_lens)
         o, final = _forward(t, c, want_final)
         ctx.set_materialize_grads(False)
-        # the final state is needed again for the decays' gradient through it
-        ctx.save_for_backward(*t, final)
+        # the final state is needed again for the decays' gradient through it; where that is not asked for, a caller
+        # may go on to step the state in place
+        ctx.save_for_backward(*t, final if ctx.needs_input_grad[3] else None)
         ctx.call = c
         ctx.dtypes = tuple(None if x is None else x.dtype for x in (q, k, v, log_decay, initial_state))
         return (o, final) if want_final else o

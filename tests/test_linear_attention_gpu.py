@@ -596,3 +596,23 @@ def test_shapes_that_padding_would_hide(dtype, dq, dk, dv, state):
     s = None if state is None else torch.zeros(1, 2, *state, device="cuda")
     with pytest.raises(ValueError):
         linear_attention_fn(z(dq), z(dk), z(dv), torch.zeros(2, device="cuda"), initial_state=s, return_final_state=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_state_that_no_backward_needs_can_be_stepped(dtype):
+    """With fixed decays no gradient reads the final state: it may be stepped in place before the backward, which
+    gives the same bits."""
+    from mamba_b200 import linear_attention_fn, linear_attention_step
+
+    t = make(1, 150, 2, 1, 16, 24, dtype, state=True, seed=42)
+
+    def once(step):
+        leaves = [t[n].detach().requires_grad_() for n in ("q", "k", "v", "s0")]
+        o, f = linear_attention_fn(*leaves[:3], t["g"], 0.3, leaves[3], None, True)
+        if step:
+            with torch.no_grad():
+                linear_attention_step(f, t["q"][:, 0], t["k"][:, 0], t["v"][:, 0], t["g"][:, 0])
+        return torch.autograd.grad([o, f], leaves, [t["do"], t["dF"]])
+
+    for a, b in zip(once(True), once(False)):
+        assert torch.equal(a, b)
