@@ -94,7 +94,8 @@ def reorder_states(states, parents):
         if at < end:
             raise ValueError("states must not share memory")
         end = at + n
-    p = parents if parents.stride(1) == 1 or w == 1 else parents.contiguous()
+    # rows of parents that share memory (one order for the whole batch) are laid out first
+    p = parents if (parents.stride(1) == 1 or w == 1) and (parents.stride(0) >= w or b <= 1) else parents.contiguous()
     L.written(states)
     for i in range(0, len(rows), L.MAX_REORDER):
         part = rows[i:i + L.MAX_REORDER]

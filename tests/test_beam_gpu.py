@@ -168,3 +168,17 @@ def test_candidates_that_are_equal_though_their_logits_are_not(dtype, b, w, voca
         scores = torch.full((b, w), low)
         scores[:, 0] = -4.0
         check(logits, scores, k)
+
+
+@pytest.mark.parametrize("b,w", [(3, 2), (4, 1), (1, 5)])
+def test_reorder_by_one_order_for_the_batch(b, w):
+    """Parents expanded over the batch (a batch stride of 0), and overlapping rows of a wider tensor."""
+    from mamba_b200 import reorder_states
+
+    order = torch.arange(w - 1, -1, -1, device="cuda")
+    wide = torch.cat([order, order])
+    for p in (order.expand(b, w), torch.as_strided(wide, (b, w), (0, 1)), torch.as_strided(torch.zeros(b + w, dtype=torch.int64, device="cuda"), (b, w), (1, 1))):
+        s = torch.randn(b * w, 3, 5, device="cuda")
+        want = s.view(b, w, 3, 5)[torch.arange(b, device="cuda")[:, None], p].flatten(0, 1)
+        reorder_states([s], p)
+        assert torch.equal(s, want)
