@@ -104,36 +104,44 @@ def mamba_simple_step(block, hidden, conv_state, ssm_state, params: _BlockParams
 
 
 class _MambaLayer:
-    """A MambaSimple mixer and its states for a batch."""
+    """A decoder's MambaSimple layer: its mixer, and where its parameters and states stand in the decoder's lists."""
 
-    def __init__(self, mixer, batch, dev):
-        self.mixer, self.params = mixer, _BlockParams(mixer)
-        p = self.params
-        self.states = [torch.zeros(batch, p.d, p.K - 1, device=dev), torch.zeros(batch, p.d, p.n, device=dev)]
+    def __init__(self, mixer, dec, dev):
+        self.mixer, self.at = mixer, len(dec.params)
+        p = _BlockParams(mixer)
+        dec.params.append(p)
+        dec.conv_states.append(torch.zeros(dec.batch, p.d, p.K - 1, device=dev))
+        dec.ssm_states.append(torch.zeros(dec.batch, p.d, p.n, device=dev))
 
-    def prefill(self, x):
-        y, *states = mamba_simple_prefill(self.mixer, x, self.params)
+    def states(self, dec):
+        return dec.conv_states[self.at], dec.ssm_states[self.at]
+
+    def prefill(self, dec, x):
+        y, *states = mamba_simple_prefill(self.mixer, x, dec.params[self.at])
         return y, states
 
-    def step(self, x):
-        return mamba_simple_step(self.mixer, x, *self.states, self.params)
+    def step(self, dec, x):
+        return mamba_simple_step(self.mixer, x, *self.states(dec), dec.params[self.at])
 
 
 class _LinearLayer:
-    """A linear-attention mixer and its state for a batch."""
+    """A decoder's linear-attention layer: its mixer, and where its state stands in the decoder's list."""
 
-    def __init__(self, mixer, batch, dev):
-        self.mixer = mixer
+    def __init__(self, mixer, dec, dev):
+        self.mixer, self.at = mixer, len(dec.linear_states)
         heads, key_heads = mixer.num_heads, mixer.num_key_heads
-        self.states = [torch.zeros(batch, heads, mixer.k_proj.weight.shape[0] // key_heads,
-                                   mixer.v_proj.weight.shape[0] // heads, device=dev)]
+        dec.linear_states.append(torch.zeros(dec.batch, heads, mixer.k_proj.weight.shape[0] // key_heads,
+                                             mixer.v_proj.weight.shape[0] // heads, device=dev))
 
-    def prefill(self, x):
+    def states(self, dec):
+        return (dec.linear_states[self.at],)
+
+    def prefill(self, dec, x):
         y, state = linear_attention_prefill(self.mixer, x)
         return y, [state]
 
-    def step(self, x):
-        return linear_attention_block_step(self.mixer, x, *self.states)
+    def step(self, dec, x):
+        return linear_attention_block_step(self.mixer, x, *self.states(dec))
 
 
 class Decoder:
@@ -148,12 +156,14 @@ class Decoder:
         self.model = model
         self.batch = batch
         dev = model.lm_head.weight.device
-        self.mixers = [_LinearLayer(layer.linear_attn, batch, dev) if getattr(layer, "linear_attn", None) is not None
-                       else _MambaLayer(layer.mamba, batch, dev) for layer in model.layers]
-        self.states = [s for m in self.mixers for s in m.states]
+        # per layer of its kind: MambaSimple parameters and states, linear-attention states.  The lists may be
+        # assigned to, or an item replaced, until the step is captured
+        self.params, self.conv_states, self.ssm_states, self.linear_states = [], [], [], []
+        self.mixers = [_LinearLayer(layer.linear_attn, self, dev) if getattr(layer, "linear_attn", None) is not None
+                       else _MambaLayer(layer.mamba, self, dev) for layer in model.layers]
         # fp32 norm weights, cast once (a per-call cast would be one more kernel per layer and step)
         norms = [layer.norm for layer in model.layers] + [model.norm]
-        self.norms = [(n.weight.detach().float().contiguous(), n.eps) for n in norms]
+        *self.norms, self.final_norm = [(n.weight.detach().float().contiguous(), n.eps) for n in norms]
         self.parts = [self._cast(branch_parts(layer, n)) for layer, n in zip(model.layers, norms[1:])]
         self.cuda_graph = cuda_graph
         self.graph = None
@@ -164,14 +174,10 @@ class Decoder:
     def _cast(parts):
         return parts and tuple(t.detach().float().contiguous() if isinstance(t, torch.Tensor) else t for t in parts)
 
-    # the per-layer states of MambaSimple layers, as lists over the layers
     @property
-    def conv_states(self):
-        return [m.states[0] for m in self.mixers if isinstance(m, _MambaLayer)]
-
-    @property
-    def ssm_states(self):
-        return [m.states[1] for m in self.mixers if isinstance(m, _MambaLayer)]
+    def states(self):
+        """The states of all layers, in the layers' order."""
+        return [s for m in self.mixers for s in m.states(self)]
 
     @torch.no_grad()
     def prefill(self, input_ids, repeat: int = 1):
@@ -181,8 +187,8 @@ class Decoder:
             raise ValueError(f"batch {input_ids.shape[0]} x {repeat} != decoder batch {self.batch}")
 
         def mixer(m, x):
-            y, states = m.prefill(x)
-            for own, new in zip(m.states, states):
+            y, states = m.prefill(self, x)
+            for own, new in zip(m.states(self), states):
                 own.unflatten(0, (-1, repeat)).copy_(new[:, None])
             return y
 
@@ -190,14 +196,15 @@ class Decoder:
 
     def _run(self, h, mixer):
         """Logits from embeddings (batch, [L,] d_model): the last position's where there are several."""
-        w, eps = self.norms[0]
+        norms = [*self.norms, self.final_norm]
+        w, eps = norms[0]
         x, res = rms_norm_fn(h, w, None, eps, True, True)
         last = len(self.mixers) - 1
         for i, m in enumerate(self.mixers):
             y = mixer(m, x)
             if i == last and y.dim() == 3:
                 x, y, res = x[:, -1], y[:, -1], res[:, -1]
-            w, eps = self.norms[i + 1]
+            w, eps = norms[i + 1]
             if i == last and self.parts[i] is None:
                 x = rms_norm_fn(y, w, res, eps)
             else:  # the residual add of this block fused with the next norm
@@ -205,7 +212,7 @@ class Decoder:
         return self.model.lm_head(x).float()
 
     def _step_eager(self, tok):
-        return self._run(self.model.embedding(tok), lambda m, x: m.step(x))
+        return self._run(self.model.embedding(tok), lambda m, x: m.step(self, x))
 
     def reorder(self, parents):
         """parents (batch / beams, beams) int64: row w of a prompt's beams becomes what row parents[:, w] was."""

@@ -171,3 +171,36 @@ def test_fused_mixer_step_matches_separate_kernels(dtype, batch, dm, N):
         assert torch.equal(cs1, cs2), t
         assert_close(f"ssm state {t}", ss1, ss2, rtol, atol)
         assert_close(f"y {t}", y1, y2, rtol, max(atol, rtol * float(y2.abs().max())))
+
+
+def test_a_decoders_lists_hold_its_parameters_and_states():
+    """params, norms, final_norm, conv_states and ssm_states are the decoder's own lists: an item that is replaced, or
+    a list that is assigned, is what the next eager step reads and updates, and what a capture then holds."""
+    from mamba_b200 import Decoder
+
+    m = _model(torch.float32)
+    ids = torch.randint(0, 97, (2, 20), generator=torch.Generator().manual_seed(11)).cuda()
+    tok = ids[:, 0].contiguous()
+
+    def prompted(graph):
+        dec = Decoder(m, 2, cuda_graph=graph)
+        dec.prefill(ids)
+        return dec
+
+    plain = prompted(False)
+    want = [plain.step(tok), plain.step(tok)]
+    assert len(plain.params) == len(plain.norms) == len(plain.conv_states) == len(plain.ssm_states) == 3
+    assert torch.equal(plain.final_norm[0], m.norm.weight.float()) and plain.final_norm[1] == m.norm.eps
+    assert plain.params[1].blk is m.layers[1].mamba and plain.norms[2][1] == m.layers[2].norm.eps
+    for graph in (False, True):
+        dec = prompted(graph)
+        old = dec.conv_states + dec.ssm_states
+        before = [t.clone() for t in old]
+        dec.conv_states = [t.clone() for t in dec.conv_states]
+        for i in range(3):
+            dec.ssm_states[i] = dec.ssm_states[i].clone()
+        for w in want:
+            assert torch.equal(dec.step(tok), w)
+        assert all(torch.equal(a, b) for a, b in zip(old, before))  # the replaced ones are not stepped
+        assert all(torch.equal(a, b) for a, b in zip(dec.conv_states + dec.ssm_states, plain.conv_states + plain.ssm_states))
+        assert all(any(a is b for b in dec.states) for a in dec.conv_states + dec.ssm_states) and len(dec.states) == 6
