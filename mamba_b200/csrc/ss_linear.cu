@@ -187,8 +187,10 @@ cudaError_t launch_all(LinTcK& T, int passes, int grads, cudaStream_t st) {
   return e;
 }
 
-bool vec16(const void* p, int es, int64_t b, int64_t l, int64_t h) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((b * es) & 15) == 0 && ((l * es) & 15) == 0 && ((h * es) & 15) == 0;
+// rows of whole 16-byte units; the stride of an axis of one element is never stepped along, here as in map_heads
+bool vec16(const LinK& P, const void* p, int heads, int es, int64_t b, int64_t l, int64_t h) {
+  auto whole = [&](int n, int64_t stride) { return n <= 1 || ((stride * es) & 15) == 0; };
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && whole(P.batch, b) && whole(P.seqlen, l) && whole(heads, h);
 }
 
 // The tensor-core kernel takes every 16-bit call whose rows are whole 16-byte units (TMA loads, vector
@@ -198,8 +200,8 @@ bool run_tc(int io, const LinK& P, int passes, cudaStream_t st, cudaError_t* e) 
   int grads = 0;
   for (int i = 0; i < passes; ++i) {
     const LinPass& A = P.pass[i];
-    if (A.dk % 8 || A.dv % 8 || !vec16(A.o, A.o_f32 ? 4 : 2, A.ob, A.ol, A.oh) ||
-        (A.dot && !vec16(A.p, 2, A.pb, A.pl, A.ph)))
+    if (A.dk % 8 || A.dv % 8 || !vec16(P, A.o, P.heads, A.o_f32 ? 4 : 2, A.ob, A.ol, A.oh) ||
+        (A.dot && !vec16(P, A.p, P.heads / A.rp, 2, A.pb, A.pl, A.ph)))
       return false;
     const struct {
       const void* p;

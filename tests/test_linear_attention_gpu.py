@@ -616,3 +616,24 @@ def test_a_state_that_no_backward_needs_can_be_stepped(dtype):
 
     for a, b in zip(once(True), once(False)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,l,h,hk", [(1, 150, 2, 1), (1, 1, 2, 2), (2, 150, 1, 1), (1, 1, 1, 1)])
+def test_strides_of_axes_of_one_do_not_matter(dtype, b, l, h, hk):
+    """The stride of an axis of one element is never stepped along: whatever it is, forward and backward run the same
+    kernels, and give the bits of the contiguous call."""
+    from mamba_b200 import linear_attention_fn
+
+    t = make(b, l, h, hk, 64, 64, dtype, seed=43)
+
+    def odd(x):
+        return torch.as_strided(x, x.shape, [7 if n == 1 else s for n, s in zip(x.shape[:-1], x.stride())] + [1])
+
+    def once(view):
+        leaves = [view(t[n]).detach().requires_grad_() for n in ("q", "k", "v")] + [t["g"].detach().requires_grad_()]
+        o = linear_attention_fn(*leaves)
+        return [o, *torch.autograd.grad(o, leaves, t["do"])]
+
+    for x, y in zip(once(odd), once(lambda x: x)):
+        assert torch.equal(x, y)
