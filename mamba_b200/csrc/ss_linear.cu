@@ -142,7 +142,7 @@ template <typename IT, int MODE>
 cudaError_t launch_tc(LinTcK& T, int pass0, int n, bool early, cudaStream_t st) {
   constexpr size_t most = std::max(TcShape<64>::kBytes, TcShape<128>::kBytes);
   static_assert(most <= 232448, "shared memory of a CTA");
-  static_assert(sizeof(TcBars) <= 512, "barriers");
+  static_assert(sizeof(TcBars) <= kBarBytes, "barriers");
   auto kern = linear_tc_kernel<IT, MODE>;
   const cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), most);
   if (e != cudaSuccess) return e;

@@ -38,9 +38,28 @@ namespace ssb {
 
 constexpr int kTcC = 128;   // tokens of a chunk
 constexpr int kTcN = 64;    // value columns of a CTA
-// log decays below this are a reset: e^-128 times anything of 16 bits is zero in fp32, and sums that hold
-// it keep a score's digits (2^-16 of a step at the first reset, more only behind a dozen in one chunk)
-constexpr float kTcReset = -128.f;
+// log decays below this are a reset: e^-88 lies below fp32's normal numbers, and ex2 flushes it to zero
+constexpr float kTcReset = -88.f;
+// The decays of a stage's chunk, from sums in 64 bits.  Sums of log decays grow with the chunk, and their
+// differences, which the weights are made of, keep only the digits that fp32 leaves them; and where the forward
+// and the reverse run are left other digits, a score next to a rounding border rounds apart, and the decays'
+// gradient, a difference of the two runs, keeps that.  So blocks of 32 tokens count for themselves, and both runs
+// form a pair's weight from the same numbers.  With z the sum from a token's block's start to it, t the block's sum
+// and s = t - z what follows the token in it (all times log2 e):
+//   X        [128]  -z, reverse z: the weight of a pair in one block is 2^{X_col - X_row}, the same bits either way
+//   factor   [128]  2^s, reverse 2^z: of a column towards the border of its block on the side of the rows that use it
+//   border   [4][4] row block w, column block x: E = 2^(sums of the blocks between them); a pair's weight is
+//                   (2^z E) 2^s, reverse (2^s E) 2^z: the same bits for neighbours, whose E is 1.  On the diagonal
+//                   the sum of the blocks before w (reverse: behind), which with z (s) is an output's.  Reverse
+//                   keeps t of block w in the unused half, at dec_own(w)
+//   update   [4]    what a block's factors are multiplied with to weight the update of the state
+//   rest     [128]  s - (t - z) in fp32, 8 bits of it, in units that t gives: s where z alone is at hand
+// 32 resets in one block leave X half a step of 2^-13, 2^-12.5 of a weight at most: below half a step of fp16.
+// Against one fp32 sum a token (1 % faster): the error of dlog_decay over 2600 tokens of log decays around -3, in
+// its norm per head, falls from 2.2e-2 to 3.1e-3 (bf16) and from 3.5e-3 to 3.3e-4 (fp16).
+constexpr int kDecFactor = kTcC, kDecBorder = 2 * kTcC, kDecUpdate = kDecBorder + 16, kDecRest = kDecUpdate + 4,
+              kDecFloats = kDecRest + kTcC / 4;
+__device__ __forceinline__ int dec_own(int w) { return kDecBorder + (w < 3 ? 4 * w + 4 : 13); }
 constexpr int kTcThreads = 19 * 32;
 constexpr uint32_t kBox = kTcC * 128;  // one TMA box: 128 rows of 128 bytes
 
@@ -172,9 +191,11 @@ __device__ __forceinline__ void store_split(unsigned char* hi, unsigned char* lo
 }
 
 // Shared memory: stages of Q, K, V as TMA writes them; V' (hi, lo); H (hi, lo); the output tile on its way to
-// the TMA store; per stage the decays: X of every token and the column factors of three blocks; barriers.
+// the TMA store; per stage the decays; barriers.
 // Wide heads have room for two stages and none for the output tile, which takes its chunk's V (needed later
 // in the stage's next chunk than Q and K).
+constexpr uint32_t kBarBytes = 352;
+
 template <int DK>
 struct TcShape {
   static constexpr int kBoxes = DK / 64;
@@ -185,17 +206,17 @@ struct TcShape {
   static constexpr uint32_t kVp = kStages * kStageBytes;
   static constexpr uint32_t kH = kVp + 2 * kBox;
   static constexpr uint32_t kOut = kH + 2 * DK * 128;
-  static constexpr uint32_t kDecStage = (kTcC + 96) * 4;
+  static constexpr uint32_t kDecStage = kDecFloats * 4;
   static constexpr uint32_t kDec = kOut + (kOwnOut ? kBox : 0);
   static constexpr uint32_t kBars = kDec + kStages * kDecStage;
-  static constexpr uint32_t kBytes = kBars + 512 + 256;  // and the rows' exponents (fp16)
+  static constexpr uint32_t kBytes = kBars + kBarBytes + 256;  // and the rows' exponents (fp16)
 };
 
 struct TcBars {
   uint64_t full[3], empty[3], v_empty[3];
   uint64_t s_full[2], p_full[2];
   uint64_t vp_full[2], vp_empty[2], l_full, l_empty, h_full, h_empty, o_full[2], o_empty[2], drain;
-  float total[3], total2[3];  // e^T of the stage's chunk, T log2 e
+  float total[3];  // e^T of the stage's chunk
   uint32_t tmem;
   int abort;
   // fp16: largest values of a chunk found by four warps, and the exponents they give
@@ -270,6 +291,14 @@ __device__ __forceinline__ float max_of2(uint32_t m) {
   return fmaxf(f.x, f.y);
 }
 
+// 2^-29 of the power of two below |t|, and its inverse: the unit of the rests of a block whose sum is t
+__device__ __forceinline__ float2 rest_unit(float t) {
+  const uint32_t e = max((__float_as_uint(t) >> 23) & 255u, 64u);
+  return make_float2(__uint_as_float((e - 29u) << 23), __uint_as_float((283u - e) << 23));
+}
+// s = t - z from its three parts
+__device__ __forceinline__ float block_rest(float t, float z, int rest) { return fmaf((float)rest, rest_unit(t).x, t - z); }
+
 // What a run writes: the segments' own states; outputs; outputs in parts or with their dot products (gradients
 // of q and k); outputs and a final state that is returned
 enum { kTcState = 0, kTcOut = 1, kTcGrad = 2, kTcOutState = 3 };
@@ -307,6 +336,11 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, wg = wid >> 2, row = tid & 127;
   auto first_token = [&](int c) { return (reverse ? n_live - 1 - c : c) * kTcC; };
   auto dec_X = [&](int st) { return reinterpret_cast<float*>(smem + S::kDec + st * S::kDecStage); };
+  // from a row's X: z, or in reverse s
+  auto dec_row = [&](int st, int w, float xi) {
+    const float* X = dec_X(st);
+    return reverse ? block_rest(X[dec_own(w)], xi, reinterpret_cast<const signed char*>(X + kDecRest)[row]) : -xi;
+  };
   const int64_t block = (int64_t)dk * dv;
   // for whole warps: the lanes go on, or give up, together
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
@@ -357,7 +391,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
     if ((wid & 3) == 0 && lane == 0) *reinterpret_cast<volatile uint32_t*>(&B.max_of[g][(i + 2) & 3]) = 0;
     return true;
   };
-  signed char* row_exp = reinterpret_cast<signed char*>(smem + S::kBars + 512);  // [2][128]
+  signed char* row_exp = reinterpret_cast<signed char*>(smem + S::kBars + kBarBytes);  // [2][128]
   constexpr bool kHalf = std::is_same<IT, __half>::value;
 
   if (wid == 16) {
@@ -411,38 +445,60 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
         g[r] = g[r] < kTcReset ? kTcReset : g[r];  // keeps NaN
       }
       if (c + 1 < cn) load(c + 1);
-      // inclusive sums, in 64 bits: a difference of two sums keeps its digits
-      const double s0 = (double)g[0], s1 = s0 + (double)g[1], s2 = s1 + (double)g[2], s3 = s2 + (double)g[3];
+      // inclusive sums in a block of 8 lanes, in 64 bits, times log2 e
+      constexpr double l2e = 1.4426950408889634;
+      const double s0 = l2e * (double)g[0], s1 = fma(l2e, (double)g[1], s0), s2 = fma(l2e, (double)g[2], s1),
+                   s3 = fma(l2e, (double)g[3], s2);
       double x = s3;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+      for (int o = 1; o < 8; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, x, o, 8);
+        if ((lane & 7) >= o) x += y;
       }
-      const double T = __shfl_sync(0xffffffffu, x, 31);
-      const double before = x - s3, after = T - before;
-      constexpr double l2e = 1.4426950408889634;
-      // X: what a token's update is weighted with (forward T - G, reverse G, times log2 e).  The decay
-      // between a row's and a column's token is e^{X_col - X_row} either way, the output's weight e^{T - X}
-      const double y0 = reverse ? before : after, ys = reverse ? l2e : -l2e, yb = y0 * l2e;
-      const float4 X = make_float4((float)fma(ys, s0, yb), (float)fma(ys, s1, yb), (float)fma(ys, s2, yb),
-                                   (float)fma(ys, s3, yb));
-      // factors of a block's 32 columns towards the block's border on the side of the rows that use them
-      const float f = __shfl_sync(0xffffffffu, X.w, reverse ? (lane & 24) - 1 : lane | 7);
-      const float4 factor = make_float4(ex2(X.x - f), ex2(X.y - f), ex2(X.z - f), ex2(X.w - f));
+      double of[4];  // the blocks' sums
+#pragma unroll
+      for (int r = 0; r < 4; ++r) of[r] = __shfl_sync(0xffffffffu, x, 8 * r + 7);
+      const double T = (of[0] + of[1]) + (of[2] + of[3]), before = x - s3, own = __shfl_sync(0xffffffffu, x, 7, 8);
+      const double z[4] = {before + s0, before + s1, before + s2, x};
+      const float tf = (float)own, unit = rest_unit(tf).y;
+      float X[4], factor[4];
+      uint32_t rest = 0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float zf = (float)z[r], s = tf - zf;
+        const float q = rintf((float)((own - z[r]) - (double)s) * unit);  // at most 96
+        const int qi = (int)fminf(fmaxf(q, -127.f), 127.f);
+        rest |= (uint32_t)(qi & 255) << (8 * r);
+        X[r] = reverse ? zf : -zf;
+        factor[r] = ex2(reverse ? zf : block_rest(tf, zf, qi));
+      }
+      // lanes 0 - 15: borders, 16 - 19: updates; the sum of blocks `lo` to before `hi`
+      const int w = lane >> 2 & 3, c4 = lane & 3;
+      const bool upd = lane >= 16, diagonal = w == c4;
+      int lo, hi;
+      if (upd) lo = reverse ? 0 : c4 + 1, hi = reverse ? c4 : 4;
+      else if (!reverse) lo = diagonal ? 0 : c4 + 1, hi = w;
+      else if (c4 < w) lo = c4 ? 3 : w - 1, hi = lo + 1;
+      else lo = w + 1, hi = diagonal ? 4 : c4;
+      double sum = 0.0;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum += r >= lo && r < hi ? of[r] : 0.0;
+      const float entry = (float)sum;
+      const bool raw = !upd && (diagonal || (reverse && c4 < w));
       seg_total += T;
       if (i >= S::kStages && !warp_wait(&B.empty[st], ph)) break;
       float* xs = dec_X(st);
-      *reinterpret_cast<float4*>(xs + 4 * lane) = X;
-      const int l = reverse ? lane - 8 : lane;  // blocks 0 - 2, reverse 1 - 3: the far block has no rows beyond it
-      if (!STATE_ONLY && l >= 0 && l < 24) *reinterpret_cast<float4*>(xs + kTcC + 4 * l) = factor;
-      if (lane == 0) B.total2[st] = (float)(T * l2e), B.total[st] = ex2((float)(T * l2e));
+      *reinterpret_cast<float4*>(xs + 4 * lane) = make_float4(X[0], X[1], X[2], X[3]);
+      *reinterpret_cast<float4*>(xs + kDecFactor + 4 * lane) = make_float4(factor[0], factor[1], factor[2], factor[3]);
+      reinterpret_cast<uint32_t*>(xs + kDecRest)[lane] = rest;
+      if (lane < 20) xs[kDecBorder + lane] = raw ? entry : ex2(entry);
+      if (lane == 0) B.total[st] = ex2((float)T);
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.full[st]);
       if (++st == S::kStages) st = 0, ph ^= 1;
     }
     if (STATE_ONLY && tile == 0 && lane == 0)
-      K.seg_decay[((int64_t)reverse * K.batch * K.heads + bh) * K.segs + seg] = (float)seg_total;
+      K.seg_decay[((int64_t)reverse * K.batch * K.heads + bh) * K.segs + seg] = (float)(seg_total * 0.6931471805599453);
   } else if (wid == 17) {
     // ------------------------------------------------------------ matrix instructions
     const uint32_t base = smem_u32(smem);
@@ -568,11 +624,12 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
         tc_after();
         const float* X = dec_X(st);
         const float xi = X[row];
+        // the row's part of its weights off the diagonal
+        const float own = pw * ex2(dec_row(st, w, xi));
         const uint32_t sp = lanes + kTmS + (i & 1) * 128;
         // 32 columns at a time.  P's columns x .. x + 31 land on S's columns x / 2 .., always behind
-        // what is still to be read; blocks on the far side of the diagonal are zero.  Off the diagonal
-        // e^{X_j - X_i} = e^{R - X_i} e^{X_j - R}, R the value at the columns' border: one exponential a
-        // row, and the columns' factors from the loading warp
+        // what is still to be read; blocks on the far side of the diagonal are zero.  Off the diagonal one
+        // exponential a row, and the columns' factors from the warp of the decays
 #pragma unroll 1
         for (int x = 0; x < 4; ++x) {
           uint32_t p[16];
@@ -580,8 +637,8 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
             float s[32];
             tmem_ld32(sp + x * 32, s);
             if (x != w) {
-              const float2 rf = f2(pw * ex2(X[reverse ? x * 32 - 1 : x * 32 + 31] - xi));
-              const float* cf = X + kTcC + (reverse ? x - 1 : x) * 32;
+              const float2 rf = f2(own * X[kDecBorder + 4 * w + x]);
+              const float* cf = X + kDecFactor + x * 32;
               tc_wait_ld();
 #pragma unroll
               for (int j = 0; j < 32; j += 4) {
@@ -640,7 +697,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
         }
       }
       __syncwarp();
-      float wv = ex2(dec_X(st)[row]);
+      float wv = dec_X(st)[kDecFactor + row] * dec_X(st)[kDecUpdate + (row >> 5)];
       int v_exp = 0;
       if constexpr (kHalf) {
         uint32_t vm = 0;
@@ -700,7 +757,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       for (int c = c0, i = 0, st = 0, ph = 0; c < cn; ++c, ++i) {
         const int t0 = first_token(c), m = min(kTcC, len - t0), t = t0 + row;
         if (!warp_wait(&B.full[st], ph)) break;
-        const float2 w = f2(A.scale * ex2(*reinterpret_cast<volatile float*>(&B.total2[st]) - dec_X(st)[row]));
+        const float2 w = f2(A.scale * ex2(dec_X(st)[kDecBorder + 5 * w4] + dec_row(st, w4, dec_X(st)[row])));
         const bool on = row < m;
         __syncwarp();
         if (lane == 0) {

@@ -637,3 +637,111 @@ def test_strides_of_axes_of_one_do_not_matter(dtype, b, l, h, hk):
 
     for x, y in zip(once(odd), once(lambda x: x)):
         assert torch.equal(x, y)
+
+
+def decay_gradient(t, scale):
+    """dlog_decay of the outputs alone in float64, from every pair of tokens: the weight of (i, j) holds the decays of
+    j < t <= i.  Also the same sum of absolute values, and the largest sum over a token's own pairs.  A reset is -1e5."""
+    q, k = (t[n].double().repeat_interleave(t["v"].shape[2] // t[n].shape[2], 2) for n in ("q", "k"))
+    b, l, h, _ = t["v"].shape
+    g = t["g"].double().clamp(min=-1e5).expand(b, l, h)
+    G = g.cumsum(1).transpose(1, 2)
+    D = torch.exp(torch.where(torch.ones(l, l, device="cuda").tril() > 0, G[..., :, None] - G[..., None, :], -torch.inf))
+    pair = lambda x, y: torch.einsum("bihd,bjhd->bhij", x, y)  # noqa: E731
+    N = scale * D * pair(q, k) * pair(t["do"].double(), t["v"].double())
+
+    def spanning(x):  # sum over j < t <= i
+        left = torch.nn.functional.pad(x, (1, 0)).cumsum(-1)[..., :-1]              # [i, t]: j < t
+        return left.flip(-2).cumsum(-2).flip(-2).diagonal(dim1=-2, dim2=-1).transpose(1, 2)
+
+    return spanning(N), spanning(N.abs()), float((N.abs().sum(-1) + N.abs().sum(-2)).max())
+
+
+def own_decay_gradient(t, scale):
+    from mamba_b200 import linear_attention_fn
+
+    g = t["g"].detach().requires_grad_()
+    return torch.autograd.grad(linear_attention_fn(t["q"], t["k"], t["v"], g, scale), g, t["do"])[0]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bias,b,l,h,hk,dk,dv", [(-3.0, 1, 200, 2, 2, 64, 64), (0.0, 2, 333, 4, 2, 128, 64), (2.0, 1, 129, 2, 1, 40, 57),
+                                                 (7.0, 1, 200, 2, 2, 64, 64), (0.0, 1, 2600, 2, 2, 128, 64), (5.0, 1, 2600, 2, 1, 64, 128),
+                                                 (-3.0, 1, 2600, 2, 2, 64, 64)])
+def test_decays_gradient_of_every_row_and_head(dtype, bias, b, l, h, hk, dk, dv):
+    """The relative 2-norm of dlog_decay's error, per row and head.  The gradient is what is left of the suffix sums of
+    two runs' dot products, so it holds only if the runs weight and round alike.  16 bits: each pair's weighted score
+    is rounded once, the same in both runs (half a step u at most, u / sqrt 3 in the mean square), the result once
+    more: sqrt(2/3) u where they are independent, and 2 u is asked for.  fp32: a dot product of some 128 fp32 terms is
+    off by 2^-24 sqrt(128), a suffix of n of them by sqrt(n) as much; of pairs that span a token with decays of
+    e^-3 a twentieth of that product is left, 2^-20.5 sqrt(200) 20 = 2^-12.4."""
+    t = make(b, l, h, hk, dk, dv, dtype, bias=bias, seed=l + int(bias))
+    want, _, _ = decay_gradient(t, 0.3)
+    got = own_decay_gradient(t, 0.3).double()
+    bound = 2.0 ** -12 if dtype == torch.float32 else 2 * HALF[dtype]
+    off = lambda x: ((x - want).norm(dim=1) / want.norm(dim=1)).max()  # noqa: E731
+    assert float(off(got)) <= bound, f"{float(off(got)):.3g} of the norm, {bound:.3g} asked for"
+    assert float(off(0 * got)) > bound and float(off(-got)) > bound
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("l,hk", [(150, 16), (1500, 4)])
+def test_one_decay_per_heads_gradient(dtype, l, hk):
+    """The same for one decay per head: a value per head, so the norm is over the 16 heads.  The sum over tokens is
+    one over more independent roundings, of a value that is rounded once itself (fp32 here)."""
+    t = make(2, l, 16, hk, 64, 64, dtype, per_head=True, seed=l)
+    want = decay_gradient(t, 0.3)[0].sum((0, 1))
+    got = own_decay_gradient(t, 0.3).double()
+    bound = 2.0 ** -12 if dtype == torch.float32 else 2 * HALF[dtype]
+    off = lambda x: float((x - want).norm() / want.norm())  # noqa: E731
+    assert off(got) <= bound and off(0 * got) > bound and off(-got) > bound, off(got)
+
+
+def with_resets(n, dtype, bias=2.0, state=False):
+    """n resets among the tokens of the second chunk of 128."""
+    t = make(1, 300, 2, 1, 64, 64, dtype, bias=bias, state=state, seed=50 + n)
+    at = 128 + torch.randperm(128, generator=torch.Generator().manual_seed(n))[:n].cuda()
+    t["g"][0, at] = float("-inf")
+    return t, at
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 2, 12, 40, 90, 128])
+def test_decays_gradient_between_resets(dtype, n):
+    """Every value against its own pairs: what stands behind a reset has to cancel out of the suffix sums.  With u the
+    half step of 16 bits, a pair's product is off by u (its score), the result by u; 2^-17 for fp32's sums.  The
+    products that cancel are sums of some 128 fp32 terms (2^-24 sqrt 128 of M, the largest sum over a token's pairs),
+    some 300 of them in a suffix: 2^-16 M."""
+    t, at = with_resets(n, dtype)
+    want, local, M = decay_gradient(t, 0.3)
+    got = own_decay_gradient(t, 0.3).double()
+    u = HALF[dtype]
+    tol = (u * 1.01 * (local + want.abs()) if dtype != torch.float32 else 2.0 ** -17 * local) + 2.0 ** -16 * M
+    worst = lambda x: float(((x - want).abs() / tol).max())  # noqa: E731
+    assert float(got[0, at].abs().max()) == 0
+    assert worst(got) <= 1, worst(got)
+    assert worst(0 * got) > 1 and worst(-got) > 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [2, 40, 128])
+@pytest.mark.parametrize("bias", [-2.0, 5.0])
+def test_gradients_with_resets(dtype, n, bias):
+    """Outputs, states and the other gradients where resets stand, few or all of a chunk's tokens, in the middle of
+    tokens that forget or last."""
+    from mamba_b200 import linear_attention_fn
+
+    t, _ = with_resets(n, dtype, bias, state=True)
+    leaves = [t[x].detach().requires_grad_() for x in ("q", "k", "v", "s0")]
+    out = linear_attention_fn(*leaves[:3], t["g"], 0.3, leaves[3], None, True)
+    grads = torch.autograd.grad(list(out), leaves, [t["do"], t["dF"]])
+    t["g"] = t["g"].double().clamp(min=-1e5)
+    want_o, want_f, want = reference(t, 0.3, True)
+    mag_o, mag_f, mags = reference(t, 0.3, True, absolute=True)
+    f32 = dtype == torch.float32
+    soft, hard = (2.0 ** -17, 2.0 ** -17) if f32 else (2 * HALF[dtype] + 2.0 ** -17, 2.0 ** -14)
+    close("o", out[0], want_o, mag_o, dtype, soft)
+    close("final", out[1], want_f, mag_f, dtype, hard)
+    for name, got, w, m, f in zip(("dq", "dk", "dv", "dinitial_state"), grads, want[:3] + want[4:], mags[:3] + mags[4:],
+                                  (soft, soft, soft, hard)):
+        close(name, got, w, m, dtype, f)
