@@ -486,8 +486,9 @@ SS_API int ss_last_cuda_error(void);
  * reset != 0 clears the bits. */
 SS_API int ss_device_status(int reset, void* stream);
 
-/* Limit, in SM clock cycles, of every bounded wait the scan kernels make for a TMA tile, for
- * the launches that follow from this process (all threads); returns the previous limit.
+/* Limit, in SM clock cycles, of every bounded wait the scan kernels make for a TMA tile, and the
+ * linear-attention kernel for a tile or a matrix instruction (in steps of some 64 ms there; 0: its first
+ * wait is a single probe), for the launches that follow from this process (all threads); returns the previous limit.
  * cycles < 0 restores the default (4e9 cycles, about 2 s).  A wait that runs out raises bit 1
  * of the device status (ss_device_status), lets the CTA's copies in flight land (bounded by
  * the default) and ends the CTA, leaving its outputs incomplete.  No counterpart in the

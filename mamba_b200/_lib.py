@@ -435,7 +435,7 @@ def maybe_check_status(device, what: str) -> None:
 
 
 def set_wait_limit(cycles: int) -> int:
-    """Limit (SM clock cycles) of the scan kernels' bounded waits for a TMA tile, for the launches
+    """Limit (SM clock cycles) of the bounded waits of the scan and linear-attention kernels, for the launches
     that follow; returns the previous one.  cycles < 0 restores the default (~2 s)."""
     return int(lib().ss_set_wait_limit(int(cycles)))
 

@@ -258,15 +258,21 @@ __device__ __forceinline__ bool mbar_try_wait_often(uint64_t* bar, uint32_t pari
 // the part of a wait that is not over at once; false: it gave up, here or in another role
 __device__ __noinline__ bool tc_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort, long long limit, int* status) {
   const long long t0 = clock64();
-  while (!mbar_try_wait_often(bar, parity)) {
+  while (limit == 0 || !mbar_try_wait_often(bar, parity)) {
     if (*abort) return false;
-    if (clock64() - t0 > limit) {
+    if (limit == 0 || clock64() - t0 > limit) {
       *abort = 1;
       if (status) atomicOr(status, kStatusTimeout);
       return false;
     }
   }
   return true;
+}
+
+// A limit of 0 makes the first wait for a stage a single probe (a choice at every wait cost 5 % of a forward)
+__device__ __noinline__ bool tc_first_wait(uint64_t* bar, volatile int* abort, long long limit, int* status) {
+  if (limit != 0 || __all_sync(0xffffffffu, mbar_test_wait(bar, 0))) return true;
+  return tc_wait_slow(bar, 0, abort, 0, status);
 }
 
 // exponent of the power of two that brings values up to m to just below 2^15 (0 where there is nothing to bring)
@@ -520,7 +526,7 @@ __device__ __forceinline__ void linear_tc_run(const LinTcK& P, int pass, int til
       }
       __syncwarp();
     };
-    const int n = cn - c0;
+    const int n = cn > c0 && tc_first_wait(&B.full[0], &B.abort, P.wait_limit, P.status) ? cn - c0 : 0;
     for (int i = 0, st = 0, ph = 0; i < n; ++i) {  // ph: the stages' phase
       if (!warp_wait(&B.full[st], ph)) break;
       tc_after();

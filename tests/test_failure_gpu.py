@@ -91,3 +91,38 @@ def test_status_check_is_silent_on_success(lib):
         mamba_b200.set_status_check(prev)
     compare(got, oracle_case(inp), torch.float32)
     mamba_b200.check_device_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear_attention_gives_up_and_recovers(lib, dtype):
+    """The tensor-core kernel with a limit of 0: the first wait of its matrix instructions is a single probe, which
+    counts as timed out; every other role waits for what then never comes, sees that and ends.  The bit is raised by
+    the forward and the backward, in one segment and in several (states, fold, main pass), and the same calls give
+    the same bits as before right after."""
+    import mamba_b200
+
+    g = torch.Generator().manual_seed(44)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda().requires_grad_()  # noqa: E731
+    for l in (200, 1500):
+        q, k, v = r(1, l, 1, 64), r(1, l, 1, 64), r(1, l, 2, 64)
+        decay = (-torch.rand(1, l, 2, generator=g)).cuda().requires_grad_()
+        dout = r(1, l, 2, 64).detach()
+        call = lambda: mamba_b200.linear_attention_fn(q, k, v, decay, return_final_state=True)  # noqa: E731
+        grads = lambda out: torch.autograd.grad(out[0], [q, k, v, decay], dout)  # noqa: E731
+        out = call()
+        want = [*out, *grads(out)]
+        lib.device_status("cuda", reset=True)
+        out = call()
+        lib.set_wait_limit(0)
+        grads(out)
+        assert lib.device_status("cuda", reset=True) & 1
+        with torch.no_grad():
+            call()
+        torch.cuda.synchronize()
+        lib.set_wait_limit(-1)
+        with pytest.raises(RuntimeError, match="bounded wait"):
+            mamba_b200.check_device_status()
+        out = call()
+        for a, b in zip([*out, *grads(out)], want):
+            assert torch.equal(a, b)
+        assert lib.device_status("cuda") == 0
