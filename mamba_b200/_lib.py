@@ -379,7 +379,13 @@ def launch(name: str, packed: bytes, device: torch.device) -> None:
 def differentiated(tensors) -> bool:
     """Whether a call goes through its autograd function: where a tensor wants a gradient, and inside a level of
     forward-mode differentiation, which the function refuses (passed by, it would leave a derivative of zero)."""
-    return _forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+    if _forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def written(tensors) -> None:

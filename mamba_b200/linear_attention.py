@@ -221,17 +221,16 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, seq_
     copied first."""
     want = bool(return_final_state)
     cut = None
-    if v.dtype in (torch.bfloat16, torch.float16):
-        _cuda_device(q, k, v, log_decay, initial_state, seq_lens)
-        h, _, dk, dv = _check_heads(q, k, v, 4)  # of what the caller passed, not of the padded copies
-        if v.numel():
-            if dk % 8 or dv % 8:
-                scale = _scale(scale, dk)
-                cut = dk, dv
-                if initial_state is not None:
-                    _check_state(initial_state, (v.shape[0], h, dk, dv), "initial_state")
-                    initial_state = torch.nn.functional.pad(initial_state, (0, -dv % 8, 0, -dk % 8))
-            q, k, v = _whole(_as(q, v.dtype)), _whole(_as(k, v.dtype)), _whole(v)
+    if v.dtype in (torch.bfloat16, torch.float16) and v.dim() == k.dim() == q.dim() == 4 and v.numel():
+        if (q.shape[3] | k.shape[3] | v.shape[3]) % 8:  # padded below: the sizes that were passed are checked first
+            _cuda_device(q, k, v, log_decay, initial_state, seq_lens)
+            h, _, dk, dv = _check_heads(q, k, v, 4)
+            scale = _scale(scale, dk)
+            cut = dk, dv
+            if initial_state is not None:
+                _check_state(initial_state, (v.shape[0], h, dk, dv), "initial_state")
+                initial_state = torch.nn.functional.pad(initial_state, (0, -dv % 8, 0, -dk % 8))
+        q, k, v = _whole(_as(q, v.dtype)), _whole(_as(k, v.dtype)), _whole(v)
     if L.differentiated((q, k, v, log_decay, initial_state)):
         out = LinearAttentionFn.apply(q, k, v, log_decay, scale, initial_state, seq_lens, want)
         o, final = out if want else (out, None)
