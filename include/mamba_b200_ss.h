@@ -454,7 +454,7 @@ SS_API int ss_linear_bwd(const ss_linear_bwd_args* args, void* stream);
 SS_API int ss_linear_step(const ss_linear_step_args* args, void* stream);
 
 /* Scratch bytes of ss_linear_fwd (backward = 0) or ss_linear_bwd (1) for these sizes, types and
- * strides (data pointers and seq_lens' values are not looked at); 0 for invalid sizes. */
+ * strides (data pointers and seq_lens' values are not looked at); 0 for sizes that the calls refuse. */
 SS_API size_t ss_linear_work_bytes(const ss_linear_args* args, int backward);
 
 /* Norms before and after a block with gate and residual scale (see ss_block_norm_args). */
@@ -469,7 +469,7 @@ SS_API size_t ss_block_norm_work_elems(int64_t rows, int dim, int io_dtype);
 /* One step of beam search (see ss_beam_args). */
 SS_API int ss_beam_select(const ss_beam_args* args, void* stream);
 
-/* Bytes of ss_beam_args.work. */
+/* Bytes of ss_beam_args.work; 0 for sizes that the call refuses. */
 SS_API size_t ss_beam_work_bytes(int batch, int beams, int vocab, int num_select);
 
 /* Reorders per-beam states in place (see ss_reorder_args). */

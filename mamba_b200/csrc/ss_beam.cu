@@ -22,6 +22,10 @@ bool sizes_ok(int batch, int beams, int vocab, int k) {
   return batch >= 0 && beams >= 1 && vocab >= 1 && k >= 1 && (int64_t)k <= (int64_t)beams * vocab;
 }
 
+bool limits_ok(int beams, int vocab, int k) {
+  return beams <= SS_MAX_BEAMS && k <= 32 && (int64_t)beams * vocab <= (1 << 30);
+}
+
 template <typename K>
 cudaError_t launch_dependent(void (*kern)(K), dim3 grid, int threads, const K& P, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
@@ -41,7 +45,7 @@ cudaError_t launch_dependent(void (*kern)(K), dim3 grid, int threads, const K& P
 extern "C" {
 
 size_t ss_beam_work_bytes(int batch, int beams, int vocab, int num_select) {
-  if (!sizes_ok(batch, beams, vocab, num_select) || batch == 0) return 0;
+  if (!sizes_ok(batch, beams, vocab, num_select) || !limits_ok(beams, vocab, num_select) || batch == 0) return 0;
   const int64_t rows = (int64_t)batch * beams;
   return (size_t)rows * slices_of(rows, vocab) * (sizeof(BeamSlice) + sizeof(u64) * num_select);
 }
@@ -50,8 +54,7 @@ int ss_beam_select(const ss_beam_args* a, void* stream) {
   if (a == nullptr) return SS_ERR_INVALID;
   if (!sizes_ok(a->batch, a->beams, a->vocab, a->num_select)) return SS_ERR_INVALID;
   if (a->io_dtype != SS_F32 && a->io_dtype != SS_BF16 && a->io_dtype != SS_F16) return SS_ERR_UNSUPPORTED;
-  if (a->beams > SS_MAX_BEAMS || a->num_select > 32 || (int64_t)a->beams * a->vocab > (1 << 30))
-    return SS_ERR_UNSUPPORTED;
+  if (!limits_ok(a->beams, a->vocab, a->num_select)) return SS_ERR_UNSUPPORTED;
   if (a->finished && (a->eos_token < 0 || a->eos_token >= a->vocab)) return SS_ERR_INVALID;
   if (a->batch == 0) return SS_OK;
   if (!a->logits || !a->scores || !a->out_scores || !a->parents || !a->tokens || !a->work ||

@@ -31,6 +31,12 @@ bool sizes_ok(const ss_linear_args& a) {
          a.key_dim >= 1 && a.value_dim >= 1;
 }
 
+// what the kernels' indexes hold
+bool limits_ok(const ss_linear_args& a) {
+  return a.key_dim <= SS_MAX_LINEAR_DIM && a.value_dim <= SS_MAX_LINEAR_DIM && (int64_t)a.batch * a.heads <= (1 << 24) &&
+         a.seqlen <= (1 << 30);
+}
+
 bool dtypes_ok(int io, int decay) {
   return (io == SS_F32 || io == SS_BF16 || io == SS_F16) && (decay == SS_F32 || decay == io);
 }
@@ -257,8 +263,7 @@ bool work_ok(const Work& w, const void* p) { return !w.bytes || (p && (reinterpr
 int check_fwd(const ss_linear_args& a) {
   if (!sizes_ok(a)) return SS_ERR_INVALID;
   if (!dtypes_ok(a.io_dtype, a.decay_dtype)) return SS_ERR_UNSUPPORTED;
-  if (a.key_dim > SS_MAX_LINEAR_DIM || a.value_dim > SS_MAX_LINEAR_DIM) return SS_ERR_UNSUPPORTED;
-  if ((int64_t)a.batch * a.heads > (1 << 24) || a.seqlen > (1 << 30)) return SS_ERR_UNSUPPORTED;  // 32-bit token indexes
+  if (!limits_ok(a)) return SS_ERR_UNSUPPORTED;
   if (!std::isnormal(a.scale)) return SS_ERR_INVALID;  // its reciprocal is needed too
   const bool empty = a.batch == 0 || a.seqlen == 0;
   if (!empty && (!a.q || !a.k || !a.v || !a.log_decay)) return SS_ERR_INVALID;
@@ -270,7 +275,7 @@ int check_fwd(const ss_linear_args& a) {
 extern "C" {
 
 size_t ss_linear_work_bytes(const ss_linear_args* a, int backward) {
-  if (a == nullptr || !sizes_ok(*a) || a->key_dim > SS_MAX_LINEAR_DIM || a->value_dim > SS_MAX_LINEAR_DIM) return 0;
+  if (a == nullptr || !sizes_ok(*a) || !limits_ok(*a)) return 0;
   return work_of(*a, backward != 0).bytes;
 }
 

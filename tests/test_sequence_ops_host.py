@@ -213,3 +213,16 @@ def test_what_goes_through_the_autograd_functions():
         with forward_ad.dual_level():
             assert L.differentiated((plain,))
     assert not L.differentiated((plain,))
+
+
+def test_workspaces_of_sizes_beyond_the_limits_are_empty():
+    """Sizes that the calls refuse, up to the largest int: no size (and no overflow on the way to one)."""
+    lib = L.lib()
+    for kw in (dict(seqlen=2 ** 31 - 1), dict(seqlen=2 ** 30 + 1), dict(batch=2 ** 23, heads=4), dict(batch=2 ** 31 - 1, heads=2 ** 31 - 1, key_heads=1)):
+        a = _linear_args(**kw)
+        assert lib.ss_linear_work_bytes(ctypes.byref(a), 0) == 0 and lib.ss_linear_work_bytes(ctypes.byref(a), 1) == 0, kw
+        assert lib.ss_linear_fwd(ctypes.byref(a), None) != L.SS_OK
+    assert lib.ss_linear_work_bytes(ctypes.byref(_linear_args(batch=1, heads=1, key_heads=1, seqlen=2 ** 30)), 1) > 2 ** 33
+    for sizes in ((1, 1, 2 ** 31 - 1, 1), (1, 32, 2 ** 26, 4), (1, 33, 100, 4), (1, 4, 100, 33), (2 ** 31 - 1, 32, 2 ** 31 - 1, 32)):
+        assert lib.ss_beam_work_bytes(*sizes) == 0, sizes
+    assert lib.ss_beam_work_bytes(1, 32, 2 ** 25, 32) > 0
