@@ -357,7 +357,7 @@ typedef struct ss_block_norm_bwd_args {
  *   finished beam: its score at eos_token, -infinity elsewhere
  * and the num_select largest of (beams x vocab), the lowest index first among equals.  A candidate
  * that is not a number, and every candidate of a beam whose score is NaN or +infinity, counts as
- * -infinity.  Candidates are compared in fp64.  beams and num_select are at most SS_MAX_BEAMS, beams * vocab
+ * -infinity.  Candidates are compared in fp64, with a logsumexp that is good to 1e-7.  beams and num_select are at most SS_MAX_BEAMS, beams * vocab
  * at most 2^30. */
 typedef struct ss_beam_args {
   int batch, beams, vocab, num_select, io_dtype;

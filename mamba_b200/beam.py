@@ -24,7 +24,9 @@ def beam_select(logits, scores, num_select=None, finished=None, eos_token_id=Non
     bool: such a beam offers itself alone, at eos_token_id with its score unchanged, and its logits
     are not read.  Candidates that are not a number count as -inf, as does every candidate of a beam
     whose score is NaN or +inf.  Returns (scores, parents, tokens), each (batch, num_select), in falling
-    order of score, equal candidates in order of (beam, token); scores fp32, indices int64.
+    order of score, equal candidates in order of (beam, token); scores fp32, indices int64.  Candidates
+    are compared in fp64; a beam's log-softmax is good to 1e-7 (its exponentials are fp32), so candidates
+    of different beams that are nearer than that may change places against exact arithmetic.
     num_select (beams when None) and beams are at most 32."""
     dev = _cuda_device(logits, scores, finished)
     if logits.dim() != 3:

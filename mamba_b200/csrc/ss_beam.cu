@@ -12,7 +12,8 @@ namespace {
 using namespace ssb;
 
 // slices of a beam's vocabulary: about three CTAs per SM over all beams (a longer slice offers fewer of its
-// logits: 192 beams x 50280 fp32 take 28 us in slices of 8 thousand, 21 us in these), at least 2048 tokens each
+// logits: 192 beams x 50280 fp32 take 55 us in slices of 8 thousand, 51 us in these, both kernels), at least 1024
+// tokens each
 int slices_of(int64_t rows, int vocab) {
   const int64_t want = std::max<int64_t>(1, (3 * 148 + rows - 1) / std::max<int64_t>(1, rows));
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, (vocab + 2047) / 2048, 64}));

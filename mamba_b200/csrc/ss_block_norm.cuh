@@ -13,15 +13,23 @@
 //
 // Bound by the memory traffic: the rows stay in registers between the statistics and their use, so
 // every tensor moves once.  A row belongs to WPR warps, each lane holding NV groups of 4 values of every
-// tensor (8 bytes of a 16-bit type, 16 of fp32): 12 values a lane keep the backward's rows, weights and
-// column sums in 128 registers, where the 24 of one warp to a row of 768 spilled (163 us a pass over
-// 16384 rows).  A row's warps meet at a barrier of their own.  A lane's columns are the same for all its
+// tensor (8 bytes of a 16-bit type, 16 of fp32): up to 12 values a lane where 8 warps hold the row so, where the
+// 24 of one warp to a row of 768 spilled (163 us a pass over 16384 rows).  128 registers hold the backward's
+// rows, weights and column sums then for gated 16-bit rows of two warps and more and for fp32 rows without a gate
+// (nothing or a few bytes spilled); gated fp32 rows spill about 300 bytes a thread, gated 16-bit rows of one warp
+// 200, and rows longer than 8 warps of 12 values (16 - 32 values a lane) up to 2 KB.  A row's warps meet at a barrier of their own.  A lane's columns are the same for all its
 // rows: their weights are loaded once, with the first row, and in the backward their two sums stay in
 // registers over the rows of a persistent CTA; the CTAs' sums meet in a second small kernel (4 us) in a fixed
 // order, so the gradients of the weights do not vary between runs.
-// Measured: 16384 rows of 768, bf16, gated: forward 27 us (126 MB, 4.7 TB/s, 72 % of the copy rate), backward
-// 43 us (201 MB, 4.6 TB/s, 71 %; 65 us with each row loaded when its turn comes); 4099 rows of 2560, fp32:
-// forward 32 us (168 MB, 5.3 TB/s), backward 45 us (252 MB, 5.6 TB/s; 51 us).
+// Measured (kernels, cold L2; shares of the copy rate), forward and backward:
+//   16384 x 768 bf16, gated       28 us 69 %    44 us 70 %  (65 us with each row loaded when its turn comes)
+//   4099 x 2560 fp32              32 us 81 %    45 us 86 %  (51 us)
+//   8192 x 768 fp32, gated        26 us 74 %    52 us 60 %
+//   32768 x 384 bf16, gated       28 us 69 %    65 us 47 %
+//   2048 x 8192 bf16, gated       60 us 43 %   185 us 22 %
+//   2048 x 8192 fp32, gated       72 us 72 %   323 us 25 %
+// 69 - 70 % is latency: 24 warps an SM wait for their rows half of the time in the forward (16 in the backward,
+// which issues in 60 % of its cycles); below 60 % it is the spills.
 #pragma once
 #include "ss_norm.cuh"
 

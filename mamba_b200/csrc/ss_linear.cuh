@@ -85,8 +85,9 @@ __device__ __forceinline__ float lin_decay(const LinK& P, int b, int t, int h, b
 // 16-bit tensor-core operands would lose half the mantissa.  A chunk is a chain of short steps with
 // barriers between them, so heads of at most DMAX = 64 run two CTAs on an SM (and are cut into twice the
 // segments); wider ones fill its shared memory alone.  8 x 1024 tokens of 12 heads of 64 x 64 take 150 us forward
-// (21 TFLOP/s) and 326 us backward, 296 and 683 us with one CTA of 4 x 4 tiles to an SM; what bounds a chunk
-// now is reading the operands' tiles from shared memory (12 wavefronts for 32 multiply-adds of a warp).
+// (21 TFLOP/s) and 326 us backward, 296 and 683 us with one CTA of 4 x 4 tiles to an SM.  What bounds a chunk now
+// is no single unit: of the main pass's cycles 64 % issue an instruction and 58 % move a wavefront of shared memory
+// (12 of them for 32 multiply-adds of a warp), and 16 warps an SM wait for one another at the barriers.
 constexpr int kLsC = 64;          // tokens of a chunk
 constexpr int kLsN = 64;          // value columns of a CTA
 constexpr int kLsThreads = 256;

@@ -22,12 +22,14 @@
 //
 // What bounds it: neither memory nor the tensor cores, but the hand-overs between the roles.  A chunk with keys
 // of 64 takes about 2.3 us a CTA (a gradient: 4400 cycles, of them 4000 in the warps that make the outputs),
-// its products 1500 cycles; a load that was issued early arrives after 3000.  Measured:
-//   8 x 2048 tokens, 24 heads of 64 x 64, bf16       76 us forward (201 MB, 2.6 TB/s), 247 us backward
-//   1 x 16384 tokens, 16 heads of 128 x 128, bf16    151 us forward (268 MB, 1.8 TB/s), 168 with the final state
-//   4 x 1999 tokens, 16 heads, 4 of keys, fp16       91 us forward, 308 us backward
+// its products 1500 cycles; a load that was issued early arrives after 3000.  All 19 warps get 96 registers, which
+// is too few for the outputs and the state: every instance spills, 136 - 320 bytes stored and 200 - 448 loaded, most
+// of it in the gradients' (outputs with their dot products, on the chain).  Measured (kernels, cold L2):
+//   8 x 2048 tokens, 24 heads of 64 x 64, bf16       73 us forward (201 MB, 2.7 TB/s), 228 us backward
+//   1 x 16384 tokens, 16 heads of 128 x 128, bf16    153 us forward (268 MB, 1.8 TB/s), 170 with the final state
+//   4 x 1999 tokens, 16 heads, 4 of keys, fp16       89 us forward, 300 us backward
 // Tried and slower: the outputs of gradients shared with the scores' warps (273 against 250 us: a chunk's scores
-// then wait for the outputs before them), 32 columns of outputs at a time (295 us: it spills).
+// then wait for the outputs before them), 32 columns of outputs at a time (295 us: it spills more).
 // Two value tiles of one head run side by side, so keys and queries come from L2 the second time.
 // Roles (19 warps): 0-3 scores, 4-7 weighted values, 8-11 outputs, 12-15 state, 16 loads, 17 matrix
 // instructions, 18 decays.  The only chain from chunk to chunk is H: L -> state warps -> Q H.

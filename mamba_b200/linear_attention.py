@@ -218,7 +218,8 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, seq_
     float32, bfloat16 and float16; the state is fp32 throughout.  Tokens are summed in chunks, so one that holds
     an infinity or NaN reaches the outputs of up to 127 tokens before it.  16-bit inputs run on the tensor cores; for
     that, inputs whose rows are not whole 16-byte units (head sizes off a multiple of 8, odd strides) are
-    copied first."""
+    copied first.  q and k are taken in v's dtype.  Differentiable once (a second or a forward-mode
+    derivative raises)."""
     want = bool(return_final_state)
     cut = None
     if v.dtype in (torch.bfloat16, torch.float16) and v.dim() == k.dim() == q.dim() == 4 and v.numel():

@@ -212,8 +212,11 @@ def block_norm_fn(y, residual, post_weight=None, pre_weight=None, gate=None, res
     post_weight (dim,): the norm after the block (none when None); gate (y's shape), through
     ``activation`` ("silu", "sigmoid" or None: as it is); residual_scale: a (dim,) tensor or a number;
     pre_weight (dim,): the norm before the next block.  Norms scale by 1 + weight (unit_offset) or
-    weight.  Everything is computed in fp32 and rounded once, x from the unrounded h.  dim is at most
-    8192.  Returns (x, h), or h alone without pre_weight; differentiable in every tensor."""
+    weight.  residual and gate are taken in y's dtype (cast to it where they come in another: an fp32
+    residual beside a 16-bit y is rounded first), and x and h are returned in it; between, everything is
+    computed in fp32 and rounded once, x from the unrounded h.  dim is at most 8192.  Returns (x, h), or h
+    alone without pre_weight; differentiable in every tensor, once (a second or a forward-mode derivative
+    raises)."""
     shape = y.shape
     if residual.shape != shape or (gate is not None and gate.shape != shape):
         raise ValueError("residual and gate must have the shape of y")
